@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define INTFA_VERSION 8
+#define INTFA_VERSION 9
 
 /* forward variants (one entry point each, below) */
 enum { INTFA_VARIANT_FULL_INT8 = 0, INTFA_VARIANT_HALF_INT8 = 1, INTFA_VARIANT_FP16 = 2 };
@@ -61,8 +61,10 @@ enum {
     INTFA_ERR_SPLITS = -8,        /* num_splits out of range */
     INTFA_ERR_VSCALE = -9,        /* v_scale_block neither a multiple of the key-block length nor 64 at head_dim 128, or
                                      vs_stride_blk below head_dim */
-    INTFA_ERR_SCRATCH = -10       /* intfa_fwd_full_int8_static: the call's split-KV partials exceed
+    INTFA_ERR_SCRATCH = -10,      /* intfa_fwd_full_int8_static: the call's split-KV partials exceed
                                      INTFA_STATIC_SCRATCH_BYTES, or the device index is beyond the table of 64 devices */
+    INTFA_ERR_PAGE = -11,         /* page_size not 16, 32, 64, 128 or 256, no page, or a block table without a column */
+    INTFA_ERR_ROPE = -12          /* rotated pairs not a multiple of 8 or more than half of head_dim, or a magnitude that is not a positive number */
 };
 
 /*
@@ -265,7 +267,7 @@ int intfa_quant_perblock_channel(const void* x, int64_t stride_b, int64_t stride
 
 /* Appends new keys (and values) to an int8 K/V cache: the counterpart, for the quantised cache this library reads, of
  * the copy the reference's cache kernel makes of knew/vnew before it attends (csrc/flash_fwd_kernel.h:690-790,
- * Append_KV; csrc/flash.h:104-112; rotary embedding and paged caches are not part of this library).  For batch entry b the
+ * Append_KV; csrc/flash.h:104-112; with rotary positions and pages: intfa_paged_append_int8).  For batch entry b the
  * rows go to positions len_b .. len_b + seqlen_new - 1 of the cache, len_b = seqlens_k[b] (device memory, clamped to
  * [0, seqlen_cache]) or seqlen_filled when seqlens_k is NULL; rows that would land at or past seqlen_cache are dropped.
  * The lengths themselves are the caller's to advance (a forward call with seqlens_k = len + seqlen_new then sees them).
@@ -292,6 +294,105 @@ typedef struct intfa_append_params {
     int32_t batch, heads_kv, seqlen_new, seqlen_cache, head_dim, dtype;
 } intfa_append_params;
 int intfa_kvcache_append_int8(const intfa_append_params* p, void* stream);
+
+/* ---- Rotary positions, and a paged int8 cache: what a server runs around the attention of one layer. */
+
+/* Rotary positions.  Pair i of a row at position t turns by the angle t * freqs[i] and is multiplied by magnitude:
+ *     (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * The pairs are elements (i, i + pairs) of the row, or (2 i, 2 i + 1) with interleaved; elements past 2 * pairs pass unchanged.
+ * The angle is formed and reduced in fp64 (positions of any size keep their angle), sine, cosine and products are fp32, and the
+ * result is rounded once.  Scaled frequencies for long contexts are a matter of freqs and magnitude. */
+typedef struct intfa_rope {
+    const double* freqs;      /* [pairs] radians per position, device memory; NULL: no rotation (the append and the attention) */
+    int32_t pairs;            /* a multiple of 8, at most head_dim / 2 */
+    int32_t interleaved;      /* 0 / 1 */
+    float   magnitude;        /* positive and finite; 1 where frequencies are not scaled */
+    int32_t reserved;         /* set to 0 */
+} intfa_rope;
+
+/* rotary(x, positions, freqs) -> out: x and out [batch, heads, seqlen, head_dim] fp16 or bf16, head_dim contiguous and one of 16, 32,
+ * 64, 128, 256, pointers and strides 16-byte aligned; out may be x itself with x's strides.  inverse turns by the negative angle
+ * (times the same magnitude): the transposed map, through which a gradient goes back. */
+typedef struct intfa_rotary_params {
+    const void* x; void* out;
+    int64_t x_stride_b, x_stride_h, x_stride_n;
+    int64_t o_stride_b, o_stride_h, o_stride_n;
+    const int32_t* positions;          /* device memory: the first row's position of each batch entry, or with positions_per_row every
+                                          row's; NULL: position_first for all entries.  Positions may be negative. */
+    int64_t pos_stride_b, pos_stride_n;
+    int32_t positions_per_row, position_first;
+    intfa_rope rope;                   /* freqs required */
+    int32_t inverse;
+    int32_t batch, heads, seqlen, head_dim, dtype;
+} intfa_rotary_params;
+int intfa_rotary(const intfa_rotary_params* p, void* stream);
+
+/* A cache of pages: int8 rows of page_size consecutive tokens of one sequence, for every K/V head, and one fp32 scale per page and
+ * head (a value is its int8 number times the scale).  Column i of a sequence's row of block_table names the page that holds its
+ * tokens i * page_size onward.  An entry outside [0, num_pages) (-1, say) names no page: it takes no rows, and its tokens are hidden
+ * from attention. */
+typedef struct intfa_paged_cache {
+    void* k; void* v;                  /* int8 [num_pages, heads_kv, page_size, head_dim], head_dim contiguous, 16-byte aligned */
+    int64_t k_stride_p, k_stride_h, k_stride_n;
+    int64_t v_stride_p, v_stride_h, v_stride_n;
+    float* k_scale; float* v_scale;    /* [num_pages, heads_kv] */
+    int64_t ks_stride_p, ks_stride_h;
+    int64_t vs_stride_p, vs_stride_h;
+    const int32_t* block_table;        /* device memory [batch, table_width], columns contiguous */
+    int64_t bt_stride_b;
+    int32_t num_pages, page_size, table_width;
+    int32_t heads_kv, head_dim;        /* head_dim: 64, 128 or 256 */
+    int32_t reserved;                  /* set to 0 */
+} intfa_paged_cache;
+
+/* Appends new keys, rotated on the way where rope.freqs is given, and new values.  Sequence b holds n = seqlens_k[b] tokens (device
+ * memory; negative counts as 0) and its row i goes to position n + i, which is also the position that it is rotated by.  Rows past the table's
+ * last column or seqlens_new[b] (optional; clamped to [0, seqlen_new]) are dropped.  The lengths are the caller's to advance.
+ * In each page and head that rows go to, for K and V alike, every step in fp32:
+ *     scale = max(A / 127, 2^-100, the page's scale before if the sequence had rows in it), A the largest magnitude of the new rows;
+ *     rows from before, if that is a larger scale than theirs: q = rint(q * (scale before / scale));
+ *     new rows: q = rint(x / scale) within +-127.
+ * A NaN becomes 0 and an infinity +-127, and neither counts for A: a page has one scale, which they would take from all its other tokens.
+ * What lies behind the new rows in a page stays as it was.  A page that rows go to must belong to one sequence of the call only (two
+ * would write it at once; the result of that is not defined, though inside the page). */
+typedef struct intfa_paged_append_params {
+    intfa_paged_cache cache;
+    const void* k_new; const void* v_new;      /* fp16 or bf16 [batch, heads_kv, seqlen_new, head_dim], as for intfa_rotary */
+    int64_t kn_stride_b, kn_stride_h, kn_stride_n;
+    int64_t vn_stride_b, vn_stride_h, vn_stride_n;
+    const int32_t* seqlens_k;
+    const int32_t* seqlens_new;
+    intfa_rope rope;
+    int32_t batch, seqlen_new, dtype;
+    int32_t reserved;                          /* set to 0 */
+} intfa_paged_append_params;
+int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream);
+
+/* Attention of new tokens over a paged cache.  q and out: [batch, heads, seqlen, head_dim] fp16 or bf16 (dtype, both alike); query
+ * head h reads K/V head h / (heads / cache.heads_kv).  Sequence b has n = seqlens_k[b] keys (clamped to [0, table_width * page_size]), its new
+ * tokens among them, and its row i of m = seqlens_q[b] (optional; clamped to [0, seqlen]; NULL: m = seqlen) stands at position n - m + i: rotated by
+ * that position first where rope.freqs is given, and with causal seeing keys 0 .. n - m + i only.  Rows from m onward and rows that
+ * see no key are zeros with lse = -infinity.  lse: as in intfa_fwd_params.
+ * Keys and values enter as the numbers that the cache stands for: the int8 values go into 16-bit matrix products as they are, exactly, and
+ * scales are applied in fp32.  Queries enter exactly, rotated ones to 22 bits; probabilities are rounded to 11 bits; sums are fp32.
+ * workspace: at least intfa_paged_attn_workspace_bytes(p) bytes of device memory, 16-byte aligned, nothing to clear; two launches that may
+ * run at the same time must not share it. */
+typedef struct intfa_paged_attn_params {
+    intfa_paged_cache cache;
+    const void* q; void* out;
+    int64_t q_stride_b, q_stride_h, q_stride_n;
+    int64_t o_stride_b, o_stride_h, o_stride_n;
+    float* lse;                                /* optional [batch, heads, seqlen] contiguous */
+    const int32_t* seqlens_k;
+    const int32_t* seqlens_q;
+    intfa_rope rope;
+    void* workspace; size_t workspace_bytes;
+    float sm_scale;
+    int32_t causal;
+    int32_t batch, heads, seqlen, dtype;
+} intfa_paged_attn_params;
+size_t intfa_paged_attn_workspace_bytes(const intfa_paged_attn_params* p);
+int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream);
 
 #ifdef __cplusplus
 }

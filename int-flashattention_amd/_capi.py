@@ -11,7 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libintfa.so")
 
-ABI_VERSION = 8          # INTFA_VERSION of include/intfa.h this mirror was written against
+ABI_VERSION = 9          # INTFA_VERSION of include/intfa.h this mirror was written against
 INTFA_F16, INTFA_BF16, INTFA_F32 = 0, 1, 2
 PROUND_REFERENCE, PROUND_RNE = 0, 1
 STATIC_SCRATCH_BYTES = 32 << 20      # INTFA_STATIC_SCRATCH_BYTES
@@ -53,13 +53,56 @@ class AppendParams(ctypes.Structure):
     )
 
 
+class Rope(ctypes.Structure):
+    """Mirror of ``intfa_rope``."""
+    _fields_ = [("freqs", ctypes.c_void_p), ("pairs", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("magnitude", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``intfa_rotary_params``."""
+    _fields_ = ([("x", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in "xo" for a in "bhn"]
+                + [("positions", ctypes.c_void_p), ("pos_stride_b", ctypes.c_int64), ("pos_stride_n", ctypes.c_int64),
+                   ("positions_per_row", ctypes.c_int32), ("position_first", ctypes.c_int32), ("rope", Rope)]
+                + [(n, ctypes.c_int32) for n in ("inverse", "batch", "heads", "seqlen", "head_dim", "dtype")])
+
+
+class PagedCache(ctypes.Structure):
+    """Mirror of ``intfa_paged_cache``."""
+    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in "kv" for a in "phn"]
+                + [("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in ("ks", "vs") for a in "ph"]
+                + [("block_table", ctypes.c_void_p), ("bt_stride_b", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "table_width", "heads_kv", "head_dim", "reserved")])
+
+
+class PagedAppendParams(ctypes.Structure):
+    """Mirror of ``intfa_paged_append_params``."""
+    _fields_ = ([("cache", PagedCache), ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in ("kn", "vn") for a in "bhn"]
+                + [("seqlens_k", ctypes.c_void_p), ("seqlens_new", ctypes.c_void_p), ("rope", Rope)]
+                + [(n, ctypes.c_int32) for n in ("batch", "seqlen_new", "dtype", "reserved")])
+
+
+class PagedAttnParams(ctypes.Structure):
+    """Mirror of ``intfa_paged_attn_params``."""
+    _fields_ = ([("cache", PagedCache), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in "qo" for a in "bhn"]
+                + [("lse", ctypes.c_void_p), ("seqlens_k", ctypes.c_void_p), ("seqlens_q", ctypes.c_void_p), ("rope", Rope),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("sm_scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("causal", "batch", "heads", "seqlen", "dtype")])
+
+
 VARIANT_FULL_INT8, VARIANT_HALF_INT8, VARIANT_FP16 = 0, 1, 2
 
 EXPORTS = ("intfa_version", "intfa_error_string", "intfa_fwd_block_n", "intfa_fwd_workspace_bytes",
            "intfa_fwd_merge_workspace_bytes", "intfa_fwd_suggest_splits",
            "intfa_fwd_full_int8", "intfa_fwd_half_int8", "intfa_fwd_fp16", "intfa_fwd_full_int8_static", "intfa_debug_qk_int32",
            "intfa_quant_pertoken", "intfa_quant_pertensor_workspace_bytes",
-           "intfa_quant_pertensor_parts_workspace_bytes", "intfa_quant_pertensor", "intfa_quant_perblock_channel", "intfa_kvcache_append_int8")
+           "intfa_quant_pertensor_parts_workspace_bytes", "intfa_quant_pertensor", "intfa_quant_perblock_channel", "intfa_kvcache_append_int8",
+           "intfa_rotary", "intfa_paged_append_int8", "intfa_paged_attn_workspace_bytes", "intfa_paged_attn_int8")
 
 _lib = None
 
@@ -108,6 +151,12 @@ def load():
     lib.intfa_quant_perblock_channel.argtypes = [vp, i64, i64, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp]
     lib.intfa_kvcache_append_int8.restype = ctypes.c_int
     lib.intfa_kvcache_append_int8.argtypes = [ctypes.POINTER(AppendParams), vp]
+    for name, block in (("intfa_rotary", RotaryParams), ("intfa_paged_append_int8", PagedAppendParams), ("intfa_paged_attn_int8", PagedAttnParams)):
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(block), vp]
+    lib.intfa_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.intfa_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
     if lib.intfa_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI version {lib.intfa_version()}, this package expects {ABI_VERSION}: rebuild it")
     _lib = lib

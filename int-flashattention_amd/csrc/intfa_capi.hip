@@ -301,6 +301,8 @@ const char* intfa_error_string(int code) {
         case INTFA_ERR_SPLITS: return "num_splits must be at most 64";
         case INTFA_ERR_VSCALE: return "v_scale_block must be a multiple of the key-block length (or 64 at head_dim 128) and vs_stride_blk at least head_dim";
         case INTFA_ERR_SCRATCH: return "the split-KV partials of this call exceed INTFA_STATIC_SCRATCH_BYTES (or the device index exceeds 63)";
+        case INTFA_ERR_PAGE: return "page_size must be 16, 32, 64, 128 or 256, with at least one page and one column in the block table";
+        case INTFA_ERR_ROPE: return "rotated pairs must be a multiple of 8 and at most half of head_dim, the magnitude a positive number";
         default: return code > 0 ? "hip error" : "unknown error";
     }
 }

@@ -36,6 +36,13 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 // compile-time switch passed as a lambda argument (selects the LDS buffer or the masked code instance of a pipeline step)
 template <bool V> struct BoolTag { static constexpr bool value = V; };
 template <int V> struct IntTag { static constexpr int value = V; };
+// f(IntTag<0>), f(IntTag<1>), ... f(IntTag<N - 1>): an unrolled loop whose index is a compile-time constant
+template <int N, int I = 0, typename F> __device__ __forceinline__ void static_for(F& f) {
+    if constexpr (I < N) {
+        f(IntTag<I>{});
+        static_for<N, I + 1>(f);
+    }
+}
 #define INTFA_GLB(p) ((const __attribute__((address_space(1))) void*)(p))
 
 // The wait states between a 32 x 32 matrix product and the first other instruction on its registers, where that instruction stands behind

@@ -1,0 +1,345 @@
+// Attention of a few query rows over a paged int8 cache.
+//
+// The rows of a K/V head (its group of query heads times the new tokens, tokens outermost) are taken in tiles of sixteen.  S^T = K Q^T
+// and O^T = V^T P^T run on v_mfma_f32_16x16x32_f16.  The cache goes from memory into registers in the layouts that the two products want,
+// without LDS:
+//   K   lane (m = l % 16, c = l / 16) loads bytes 64 j + 16 c .. + 15 of key row m: sixteen elements of the row, eight each for products
+//       2 j and 2 j + 1.  Which elements a product takes together is free as long as Q's fragments are laid out the same.
+//   P   leaves the first product with keys 4 c + i of each 16-key granule in lane (query n = l % 16, c), and the granules 2 t and 2 t + 1 are
+//       the eight slots of lane c in the second one: P goes from accumulator to operand in its lane.
+//   V   lane (x = l % 16, c) therefore loads D / 16 bytes, x * D / 16 onward, of key rows 4 c + i of each granule: whole rows, and element j of
+//       each is what tile j of V^T (row x: column x * D / 16 + j of V) takes.  The transposition is a byte select inside the lane.
+// int8 to fp16 is exact: byte ^ 0x80 under the exponent of 1024 is 1152 + value.
+#pragma once
+#include "intfa_paged_host.h"
+#include "intfa_splitkv.h"
+
+namespace intfa {
+
+constexpr int kPagedWaves = 4;
+constexpr float kPShift = 14.f;       // P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales
+
+// Four int8 of a word as fp16
+__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    const v2h bias = {(_Float16)-1152.f, (_Float16)-1152.f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + bias);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + bias);
+}
+// Byte `b` of two words as a pair of fp16
+template <int B> __device__ __forceinline__ uint32_t i8_pair_to_f16(uint32_t first, uint32_t second) {
+    const uint32_t u = __builtin_amdgcn_perm(second, first, 0x0c000c00u | (uint32_t)(4 + B) << 16 | (uint32_t)B) ^ 0x64806480u;
+    const v2h bias = {(_Float16)-1152.f, (_Float16)-1152.f};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, u) + bias);
+}
+
+// ---- which rows a workgroup has
+struct PagedTile { int z, hk, tile, n, m; };      // n: keys of the sequence, m: its new tokens
+__device__ __forceinline__ PagedTile paged_tile(const PagedParams& p, int index) {
+    PagedTile t;
+    const int zh = fast_div(index, p.d_tiles);
+    t.tile = index - zh * p.tiles;
+    t.z = fast_div(zh, p.d_heads_kv);
+    t.hk = zh - t.z * p.heads_kv;
+    const int most = p.table_width << p.page_log2, n = p.seqlens_k[t.z];
+    t.n = n < 0 ? 0 : n < most ? n : most;
+    t.m = p.seqlen;
+    if (p.seqlens_q != nullptr) {
+        const int m = p.seqlens_q[t.z];
+        t.m = m < 0 ? 0 : m < t.m ? m : t.m;
+    }
+    return t;
+}
+// Keys that row r (of the K/V head's) sees: the first so many.
+__device__ __forceinline__ int paged_row_keys(const PagedParams& p, const PagedTile& t, int r) {
+    const int i = fast_div(r, p.d_group);
+    if (r >= p.rows || i >= t.m) return 0;
+    const int seen = t.n - t.m + i + 1;
+    return !p.causal ? t.n : seen < 0 ? 0 : seen;
+}
+
+// Rows first .. first + R - 1 to LDS as fp16 with a power of two of their own taken out (`factor` gets it back, with the softmax's scale in base 2):
+// the largest element of a row is brought to 2^8, so that neither the range of bf16 nor a rotation leaves fp16's, and what lies under fp16's
+// smallest step is 2^-32 of it.  16-bit queries are held exactly that way; rotated ones are not 16-bit numbers, and what their rounding leaves goes
+// to q_rest for a second product (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).
+template <int D, int DT, int R, int THREADS>
+__device__ __forceinline__ void paged_stage_q(const PagedParams& p, const PagedTile& t, int first_row, char* q_lds, char* q_rest, float* factor) {
+    constexpr int U = D / 16;      // units of sixteen elements, one lane each; a row is U neighbouring lanes
+    const bool rope = p.rope.freqs != nullptr, interleaved = p.rope.interleaved != 0;
+    const int pairs = rope ? p.rope.pairs : 0;
+    for (int i = threadIdx.x; i < R * U; i += THREADS) {
+        const int r = i / U, u = i % U, row = first_row + r, token = fast_div(row, p.d_group);
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = 0.f;
+        int first, second;
+        rope_unit(u, pairs, interleaved, first, second);
+        if (row < p.rows && token < t.m) {
+            const char* src = p.q + t.z * p.q_sb + (t.hk * p.group + row - token * p.group) * p.q_sh + token * p.q_sn;
+            unpack8<DT>(*(const v4i*)(src + 2 * first), x);
+            unpack8<DT>(*(const v4i*)(src + 2 * second), x + 8);
+            if (8 * u < pairs) {
+                float c[8], s[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rope_angle(p.rope.freqs[8 * u + j], t.n - t.m + token, p.rope.magnitude, c[j], s[j]);
+                rope_turn_unit(x, c, s, interleaved);
+            }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint32_t a = __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu;
+            top = top > a ? top : a;
+        }
+#pragma unroll
+        for (int w = 1; w < U; w <<= 1) {
+            const uint32_t a = (uint32_t)__shfl_xor((int)top, w);
+            top = top > a ? top : a;
+        }
+        int e = (int)(top >> 23) - 127;
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        const float down = __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x[2 * j] * down, x[2 * j + 1] * down}, v2h));
+        *(v4i*)(q_lds + (r * D + first) * 2) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
+        *(v4i*)(q_lds + (r * D + second) * 2) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
+        if (rope) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const v2f near = __builtin_convertvector(__builtin_bit_cast(v2h, h[j]), v2f);
+                h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x[2 * j] * down - near[0], x[2 * j + 1] * down - near[1]}, v2h));
+            }
+            *(v4i*)(q_rest + (r * D + first) * 2) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
+            *(v4i*)(q_rest + (r * D + second) * 2) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
+        }
+        if (u == 0) factor[r] = __builtin_bit_cast(float, (uint32_t)(127 + e - 8) << 23) * p.qk_scale_log2;
+    }
+}
+
+template <int D, int DT, int RT>
+__global__ void __launch_bounds__(64 * kPagedWaves) paged_decode_kernel(const PagedParams p) {
+    constexpr int R = 16 * RT, STEP = D == 256 ? 32 : 64, G = STEP / 16, KJ = D / 64, VB = D / 16, VD = VB / 4, DT16 = D / 16;
+    constexpr int W = kPagedWaves, THREADS = 64 * W;
+    typedef uint32_t VRow __attribute__((ext_vector_type(VD)));
+    __shared__ __align__(16) char q_lds[R * D * 2];
+    __shared__ __align__(16) char q_rest[R * D * 2];
+    __shared__ float factor_lds[R];
+    __shared__ __align__(16) float o_lds[W * 16 * D];
+    __shared__ float m_lds[W * R], l_lds[W * R];
+    const PagedTile t = paged_tile(p, (int)blockIdx.x);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), x = lane & 15, c = lane >> 4;
+    const int row0 = t.tile * R;
+    paged_stage_q<D, DT, R, THREADS>(p, t, row0, q_lds, q_rest, factor_lds);
+    const bool rope = p.rope.freqs != nullptr;
+    __syncthreads();
+    int seen[RT], least = 0x7fffffff, most = 0;
+    float factor[RT], m[RT], l[RT];
+    v4f o[RT][DT16];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        seen[rt] = paged_row_keys(p, t, row0 + 16 * rt + x);
+        factor[rt] = factor_lds[16 * rt + x];
+        m[rt] = -INFINITY;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < DT16; ++j) o[rt][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    for (int r = 0; r < R; ++r) {
+        const int s = paged_row_keys(p, t, row0 + r);
+        most = s > most ? s : most;
+        least = s < least ? s : least;
+    }
+    const char* const k_head = p.k + t.hk * p.k_sh;
+    const char* const v_head = p.v + t.hk * p.v_sh;
+    const int32_t* const table = p.table + t.z * p.bt_sb;
+    for (int key0 = wave * STEP; key0 < most; key0 += W * STEP) {
+        v4i k[G][KJ];
+        VRow v[G][4];
+        float ks[G], vs[G];
+        bool all_pages = true, has_page[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int key = key0 + 16 * g, column = key >> p.page_log2, in_page = key & ((1 << p.page_log2) - 1);
+            const int id = table[column < p.table_width ? column : p.table_width - 1];
+            has_page[g] = key < most && (unsigned)id < (unsigned)p.num_pages;      // (behind the last key the table may hold anything)
+            all_pages = all_pages && has_page[g];
+            const int at = has_page[g] ? id : 0;
+            const char* const kp = k_head + at * p.k_sp;
+            const char* const vp = v_head + at * p.v_sp;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) k[g][j] = *(const v4i*)(kp + ((in_page + x) * p.k_sn + 64 * j + 16 * c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[g][i] = *(const VRow*)(vp + ((in_page + 4 * c + i) * p.v_sn + x * VB));
+            ks[g] = p.k_scale[at * p.ks_sp + t.hk * p.ks_sh];
+            vs[g] = p.v_scale[at * p.vs_sp + t.hk * p.vs_sh];
+        }
+        // V's scales relative to the largest of the step's go into P, that one into the sum
+        float v_top = 0x1p-120f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) v_top = fmaxf(v_top, has_page[g] ? fabsf(vs[g]) : 0.f);
+        float v_rel[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) v_rel[g] = has_page[g] ? vs[g] / v_top : 0.f;
+        v8h kf[G][2 * KJ];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t w[4];
+                    i8x4_to_f16((uint32_t)k[g][j][2 * u], w[0], w[1]);
+                    i8x4_to_f16((uint32_t)k[g][j][2 * u + 1], w[2], w[3]);
+                    kf[g][2 * j + u] = __builtin_bit_cast(v8h, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+                }
+        v8h pf[RT][G / 2];
+        float alpha[RT];
+        bool rescale = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            v4f s[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                s[g] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 2 * KJ; ++j) {
+                    const v8h qf = *(const v8h*)(q_lds + ((16 * rt + x) * D + 64 * (j / 2) + 16 * c + 8 * (j & 1)) * 2);
+                    s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[g][j], qf, s[g], 0, 0, 0);
+                }
+                if (rope) {
+#pragma unroll
+                    for (int j = 0; j < 2 * KJ; ++j) {
+                        const v8h qf = *(const v8h*)(q_rest + ((16 * rt + x) * D + 64 * (j / 2) + 16 * c + 8 * (j & 1)) * 2);
+                        s[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[g][j], qf, s[g], 0, 0, 0);
+                    }
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float f = factor[rt] * ks[g];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[g][i] *= f;
+                    if (key0 + STEP > least || !all_pages) {
+                        if (key0 + 16 * g + 4 * c + i >= seen[rt] || !has_page[g]) s[g][i] = -INFINITY;
+                    }
+                    top = fmaxf(top, s[g][i]);
+                }
+            }
+            top = reduce_row_lanes(top, [](float a, float b) { return fmaxf(a, b); });
+            const float m_new = fmaxf(m[rt], top), frame = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
+            alpha[rt] = m_new == -INFINITY ? 1.f : fast_exp2(m[rt] - m_new);
+            m[rt] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[g][i] = fast_exp2(s[g][i] - frame);
+                    sum += s[g][i];
+                    s[g][i] *= v_rel[g];
+                }
+            l[rt] = l[rt] * alpha[rt] + sum;
+#pragma unroll
+            for (int h = 0; h < G / 2; ++h) {
+                v8h f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f[i] = (_Float16)s[2 * h][i];
+                    f[4 + i] = (_Float16)s[2 * h + 1][i];
+                }
+                pf[rt][h] = f;
+            }
+            rescale = rescale || alpha[rt] != 1.f;
+        }
+        if (__any(rescale)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int j = 0; j < DT16; ++j) o[rt][j] *= alpha[rt];
+        }
+        auto tile = [&](auto jt) __attribute__((always_inline)) {
+            constexpr int j = decltype(jt)::value;
+            v8h vf[G / 2];
+#pragma unroll
+            for (int h = 0; h < G / 2; ++h) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = i8_pair_to_f16<j % 4>(v[2 * h + i / 2][2 * (i & 1)][j / 4], v[2 * h + i / 2][2 * (i & 1) + 1][j / 4]);
+                vf[h] = __builtin_bit_cast(v8h, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                v4f a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < G / 2; ++h) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[h], pf[rt][h], a, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[rt][j][i] = fmaf(a[i], v_top, o[rt][j][i]);
+            }
+        };
+        static_for<DT16>(tile);
+    }
+    // ---- the waves' parts of a row meet in LDS
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = reduce_row_lanes(l[rt], [](float a, float b) { return a + b; });
+        if (c == 0) {
+            m_lds[wave * R + 16 * rt + x] = m[rt];
+            l_lds[wave * R + 16 * rt + x] = l[rt];
+        }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        if (rt > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < DT16; ++j) o_lds[(wave * 16 + x) * D + (4 * c + i) * DT16 + j] = o[rt][j][i];
+        __syncthreads();
+        const int r = (int)threadIdx.x / 16, part = (int)threadIdx.x % 16, row = row0 + 16 * rt + r;      // D / 16 columns of one row
+        static_assert(THREADS == 256, "a thread per row and sixteenth of it");
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, m_lds[w * R + 16 * rt + r]);
+        const bool empty = top == -INFINITY;
+        float sum = 0.f, weight[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            weight[w] = empty ? 0.f : fast_exp2(m_lds[w * R + 16 * rt + r] - top);
+            sum += weight[w] * l_lds[w * R + 16 * rt + r];
+        }
+        const float inv = empty ? 0.f : 1.f / sum;
+        const int token = fast_div(row, p.d_group);
+        const int head = t.hk * p.group + row - token * p.group;
+        if (row < p.rows) {
+            char* const dst = p.out + t.z * p.o_sb + head * p.o_sh + token * p.o_sn + part * DT16 * 2;
+#pragma unroll
+            for (int j = 0; j < DT16; j += 4) {
+                v4f a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * D + part * DT16 + j);
+                store_out4<DT>(dst + j * 2, a * inv);
+            }
+            if (p.lse != nullptr && part == 0)
+                p.lse[((int64_t)t.z * p.heads + head) * p.seqlen + token] = empty ? -INFINITY : top + __builtin_log2f(sum) - kPShift;
+        }
+    }
+}
+
+template <int D> int launch_paged(const PagedParams& p, const PagedSel& sel, hipStream_t stream) {
+    const dim3 grid((unsigned)(p.batch * p.heads_kv * p.tiles));
+#define INTFA_CALL(DT, RT) hipLaunchKernelGGL((paged_decode_kernel<D, DT, RT>), grid, dim3(64 * kPagedWaves), 0, stream, p)
+    if (sel.io_dt == 0) {
+        if (sel.row_tiles == 1) INTFA_CALL(0, 1); else INTFA_CALL(0, 2);
+    } else {
+        if (sel.row_tiles == 1) INTFA_CALL(1, 1); else INTFA_CALL(1, 2);
+    }
+#undef INTFA_CALL
+    return (int)hipGetLastError();
+}
+
+}  // namespace intfa

@@ -1,0 +1,242 @@
+// Rotary positions, and the append of rotated keys and of values to a paged int8 cache.  See include/intfa.h for the formulas.
+#include "intfa_paged_host.h"
+
+using namespace intfa;
+
+namespace {
+
+// ---- rotary
+struct RotaryParams {
+    const char* x; char* out;
+    int64_t x_sb, x_sh, x_sn, o_sb, o_sh, o_sn;      // bytes
+    const int32_t* positions;
+    int64_t pos_sb, pos_sn;
+    int32_t per_row, first;
+    RopeArgs rope;
+    int32_t heads, seqlen, units, heads_each;        // units of sixteen elements per row; heads per thread
+    int64_t threads;                                 // batch * seqlen * units
+    FastDiv d_units, d_seqlen;
+    float sign;
+};
+
+// A thread takes one unit of one token and turns it in heads_each heads by the same eight angles.
+template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+    const int64_t lin = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (lin >= p.threads) return;
+    const int token = fast_div((int)lin, p.d_units), u = (int)lin - token * p.units;
+    const int b = fast_div(token, p.d_seqlen), n = token - b * p.seqlen;
+    int first, second;
+    const bool turns = 8 * u < p.rope.pairs, interleaved = p.rope.interleaved != 0;
+    rope_unit(u, p.rope.pairs, interleaved, first, second);
+    float c[8], s[8];
+    if (turns) {
+        const int position = p.positions == nullptr ? p.first + n : p.per_row ? p.positions[b * p.pos_sb + n * p.pos_sn] : p.positions[b * p.pos_sb] + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            rope_angle(p.rope.freqs[8 * u + i], position, p.rope.magnitude, c[i], s[i]);
+            s[i] *= p.sign;
+        }
+    }
+    const int h0 = (int)blockIdx.y * p.heads_each, h1 = h0 + p.heads_each < p.heads ? h0 + p.heads_each : p.heads;
+    for (int h = h0; h < h1; ++h) {
+        const char* src = p.x + b * p.x_sb + h * p.x_sh + n * p.x_sn;
+        char* dst = p.out + b * p.o_sb + h * p.o_sh + n * p.o_sn;
+        const v4i lo = *(const v4i*)(src + 2 * first), hi = *(const v4i*)(src + 2 * second);
+        if (!turns) {
+            *(v4i*)(dst + 2 * first) = lo;
+            *(v4i*)(dst + 2 * second) = hi;
+            continue;
+        }
+        float x[16];
+        unpack8<DT>(lo, x);
+        unpack8<DT>(hi, x + 8);
+        rope_turn_unit(x, c, s, interleaved);
+        *(v4i*)(dst + 2 * first) = pack8<DT>(x);
+        *(v4i*)(dst + 2 * second) = pack8<DT>(x + 8);
+    }
+}
+
+// ---- append to pages
+struct PagedSide {
+    const char* src; char* cache; float* scale;
+    int64_t n_sb, n_sh, n_sn;            // bytes
+    int64_t c_sp, c_sh, c_sn;            // bytes
+    int64_t s_sp, s_sh;                  // elements
+};
+struct PagedAppendParams {
+    PagedSide k, v;
+    const int32_t* table; int64_t bt_sb;
+    const int32_t* seqlens_k; const int32_t* seqlens_new;
+    RopeArgs rope;
+    int32_t heads, seqlen_new, page_log2, num_pages, table_width, units, slots;      // slots: pages that a sequence may reach
+    FastDiv d_slots, d_heads;
+};
+
+constexpr float kLeastScale = 0x1p-100f;
+constexpr int kAppendThreads = 256;
+
+__device__ __forceinline__ float finite_magnitude(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.f;      // (false for NaN too)
+}
+// rint(x / scale) within +-127, 0 for NaN.  The quotient is the correctly rounded one (the scale is at least 2^-100, and not infinite
+// unless the cache held such a scale: then everything is 0).
+__device__ __forceinline__ uint32_t quantise(float x, float scale) {
+    const float q = rintf(x / scale);
+    return (uint32_t)(q >= 127.f ? 127 : q <= -127.f ? -127 : q == q ? (int)q : 0) & 0xffu;
+}
+
+// One workgroup per page slot of a sequence, head, and K or V.
+template <int DT> __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppendParams p) {
+    __shared__ float red[kAppendThreads / 64];
+    const int zh = fast_div((int)blockIdx.x, p.d_slots), slot = (int)blockIdx.x - zh * p.slots;
+    const int z = fast_div(zh, p.d_heads), h = zh - z * p.heads;
+    const bool is_v = blockIdx.y != 0;
+    const PagedSide& side = is_v ? p.v : p.k;
+    const int page = 1 << p.page_log2;
+    int held = p.seqlens_k[z], fresh = p.seqlen_new;
+    held = held < 0 ? 0 : held;
+    if (p.seqlens_new != nullptr) {
+        const int m = p.seqlens_new[z];
+        fresh = m < 0 ? 0 : m < fresh ? m : fresh;
+    }
+    const int column = (held >> p.page_log2) + slot;
+    if (column >= p.table_width) return;
+    const int64_t start = (int64_t)column << p.page_log2;                       // position of the page's first row
+    const int row0 = start < held ? (int)(held - start) : 0;                    // rows [row0, row1) are new
+    const int64_t past = (int64_t)held + fresh - start;
+    const int row1 = past < page ? (int)past : page;
+    if (row1 <= row0) return;
+    const int id = p.table[z * p.bt_sb + column];
+    if ((unsigned)id >= (unsigned)p.num_pages) return;
+    const char* const src = side.src + z * side.n_sb + h * side.n_sh + (start + row0 - held) * side.n_sn;
+    char* const dst = side.cache + id * side.c_sp + h * side.c_sh;
+    float* const scale_at = side.scale + id * side.s_sp + h * side.s_sh;
+    const bool rope = !is_v && p.rope.freqs != nullptr, interleaved = p.rope.interleaved != 0;
+    const int pairs = rope ? p.rope.pairs : 0, units = (row1 - row0) * p.units;
+    auto load = [&](int i, float (&x)[16], int& row, int& first, int& second) __attribute__((always_inline)) {
+        row = i / p.units;
+        const int u = i - row * p.units;
+        rope_unit(u, pairs, interleaved, first, second);
+        unpack8<DT>(*(const v4i*)(src + row * side.n_sn + 2 * first), x);
+        unpack8<DT>(*(const v4i*)(src + row * side.n_sn + 2 * second), x + 8);
+        if (8 * u < pairs) {
+            float c[8], s[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rope_angle(p.rope.freqs[8 * u + j], (int)(start + row0 + row), p.rope.magnitude, c[j], s[j]);
+            rope_turn_unit(x, c, s, interleaved);
+        }
+    };
+    float top = 0.f;
+    for (int i = threadIdx.x; i < units; i += kAppendThreads) {
+        float x[16];
+        int row, first, second;
+        load(i, x, row, first, second);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+    }
+    for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    const float before = row0 > 0 ? *scale_at : 0.f;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float scale = fmaxf(fmaxf(top / 127.0f, kLeastScale), before);
+    if (scale != before) {
+        const float ratio = before / scale;
+        const int words = row0 * p.units * 4;
+        for (int i = threadIdx.x; i < words; i += kAppendThreads) {
+            const int row = i / (p.units * 4);
+            uint32_t* const at = (uint32_t*)(dst + row * side.c_sn) + (i - row * p.units * 4);
+            const uint32_t w = *at;
+            uint32_t r = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r |= ((uint32_t)(int)rintf((float)(int8_t)(w >> (8 * j)) * ratio) & 0xffu) << (8 * j);
+            *at = r;
+        }
+    }
+    for (int i = threadIdx.x; i < units; i += kAppendThreads) {
+        float x[16];
+        int row, first, second;
+        load(i, x, row, first, second);
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            q[j] = quantise(x[4 * j], scale) | quantise(x[4 * j + 1], scale) << 8 | quantise(x[4 * j + 2], scale) << 16 | quantise(x[4 * j + 3], scale) << 24;
+        *(v2i*)(dst + (row0 + row) * side.c_sn + first) = (v2i){(int)q[0], (int)q[1]};
+        *(v2i*)(dst + (row0 + row) * side.c_sn + second) = (v2i){(int)q[2], (int)q[3]};
+    }
+    if (threadIdx.x == 0) *scale_at = scale;      // (every thread read it ahead of the barrier)
+}
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
+bool strides16(int64_t a, int64_t b, int64_t c) { return a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }      // of 16-bit elements
+
+}  // namespace
+
+extern "C" {
+
+int intfa_rotary(const intfa_rotary_params* p, void* stream) {
+    if (p == nullptr || p->x == nullptr || p->out == nullptr || p->rope.freqs == nullptr) return INTFA_ERR_NULL;
+    if (p->batch <= 0 || p->heads <= 0) return INTFA_ERR_SHAPE;
+    if (p->seqlen <= 0) return INTFA_ERR_SEQLEN;
+    const int d = p->head_dim;
+    if (d != 16 && d != 32 && d != 64 && d != 128 && d != 256) return INTFA_ERR_HEAD_DIM;
+    if (p->dtype != INTFA_F16 && p->dtype != INTFA_BF16) return INTFA_ERR_DTYPE;
+    if (!rope_valid(&p->rope, d)) return INTFA_ERR_ROPE;
+    if (!aligned(p->x, 16) || !aligned(p->out, 16) || !aligned(p->rope.freqs, 8) || !aligned(p->positions, 4) ||
+        !strides16(p->x_stride_b, p->x_stride_h, p->x_stride_n) || !strides16(p->o_stride_b, p->o_stride_h, p->o_stride_n)) return INTFA_ERR_ALIGN;
+    RotaryParams rp{};
+    rp.units = d / 16;
+    rp.threads = (int64_t)p->batch * p->seqlen * rp.units;
+    if (rp.threads >= (1ll << 31) - 256 || p->heads > 65535) return INTFA_ERR_SHAPE;
+    rp.x = (const char*)p->x; rp.out = (char*)p->out;
+    rp.x_sb = p->x_stride_b * 2; rp.x_sh = p->x_stride_h * 2; rp.x_sn = p->x_stride_n * 2;
+    rp.o_sb = p->o_stride_b * 2; rp.o_sh = p->o_stride_h * 2; rp.o_sn = p->o_stride_n * 2;
+    rp.positions = p->positions; rp.pos_sb = p->pos_stride_b; rp.pos_sn = p->pos_stride_n;
+    rp.per_row = p->positions_per_row; rp.first = p->position_first;
+    rp.rope = {p->rope.freqs, p->rope.pairs, p->rope.interleaved, p->rope.magnitude};
+    rp.heads = p->heads; rp.seqlen = p->seqlen;
+    rp.d_units = make_fast_div(rp.units); rp.d_seqlen = make_fast_div(p->seqlen);
+    rp.sign = p->inverse ? -1.0f : 1.0f;
+    rp.heads_each = 1;
+    const int blocks = (int)((rp.threads + 255) / 256);
+    const dim3 grid(blocks, p->heads);
+    if (p->dtype == INTFA_F16) hipLaunchKernelGGL(rotary_kernel<0>, grid, dim3(256), 0, (hipStream_t)stream, rp);
+    else hipLaunchKernelGGL(rotary_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, rp);
+    return (int)hipGetLastError();
+}
+
+int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream) {
+    if (p == nullptr || p->k_new == nullptr || p->v_new == nullptr || p->seqlens_k == nullptr) return INTFA_ERR_NULL;
+    const intfa_paged_cache& c = p->cache;
+    const int rc = paged_cache_check(&c);
+    if (rc != INTFA_OK) return rc;
+    if (p->batch <= 0) return INTFA_ERR_SHAPE;
+    if (p->seqlen_new <= 0 || p->seqlen_new > 1 << 30) return INTFA_ERR_SEQLEN;
+    if (p->dtype != INTFA_F16 && p->dtype != INTFA_BF16) return INTFA_ERR_DTYPE;
+    if (p->rope.freqs != nullptr && !rope_valid(&p->rope, c.head_dim)) return INTFA_ERR_ROPE;
+    if (!aligned(p->k_new, 16) || !aligned(p->v_new, 16) || !aligned(p->seqlens_k, 4) || !aligned(p->seqlens_new, 4) || !aligned(p->rope.freqs, 8) ||
+        !strides16(p->kn_stride_b, p->kn_stride_h, p->kn_stride_n) || !strides16(p->vn_stride_b, p->vn_stride_h, p->vn_stride_n)) return INTFA_ERR_ALIGN;
+    PagedAppendParams ap{};
+    ap.k = {(const char*)p->k_new, (char*)c.k, c.k_scale, p->kn_stride_b * 2, p->kn_stride_h * 2, p->kn_stride_n * 2,
+            c.k_stride_p, c.k_stride_h, c.k_stride_n, c.ks_stride_p, c.ks_stride_h};
+    ap.v = {(const char*)p->v_new, (char*)c.v, c.v_scale, p->vn_stride_b * 2, p->vn_stride_h * 2, p->vn_stride_n * 2,
+            c.v_stride_p, c.v_stride_h, c.v_stride_n, c.vs_stride_p, c.vs_stride_h};
+    ap.table = c.block_table; ap.bt_sb = c.bt_stride_b;
+    ap.seqlens_k = p->seqlens_k; ap.seqlens_new = p->seqlens_new;
+    ap.rope = {p->rope.freqs, p->rope.pairs, p->rope.interleaved, p->rope.magnitude};
+    ap.heads = c.heads_kv; ap.seqlen_new = p->seqlen_new;
+    ap.page_log2 = __builtin_ctz((unsigned)c.page_size); ap.num_pages = c.num_pages; ap.table_width = c.table_width;
+    ap.units = c.head_dim / 16;
+    ap.slots = (p->seqlen_new + c.page_size - 2) / c.page_size + 1;
+    ap.slots = ap.slots < c.table_width ? ap.slots : c.table_width;
+    const int64_t grid = (int64_t)p->batch * c.heads_kv * ap.slots;
+    if (grid >= 1ll << 31) return INTFA_ERR_SHAPE;
+    ap.d_slots = make_fast_div(ap.slots); ap.d_heads = make_fast_div(c.heads_kv);
+    const dim3 g((unsigned)grid, 2);
+    if (p->dtype == INTFA_F16) hipLaunchKernelGGL(paged_append_kernel<0>, g, dim3(kAppendThreads), 0, (hipStream_t)stream, ap);
+    else hipLaunchKernelGGL(paged_append_kernel<1>, g, dim3(kAppendThreads), 0, (hipStream_t)stream, ap);
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

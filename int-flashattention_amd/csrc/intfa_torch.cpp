@@ -323,7 +323,7 @@ Tensor quant_input(const Tensor& x) {
     require_4d(x, "x");
     return row_major(x, x.size(-1), 2);
 }
-PyObject* quant_result(Tensor&& q8, Tensor&& scale) {
+PyObject* tensor_pair(Tensor&& q8, Tensor&& scale) {
     PyObject* pair = PyTuple_New(2);
     if (pair == nullptr) throw python_error();
     PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(q8)));
@@ -343,7 +343,7 @@ PyObject* quant_pertoken(PyObject*, PyObject* arg) {
     });
     check_rc(rc, "intfa_quant_pertoken");
     dev.used(x);
-    return quant_result(std::move(q8), std::move(scale));
+    return tensor_pair(std::move(q8), std::move(scale));
     END_HANDLE_TH_ERRORS
 }
 
@@ -361,7 +361,7 @@ PyObject* quant_pertensor(PyObject*, PyObject* arg) {
     });
     check_rc(rc, "intfa_quant_pertensor");
     dev.used(x);
-    return quant_result(std::move(q8), std::move(scale));
+    return tensor_pair(std::move(q8), std::move(scale));
     END_HANDLE_TH_ERRORS
 }
 
@@ -383,7 +383,7 @@ PyObject* quant_perblock_channel(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
     check_rc(rc, "intfa_quant_perblock_channel");
     dev.used(x);
-    return quant_result(std::move(q8), std::move(scale));
+    return tensor_pair(std::move(q8), std::move(scale));
     END_HANDLE_TH_ERRORS
 }
 
@@ -440,9 +440,189 @@ PyObject* kvcache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions and the paged cache
+void require_on(const Tensor& t, const Tensor& like, const char* name) {
+    if (t.device() != like.device())
+        fail(PyExc_ValueError, std::string(name) + " must be on " + like.device().str() + " like the others, got " + t.device().str());
+}
+// freqs: float64 [pairs] on the device of `like`, or None
+intfa_rope rope_arg(const Tensor& freqs, bool interleaved, double magnitude, const Tensor& like, int64_t d, Tensor* held) {
+    intfa_rope r{};
+    if (!freqs.defined()) return r;
+    if (freqs.scalar_type() != ScalarType::Double || freqs.dim() != 1) fail(PyExc_ValueError, "freqs must be a one-dimensional float64 tensor (see rotary_frequencies)");
+    require_on(freqs, like, "freqs");
+    if (freqs.size(0) == 0 || freqs.size(0) % 8 != 0 || 2 * freqs.size(0) > d)
+        fail(PyExc_ValueError, "freqs must hold a multiple of 8 frequencies and at most head_dim / 2, got " + std::to_string(freqs.size(0)) + " for head_dim " + std::to_string(d));
+    *held = freqs.contiguous();
+    r.freqs = held->data_ptr<double>();
+    r.pairs = (int)freqs.size(0);
+    r.interleaved = interleaved ? 1 : 0;
+    r.magnitude = (float)magnitude;
+    if (!(r.magnitude > 0.f) || r.magnitude > 3.402823466e38f) fail(PyExc_ValueError, "magnitude must be a positive number");
+    return r;
+}
+// int32 [n] on the device of `like`, contiguous
+Tensor lengths_arg(const Tensor& t, int64_t n, const Tensor& like, const char* name) {
+    if (t.scalar_type() != ScalarType::Int || t.dim() != 1 || t.size(0) != n) fail(PyExc_ValueError, std::string(name) + " must be an int32 tensor of shape (" + std::to_string(n) + ",)");
+    require_on(t, like, name);
+    return t.contiguous();
+}
+
+// rotary(x, positions, freqs, interleaved, inverse, magnitude)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 6, "rotary");
+    const Tensor &x_in = tensor_arg(a[0], "x"), &freqs = tensor_arg(a[2], "freqs");
+    if (!x_in.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd.rotary runs on the GPU only; got a CPU tensor");
+    if (quant_dtype(x_in) < 0) fail(PyExc_TypeError, "rotary takes fp16 or bf16 tensors, got " + dtype_text(x_in.scalar_type()));
+    require_4d(x_in, "x");
+    const int64_t Z = x_in.size(0), H = x_in.size(1), N = x_in.size(2), d = x_in.size(3);
+    const CallDevice dev(x_in);
+    const Tensor x = row_major(x_in, d, 2);
+    intfa_rotary_params p{};
+    Tensor freqs_, positions;
+    p.rope = rope_arg(freqs, bool_arg(a[3]), float_arg(a[5]), x, d, &freqs_);
+    if (PyLong_Check(a[1])) {
+        p.position_first = int32_arg(a[1], "positions");
+    } else {
+        const Tensor& t = tensor_arg(a[1], "positions");
+        const bool per_row = t.dim() == 2;
+        if (t.scalar_type() != ScalarType::Int || (t.dim() != 1 && !per_row) || t.size(0) != Z || (per_row && t.size(1) != N))
+            fail(PyExc_ValueError, "positions must be an int, an int32 [Z] tensor (the first row's of each entry) or an int32 [Z, N] tensor");
+        require_on(t, x, "positions");
+        positions = t;
+        p.positions = t.data_ptr<int32_t>();
+        p.positions_per_row = per_row ? 1 : 0;
+        p.pos_stride_b = t.stride(0); p.pos_stride_n = per_row ? t.stride(1) : 0;
+    }
+    Tensor out = dev.empty(x.sizes(), x.scalar_type());
+    if (out.numel() == 0) return THPVariable_Wrap(std::move(out));
+    p.x = x.data_ptr(); p.out = out.data_ptr();
+    set_strides(&p.x_stride_b, x); set_strides(&p.o_stride_b, out);
+    p.inverse = bool_arg(a[4]) ? 1 : 0;
+    p.batch = (int)Z; p.heads = (int)H; p.seqlen = (int)N; p.head_dim = (int)d; p.dtype = quant_dtype(x);
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_rotary(&p, st); }), "intfa_rotary");
+    dev.used(x); dev.used(freqs_); dev.used(positions);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// The pages, their scales and the block table: a[0 .. 3] k_cache, k_scale, v_cache, v_scale; checked against [Z] sequences.
+intfa_paged_cache paged_cache_arg(const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table, int64_t Z, const Tensor& like) {
+    if (kc.scalar_type() != ScalarType::Char || vc.scalar_type() != ScalarType::Char || kc.dim() != 4 || vc.sizes() != kc.sizes())
+        fail(PyExc_ValueError, "k_cache and v_cache must be int8 [pages, H_kv, page_size, d] tensors of one shape");
+    const int64_t pages = kc.size(0), H = kc.size(1), page = kc.size(2), d = kc.size(3);
+    if (ks.scalar_type() != ScalarType::Float || vs.scalar_type() != ScalarType::Float || ks.dim() != 2 || vs.dim() != 2 || ks.size(0) != pages ||
+        ks.size(1) != H || vs.size(0) != pages || vs.size(1) != H) fail(PyExc_ValueError, "k_scale and v_scale must be float32 [pages, H_kv] tensors");
+    if (table.scalar_type() != ScalarType::Int || table.dim() != 2 || table.size(0) != Z || (table.size(1) > 1 && table.stride(1) != 1))
+        fail(PyExc_ValueError, "block_table must be an int32 [Z, columns] tensor with contiguous columns");
+    require_on(kc, like, "k_cache"); require_on(vc, like, "v_cache"); require_on(ks, like, "k_scale"); require_on(vs, like, "v_scale");
+    require_on(table, like, "block_table");
+    if (d != 64 && d != 128 && d != 256) fail(PyExc_AssertionError, "head_dim of a paged cache must be 64, 128 or 256");
+    if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256) fail(PyExc_ValueError, "page_size must be 16, 32, 64, 128 or 256, got " + std::to_string(page));
+    if (pages == 0 || pages > INT_MAX || table.size(1) == 0 || table.size(1) > INT_MAX) fail(PyExc_ValueError, "a paged cache needs at least one page and one column of block_table");
+    for (const Tensor* t : {&kc, &vc}) {
+        bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+        for (int i = 0; i < 3; ++i) ok = ok && t->stride(i) % 16 == 0;
+        if (!ok) fail(PyExc_ValueError, "rows of k_cache and v_cache must be contiguous, and pages, heads and rows 16-byte aligned (the cache is used in place)");
+    }
+    intfa_paged_cache c{};
+    c.k = kc.data_ptr(); c.v = vc.data_ptr();
+    set_strides(&c.k_stride_p, kc); set_strides(&c.v_stride_p, vc);
+    c.k_scale = ks.data_ptr<float>(); c.v_scale = vs.data_ptr<float>();
+    c.ks_stride_p = ks.stride(0); c.ks_stride_h = ks.stride(1); c.vs_stride_p = vs.stride(0); c.vs_stride_h = vs.stride(1);
+    c.block_table = table.data_ptr<int32_t>(); c.bt_stride_b = table.stride(0);
+    c.num_pages = (int)pages; c.page_size = (int)page; c.table_width = (int)table.size(1); c.heads_kv = (int)H; c.head_dim = (int)d;
+    return c;
+}
+
+// paged_kvcache_append(k_cache, k_scale, v_cache, v_scale, k_new, v_new, block_table, seqlens_k, freqs, interleaved, magnitude, seqlens_new)
+PyObject* paged_kvcache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 12, "paged_kvcache_append");
+    const Tensor &kc = tensor_arg(a[0], "k_cache"), &ks = tensor_arg(a[1], "k_scale"), &vc = tensor_arg(a[2], "v_cache"), &vs = tensor_arg(a[3], "v_scale");
+    const Tensor &k_new = tensor_arg(a[4], "k_new"), &v_new = tensor_arg(a[5], "v_new"), &table = tensor_arg(a[6], "block_table");
+    const Tensor &lens = tensor_arg(a[7], "seqlens_k"), &freqs = optional_tensor_arg(a[8], "freqs"), &fresh = optional_tensor_arg(a[11], "seqlens_new");
+    if (!k_new.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd.paged_kvcache_append runs on the GPU only; got a CPU tensor");
+    if (quant_dtype(k_new) < 0 || v_new.scalar_type() != k_new.scalar_type()) fail(PyExc_TypeError, "new keys and values must both be fp16 or both bf16");
+    require_4d(k_new, "k_new"); require_4d(v_new, "v_new");
+    require_on(v_new, k_new, "v_new");
+    const int64_t Z = k_new.size(0);
+    intfa_paged_append_params p{};
+    p.cache = paged_cache_arg(kc, ks, vc, vs, table, Z, k_new);
+    if (k_new.sizes() != v_new.sizes() || k_new.size(1) != kc.size(1) || k_new.size(3) != kc.size(3))
+        fail(PyExc_ValueError, "k_new and v_new must be [Z, H_kv, N_new, d] with the cache's H_kv and d");
+    const CallDevice dev(k_new);
+    const Tensor kn = row_major(k_new, k_new.size(3), 2), vn = row_major(v_new, v_new.size(3), 2);
+    Tensor freqs_, fresh_;
+    const Tensor lens_ = lengths_arg(lens, Z, k_new, "seqlens_k");
+    if (fresh.defined()) fresh_ = lengths_arg(fresh, Z, k_new, "seqlens_new");
+    p.rope = rope_arg(freqs, bool_arg(a[9]), float_arg(a[10]), k_new, kc.size(3), &freqs_);
+    if (kn.numel() == 0) Py_RETURN_NONE;
+    p.k_new = kn.data_ptr(); p.v_new = vn.data_ptr();
+    set_strides(&p.kn_stride_b, kn); set_strides(&p.vn_stride_b, vn);
+    p.seqlens_k = lens_.data_ptr<int32_t>();
+    p.seqlens_new = fresh_.defined() ? fresh_.data_ptr<int32_t>() : nullptr;
+    p.batch = (int)Z; p.seqlen_new = (int)kn.size(2); p.dtype = quant_dtype(kn);
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_paged_append_int8(&p, st); }), "intfa_paged_append_int8");
+    for (const Tensor* t : {&kc, &ks, &vc, &vs, &table, &kn, &vn, &lens_, const_cast<const Tensor*>(&fresh_), const_cast<const Tensor*>(&freqs_)}) dev.used(*t);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens_k, causal, sm_scale, freqs, interleaved, magnitude, seqlens_q, return_lse)
+PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 14, "attention_paged");
+    const Tensor &q_in = tensor_arg(a[0], "q"), &kc = tensor_arg(a[1], "k_cache"), &vc = tensor_arg(a[2], "v_cache");
+    const Tensor &ks = tensor_arg(a[3], "k_scale"), &vs = tensor_arg(a[4], "v_scale"), &table = tensor_arg(a[5], "block_table");
+    const Tensor &lens = tensor_arg(a[6], "seqlens_k"), &freqs = optional_tensor_arg(a[9], "freqs"), &rows = optional_tensor_arg(a[12], "seqlens_q");
+    require_gpu(q_in);
+    if (quant_dtype(q_in) < 0) fail(PyExc_TypeError, "q must be fp16 or bf16, got " + dtype_text(q_in.scalar_type()));
+    require_4d(q_in, "q");
+    const int64_t Z = q_in.size(0), H = q_in.size(1), N = q_in.size(2), d = q_in.size(3);
+    intfa_paged_attn_params p{};
+    p.cache = paged_cache_arg(kc, ks, vc, vs, table, Z, q_in);
+    if (d != kc.size(3)) fail(PyExc_AssertionError, "q and the cache must have the same head_dim");
+    if (kc.size(1) == 0 || H % kc.size(1) != 0)
+        fail(PyExc_ValueError, "the number of query heads (" + std::to_string(H) + ") must be a multiple of the number of K/V heads (" + std::to_string(kc.size(1)) + ")");
+    const CallDevice dev(q_in);
+    const Tensor q = row_major(q_in, d, 2);
+    Tensor freqs_, rows_, lse, ws, out = dev.empty({Z, H, N, d}, q.scalar_type());
+    const bool return_lse = bool_arg(a[13]);
+    if (return_lse) lse = dev.empty({Z, H, N}, ScalarType::Float);
+    const Tensor lens_ = lengths_arg(lens, Z, q, "seqlens_k");
+    if (rows.defined()) rows_ = lengths_arg(rows, Z, q, "seqlens_q");
+    p.rope = rope_arg(freqs, bool_arg(a[10]), float_arg(a[11]), q, d, &freqs_);
+    p.causal = bool_arg(a[7]) ? 1 : 0;
+    p.sm_scale = (float)float_arg(a[8]);
+    if (out.numel() != 0) {
+        p.q = q.data_ptr(); p.out = out.data_ptr();
+        p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+        set_strides(&p.q_stride_b, q); set_strides(&p.o_stride_b, out);
+        p.seqlens_k = lens_.data_ptr<int32_t>();
+        p.seqlens_q = rows_.defined() ? rows_.data_ptr<int32_t>() : nullptr;
+        p.batch = (int)Z; p.heads = (int)H; p.seqlen = (int)N; p.dtype = quant_dtype(q);
+        p.workspace_bytes = intfa_paged_attn_workspace_bytes(&p);
+        if (p.workspace_bytes > 0) {
+            ws = dev.empty({(int64_t)p.workspace_bytes}, ScalarType::Byte);
+            p.workspace = ws.data_ptr();
+        }
+        void* const st = dev.raw_stream();
+        check_rc(unlocked([&] { return intfa_paged_attn_int8(&p, st); }), "intfa_paged_attn_int8");
+        for (const Tensor* t : {&q, &kc, &vc, &ks, &vs, &table, &lens_, const_cast<const Tensor*>(&rows_), const_cast<const Tensor*>(&freqs_)}) dev.used(*t);
+    }
+    if (!return_lse) return THPVariable_Wrap(std::move(out));
+    return tensor_pair(std::move(out), std::move(lse));
+    END_HANDLE_TH_ERRORS
+}
+
 #define INTFA_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     INTFA_FAST(forward), INTFA_FAST(check_head_dims), INTFA_FAST(debug_qk_int32), INTFA_FAST(quant_perblock_channel), INTFA_FAST(kvcache_append),
+    INTFA_FAST(rotary), INTFA_FAST(paged_kvcache_append), INTFA_FAST(attention_paged),
     {"quant_pertoken", quant_pertoken, METH_O, nullptr}, {"quant_pertensor", quant_pertensor, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "host side of the entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

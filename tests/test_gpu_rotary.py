@@ -1,0 +1,102 @@
+"""Rotary positions against their formula in float64: layouts, parts of the head, strides, far positions, the gradient."""
+import pytest
+import torch
+
+import int_flashattention_amd as M
+from paged_reference import rotate
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def check(out, x, positions, freqs, magnitude=1.0, interleaved=False, inverse=False):
+    """Half a step of the result; cos and sin within 8e-7 (the reduced angle in fp32 2e-7, the function 4 units of 2^-24 and its rounding,
+    the two products and their sum one of 2^-24 each), so 1e-6 of |a| + |b|; fp16's smallest step."""
+    want = rotate(x, positions, freqs, magnitude, interleaved, inverse)
+    r, half = 2 * freqs.numel(), freqs.numel()
+    size = x.double().abs().clone()
+    a, b = (size[..., 0:r:2], size[..., 1:r:2]) if interleaved else (size[..., :half], size[..., half:r])
+    both = (a + b).repeat_interleave(2, -1) if interleaved else torch.cat([a + b, a + b], -1)
+    size[..., :r] = both
+    tolerance = torch.finfo(x.dtype).eps / 2 * want.abs() * (1 + 1e-6) + 1e-6 * magnitude * size + 2.0 ** -25
+    assert ((out.cpu().double() - want).abs() <= tolerance).all()
+    assert torch.equal(out[..., r:].cpu(), x[..., r:])
+
+
+@pytest.mark.parametrize("Z,H,N,d,rot,interleaved,inverse,dtype", [
+    (1, 1, 1, 16, 16, False, False, torch.float16),
+    (2, 3, 5, 32, 16, True, False, torch.bfloat16),
+    (1, 32, 1, 128, 128, False, False, torch.float16),
+    (3, 5, 67, 64, 32, True, True, torch.float16),
+    (2, 9, 33, 128, 64, False, True, torch.bfloat16),
+    (1, 4, 130, 256, 256, False, False, torch.bfloat16),
+    (1, 2, 257, 256, 80, True, False, torch.float16),
+    (2, 12, 300, 64, 64, False, False, torch.float16),
+])
+def test_formula(Z, H, N, d, rot, interleaved, inverse, dtype):
+    g = torch.Generator().manual_seed(Z * 1000 + N)
+    x = torch.randn((Z, H, N, d), generator=g).to(dtype)
+    freqs, magnitude = M.rotary_frequencies(rot, device=DEV, scaling="parts", factor=4.0, original_length=2048)
+    first = torch.randint(0, 5000, (Z,), generator=g, dtype=torch.int32)
+    rows = torch.arange(N)
+    out = M.rotary(x.to(DEV), first.to(DEV), freqs, interleaved=interleaved, inverse=inverse, magnitude=magnitude)
+    assert out.is_contiguous() and out.dtype == dtype
+    check(out, x, first[:, None] + rows, freqs.cpu(), magnitude, interleaved, inverse)
+    each = torch.randint(-100, 100000, (Z, N), generator=g, dtype=torch.int32)
+    check(M.rotary(x.to(DEV), each.to(DEV), freqs, interleaved=interleaved, inverse=inverse), x, each, freqs.cpu(), 1.0, interleaved, inverse)
+    check(M.rotary(x.to(DEV), 17, freqs, interleaved=interleaved, inverse=inverse), x, (17 + rows).expand(Z, N), freqs.cpu(), 1.0, interleaved, inverse)
+
+
+def test_strides_and_one_position_for_all_rows():
+    g = torch.Generator().manual_seed(5)
+    freqs, _ = M.rotary_frequencies(64, device=DEV)
+    y = torch.randn((2, 37, 6, 128), generator=g).half()                       # [Z, N, H, d]
+    x = y.transpose(1, 2)
+    pos = torch.tensor([[40], [7]], dtype=torch.int32)
+    out = M.rotary(y.to(DEV).transpose(1, 2), pos.to(DEV).expand(2, 37), freqs)   # a row stride of zero: every row at the same position
+    check(out, x, pos.expand(2, 37), freqs.cpu())
+    odd = torch.randn((2, 3, 9, 130), generator=g).bfloat16()[..., 1:129]       # rows that are not 16-byte aligned
+    check(M.rotary(odd.to(DEV), 3, freqs), odd.contiguous(), (3 + torch.arange(9)).expand(2, 9), freqs.cpu())
+
+
+def test_far_positions_keep_their_angle():
+    freqs, _ = M.rotary_frequencies(128, base=500000.0, device=DEV)
+    x = torch.randn((1, 2, 6, 128), generator=torch.Generator().manual_seed(6)).half()
+    pos = torch.tensor([[2 ** 31 - 1, 2 ** 30 + 12345, 16777217, 1 << 20, -(2 ** 31), -1]], dtype=torch.int32)
+    check(M.rotary(x.to(DEV), pos.to(DEV), freqs), x, pos, freqs.cpu())
+
+
+def test_values_that_are_not_finite_stay_in_their_pair():
+    freqs, _ = M.rotary_frequencies(32, device=DEV)
+    x = torch.randn((1, 1, 4, 64), generator=torch.Generator().manual_seed(7)).half()
+    x[0, 0, 1, 3], x[0, 0, 2, 40] = float("nan"), float("inf")
+    out = M.rotary(x.to(DEV), 5, freqs).cpu()
+    bad = torch.zeros(64, dtype=torch.bool)
+    bad[3] = bad[3 + 16] = True
+    assert out[0, 0, 1][bad].isnan().all() and out[0, 0, 1][~bad].isfinite().all()
+    assert out[0, 0, 2, 40] == float("inf") and out[0, 0, 2].isfinite().sum() == 63
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_gradient(interleaved):
+    """The map is linear: its gradient is the transposed map, <R x, y> = <x, R^T y>, and the difference quotient is exact."""
+    g = torch.Generator().manual_seed(8)
+    freqs, magnitude = M.rotary_frequencies(48, device=DEV, scaling="parts", factor=8.0, original_length=1024)
+    x = torch.randn((2, 3, 11, 64), generator=g).bfloat16()
+    y = torch.randn((2, 3, 11, 64), generator=g).bfloat16()
+    first = torch.tensor([3, 900], dtype=torch.int32)
+    leaf = x.to(DEV).requires_grad_()
+    out = M.rotary(leaf, first.to(DEV), freqs, interleaved=interleaved, magnitude=magnitude)
+    out.backward(y.to(DEV))
+    pos = first[:, None] + torch.arange(11)
+    check(leaf.grad, y, pos, freqs.cpu(), magnitude, interleaved, inverse=True)
+    ref = rotate(x, pos, freqs.cpu(), magnitude, interleaved)
+    d = torch.zeros_like(x).double()
+    d[0, 1, 4, 5] = 1.0
+    quotient = ((rotate(x.double() + d, pos, freqs.cpu(), magnitude, interleaved) - ref) * y.double()).sum()
+    assert abs(leaf.grad[0, 1, 4, 5].item() - quotient.item()) <= 2.0 ** -8 * abs(quotient.item()) + 1e-5
+    leaf.grad = None
+    M.rotary(leaf, 4, freqs, interleaved=interleaved).sum().backward()           # (the gradient of a sum: one value, expanded)
+    check(leaf.grad, torch.ones_like(x), (4 + torch.arange(11)).expand(2, 11), freqs.cpu(), 1.0, interleaved, inverse=True)
+    with torch.no_grad():
+        assert not M.rotary(leaf, 4, freqs).requires_grad
