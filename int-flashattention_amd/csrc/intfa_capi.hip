@@ -14,6 +14,13 @@ using namespace intfa;
 // the array's name is only a handle for hipGetSymbolAddress, never an address to hand to a kernel.
 static __device__ __align__(256) unsigned char scratch[INTFA_STATIC_SCRATCH_BYTES];
 
+// Epochs of the launches that merge their splits themselves: 56 bits in the upper bits of the word, counted from a random
+// start so that a ticket word holding old data of another process's making is not taken for one of ours.
+uint64_t intfa::next_epoch() {
+    static std::atomic<uint64_t> count{((uint64_t)std::random_device{}() << 32 | std::random_device{}()) | 1u};
+    return count.fetch_add(1, std::memory_order_relaxed) << 8;
+}
+
 namespace {
 
 constexpr int kMaxDevices = 64;
@@ -130,13 +137,6 @@ size_t ticket_offset(const intfa_fwd_params* p) { return (workspace_bytes_for(p)
 size_t merge_workspace_bytes_for(const intfa_fwd_params* p) {
     if (workspace_bytes_for(p) == 0) return 0;
     return ticket_offset(p) + (size_t)p->batch * p->heads * ((p->seqlen + 15) / 16) * kTicketStride * sizeof(uint64_t);
-}
-
-// Epochs of the launches that merge their splits themselves: 56 bits in the upper bits of the word, counted from a random
-// start so that a ticket word holding old data of another process's making is not taken for one of ours.
-uint64_t next_epoch() {
-    static std::atomic<uint64_t> count{((uint64_t)std::random_device{}() << 32 | std::random_device{}()) | 1u};
-    return count.fetch_add(1, std::memory_order_relaxed) << 8;
 }
 
 int setup_split(const intfa_fwd_params* p, int block_n, KParams* kp) {

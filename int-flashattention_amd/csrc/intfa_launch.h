@@ -25,6 +25,8 @@ struct LaunchSel {
     bool crowded;    // ... full-int8: more workgroups than the form with the longer pipeline has room for
 };
 
+uint64_t next_epoch();                // (intfa_capi.hip)
+
 inline FastDiv make_fast_div(int d) {
     int l = 0;
     while ((1ll << l) < (long long)d) ++l;                   // ceil(log2 d), d >= 1

@@ -1,5 +1,6 @@
 // C entry of the attention over a paged int8 cache: argument checks, kernel selection and launch.  See include/intfa.h.
 #include "intfa_paged_host.h"
+#include "intfa_splitkv.h"
 
 using namespace intfa;
 
@@ -23,16 +24,41 @@ int check(const intfa_paged_attn_params* p) {
     return INTFA_OK;
 }
 
+// How a call is dealt: rows per tile, keys per unit, workgroups; and the layout of its workspace.
+struct Plan { PagedSel sel; int rows, tiles, unit_log2, grid, slot_rows; size_t stats_at, tickets_at, bytes; };
+Plan make_plan(const intfa_paged_attn_params* p) {
+    const intfa_paged_cache& c = p->cache;
+    Plan a{};
+    a.rows = p->heads / c.heads_kv * p->seqlen;
+    a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, a.rows <= 16 ? 1 : 2};
+    a.slot_rows = 16 * a.sel.row_tiles;
+    a.tiles = (a.rows + a.slot_rows - 1) / a.slot_rows;
+    a.unit_log2 = c.head_dim == 256 ? 7 : 8;
+    const int64_t items = (int64_t)p->batch * c.heads_kv * a.tiles, keys = (int64_t)c.table_width * c.page_size;
+    const int slots = kComputeUnits * (c.head_dim == 256 || a.sel.row_tiles > 1 ? 1 : 2);
+    auto units = [&] { return items * ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2); };
+    a.grid = (int)(units() < slots ? units() : slots);
+    while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)
+    if (units() * a.grid >= 1ll << 32) a.grid = (int)(((1ll << 32) - 1) / units());
+    const size_t slot_rows = (size_t)a.grid * 2 * a.slot_rows;
+    a.stats_at = slot_rows * c.head_dim * sizeof(float);
+    a.tickets_at = a.stats_at + slot_rows * 2 * sizeof(float);
+    a.bytes = a.tickets_at + (size_t)items * kTicketStride * sizeof(uint64_t);
+    return a;
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t intfa_paged_attn_workspace_bytes(const intfa_paged_attn_params* p) { return 0; }
+size_t intfa_paged_attn_workspace_bytes(const intfa_paged_attn_params* p) { return check(p) == INTFA_OK ? make_plan(p).bytes : 0; }
 
 int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream) {
     const int rc = check(p);
     if (rc != INTFA_OK) return rc;
     const intfa_paged_cache& c = p->cache;
+    const Plan a = make_plan(p);
+    if (p->workspace == nullptr || p->workspace_bytes < a.bytes || !aligned(p->workspace, 16)) return INTFA_ERR_WORKSPACE;
     PagedParams kp{};
     kp.q = (const char*)p->q; kp.out = (char*)p->out; kp.lse = p->lse;
     kp.k = (const char*)c.k; kp.v = (const char*)c.v; kp.k_scale = c.k_scale; kp.v_scale = c.v_scale;
@@ -48,9 +74,13 @@ int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream) {
     kp.causal = p->causal != 0;
     kp.qk_scale_log2 = p->sm_scale * 1.4426950408889634f;
     kp.rope = {p->rope.freqs, p->rope.pairs, p->rope.interleaved, p->rope.magnitude};
-    PagedSel sel{c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, kp.rows <= 16 ? 1 : 2};
-    kp.tiles = (kp.rows + 16 * sel.row_tiles - 1) / (16 * sel.row_tiles);
+    kp.tiles = a.tiles; kp.unit_log2 = a.unit_log2; kp.grid = a.grid;
+    kp.parts = (float*)p->workspace;
+    kp.part_stats = (float*)((char*)p->workspace + a.stats_at);
+    kp.ticket = (uint64_t*)((char*)p->workspace + a.tickets_at);
+    kp.epoch = next_epoch() << 8;
     kp.d_group = make_fast_div(kp.group); kp.d_tiles = make_fast_div(kp.tiles); kp.d_heads_kv = make_fast_div(kp.heads_kv);
+    const PagedSel& sel = a.sel;
     hipStream_t st = (hipStream_t)stream;
     return c.head_dim == 64 ? launch_paged_d64(kp, sel, st) : c.head_dim == 128 ? launch_paged_d128(kp, sel, st) : launch_paged_d256(kp, sel, st);
 }

@@ -33,25 +33,83 @@ template <int B> __device__ __forceinline__ uint32_t i8_pair_to_f16(uint32_t fir
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, u) + bias);
 }
 
-// ---- which rows a workgroup has
-struct PagedTile { int z, hk, tile, n, m; };      // n: keys of the sequence, m: its new tokens
-__device__ __forceinline__ PagedTile paged_tile(const PagedParams& p, int index) {
-    PagedTile t;
-    const int zh = fast_div(index, p.d_tiles);
-    t.tile = index - zh * p.tiles;
-    t.z = fast_div(zh, p.d_heads_kv);
-    t.hk = zh - t.z * p.heads_kv;
-    const int most = p.table_width << p.page_log2, n = p.seqlens_k[t.z];
-    t.n = n < 0 ? 0 : n < most ? n : most;
+// ---- who works on what
+// The keys of all sequences, K/V heads and row tiles (the items, in that order) are one line of units of 2^unit_log2 keys, at least one per item, and
+// every workgroup takes an equal piece of it: whatever the lengths, all compute units end together.  An item that lies in several pieces is merged
+// by the workgroup that finishes its part last.
+struct PagedItem { int z, hk, tile, n, m, units; };      // n: keys of the sequence, m: its new tokens, units: of each of its items
+__device__ __forceinline__ int paged_keys(const PagedParams& p, int z) {
+    const int most = p.table_width << p.page_log2, n = p.seqlens_k[z];
+    return n < 0 ? 0 : n < most ? n : most;
+}
+__device__ __forceinline__ int paged_units(const PagedParams& p, int n) {
+    const int u = (n + (1 << p.unit_log2) - 1) >> p.unit_log2;
+    return u > 1 ? u : 1;
+}
+__device__ __forceinline__ void paged_sequence(const PagedParams& p, int z, PagedItem& t) {
+    t.z = z;
+    t.n = paged_keys(p, z);
+    t.units = paged_units(p, t.n);
     t.m = p.seqlen;
     if (p.seqlens_q != nullptr) {
-        const int m = p.seqlens_q[t.z];
+        const int m = p.seqlens_q[z];
         t.m = m < 0 ? 0 : m < t.m ? m : t.m;
     }
-    return t;
 }
+// Finds this workgroup's piece [first, end) of the line, and the item that `first` lies in: it begins at unit `start`.  The line is cut for `grid`
+// workgroups, those of the launch or as many as there are units: none of them has an empty piece (first == end: not one of them).  The host
+// keeps the number of units times that of workgroups below 2^32.
+// (Sequences are dealt to the threads in runs; one scan gives the total and every run's place.)
+template <int THREADS> __device__ __forceinline__ uint32_t paged_find(const PagedParams& p, uint32_t* lds, PagedItem& t, uint32_t& first, uint32_t& end, uint32_t& start, uint32_t& grid) {
+    const int per = p.heads_kv * p.tiles, run = (p.batch + THREADS - 1) / THREADS, z0 = (int)threadIdx.x * run;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t mine = 0;
+    for (int z = z0; z < z0 + run && z < p.batch; ++z) mine += (uint32_t)paged_units(p, paged_keys(p, z)) * (uint32_t)per;
+    uint32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 63) lds[wave] = upto;
+    __syncthreads();
+    uint32_t total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+        if (w == wave) before = total;
+        total += lds[w];
+    }
+    grid = (uint32_t)p.grid < total ? (uint32_t)p.grid : total;
+    first = end = 0;
+    if (blockIdx.x >= grid) return total;
+    first = (uint32_t)blockIdx.x * total / grid;
+    end = ((uint32_t)blockIdx.x + 1) * total / grid;
+    uint32_t at = before + upto - mine;
+    if (first >= at && first < at + mine) {
+        int z = z0;
+        uint32_t units = (uint32_t)paged_units(p, paged_keys(p, z)) * (uint32_t)per;
+        for (; first >= at + units; units = (uint32_t)paged_units(p, paged_keys(p, z)) * (uint32_t)per) {
+            at += units;
+            ++z;
+        }
+        lds[8] = (uint32_t)z;
+        lds[9] = at;
+    }
+    __syncthreads();
+    const int z = __builtin_amdgcn_readfirstlane((int)lds[8]);
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds[9]);
+    paged_sequence(p, z, t);
+    const uint32_t item = (first - at) / (uint32_t)t.units;
+    start = at + item * (uint32_t)t.units;
+    t.hk = fast_div((int)item, p.d_tiles);
+    t.tile = (int)item - t.hk * p.tiles;
+    return total;
+}
+// The workgroup that has unit u of a line of `total`.
+__device__ __forceinline__ int paged_owner(uint32_t u, uint32_t total, uint32_t grid) { return (int)(((u + 1) * grid - 1) / total); }
+
 // Keys that row r (of the K/V head's) sees: the first so many.
-__device__ __forceinline__ int paged_row_keys(const PagedParams& p, const PagedTile& t, int r) {
+__device__ __forceinline__ int paged_row_keys(const PagedParams& p, const PagedItem& t, int r) {
     const int i = fast_div(r, p.d_group);
     if (r >= p.rows || i >= t.m) return 0;
     const int seen = t.n - t.m + i + 1;
@@ -63,7 +121,7 @@ __device__ __forceinline__ int paged_row_keys(const PagedParams& p, const PagedT
 // smallest step is 2^-32 of it.  16-bit queries are held exactly that way; rotated ones are not 16-bit numbers, and what their rounding leaves goes
 // to q_rest for a second product (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).
 template <int D, int DT, int R, int THREADS>
-__device__ __forceinline__ void paged_stage_q(const PagedParams& p, const PagedTile& t, int first_row, char* q_lds, char* q_rest, float* factor) {
+__device__ __forceinline__ void paged_stage_q(const PagedParams& p, const PagedItem& t, int first_row, char* q_lds, char* q_rest, float* factor) {
     constexpr int U = D / 16;      // units of sixteen elements, one lane each; a row is U neighbouring lanes
     const bool rope = p.rope.freqs != nullptr, interleaved = p.rope.interleaved != 0;
     const int pairs = rope ? p.rope.pairs : 0;
@@ -118,6 +176,111 @@ __device__ __forceinline__ void paged_stage_q(const PagedParams& p, const PagedT
     }
 }
 
+// ---- partial results: a slot of R rows for a workgroup's first item (2 g) and one for its last (2 g + 1), the only ones that it can have parts of.
+// Written and read past the XCDs' L2s, which are not coherent with each other (see intfa_splitkv.h).
+struct PagedParts {
+    BufferRsrc o, s;
+    __device__ __forceinline__ PagedParts(const PagedParams& p, int R, int D, int slot) {
+        o = __builtin_amdgcn_make_buffer_rsrc(p.parts + (int64_t)slot * R * D, 0, R * D * 4, 0x00020000);
+        s = __builtin_amdgcn_make_buffer_rsrc(p.part_stats + (int64_t)slot * R * 2, 0, R * 8, 0x00020000);
+    }
+    __device__ __forceinline__ void put(uint32_t row, int D, int col, v4f x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), o, (row * (uint32_t)D + (uint32_t)col) * 4u, 0, kSplitAux);
+    }
+    __device__ __forceinline__ void put_stats(uint32_t row, float m, float l) const {
+        typedef unsigned v2u __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64((v2u){__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, l)}, s, row * 8u, 0, kSplitAux);
+    }
+};
+
+// An item's ticket: the launch's epoch (upper 48 bits) and its arrivals so far.  The word is not cleared: whoever finds one of another epoch
+// takes it for (epoch, 0), and the last one leaves zero behind, so that the replays of a captured graph, whose epoch is a constant, find none of
+// their own.  True for the last of `pieces` arrivals.
+__device__ __forceinline__ bool paged_last_arrival(const PagedParams& p, uint32_t* lds, int item, int pieces) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's part has reached the point of coherence
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint64_t* const w = p.ticket + (int64_t)item * kTicketStride;
+        uint64_t seen = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if ((seen ^ p.epoch) >= 1u << 16)
+            __hip_atomic_compare_exchange_strong(w, &seen, p.epoch, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = __hip_atomic_fetch_add(w, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (p.epoch | (uint64_t)(pieces - 1));
+        if (last) __hip_atomic_store(w, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        lds[10] = last;
+    }
+    __syncthreads();
+    const bool last = __builtin_amdgcn_readfirstlane((int)lds[10]) != 0;
+    if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    return last;
+}
+
+// Merges the rows of an item from its pieces: those of workgroups `one` onward, all of them first items of theirs but the one that the item begins in
+// the middle of (first_is_first: it begins at that workgroup's first unit).
+template <int D, int DT, int R, int THREADS>
+__device__ __forceinline__ void paged_merge(const PagedParams& p, const PagedItem& t, int row0, int one, int pieces, bool first_is_first, float* lds) {
+    constexpr int LPR = D / 4, GROUPS = THREADS / LPR;      // lanes per row; rows, or shares of a row's pieces, side by side
+    const int nrows = p.rows - row0 < R ? p.rows - row0 : R;
+    const int col = ((int)threadIdx.x % LPR) * 4, group = (int)threadIdx.x / LPR;
+    int shares = 1;                                         // of a row's pieces
+    while (shares * 2 * nrows <= GROUPS) shares *= 2;
+    const int side = GROUPS / shares, share = group / side;
+    const BufferRsrc o = __builtin_amdgcn_make_buffer_rsrc(p.parts + (int64_t)one * 2 * R * D, 0, -1, 0x00020000);
+    const BufferRsrc s = __builtin_amdgcn_make_buffer_rsrc(p.part_stats + (int64_t)one * 2 * R * 2, 0, -1, 0x00020000);
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    auto slot_of = [&](int i) __attribute__((always_inline)) { return (uint32_t)(2 * i + (i == 0 && !first_is_first)); };
+    for (int r0 = 0; r0 < nrows; r0 += side) {
+        const int r = r0 + group % side, rr = r < nrows ? r : nrows - 1;
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        for (int i0 = share; i0 < pieces; i0 += 4 * shares) {
+            v4f x[4];
+            float ms[4], ls[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * shares < pieces ? i0 + u * shares : i0;
+                const uint32_t row = slot_of(i) * R + (uint32_t)rr;
+                const v2u st = __builtin_amdgcn_raw_buffer_load_b64(s, row * 8u, 0, kSplitAux);
+                x[u] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, (row * (uint32_t)D + (uint32_t)col) * 4u, 0, kSplitAux));
+                ms[u] = i0 + u * shares < pieces ? __builtin_bit_cast(float, (unsigned)st[0]) : -INFINITY;
+                ls[u] = __builtin_bit_cast(float, (unsigned)st[1]);
+            }
+            const float top = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m);
+            const float frame = top == -INFINITY ? 0.f : top;
+            const float a = fast_exp2(m - frame);
+            acc *= a;
+            l *= a;
+            m = top;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float w = fast_exp2(ms[u] - frame);
+                acc += w * x[u];
+                l += w * ls[u];
+            }
+        }
+        if (shares > 1) {                                   // (one row per group then: every thread comes here once)
+            __syncthreads();
+            float* const mine = lds + threadIdx.x * 6;
+            mine[0] = acc[0]; mine[1] = acc[1]; mine[2] = acc[2]; mine[3] = acc[3]; mine[4] = m; mine[5] = l;
+            __syncthreads();
+            if (share > 0) return;
+            for (int k = 1; k < shares; ++k) {
+                const float* const other = lds + ((group + k * side) * LPR + (int)threadIdx.x % LPR) * 6;
+                const float top = fmaxf(m, other[4]), frame = top == -INFINITY ? 0.f : top, a = fast_exp2(m - frame), w = fast_exp2(other[4] - frame);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = a * acc[j] + w * other[j];
+                l = a * l + w * other[5];
+                m = top;
+            }
+        }
+        if (r >= nrows) continue;
+        const int row = row0 + r, token = fast_div(row, p.d_group), head = t.hk * p.group + row - token * p.group;
+        const bool empty = m == -INFINITY;
+        store_out4<DT>(p.out + t.z * p.o_sb + head * p.o_sh + token * p.o_sn + col * 2, acc * (empty ? 0.f : 1.f / l));
+        if (p.lse != nullptr && col == 0)
+            p.lse[((int64_t)t.z * p.heads + head) * p.seqlen + token] = empty ? -INFINITY : m + __builtin_log2f(l) - kPShift;
+    }
+}
+
 template <int D, int DT, int RT>
 __global__ void __launch_bounds__(64 * kPagedWaves) paged_decode_kernel(const PagedParams p) {
     constexpr int R = 16 * RT, STEP = D == 256 ? 32 : 64, G = STEP / 16, KJ = D / 64, VB = D / 16, VD = VB / 4, DT16 = D / 16;
@@ -128,11 +291,19 @@ __global__ void __launch_bounds__(64 * kPagedWaves) paged_decode_kernel(const Pa
     __shared__ float factor_lds[R];
     __shared__ __align__(16) float o_lds[W * 16 * D];
     __shared__ float m_lds[W * R], l_lds[W * R];
-    const PagedTile t = paged_tile(p, (int)blockIdx.x);
+    __shared__ uint32_t find_lds[16];
+    PagedItem t;
+    uint32_t first, end, start, grid;
+    const uint32_t total = paged_find<THREADS>(p, find_lds, t, first, end, start, grid);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), x = lane & 15, c = lane >> 4;
-    const int row0 = t.tile * R;
-    paged_stage_q<D, DT, R, THREADS>(p, t, row0, q_lds, q_rest, factor_lds);
     const bool rope = p.rope.freqs != nullptr;
+  for (uint32_t at = first; at < end;) {
+    const int row0 = t.tile * R;
+    // keys [key_first, key_end) of the item are this workgroup's
+    const uint32_t item_end = start + (uint32_t)t.units;
+    const bool whole = at == start && item_end <= end;
+    const int key_first = (int)(at - start) << p.unit_log2;
+    paged_stage_q<D, DT, R, THREADS>(p, t, row0, q_lds, q_rest, factor_lds);
     __syncthreads();
     int seen[RT], least = 0x7fffffff, most = 0;
     float factor[RT], m[RT], l[RT];
@@ -151,10 +322,14 @@ __global__ void __launch_bounds__(64 * kPagedWaves) paged_decode_kernel(const Pa
         most = s > most ? s : most;
         least = s < least ? s : least;
     }
+    if (item_end > end) {
+        const int limit = (int)(end - start) << p.unit_log2;
+        most = most < limit ? most : limit;
+    }
     const char* const k_head = p.k + t.hk * p.k_sh;
     const char* const v_head = p.v + t.hk * p.v_sh;
     const int32_t* const table = p.table + t.z * p.bt_sb;
-    for (int key0 = wave * STEP; key0 < most; key0 += W * STEP) {
+    for (int key0 = key_first + wave * STEP; key0 < most; key0 += W * STEP) {
         v4i k[G][KJ];
         VRow v[G][4];
         float ks[G], vs[G];
@@ -312,26 +487,56 @@ __global__ void __launch_bounds__(64 * kPagedWaves) paged_decode_kernel(const Pa
             weight[w] = empty ? 0.f : fast_exp2(m_lds[w * R + 16 * rt + r] - top);
             sum += weight[w] * l_lds[w * R + 16 * rt + r];
         }
-        const float inv = empty ? 0.f : 1.f / sum;
         const int token = fast_div(row, p.d_group);
         const int head = t.hk * p.group + row - token * p.group;
         if (row < p.rows) {
-            char* const dst = p.out + t.z * p.o_sb + head * p.o_sh + token * p.o_sn + part * DT16 * 2;
+            if (whole) {
+                const float inv = empty ? 0.f : 1.f / sum;
+                char* const dst = p.out + t.z * p.o_sb + head * p.o_sh + token * p.o_sn + part * DT16 * 2;
 #pragma unroll
-            for (int j = 0; j < DT16; j += 4) {
-                v4f a = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < DT16; j += 4) {
+                    v4f a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * D + part * DT16 + j);
-                store_out4<DT>(dst + j * 2, a * inv);
+                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * D + part * DT16 + j);
+                    store_out4<DT>(dst + j * 2, a * inv);
+                }
+                if (p.lse != nullptr && part == 0)
+                    p.lse[((int64_t)t.z * p.heads + head) * p.seqlen + token] = empty ? -INFINITY : top + __builtin_log2f(sum) - kPShift;
+            } else {
+                const PagedParts mine(p, R, D, 2 * (int)blockIdx.x + (at != first));
+#pragma unroll
+                for (int j = 0; j < DT16; j += 4) {
+                    v4f a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * D + part * DT16 + j);
+                    mine.put((uint32_t)(16 * rt + r), D, part * DT16 + j, a);
+                }
+                if (part == 0) mine.put_stats((uint32_t)(16 * rt + r), top, sum);
             }
-            if (p.lse != nullptr && part == 0)
-                p.lse[((int64_t)t.z * p.heads + head) * p.seqlen + token] = empty ? -INFINITY : top + __builtin_log2f(sum) - kPShift;
         }
     }
+    if (!whole) {
+        const int one = paged_owner(start, total, grid), last = paged_owner(item_end - 1, total, grid);
+        if (paged_last_arrival(p, find_lds, (t.z * p.heads_kv + t.hk) * p.tiles + t.tile, last - one + 1))
+            paged_merge<D, DT, R, THREADS>(p, t, row0, one, last - one + 1, (uint32_t)one * total / grid == start, o_lds);
+    }
+    // ---- the next item of the line
+    at = item_end;
+    if (at >= end) break;
+    start = at;
+    if (++t.tile == p.tiles) {
+        t.tile = 0;
+        if (++t.hk == p.heads_kv) {
+            t.hk = 0;
+            paged_sequence(p, t.z + 1, t);
+        }
+    }
+    __syncthreads();
+  }
 }
 
 template <int D> int launch_paged(const PagedParams& p, const PagedSel& sel, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.batch * p.heads_kv * p.tiles));
+    const dim3 grid((unsigned)p.grid);
 #define INTFA_CALL(DT, RT) hipLaunchKernelGGL((paged_decode_kernel<D, DT, RT>), grid, dim3(64 * kPagedWaves), 0, stream, p)
     if (sel.io_dt == 0) {
         if (sel.row_tiles == 1) INTFA_CALL(0, 1); else INTFA_CALL(0, 2);

@@ -36,9 +36,13 @@ struct PagedParams {
     int32_t k_sn, v_sn;                              // bytes
     int32_t batch, heads, heads_kv, group, seqlen, rows;      // group: query heads per K/V head; rows = group * seqlen
     int32_t page_log2, num_pages, table_width, causal;
-    int32_t tiles;                                   // workgroups along the rows of a K/V head
+    int32_t tiles;                                   // row tiles of a K/V head
+    int32_t unit_log2;                               // keys that are dealt together
+    int32_t grid;                                    // workgroups of the launch
     float qk_scale_log2;
     RopeArgs rope;
+    float* parts; float* part_stats;                 // partial results: two slots per workgroup (intfa_paged_decode.h)
+    uint64_t* ticket; uint64_t epoch;
     FastDiv d_group, d_tiles, d_heads_kv;
 };
 
