@@ -365,7 +365,7 @@ template <int D> struct PagedStream {
         for (int g = 0; g < G; ++g) {
             const char* const kp = k_head + (named(key0, g) ? id[g] : 0) * k_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * k_sn;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) k[g][j] = *(const v4i*)(kp + k_lane + 64 * j);
+            for (int j = 0; j < KJ; ++j) k[g][j] = __builtin_nontemporal_load((const v4i*)(kp + k_lane + 64 * j));
         }
     }
     __device__ __forceinline__ void load_v(int key0) {
@@ -375,7 +375,7 @@ template <int D> struct PagedStream {
             const int at = has[g] ? id[g] : 0;
             const char* const vp = v_head + at * v_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * v_sn;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[g][i] = *(const VRow*)(vp + i * v_sn + v_lane);
+            for (int i = 0; i < 4; ++i) v[g][i] = __builtin_nontemporal_load((const VRow*)(vp + i * v_sn + v_lane));
             ks[g] = k_scale[at * ks_sp];
             vs[g] = v_scale[at * vs_sp];
         }
