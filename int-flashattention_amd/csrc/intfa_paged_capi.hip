@@ -36,7 +36,7 @@ Plan make_plan(const intfa_paged_attn_params* p) {
     a.unit_log2 = c.head_dim == 256 ? 7 : 8;
     const int64_t items = (int64_t)p->batch * c.heads_kv * a.tiles, keys = (int64_t)c.table_width * c.page_size;
     const int slots = kComputeUnits * (c.head_dim == 256 || a.sel.row_tiles > 1 ? 1 : 2);
-    auto units = [&] { return items * ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2); };
+    auto units = [&] { return items * (kPagedLead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
     a.grid = (int)(units() < slots ? units() : slots);
     while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)
     if (units() * a.grid >= 1ll << 32) a.grid = (int)(((1ll << 32) - 1) / units());

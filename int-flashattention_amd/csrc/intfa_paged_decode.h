@@ -24,6 +24,16 @@ __device__ __forceinline__ PagedArgs paged_args() {
     asm volatile("" : "+s"(p));
     return p;
 }
+// The same at the start of a kernel, with all lines of the block requested at once: it is cold in each launch, and the prologue's first dozen reads of it
+// would each be a trip to memory of their own.
+__device__ __forceinline__ PagedArgs paged_args_first() {
+    PagedArgs p = (PagedArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    typedef const __attribute__((address_space(4))) int* Words;
+    const Words w = (Words)p;
+    static_assert((sizeof(PagedParams) - 1) / 64 == 5, "the statement names a word of each line");
+    asm("" : "+s"(p) : "s"(w[0]), "s"(w[16]), "s"(w[32]), "s"(w[48]), "s"(w[64]), "s"(w[80]));
+    return p;
+}
 
 constexpr int kPagedWaves = 4;
 constexpr float kPShift = 14.f;       // P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales
@@ -51,15 +61,17 @@ typedef const __attribute__((address_space(4))) float* PagedFloats;
 // ---- who works on what
 // The keys of all sequences, K/V heads and row tiles (the items, in that order) are one line of units of 2^unit_log2 keys, at least one per item, and
 // every workgroup takes an equal piece of it: whatever the lengths, all compute units end together.  An item that lies in several pieces is merged
-// by the workgroup that finishes its part last.
-struct PagedItem { int z, hk, tile, n, m, units; };      // n: keys of the sequence, m: its new tokens, units: of each of its items
+// by the workgroup that finishes its part last.  Each item has kPagedLead units without keys ahead of its own: beginning an item and ending one take a
+// workgroup about as long as their keys would (8 us, where a unit takes 4 with the whole card reading), and without them the workgroups that have parts
+// of two items came in last (ragged batch of 16, 512 workgroups of 5.3 units: 42 -> 47 us).
+struct PagedItem { int z, hk, tile, n, m, units; };      // n: keys of the sequence, m: its new tokens, units: of each of its items, with the lead
 __device__ __forceinline__ int paged_keys(PagedArgs p, int z) {
     const int most = p->table_width << p->page_log2, n = p->seqlens_k[z];
     return n < 0 ? 0 : n < most ? n : most;
 }
 __device__ __forceinline__ int paged_units(PagedArgs p, int n) {
     const int u = (n + (1 << p->unit_log2) - 1) >> p->unit_log2;
-    return u > 1 ? u : 1;
+    return (u > 1 ? u : 1) + kPagedLead;
 }
 __device__ __forceinline__ void paged_sequence(PagedArgs p, int z, PagedItem& t) {
     const int most = p->table_width << p->page_log2, n = ((PagedInts)p->seqlens_k)[z];
@@ -279,31 +291,37 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
         const int r = r0 + group % side, rr = r < nrows ? r : nrows - 1;
         v4f acc = {0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
-        for (int i0 = share; i0 < pieces; i0 += 4 * shares) {
-            v4f x[4];
-            float ms[4], ls[4];
+        auto add = [&](auto many) __attribute__((always_inline)) {      // (so many loads under way together: each takes a microsecond)
+            constexpr int U = decltype(many)::value;
+            for (int i0 = share; i0 < pieces; i0 += U * shares) {      // (U loads under way together: each takes a microsecond)
+                v4f x[U];
+                float ms[U], ls[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = i0 + u * shares < pieces ? i0 + u * shares : i0;
-                const uint32_t row = slot_of(i) * R + (uint32_t)rr;
-                const v2u st = __builtin_amdgcn_raw_buffer_load_b64(s, row * 8u, 0, kSplitAux);
-                x[u] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, (row * (uint32_t)D + (uint32_t)col) * 4u, 0, kSplitAux));
-                ms[u] = i0 + u * shares < pieces ? __builtin_bit_cast(float, (unsigned)st[0]) : -INFINITY;
-                ls[u] = __builtin_bit_cast(float, (unsigned)st[1]);
-            }
-            const float top = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m);
-            const float frame = top == -INFINITY ? 0.f : top;
-            const float a = fast_exp2(m - frame);
-            acc *= a;
-            l *= a;
-            m = top;
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * shares < pieces ? i0 + u * shares : i0;
+                    const uint32_t row = slot_of(i) * R + (uint32_t)rr;
+                    const v2u st = __builtin_amdgcn_raw_buffer_load_b64(s, row * 8u, 0, kSplitAux);
+                    x[u] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, (row * (uint32_t)D + (uint32_t)col) * 4u, 0, kSplitAux));
+                    ms[u] = i0 + u * shares < pieces ? __builtin_bit_cast(float, (unsigned)st[0]) : -INFINITY;
+                    ls[u] = __builtin_bit_cast(float, (unsigned)st[1]);
+                }
+                float top = m;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float w = fast_exp2(ms[u] - frame);
-                acc += w * x[u];
-                l += w * ls[u];
+                for (int u = 0; u < U; ++u) top = fmaxf(top, ms[u]);
+                const float frame = top == -INFINITY ? 0.f : top;
+                const float a = fast_exp2(m - frame);
+                acc *= a;
+                l *= a;
+                m = top;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float w = fast_exp2(ms[u] - frame);
+                    acc += w * x[u];
+                    l += w * ls[u];
+                }
             }
-        }
+        };
+        if (pieces <= 4 * shares) add(IntTag<4>{}); else add(IntTag<16>{});
         if (shares > 1) {                                   // (one row per group then: every thread comes here once)
             __syncthreads();
             float* const mine = lds + threadIdx.x * 6;
@@ -395,7 +413,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     static_assert(R * (D / 2) * 8 <= W * 16 * O_ROW * 4, "the angles lie there first");
     __shared__ float m_lds[W * R], l_lds[W * R];
     __shared__ uint32_t arrival_lds;
-    PagedArgs p = paged_args();
+    PagedArgs p = paged_args_first();
     PagedItem t;
     uint32_t first, end, start, grid;
     const uint32_t total = paged_find(p, t, first, end, start, grid);
@@ -404,8 +422,9 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     const int row0 = t.tile * R;
     // this workgroup's part of the item: keys key_first .. most - 1
     const uint32_t item_end = start + (uint32_t)t.units;
-    const bool whole = at == start && item_end <= end;
-    const int key_first = (int)(at - start) << p->unit_log2;
+    if (end <= start + (uint32_t)kPagedLead) break;        // (no key of the last item)
+    const bool whole = at <= start + (uint32_t)kPagedLead && item_end <= end;
+    const int key_first = (at - start > (uint32_t)kPagedLead ? (int)(at - start) - kPagedLead : 0) << p->unit_log2;
     uint64_t ticket_seen = 0;
     if (!whole && threadIdx.x == 0) ticket_seen = __hip_atomic_load(paged_ticket(p, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     Queries queries;
@@ -417,7 +436,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     int most = queries.first_token < t.m ? paged_token_keys(p, t, last_token) : 0;
     const int least = paged_token_keys(p, t, queries.first_token);
     if (item_end > end) {
-        const int limit = (int)(end - start) << p->unit_log2;
+        const int limit = (int)(end - start - (uint32_t)kPagedLead) << p->unit_log2;
         most = most < limit ? most : limit;
     }
     // the first keys are on their way while the queries are staged
@@ -647,9 +666,9 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         }
     }
     if (!whole) {
-        const int one = paged_owner(start, total, grid), last = paged_owner(item_end - 1, total, grid);
+        const int one = paged_owner(start + (uint32_t)kPagedLead, total, grid), last = paged_owner(item_end - 1, total, grid);
         if (paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, last - one + 1))
-            paged_merge<D, DT, R, THREADS>(p, t, row0, one, last - one + 1, (uint32_t)one * total / grid == start, o_lds);
+            paged_merge<D, DT, R, THREADS>(p, t, row0, one, last - one + 1, (uint32_t)one * total / grid >= start, o_lds);
     }
     // ---- the next item of the line
     at = item_end;

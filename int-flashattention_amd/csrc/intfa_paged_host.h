@@ -26,6 +26,7 @@ inline int paged_cache_check(const intfa_paged_cache* c) {
     return INTFA_OK;
 }
 
+constexpr int kPagedLead = 2;          // units ahead of an item's keys (intfa_paged_decode.h)
 struct PagedParams {
     const char* q; char* out; float* lse;
     const char* k; const char* v; const float* k_scale; const float* v_scale;
