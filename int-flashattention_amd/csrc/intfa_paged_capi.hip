@@ -30,7 +30,7 @@ Plan make_plan(const intfa_paged_attn_params* p) {
     const intfa_paged_cache& c = p->cache;
     Plan a{};
     a.rows = p->heads / c.heads_kv * p->seqlen;
-    a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, a.rows <= 16 ? 1 : 2};
+    a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, a.rows <= 16 ? 1 : 2, c.page_size >= (c.head_dim == 256 ? 32 : 64)};
     a.slot_rows = 16 * a.sel.row_tiles;
     a.tiles = (a.rows + a.slot_rows - 1) / a.slot_rows;
     a.unit_log2 = c.head_dim == 256 ? 7 : 8;

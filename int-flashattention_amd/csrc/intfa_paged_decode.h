@@ -347,16 +347,22 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
     }
 }
 
-// Keys that a wave takes at a time, as they come from memory, and where they come from.  K's registers are refilled once the scores are formed, V's once
-// their products are, so that one of the two is on its way under everything that a step does.  The table's entries, which the addresses wait for, are
-// requested a step ahead of that, and the scales with the keys.
-template <int D> struct PagedStream {
+// Keys that a wave takes at a time, as they come from memory.
+template <int D> struct PagedStep {
     static constexpr int KEYS = D == 256 ? 32 : 64, G = KEYS / 16, KJ = D / 64, VB = D / 16, VD = VB / 4;
     typedef uint32_t VRow __attribute__((ext_vector_type(VD)));
     v4i k[G][KJ];
     VRow v[G][4];
     float ks[G], vs[G];
     bool has[G];                  // the granule has a key that some row sees, and the table names its page
+};
+// Where they come from.  K's registers are refilled once the scores are formed, V's once their products are, so that one of the two is on its way
+// under everything that a step does.  The table's entries, which the addresses wait for, are requested a step ahead of that.
+// (Two sets of registers, with everything requested a whole step ahead, leave room for one wave per SIMD: 32 x 32 heads of 4096 keys 171 -> 185 us.)
+// ONE: a page holds a step's keys (page_size at least KEYS), which takes a quarter of the scalar work.
+template <int D, bool ONE> struct PagedStream {
+    typedef PagedStep<D> Step;
+    static constexpr int G = Step::G, IDS = ONE ? 1 : G;
     const char* k_head; const char* v_head;
     PagedInts table;
     PagedFloats k_scale, v_scale;
@@ -364,45 +370,58 @@ template <int D> struct PagedStream {
     int k_sn, v_sn, page_log2, num_pages, last_column;
     int most;                     // keys past `most` are not this workgroup's
     uint32_t k_lane, v_lane;
-    int id[G];
+    int id[IDS];
     __device__ __forceinline__ PagedStream(PagedArgs p, const PagedItem& t, int most_, int x, int c)
         : k_head(p->k + t.hk * p->k_sh), v_head(p->v + t.hk * p->v_sh), table((PagedInts)(p->table + t.z * p->bt_sb)),
           k_scale((PagedFloats)(p->k_scale + t.hk * p->ks_sh)), v_scale((PagedFloats)(p->v_scale + t.hk * p->vs_sh)), k_sp(p->k_sp), v_sp(p->v_sp), ks_sp(p->ks_sp),
           vs_sp(p->vs_sp), k_sn(p->k_sn), v_sn(p->v_sn), page_log2(p->page_log2), num_pages(p->num_pages), last_column(p->table_width - 1), most(most_),
-          k_lane((uint32_t)(x * p->k_sn + 16 * c)), v_lane((uint32_t)(4 * c * p->v_sn + x * VB)) {}
+          k_lane((uint32_t)(x * p->k_sn + 16 * c)), v_lane((uint32_t)(4 * c * p->v_sn + x * Step::VB)) {}
     __device__ __forceinline__ void look(int key0) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < IDS; ++g) {
             const int column = (key0 + 16 * g) >> page_log2;
             id[g] = table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
         }
     }
-    __device__ __forceinline__ bool named(int key0, int g) const { return key0 + 16 * g < most && (unsigned)id[g] < (unsigned)num_pages; }
-    __device__ __forceinline__ void load_k(int key0) {
+    __device__ __forceinline__ bool named(int g) const { return (unsigned)id[g] < (unsigned)num_pages; }
+    __device__ __forceinline__ void load_k(int key0, Step& s) const {
+        const char* kp[IDS];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const char* const kp = k_head + (named(key0, g) ? id[g] : 0) * k_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * k_sn;
+        for (int g = 0; g < IDS; ++g) kp[g] = k_head + (named(g) ? id[g] : 0) * k_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * k_sn;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) k[g][j] = __builtin_nontemporal_load((const v4i*)(kp + k_lane + 64 * j));
-        }
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < Step::KJ; ++j)
+                s.k[g][j] = __builtin_nontemporal_load((const v4i*)((ONE ? kp[0] + 16 * g * k_sn : kp[ONE ? 0 : g]) + k_lane + 64 * j));
     }
-    __device__ __forceinline__ void load_v(int key0) {
+    __device__ __forceinline__ void load_v(int key0, Step& s) const {
+        const char* vp[IDS];
+#pragma unroll
+        for (int g = 0; g < IDS; ++g) {
+            const int at = named(g) ? id[g] : 0;
+            vp[g] = v_head + at * v_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * v_sn;
+            s.ks[g] = k_scale[at * ks_sp];
+            s.vs[g] = v_scale[at * vs_sp];
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            has[g] = named(key0, g);
-            const int at = has[g] ? id[g] : 0;
-            const char* const vp = v_head + at * v_sp + ((key0 + 16 * g) & ((1 << page_log2) - 1)) * v_sn;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[g][i] = __builtin_nontemporal_load((const VRow*)(vp + i * v_sn + v_lane));
-            ks[g] = k_scale[at * ks_sp];
-            vs[g] = v_scale[at * vs_sp];
+            s.has[g] = named(ONE ? 0 : g) && key0 + 16 * g < most;
+            if (ONE) {
+                s.ks[g] = s.ks[0];
+                s.vs[g] = s.vs[0];
+            }
         }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s.v[g][i] = __builtin_nontemporal_load((const typename Step::VRow*)((ONE ? vp[0] + (16 * g + i) * v_sn : vp[ONE ? 0 : g] + i * v_sn) + v_lane));
     }
 };
 
-template <int D, int DT, int RT>
+template <int D, int DT, int RT, bool ONE>
 __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) paged_decode_kernel(const PagedParams) {
-    constexpr int R = 16 * RT, STEP = PagedStream<D>::KEYS, G = STEP / 16, KJ = D / 64, DT16 = D / 16;
+    constexpr int R = 16 * RT, STEP = PagedStep<D>::KEYS, G = STEP / 16, KJ = D / 64, DT16 = D / 16;
     constexpr int W = kPagedWaves, THREADS = 64 * W, STRIDE = W * STEP;
     typedef PagedQueries<D, DT, R, THREADS> Queries;
     constexpr int O_ROW = D + 4;                           // floats (4 more: the banks)
@@ -410,7 +429,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     __shared__ __align__(16) char q_rest[R * Queries::ROW];
     __shared__ float factor_lds[R];
     __shared__ __align__(16) float o_lds[W * 16 * O_ROW];
-    static_assert(R * (D / 2) * 8 <= W * 16 * O_ROW * 4, "the angles lie there first");
+    static_assert(R * (D / 2) * 8 <= W * 16 * O_ROW * 4 && THREADS * 6 <= W * 16 * O_ROW, "the angles lie there first, and a merge's sums last");
     __shared__ float m_lds[W * R], l_lds[W * R];
     __shared__ uint32_t arrival_lds;
     PagedArgs p = paged_args_first();
@@ -440,13 +459,14 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         most = most < limit ? most : limit;
     }
     // the first keys are on their way while the queries are staged
-    PagedStream<D> now(p, t, most, x, c);
+    PagedStream<D, ONE> stream(p, t, most, x, c);
+    PagedStep<D> now;
     int key0 = key_first + wave * STEP;
     if (key0 < most) {
-        now.look(key0);
-        now.load_k(key0);
-        now.load_v(key0);
-        now.look(key0 + STRIDE);
+        stream.look(key0);
+        stream.load_k(key0, now);
+        stream.load_v(key0, now);
+        stream.look(key0 + STRIDE);
     }
     int seen[RT];
     float factor[RT], m[RT], l[RT];
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
                 }
             }
         }
-        if (more) now.load_k(key0 + STRIDE);
+        if (more) stream.load_k(key0 + STRIDE, now);
         v8h pf[RT][G / 2];
         float alpha[RT];
         bool rescale = false;
@@ -603,8 +623,8 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         };
         static_for<DT16>(tile);
         if (more) {
-            now.load_v(key0 + STRIDE);
-            now.look(key0 + 2 * STRIDE);
+            stream.load_v(key0 + STRIDE, now);
+            stream.look(key0 + 2 * STRIDE);
         }
     }
     p = paged_args();
@@ -687,7 +707,9 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
 
 template <int D> int launch_paged(const PagedParams& p, const PagedSel& sel, hipStream_t stream) {
     const dim3 grid((unsigned)p.grid);
-#define INTFA_CALL(DT, RT) hipLaunchKernelGGL((paged_decode_kernel<D, DT, RT>), grid, dim3(64 * kPagedWaves), 0, stream, p)
+#define INTFA_CALL(DT, RT) do { \
+        if (sel.one_page) hipLaunchKernelGGL((paged_decode_kernel<D, DT, RT, true>), grid, dim3(64 * kPagedWaves), 0, stream, p); \
+        else hipLaunchKernelGGL((paged_decode_kernel<D, DT, RT, false>), grid, dim3(64 * kPagedWaves), 0, stream, p); } while (0)
     if (sel.io_dt == 0) {
         if (sel.row_tiles == 1) INTFA_CALL(0, 1); else INTFA_CALL(0, 2);
     } else {

@@ -47,7 +47,7 @@ struct PagedParams {
     FastDiv d_group, d_tiles, d_heads_kv;
 };
 
-struct PagedSel { int head_dim, io_dt, row_tiles; };
+struct PagedSel { int head_dim, io_dt, row_tiles; bool one_page; };      // one_page: a page holds the keys that a wave takes at a time
 #define INTFA_DECL_PAGED(name) int name(const PagedParams& p, const PagedSel& sel, hipStream_t stream)
 INTFA_DECL_PAGED(launch_paged_d64);
 INTFA_DECL_PAGED(launch_paged_d128);
