@@ -30,12 +30,13 @@ Plan make_plan(const intfa_paged_attn_params* p) {
     const intfa_paged_cache& c = p->cache;
     Plan a{};
     a.rows = p->heads / c.heads_kv * p->seqlen;
-    a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, a.rows <= 16 ? 1 : 2, c.page_size >= (c.head_dim == 256 ? 32 : 64)};
-    a.slot_rows = 16 * a.sel.row_tiles;
+    const bool prefill = a.rows > 32;
+    a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, prefill ? 0 : a.rows <= 16 ? 1 : 2, c.page_size >= (!prefill && c.head_dim == 256 ? 32 : 64)};
+    a.slot_rows = prefill ? paged_prefill_rows(c.head_dim) : 16 * a.sel.row_tiles;
     a.tiles = (a.rows + a.slot_rows - 1) / a.slot_rows;
-    a.unit_log2 = c.head_dim == 256 ? 7 : 8;
+    a.unit_log2 = !prefill && c.head_dim == 256 ? 7 : 8;
     const int64_t items = (int64_t)p->batch * c.heads_kv * a.tiles, keys = (int64_t)c.table_width * c.page_size;
-    const int slots = kComputeUnits * (c.head_dim == 256 || a.sel.row_tiles > 1 ? 1 : 2);
+    const int slots = kComputeUnits * (prefill ? paged_prefill_wgs(c.head_dim) : c.head_dim == 256 || a.sel.row_tiles > 1 ? 1 : 2);
     auto units = [&] { return items * (kPagedLead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
     a.grid = (int)(units() < slots ? units() : slots);
     while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)
@@ -82,6 +83,8 @@ int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream) {
     kp.d_group = make_fast_div(kp.group); kp.d_tiles = make_fast_div(kp.tiles); kp.d_heads_kv = make_fast_div(kp.heads_kv);
     const PagedSel& sel = a.sel;
     hipStream_t st = (hipStream_t)stream;
+    if (sel.row_tiles == 0)
+        return c.head_dim == 64 ? launch_paged_prefill_d64(kp, sel, st) : c.head_dim == 128 ? launch_paged_prefill_d128(kp, sel, st) : launch_paged_prefill_d256(kp, sel, st);
     return c.head_dim == 64 ? launch_paged_d64(kp, sel, st) : c.head_dim == 128 ? launch_paged_d128(kp, sel, st) : launch_paged_d256(kp, sel, st);
 }
 

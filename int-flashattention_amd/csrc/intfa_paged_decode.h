@@ -11,267 +11,12 @@
 //       each is what tile j of V^T (row x: column x * D / 16 + j of V) takes.  The transposition is a byte select inside the lane.
 // int8 to fp16 is exact: byte ^ 0x80 under the exponent of 1024 is 1152 + value.
 #pragma once
-#include "intfa_paged_host.h"
-#include "intfa_splitkv.h"
+#include "intfa_paged_device.h"
 
 namespace intfa {
 
-// The kernel's own argument block; its fields are scalar loads, made where they are used: paged_args() gives a pointer that the compiler takes for
-// a new one (a hundred fields and what follows from them held from the prologue to the end would not fit the scalar registers).
-typedef const __attribute__((address_space(4))) PagedParams* PagedArgs;
-__device__ __forceinline__ PagedArgs paged_args() {
-    PagedArgs p = (PagedArgs)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    return p;
-}
-// The same at the start of a kernel, with all lines of the block requested at once: it is cold in each launch, and the prologue's first dozen reads of it
-// would each be a trip to memory of their own.
-__device__ __forceinline__ PagedArgs paged_args_first() {
-    PagedArgs p = (PagedArgs)__builtin_amdgcn_kernarg_segment_ptr();
-    typedef const __attribute__((address_space(4))) int* Words;
-    const Words w = (Words)p;
-    static_assert((sizeof(PagedParams) - 1) / 64 == 5, "the statement names a word of each line");
-    asm("" : "+s"(p) : "s"(w[0]), "s"(w[16]), "s"(w[32]), "s"(w[48]), "s"(w[64]), "s"(w[80]));
-    return p;
-}
-
 constexpr int kPagedWaves = 4;
 constexpr float kPShift = 14.f;       // P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales
-
-// Four int8 of a word as fp16
-__device__ __forceinline__ void i8x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    w ^= 0x80808080u;
-    const v2h bias = {(_Float16)-1152.f, (_Float16)-1152.f};
-    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + bias);
-    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + bias);
-}
-// Byte `b` of two words as a pair of fp16
-template <int B> __device__ __forceinline__ uint32_t i8_pair_to_f16(uint32_t first, uint32_t second) {
-    const uint32_t u = __builtin_amdgcn_perm(second, first, 0x0c000c00u | (uint32_t)(4 + B) << 16 | (uint32_t)B) ^ 0x64806480u;
-    const v2h bias = {(_Float16)-1152.f, (_Float16)-1152.f};
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, u) + bias);
-}
-
-__device__ __forceinline__ int paged_div(int n, const __attribute__((address_space(4))) FastDiv& d) { return fast_div(n, FastDiv{d.m, d.s}); }
-
-// (scalar loads of device memory that nothing in the launch writes)
-typedef const __attribute__((address_space(4))) int32_t* PagedInts;
-typedef const __attribute__((address_space(4))) float* PagedFloats;
-
-// ---- who works on what
-// The keys of all sequences, K/V heads and row tiles (the items, in that order) are one line of units of 2^unit_log2 keys, at least one per item, and
-// every workgroup takes an equal piece of it: whatever the lengths, all compute units end together.  An item that lies in several pieces is merged
-// by the workgroup that finishes its part last.  Each item has kPagedLead units without keys ahead of its own: beginning an item and ending one take a
-// workgroup about as long as their keys would (8 us, where a unit takes 4 with the whole card reading), and without them the workgroups that have parts
-// of two items came in last (ragged batch of 16, 512 workgroups of 5.3 units: 42 -> 47 us).
-struct PagedItem { int z, hk, tile, n, m, units; };      // n: keys of the sequence, m: its new tokens, units: of each of its items, with the lead
-__device__ __forceinline__ int paged_keys(PagedArgs p, int z) {
-    const int most = p->table_width << p->page_log2, n = p->seqlens_k[z];
-    return n < 0 ? 0 : n < most ? n : most;
-}
-__device__ __forceinline__ int paged_units(PagedArgs p, int n) {
-    const int u = (n + (1 << p->unit_log2) - 1) >> p->unit_log2;
-    return (u > 1 ? u : 1) + kPagedLead;
-}
-__device__ __forceinline__ void paged_sequence(PagedArgs p, int z, PagedItem& t) {
-    const int most = p->table_width << p->page_log2, n = ((PagedInts)p->seqlens_k)[z];
-    t.z = z;
-    t.n = n < 0 ? 0 : n < most ? n : most;
-    t.units = paged_units(p, t.n);
-    t.m = p->seqlen;
-    if (p->seqlens_q != nullptr) {
-        const int m = ((PagedInts)p->seqlens_q)[z];
-        t.m = m < 0 ? 0 : m < t.m ? m : t.m;
-    }
-}
-// Finds this workgroup's piece [first, end) of the line, and the item that `first` lies in: it begins at unit `start`.  The line is cut for `grid`
-// workgroups, those of the launch or as many as there are units: none of them has an empty piece (first == end: not one of them).  The host
-// keeps the number of units times that of workgroups below 2^32.
-// (Every wave finds it for itself, without LDS: sequences are dealt to the lanes in runs, of one up to 64 sequences, and a scan gives the total and
-// every run's place.)
-__device__ __forceinline__ uint32_t paged_find(PagedArgs p, PagedItem& t, uint32_t& first, uint32_t& end, uint32_t& start, uint32_t& grid) {
-    const int per = p->heads_kv * p->tiles, run = (p->batch + 63) / 64, lane = threadIdx.x & 63, z0 = lane * run;
-    uint32_t mine = 0;
-    for (int z = z0; z < z0 + run && z < p->batch; ++z) mine += (uint32_t)paged_units(p, paged_keys(p, z)) * (uint32_t)per;
-    uint32_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
-        if (lane >= d) upto += o;
-    }
-    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    grid = (uint32_t)p->grid < total ? (uint32_t)p->grid : total;
-    first = end = 0;
-    if (blockIdx.x >= grid) return total;
-    first = (uint32_t)blockIdx.x * total / grid;
-    end = ((uint32_t)blockIdx.x + 1) * total / grid;
-    // the lane whose run holds `first`, and the sequence in it
-    const int holder = __builtin_ctzll(__ballot(first < upto));
-    uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), holder);
-    int z = holder * run;
-    paged_sequence(p, z, t);
-    while (first >= at + (uint32_t)(t.units * per)) {
-        at += (uint32_t)(t.units * per);
-        paged_sequence(p, ++z, t);
-    }
-    const uint32_t item = (first - at) / (uint32_t)t.units;
-    start = at + item * (uint32_t)t.units;
-    t.hk = paged_div((int)item, p->d_tiles);
-    t.tile = (int)item - t.hk * p->tiles;
-    return total;
-}
-// The workgroup that has unit u of a line of `total`.
-__device__ __forceinline__ int paged_owner(uint32_t u, uint32_t total, uint32_t grid) { return (int)(((u + 1) * grid - 1) / total); }
-
-// Keys that token i of the sequence sees: the first so many.
-__device__ __forceinline__ int paged_token_keys(PagedArgs p, const PagedItem& t, int i) {
-    const int seen = t.n - t.m + i + 1;
-    return !p->causal || seen > t.n ? t.n : seen < 0 ? 0 : seen;
-}
-
-// The rows of a tile on their way to LDS: requested first, ahead of the cache's (loads come back in order), then turned and stored.  A row is D / 16
-// units of sixteen elements, a lane each.
-template <int D, int DT, int R, int THREADS> struct PagedQueries {
-    static constexpr int U = D / 16, N = (R * U + THREADS - 1) / THREADS, ROW = 2 * D + 16;      // ROW: bytes in LDS (16 more: sixteen rows in sixteen banks)
-    v4i x[N][2];
-    double freq;
-    int first_token, tokens;
-    bool rope, interleaved;
-    int pairs;
-    __device__ __forceinline__ void request(PagedArgs p, const PagedItem& t, int row0) {
-        rope = p->rope.freqs != nullptr;
-        interleaved = p->rope.interleaved != 0;
-        pairs = rope ? p->rope.pairs : 0;
-        const int row_last = row0 + R < p->rows ? row0 + R - 1 : p->rows - 1;
-        first_token = paged_div(row0, p->d_group);
-        tokens = paged_div(row_last, p->d_group) - first_token + 1;
-        freq = 0.0;
-        if ((int)threadIdx.x < pairs) freq = p->rope.freqs[threadIdx.x];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int i = (int)threadIdx.x + k * THREADS, r = i / U, u = i % U, row = row0 + r, token = paged_div(row, p->d_group);
-            int first, second;
-            rope_unit(u, pairs, interleaved, first, second);
-            x[k][0] = x[k][1] = (v4i){0, 0, 0, 0};
-            if (i < R * U && row < p->rows) {
-                const char* src = p->q + t.z * p->q_sb + (t.hk * p->group + row - token * p->group) * p->q_sh + token * p->q_sn;
-                x[k][0] = *(const v4i*)(src + 2 * first);
-                x[k][1] = *(const v4i*)(src + 2 * second);
-            }
-        }
-    }
-    // The angles of the tile's tokens, each once: angles[token * pairs + pair] = (cos, sin).  Threads beyond the pairs take further tokens.
-    __device__ __forceinline__ void turn_angles(PagedArgs p, const PagedItem& t, v2f* angles) const {
-        const float magnitude = p->rope.magnitude;
-        const int position = t.n - t.m + first_token;
-        for (int i = threadIdx.x; i < tokens * pairs; i += THREADS) {
-            const int token = i / pairs, pair = i - token * pairs;
-            float c, s;
-            rope_angle(pair == (int)threadIdx.x ? freq : p->rope.freqs[pair], position + token, magnitude, c, s);
-            angles[i] = (v2f){c, s};
-        }
-    }
-    // To LDS as fp16 with a power of two of the row's own taken out (`factor` gets it back, with the softmax's scale in base 2): the row's largest element
-    // is brought to 2^8, so that neither the range of bf16 nor a rotation leaves fp16's, and what lies under fp16's smallest step is 2^-32 of it.
-    // 16-bit queries are held exactly that way; rotated ones are not 16-bit numbers, and what their rounding leaves goes to q_rest for a second product
-    // (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).
-    __device__ __forceinline__ void stage(PagedArgs p, int row0, const v2f* angles, char* q_lds, char* q_rest, float* factor) const {
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int i = (int)threadIdx.x + k * THREADS, r = i / U, u = i % U;
-            if (R * U % THREADS != 0 && i >= R * U) continue;
-            int first, second;
-            rope_unit(u, pairs, interleaved, first, second);
-            float y[16];
-            unpack8<DT>(x[k][0], y);
-            unpack8<DT>(x[k][1], y + 8);
-            if (8 * u < pairs) {
-                int token = paged_div(row0 + r, p->d_group) - first_token;
-                token = token < tokens ? token : tokens - 1;
-                float c[8], s[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const v2f a = angles[token * pairs + 8 * u + j];
-                    c[j] = a[0];
-                    s[j] = a[1];
-                }
-                rope_turn_unit(y, c, s, interleaved);
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uint32_t a = __builtin_bit_cast(uint32_t, y[j]) & 0x7fffffffu;
-                top = top > a ? top : a;
-            }
-#pragma unroll
-            for (int w = 1; w < U; w <<= 1) {
-                const uint32_t a = (uint32_t)__shfl_xor((int)top, w);
-                top = top > a ? top : a;
-            }
-            int e = (int)(top >> 23) - 127;
-            e = e < -100 ? -100 : e > 100 ? 100 : e;
-            const float down = __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){y[2 * j] * down, y[2 * j + 1] * down}, v2h));
-            *(v4i*)(q_lds + r * ROW + 2 * first) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
-            *(v4i*)(q_lds + r * ROW + 2 * second) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
-            if (rope) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const v2f near = __builtin_convertvector(__builtin_bit_cast(v2h, h[j]), v2f);
-                    h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){y[2 * j] * down - near[0], y[2 * j + 1] * down - near[1]}, v2h));
-                }
-                *(v4i*)(q_rest + r * ROW + 2 * first) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
-                *(v4i*)(q_rest + r * ROW + 2 * second) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
-            }
-            if (u == 0) factor[r] = __builtin_bit_cast(float, (uint32_t)(127 + e - 8) << 23) * p->qk_scale_log2;
-        }
-    }
-};
-
-// ---- partial results: a slot of R rows for a workgroup's first item (2 g) and one for its last (2 g + 1), the only ones that it can have parts of.
-// Written and read past the XCDs' L2s, which are not coherent with each other (see intfa_splitkv.h).
-struct PagedParts {
-    BufferRsrc o, s;
-    __device__ __forceinline__ PagedParts(PagedArgs p, int R, int D, int slot) {
-        o = __builtin_amdgcn_make_buffer_rsrc(p->parts + (int64_t)slot * R * D, 0, R * D * 4, 0x00020000);
-        s = __builtin_amdgcn_make_buffer_rsrc(p->part_stats + (int64_t)slot * R * 2, 0, R * 8, 0x00020000);
-    }
-    __device__ __forceinline__ void put(uint32_t row, int D, int col, v4f x) const {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), o, (row * (uint32_t)D + (uint32_t)col) * 4u, 0, kSplitAux);
-    }
-    __device__ __forceinline__ void put_stats(uint32_t row, float m, float l) const {
-        typedef unsigned v2u __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64((v2u){__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, l)}, s, row * 8u, 0, kSplitAux);
-    }
-};
-
-// An item's ticket: the launch's epoch (upper 48 bits) and its arrivals so far.  The word is not cleared: every piece looks at it when it starts, and one
-// that finds another epoch's exchanges it for (epoch, 0) before its own arrival (a word exchanged by another since then is left alone).  The last
-// arrival leaves zero behind, so that the replays of a captured graph, whose epoch is a constant, find none of their own.
-__device__ __forceinline__ uint64_t* paged_ticket(PagedArgs p, const PagedItem& t) {
-    return p->ticket + (int64_t)((t.z * p->heads_kv + t.hk) * p->tiles + t.tile) * kTicketStride;
-}
-__device__ __forceinline__ void paged_open_ticket(PagedArgs p, uint64_t* word, uint64_t seen) {
-    if (threadIdx.x == 0 && (seen ^ p->epoch) >= 1u << 16)
-        __hip_atomic_compare_exchange_strong(word, &seen, p->epoch, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// True for the last of `pieces` arrivals.
-__device__ __forceinline__ bool paged_last_arrival(PagedArgs p, uint64_t* word, uint32_t* lds, int pieces) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's part has reached the point of coherence
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const bool last = __hip_atomic_fetch_add(word, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (p->epoch | (uint64_t)(pieces - 1));
-        if (last) __hip_atomic_store(word, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *lds = last;
-    }
-    __syncthreads();
-    const bool last = __builtin_amdgcn_readfirstlane((int)*lds) != 0;
-    if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    return last;
-}
 
 // Merges the rows of an item from its pieces: those of workgroups `one` onward, all of them first items of theirs but the one that the item begins in
 // the middle of (first_is_first: it begins at that workgroup's first unit).
@@ -434,34 +179,23 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     __shared__ uint32_t arrival_lds;
     PagedArgs p = paged_args_first();
     PagedItem t;
-    uint32_t first, end, start, grid;
-    const uint32_t total = paged_find(p, t, first, end, start, grid);
+    PagedPiece piece = paged_find(p, R, t);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), x = lane & 15, c = lane >> 4;
-  for (uint32_t at = first; at < end;) {
+  while (piece.start < piece.end) {
     const int row0 = t.tile * R;
-    // this workgroup's part of the item: keys key_first .. most - 1
-    const uint32_t item_end = start + (uint32_t)t.units;
-    if (end <= start + (uint32_t)kPagedLead) break;        // (no key of the last item)
-    const bool whole = at <= start + (uint32_t)kPagedLead && item_end <= end;
-    const int key_first = (at - start > (uint32_t)kPagedLead ? (int)(at - start) - kPagedLead : 0) << p->unit_log2;
+    const PagedPart part = paged_part(p, t, piece);
+    if (part.none) break;
     uint64_t ticket_seen = 0;
-    if (!whole && threadIdx.x == 0) ticket_seen = __hip_atomic_load(paged_ticket(p, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!part.whole && threadIdx.x == 0) ticket_seen = __hip_atomic_load(paged_ticket(p, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     Queries queries;
     queries.request(p, t, row0);
     const bool rope = queries.rope;
     // (a row past the last one or a token past the sequence's new ones counts like the others here; what it gives is not used)
-    int last_token = queries.first_token + queries.tokens - 1;
-    last_token = last_token < t.m ? last_token : t.m - 1;
-    int most = queries.first_token < t.m ? paged_token_keys(p, t, last_token) : 0;
-    const int least = paged_token_keys(p, t, queries.first_token);
-    if (item_end > end) {
-        const int limit = (int)(end - start - (uint32_t)kPagedLead) << p->unit_log2;
-        most = most < limit ? most : limit;
-    }
+    const int most = part.key_end, least = paged_token_keys(p, t, t.first_token);
     // the first keys are on their way while the queries are staged
     PagedStream<D, ONE> stream(p, t, most, x, c);
     PagedStep<D> now;
-    int key0 = key_first + wave * STEP;
+    int key0 = part.key_first + wave * STEP;
     if (key0 < most) {
         stream.look(key0);
         stream.load_k(key0, now);
@@ -484,7 +218,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         __syncthreads();
     }
     queries.stage(p, row0, (const v2f*)o_lds, q_lds, q_rest, factor_lds);
-    if (!whole) paged_open_ticket(p, paged_ticket(p, t), ticket_seen);
+    if (!part.whole) paged_open_ticket(p, paged_ticket(p, t), ticket_seen);
     __syncthreads();
     const char* const q_lane = q_lds + x * Queries::ROW + 32 * c;
     const char* const q_rest_lane = q_rest + x * Queries::ROW + 32 * c;
@@ -645,13 +379,13 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
 #pragma unroll
             for (int j = 0; j < DT16; ++j) o_lds[(wave * 16 + x) * O_ROW + (4 * c + i) * DT16 + j] = o[rt][j][i];
         __syncthreads();
-        const int r = (int)threadIdx.x / 16, part = (int)threadIdx.x % 16, row = row0 + 16 * rt + r;      // D / 16 columns of one row
+        const int r = (int)threadIdx.x / 16, cols = (int)threadIdx.x % 16, row = row0 + 16 * rt + r;      // D / 16 columns of one row
         static_assert(THREADS == 256, "a thread per row and sixteenth of it");
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < W; ++w) top = fmaxf(top, m_lds[w * R + 16 * rt + r]);
         const int token = paged_div(row, p->d_group);
-        const bool empty = top == -INFINITY || (whole && token >= t.m);
+        const bool empty = top == -INFINITY || (part.whole && token >= t.m);
         float sum = 0.f, weight[W];
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -660,47 +394,34 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         }
         const int head = t.hk * p->group + row - token * p->group;
         if (row < p->rows) {
-            if (whole) {
+            if (part.whole) {
                 const float inv = empty ? 0.f : 1.f / sum;
-                char* const dst = p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + part * DT16 * 2;
+                char* const dst = p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + cols * DT16 * 2;
 #pragma unroll
                 for (int j = 0; j < DT16; j += 4) {
                     v4f a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * O_ROW + part * DT16 + j);
+                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * O_ROW + cols * DT16 + j);
                     store_out4<DT>(dst + j * 2, a * inv);
                 }
-                if (p->lse != nullptr && part == 0)
+                if (p->lse != nullptr && cols == 0)
                     p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = empty ? -INFINITY : top + __builtin_log2f(sum) - kPShift;
             } else {
-                const PagedParts mine(p, R, D, 2 * (int)blockIdx.x + (at != first));
+                const PagedParts mine(p, R, D, (int)part.slot);
 #pragma unroll
                 for (int j = 0; j < DT16; j += 4) {
                     v4f a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * O_ROW + part * DT16 + j);
-                    mine.put((uint32_t)(16 * rt + r), D, part * DT16 + j, a);
+                    for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * O_ROW + cols * DT16 + j);
+                    mine.put((uint32_t)(16 * rt + r), D, cols * DT16 + j, a);
                 }
-                if (part == 0) mine.put_stats((uint32_t)(16 * rt + r), top, sum);
+                if (cols == 0) mine.put_stats((uint32_t)(16 * rt + r), top, sum);
             }
         }
     }
-    if (!whole) {
-        const int one = paged_owner(start + (uint32_t)kPagedLead, total, grid), last = paged_owner(item_end - 1, total, grid);
-        if (paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, last - one + 1))
-            paged_merge<D, DT, R, THREADS>(p, t, row0, one, last - one + 1, (uint32_t)one * total / grid >= start, o_lds);
-    }
-    // ---- the next item of the line
-    at = item_end;
-    if (at >= end) break;
-    start = at;
-    if (++t.tile == p->tiles) {
-        t.tile = 0;
-        if (++t.hk == p->heads_kv) {
-            t.hk = 0;
-            paged_sequence(p, t.z + 1, t);
-        }
-    }
+    if (!part.whole && paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, part.pieces))
+        paged_merge<D, DT, R, THREADS>(p, t, row0, part.one, part.pieces, part.first_is_first, o_lds);
+    if (!paged_next(p, R, t, piece)) break;
     __syncthreads();
   }
 }

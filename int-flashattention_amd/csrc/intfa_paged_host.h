@@ -47,10 +47,16 @@ struct PagedParams {
     FastDiv d_group, d_tiles, d_heads_kv;
 };
 
-struct PagedSel { int head_dim, io_dt, row_tiles; bool one_page; };      // one_page: a page holds the keys that a wave takes at a time
+struct PagedSel { int head_dim, io_dt, row_tiles; bool one_page; };      // row_tiles: of 16 rows, 0 for the prefill kernel; one_page: a page holds the keys that are taken at a time
 #define INTFA_DECL_PAGED(name) int name(const PagedParams& p, const PagedSel& sel, hipStream_t stream)
 INTFA_DECL_PAGED(launch_paged_d64);
 INTFA_DECL_PAGED(launch_paged_d128);
 INTFA_DECL_PAGED(launch_paged_d256);
+INTFA_DECL_PAGED(launch_paged_prefill_d64);
+INTFA_DECL_PAGED(launch_paged_prefill_d128);
+INTFA_DECL_PAGED(launch_paged_prefill_d256);
+// rows of a tile and workgroups per compute unit of the prefill kernel (intfa_paged_prefill.h)
+inline int paged_prefill_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
+inline int paged_prefill_wgs(int head_dim) { return head_dim == 64 ? 2 : 1; }
 
 }  // namespace intfa

@@ -1,0 +1,373 @@
+// Attention of many query rows (a chunk of a prompt, or a whole one) over a paged int8 cache.
+//
+// A wave owns 32 rows of a tile and all waves walk the same key blocks of 64.  S^T = K Q^T and O^T = V^T P^T run on v_mfma_f32_32x32x16_f16 with the
+// rows as columns, so that the statistics of a row are one lane's (and its pair's, l ^ 32) and P goes from accumulator to operand in its lane.  The products
+// take fp16, and what a block needs of it is made once for all waves: the threads fetch the block's bytes two blocks ahead, turn them into fp16 (exactly:
+// intfa_paged_device.h) and store them to LDS, K by rows of keys, V transposed.
+//   V^T  a thread takes four consecutive keys by four columns: a word each of four rows, whose bytes it selects into four pairs of pairs.  A row of V^T
+//        holds the keys in the order in which P's lanes have them: 16 t + 8 j + 4 h + i at 32 t + 16 h + 8 j + 2 i bytes (h: the lane's half).  Column
+//        4 q + b is row b D / 4 + q: neighbouring threads (q) then store to neighbouring rows, in different banks, and a lane's accumulators of the
+//        tiles are four neighbouring columns.
+// A row's scale of scores and a page's go into one multiplier of the exponent's fused multiply-add (a page's scale is not negative: the maximum of the
+// products is that of the scores).  V's scale goes there too, as log2(scale / reference), the reference being the unit of the accumulators: it follows the
+// page's scale where that leaves 2^-10 .. 2 of it.  A row's maximum is followed where it grows by more than 2^6, so that most blocks rescale nothing.
+#pragma once
+#include "intfa_paged_device.h"
+
+namespace intfa {
+
+constexpr float kPrefillShift = 8.f, kPrefillSlack = 6.f;      // P is held as up to 2^(8 + 6 + 1) p, within fp16
+
+template <int D> struct PrefillShape {
+    static constexpr int WAVES = D == 128 ? 8 : 4, ROWS = 32 * WAVES, THREADS = 64 * WAVES, KEYS = 64;
+    static constexpr int WGS = D == 64 ? 2 : 1;            // workgroups per compute unit
+    static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * KEYS + 16;      // bytes in LDS (16 more: the banks)
+    static constexpr int K_BYTES = KEYS * K_ROW, V_BYTES = D * V_ROW, BLOCK = K_BYTES + V_BYTES;
+    static constexpr int UNITS = KEYS * D / 16 / THREADS;  // of sixteen bytes, for K and for V, per thread and block
+    static constexpr int PASS = D == 256 ? 32 : 64;        // rows whose queries are staged at a time
+    static_assert(UNITS >= 1 && UNITS * THREADS * 16 == KEYS * D, "");
+};
+
+// A block's bytes on their way, of one thread
+template <int D> struct PrefillBytes {
+    v4i k[PrefillShape<D>::UNITS];
+    uint32_t v[PrefillShape<D>::UNITS][4];
+};
+
+// REST: rotated queries, whose scores take a second product (PagedQueries::stage).  ONE: a page holds a block's keys.
+template <int D, int DT, bool REST, bool ONE>
+__global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS * PrefillShape<D>::WAVES / 4) paged_prefill_kernel(const PagedParams) {
+    typedef PrefillShape<D> S;
+    constexpr int THREADS = S::THREADS, R = S::ROWS, KS = D / 16, DTILES = D / 32, G = 4, UNITS = S::UNITS, NB = D / 4;
+    typedef PagedQueries<D, DT, S::PASS, THREADS> Queries;
+    constexpr int ANGLES_AT = 2 * S::PASS * Queries::ROW;
+    static_assert(ANGLES_AT + S::PASS * (D / 2) * 8 <= 2 * S::BLOCK, "the queries and their angles pass through the blocks' place");
+    __shared__ __align__(16) char lds[2 * S::BLOCK];
+    __shared__ float factor_lds[S::PASS];
+    __shared__ uint32_t arrival_lds;
+    PagedArgs p = paged_args_first();
+    PagedItem t;
+    PagedPiece piece = paged_find(p, R, t);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lq = lane & 31, lh = lane >> 5;
+  while (piece.start < piece.end) {
+    const PagedPart part = paged_part(p, t, piece);
+    if (part.none) break;
+    const int row0 = t.tile * R, row = row0 + 32 * wave + lq, token = paged_div(row, p->d_group);
+    uint64_t ticket_seen = 0;
+    if (!part.whole && threadIdx.x == 0) ticket_seen = __hip_atomic_load(paged_ticket(p, t), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // ---- queries: through LDS into the waves that own them
+    v8h q[KS], q_rest[REST ? KS : 1];
+    float factor = 0.f;
+    for (int pass = 0; pass < R / S::PASS; ++pass) {
+        Queries queries;
+        queries.request(p, t, row0 + pass * S::PASS);
+        if (pass > 0) __syncthreads();
+        if (REST) {
+            queries.turn_angles(p, t, (v2f*)(lds + ANGLES_AT));
+            __syncthreads();
+        }
+        queries.stage(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
+        __syncthreads();
+        if (32 * wave / S::PASS == pass) {
+            const char* const mine = lds + (32 * wave % S::PASS + lq) * Queries::ROW + 16 * lh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                q[ks] = *(const v8h*)(mine + 32 * ks);
+                if (REST) q_rest[REST ? ks : 0] = *(const v8h*)(mine + S::PASS * Queries::ROW + 32 * ks);
+            }
+            factor = factor_lds[32 * wave % S::PASS + lq];
+        }
+    }
+    // ---- where the keys come from
+    const char* const k_head = p->k + t.hk * p->k_sh;
+    const char* const v_head = p->v + t.hk * p->v_sh;
+    const int32_t* const table = p->table + t.z * p->bt_sb;
+    const PagedInts table_s = (PagedInts)table;
+    const PagedFloats k_scale = (PagedFloats)(p->k_scale + t.hk * p->ks_sh), v_scale = (PagedFloats)(p->v_scale + t.hk * p->vs_sh);
+    const int64_t k_sp = p->k_sp, v_sp = p->v_sp, ks_sp = p->ks_sp, vs_sp = p->vs_sp;
+    const int k_sn = p->k_sn, v_sn = p->v_sn, page_log2 = p->page_log2, num_pages = p->num_pages, last_column = p->table_width - 1;
+    const int page_mask = (1 << page_log2) - 1, most = part.key_end;
+    auto column = [&](int key) __attribute__((always_inline)) { const int c = key >> page_log2; return c < last_column ? c : last_column; };
+    // (the pages of a thread's own keys, where a block has several)
+    int k_id[UNITS], v_id[UNITS];
+    auto look = [&](int key0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int u = (int)threadIdx.x + i * THREADS;
+            if (ONE) {
+                if (i == 0) k_id[0] = table_s[column(key0)];
+            } else {
+                k_id[i] = table[column(key0 + u / (D / 16))];
+                v_id[i] = table[column(key0 + 4 * (u / NB))];
+            }
+        }
+    };
+    auto fetch = [&](int key0, PrefillBytes<D>& b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int u = (int)threadIdx.x + i * THREADS, kk = u / (D / 16), vk = 4 * (u / NB);
+            const int kid = ONE ? k_id[0] : k_id[i], vid = ONE ? k_id[0] : v_id[i];
+            const char* const kp = k_head + ((unsigned)kid < (unsigned)num_pages ? kid : 0) * k_sp + (ONE ? (key0 & page_mask) * k_sn : 0);
+            const char* const vp = v_head + ((unsigned)vid < (unsigned)num_pages ? vid : 0) * v_sp + (ONE ? (key0 & page_mask) * v_sn : 0);
+            b.k[i] = *(const v4i*)(kp + (uint32_t)((ONE ? kk : (key0 + kk) & page_mask) * k_sn + 16 * (u % (D / 16))));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b.v[i][j] = *(const uint32_t*)(vp + (uint32_t)(((ONE ? vk : (key0 + vk) & page_mask) + j) * v_sn + 4 * (u % NB)));
+        }
+    };
+    auto store = [&](const PrefillBytes<D>& b, char* block) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int u = (int)threadIdx.x + i * THREADS;
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) i8x4_to_f16((uint32_t)b.k[i][j], w[2 * j], w[2 * j + 1]);
+            char* const kd = block + (u / (D / 16)) * S::K_ROW + 32 * (u % (D / 16));
+            *(v4i*)kd = (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+            *(v4i*)(kd + 16) = (v4i){(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
+            const int four = u / NB;                       // which four keys: 4 (2 j + h) of 16 t
+            char* const vd = block + S::K_BYTES + (u % NB) * S::V_ROW + 32 * (four >> 2) + 16 * (four & 1) + 8 * ((four >> 1) & 1);
+            auto quad = [&](auto bt) __attribute__((always_inline)) {
+                constexpr int B = decltype(bt)::value;
+                *(v2i*)(vd + B * NB * S::V_ROW) = (v2i){(int)i8_pair_to_f16<B>(b.v[i][0], b.v[i][1]), (int)i8_pair_to_f16<B>(b.v[i][2], b.v[i][3])};
+            };
+            static_for<4>(quad);
+        }
+    };
+    // scales of a block, and whether the table names its pages (scalars)
+    struct Scales { float k[G], v[G]; bool has[G]; };
+    auto scales_of = [&](int key0, Scales& s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (ONE && g > 0) {
+                s.k[g] = s.k[0]; s.v[g] = s.v[0];
+                s.has[g] = s.has[0] && key0 + 16 * g < most;
+                continue;
+            }
+            const int id = table_s[column(key0 + 16 * g)];
+            s.has[g] = (unsigned)id < (unsigned)num_pages && key0 + 16 * g < most;
+            const int at = s.has[g] ? id : 0;
+            s.k[g] = k_scale[at * ks_sp];
+            s.v[g] = v_scale[at * vs_sp];
+        }
+    };
+    const int seen = paged_token_keys(p, t, token), least = paged_token_keys(p, t, t.first_token);
+    v16f acc[DTILES];
+#pragma unroll
+    for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+    float m = -INFINITY, l = 0.f, v_unit = 1.f, v_peak = 0.f;
+    int key0 = part.key_first;
+    PrefillBytes<D> even, odd;
+    Scales scales;
+    if (key0 < most) {
+        look(key0);
+        fetch(key0, even);
+        look(key0 + 64);
+        if (key0 + 64 < most) fetch(key0 + 64, odd);
+        look(key0 + 128);
+        scales_of(key0, scales);
+    }
+    if (!part.whole) paged_open_ticket(p, paged_ticket(p, t), ticket_seen);
+    __syncthreads();                                       // (the queries have been read)
+    if (key0 < most) store(even, lds);
+    __syncthreads();
+    auto block = [&](const char* now, char* then, PrefillBytes<D>& next, PrefillBytes<D>& after) __attribute__((always_inline)) {
+        // `next` holds the bytes of the block behind this one, `after` takes those of the one behind that
+        if (key0 + 128 < most) fetch(key0 + 128, after);
+        look(key0 + 192);
+        if (key0 + 64 < most) store(next, then);
+        const Scales sc = scales;
+        scales_of(key0 + 64, scales);
+        v16f s[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[half][r] = 0.f;
+            const char* const kl = now + (32 * half + lq) * S::K_ROW + 16 * lh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const v8h kf = *(const v8h*)(kl + 32 * ks);
+                s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[ks], s[half], 0, 0, 0);
+                if (REST) s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q_rest[REST ? ks : 0], s[half], 0, 0, 0);
+            }
+        }
+        // ---- hidden keys
+        bool masked = key0 + 64 > least;
+#pragma unroll
+        for (int g = 0; g < G; ++g) masked = masked || !sc.has[g];
+        if (masked) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = key0 + 32 * half + 8 * (r / 4) + 4 * lh + r % 4;
+                    s[half][r] = key < seen && sc.has[2 * half + r / 8] ? s[half][r] : -INFINITY;
+                }
+        }
+        // ---- V's unit: the page's scale, or the largest of the block's
+        float v_top = sc.has[0] ? sc.v[0] : 0.f;
+        if (!ONE) {
+#pragma unroll
+            for (int g = 1; g < G; ++g) v_top = fmaxf(v_top, sc.has[g] ? sc.v[g] : 0.f);
+        }
+        v_peak = fmaxf(v_peak, v_top);
+        if (v_top > 2.f * v_unit || v_top < 0x1p-10f * v_unit) {
+            const float unit = fmaxf(fmaxf(v_top, v_peak * 0x1p-60f), 0x1p-100f), scale = v_unit / unit;
+            v_unit = unit;
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[dt][r] *= scale;
+        }
+        const float v_ratio = v_top > 0.f ? v_top / v_unit : 1.f, v_log = __builtin_amdgcn_logf(v_ratio), v_back = 1.f / v_ratio;
+        // ---- softmax
+        float f[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) f[g] = fmaxf(factor * (ONE ? sc.k[0] : sc.k[g]), 0x1p-126f);      // (never zero: hidden keys are -infinity times it)
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float raw = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) raw = fmaxf(raw, s[g / 2][8 * (g % 2) + r]);
+            top = fmaxf(top, raw * f[g]);
+        }
+        top = half_pair_max(top);
+        if (__any(top > m + kPrefillSlack)) {
+            const float grown = fmaxf(m, top), alpha = grown == -INFINITY ? 1.f : fast_exp2(m - grown);
+            m = grown;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
+        }
+        const float frame = (m == -INFINITY ? 0.f : m) - kPrefillShift - v_log;
+        float sum = 0.f;
+        v8h pf[4];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float rel = ONE || v_top <= 0.f ? 1.f : (sc.has[g] ? sc.v[g] : 0.f) / v_top;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                float e = fast_exp2(fmaf(s[g / 2][8 * (g % 2) + r], f[g], -frame));
+                sum += e;
+                if (!ONE) e *= rel;
+                pf[g][r] = (_Float16)e;
+            }
+        }
+        l = fmaf(sum, v_back, l);
+        // ---- O^T += V^T P^T
+        if (v_top > 0.f) {
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt) {
+                const char* const vl = now + S::K_BYTES + (32 * dt + lq) * S::V_ROW + 16 * lh;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(vl + 32 * g), pf[g], acc[dt], 0, 0, 0);
+            }
+        }
+        key0 += 64;
+        __syncthreads();
+    };
+    while (key0 < most) {
+        block(lds, lds + S::BLOCK, odd, even);
+        if (key0 >= most) break;
+        block(lds + S::BLOCK, lds, even, odd);
+    }
+    p = paged_args();
+    l = half_pair_sum(l);
+    // ---- a lane's values: columns 4 (8 a + 4 lh + i) + b of its row, b = 0 .. 3 from as many tiles
+    auto value = [&](int a, int i) __attribute__((always_inline)) {
+        v4f x;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = acc[(b * NB + 8 * a) / 32][4 * ((b * NB / 8 + a) % 4) + i];
+        return x;
+    };
+    bool done = part.whole;
+    float weight = v_unit;                                 // of the accumulators
+    if (!part.whole) {
+        const PagedParts mine(p, R, D, (int)part.slot);
+#pragma unroll
+        for (int a = 0; a < D / 32; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine.put((uint32_t)(32 * wave + lq), D, 4 * (8 * a + 4 * lh + i), value(a, i) * v_unit);
+        if (lh == 0) mine.put_stats((uint32_t)(32 * wave + lq), m, l);
+        if (paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, part.pieces)) {
+            // the pieces in their order, each wave its own rows in its own layout
+            typedef unsigned v2u __attribute__((ext_vector_type(2)));
+            done = true;
+            weight = 1.f;
+            m = -INFINITY;
+            l = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+            for (int k = 0; k < part.pieces; ++k) {
+                const int slot = 2 * (part.one + k) + (k == 0 && !part.first_is_first);
+                const BufferRsrc o = __builtin_amdgcn_make_buffer_rsrc(p->parts + (int64_t)slot * R * D, 0, R * D * 4, 0x00020000);
+                const BufferRsrc st = __builtin_amdgcn_make_buffer_rsrc(p->part_stats + (int64_t)slot * R * 2, 0, R * 8, 0x00020000);
+                const uint32_t r0 = (uint32_t)(32 * wave + lq);
+                const v2u ml = __builtin_amdgcn_raw_buffer_load_b64(st, r0 * 8u, 0, kSplitAux);
+                const float mk = __builtin_bit_cast(float, (unsigned)ml[0]), top = fmaxf(m, mk), base = top == -INFINITY ? 0.f : top;
+                const float alpha = fast_exp2(m - base), w = fast_exp2(mk - base);
+                l = l * alpha + w * __builtin_bit_cast(float, (unsigned)ml[1]);
+                m = top;
+#pragma unroll
+                for (int a0 = 0; a0 < D / 32; a0 += 2) {
+                    v4f x[2][4];
+#pragma unroll
+                    for (int a = a0; a < a0 + 2; ++a)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[a - a0][i] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, (r0 * (uint32_t)D + (uint32_t)(4 * (8 * a + 4 * lh + i))) * 4u, 0, kSplitAux));
+#pragma unroll
+                    for (int a = a0; a < a0 + 2; ++a)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                const int dt = (b * NB + 8 * a) / 32, r = 4 * ((b * NB / 8 + a) % 4) + i;
+                                acc[dt][r] = alpha * acc[dt][r] + w * x[a - a0][i][b];
+                            }
+                    asm volatile("" ::: "memory");         // (these before the next ones are requested: room for all of a row is not there)
+                }
+            }
+        }
+    }
+    if (done && row < p->rows) {
+        const bool empty = m == -INFINITY || token >= t.m;
+        const float inv = empty ? 0.f : weight / l;
+        const int head = t.hk * p->group + row - token * p->group;
+        char* const dst = p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + 32 * lh;
+#pragma unroll
+        for (int a = 0; a < D / 32; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v4f x = value(a, i) * inv;
+                if (token >= t.m) x = (v4f){0.f, 0.f, 0.f, 0.f};
+                store_out4<DT>(dst + 64 * a + 8 * i, x);
+            }
+        if (p->lse != nullptr && lh == 0)
+            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = empty ? -INFINITY : m + __builtin_log2f(l) - kPrefillShift;
+    }
+    if (!paged_next(p, R, t, piece)) break;
+    __syncthreads();
+  }
+}
+
+template <int D> int launch_paged_prefill(const PagedParams& p, const PagedSel& sel, hipStream_t stream) {
+    const dim3 grid((unsigned)p.grid), threads(PrefillShape<D>::THREADS);
+    const bool rest = p.rope.freqs != nullptr;
+#define INTFA_CALL(DT, REST, ONE) hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, ONE>), grid, threads, 0, stream, p)
+#define INTFA_CALL_DT(DT) do { \
+        if (rest) { if (sel.one_page) INTFA_CALL(DT, true, true); else INTFA_CALL(DT, true, false); } \
+        else { if (sel.one_page) INTFA_CALL(DT, false, true); else INTFA_CALL(DT, false, false); } } while (0)
+    if (sel.io_dt == 0) INTFA_CALL_DT(0); else INTFA_CALL_DT(1);
+#undef INTFA_CALL_DT
+#undef INTFA_CALL
+    return (int)hipGetLastError();
+}
+
+}  // namespace intfa
