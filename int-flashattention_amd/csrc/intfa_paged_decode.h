@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         queries.turn_angles(p, t, (v2f*)o_lds);
         __syncthreads();
     }
-    queries.stage(p, row0, (const v2f*)o_lds, q_lds, q_rest, factor_lds);
+    queries.template stage<true>(p, row0, (const v2f*)o_lds, q_lds, q_rest, factor_lds);
     if (!part.whole) paged_open_ticket(p, paged_ticket(p, t), ticket_seen);
     __syncthreads();
     const char* const q_lane = q_lds + x * Queries::ROW + 32 * c;

@@ -208,8 +208,8 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
     // To LDS as fp16 with a power of two of the row's own taken out (`factor` gets it back, with the softmax's scale in base 2): the row's largest element
     // is brought to 2^8, so that neither the range of bf16 nor a rotation leaves fp16's, and what lies under fp16's smallest step is 2^-32 of it.
     // 16-bit queries are held exactly that way; rotated ones are not 16-bit numbers, and what their rounding leaves goes to q_rest for a second product
-    // (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).
-    __device__ __forceinline__ void stage(PagedArgs p, int row0, const v2f* angles, char* q_lds, char* q_rest, float* factor) const {
+    // (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).  Without REST they stay rounded to 11 bits.
+    template <bool REST> __device__ __forceinline__ void stage(PagedArgs p, int row0, const v2f* angles, char* q_lds, char* q_rest, float* factor) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int i = (int)threadIdx.x + k * THREADS, r = i / U, u = i % U;
@@ -251,7 +251,7 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
                 h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){y[2 * j] * down, y[2 * j + 1] * down}, v2h));
             *(v4i*)(q_lds + r * ROW + 2 * first) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
             *(v4i*)(q_lds + r * ROW + 2 * second) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
-            if (rope) {
+            if (REST && rope) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const v2f near = __builtin_convertvector(__builtin_bit_cast(v2h, h[j]), v2f);

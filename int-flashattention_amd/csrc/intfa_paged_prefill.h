@@ -34,7 +34,8 @@ template <int D> struct PrefillBytes {
     uint32_t v[PrefillShape<D>::UNITS][4];
 };
 
-// REST: rotated queries, whose scores take a second product (PagedQueries::stage).  ONE: a page holds a block's keys.
+// REST: rotated fp16 queries, whose scores take a second product (PagedQueries::stage).  Rotated bf16 queries stay rounded to 11 bits here, three more than
+// they came with: a second product costs a third more matrix work and the registers for it (chunk 145 -> 187 us).  ONE: a page holds a block's keys.
 template <int D, int DT, bool REST, bool ONE>
 __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS * PrefillShape<D>::WAVES / 4) paged_prefill_kernel(const PagedParams) {
     typedef PrefillShape<D> S;
@@ -62,11 +63,11 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
         Queries queries;
         queries.request(p, t, row0 + pass * S::PASS);
         if (pass > 0) __syncthreads();
-        if (REST) {
+        if (queries.rope) {
             queries.turn_angles(p, t, (v2f*)(lds + ANGLES_AT));
             __syncthreads();
         }
-        queries.stage(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
+        queries.template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
         __syncthreads();
         if (32 * wave / S::PASS == pass) {
             const char* const mine = lds + (32 * wave % S::PASS + lq) * Queries::ROW + 16 * lh;
@@ -88,25 +89,28 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     const int k_sn = p->k_sn, v_sn = p->v_sn, page_log2 = p->page_log2, num_pages = p->num_pages, last_column = p->table_width - 1;
     const int page_mask = (1 << page_log2) - 1, most = part.key_end;
     auto column = [&](int key) __attribute__((always_inline)) { const int c = key >> page_log2; return c < last_column ? c : last_column; };
-    // (the pages of a thread's own keys, where a block has several)
-    int k_id[UNITS], v_id[UNITS];
+    // Table entries are requested two blocks ahead of the bytes and the scales that they lead to.  Nothing here is conditional: behind the last block the
+    // last column's page is read again, so that the compiler can count what is under way.
+    int k_id[UNITS], v_id[UNITS];                          // of a thread's own keys, where a block has several pages
+    int s_id[ONE ? 1 : G];                                 // of the block's granules (scalars)
     auto look = [&](int key0) __attribute__((always_inline)) {
+        if (ONE) return;
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
             const int u = (int)threadIdx.x + i * THREADS;
-            if (ONE) {
-                if (i == 0) k_id[0] = table_s[column(key0)];
-            } else {
-                k_id[i] = table[column(key0 + u / (D / 16))];
-                v_id[i] = table[column(key0 + 4 * (u / NB))];
-            }
+            k_id[i] = table[column(key0 + u / (D / 16))];
+            v_id[i] = table[column(key0 + 4 * (u / NB))];
         }
     };
-    auto fetch = [&](int key0, PrefillBytes<D>& b) __attribute__((always_inline)) {
+    auto look_scalar = [&](int key0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < (ONE ? 1 : G); ++g) s_id[g] = table_s[column(key0 + 16 * g)];
+    };
+    auto fetch = [&](int key0, int one_id, PrefillBytes<D>& b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
             const int u = (int)threadIdx.x + i * THREADS, kk = u / (D / 16), vk = 4 * (u / NB);
-            const int kid = ONE ? k_id[0] : k_id[i], vid = ONE ? k_id[0] : v_id[i];
+            const int kid = ONE ? one_id : k_id[i], vid = ONE ? one_id : v_id[i];
             const char* const kp = k_head + ((unsigned)kid < (unsigned)num_pages ? kid : 0) * k_sp + (ONE ? (key0 & page_mask) * k_sn : 0);
             const char* const vp = v_head + ((unsigned)vid < (unsigned)num_pages ? vid : 0) * v_sp + (ONE ? (key0 & page_mask) * v_sn : 0);
             b.k[i] = *(const v4i*)(kp + (uint32_t)((ONE ? kk : (key0 + kk) & page_mask) * k_sn + 16 * (u % (D / 16))));
@@ -133,19 +137,18 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
             static_for<4>(quad);
         }
     };
-    // scales of a block, and whether the table names its pages (scalars)
+    // scales of a block, and whether the table names its pages (scalars, by the entries in s_id)
     struct Scales { float k[G], v[G]; bool has[G]; };
     auto scales_of = [&](int key0, Scales& s) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            const int id = s_id[ONE ? 0 : g];
+            s.has[g] = (unsigned)id < (unsigned)num_pages && key0 + 16 * g < most;
             if (ONE && g > 0) {
                 s.k[g] = s.k[0]; s.v[g] = s.v[0];
-                s.has[g] = s.has[0] && key0 + 16 * g < most;
                 continue;
             }
-            const int id = table_s[column(key0 + 16 * g)];
-            s.has[g] = (unsigned)id < (unsigned)num_pages && key0 + 16 * g < most;
-            const int at = s.has[g] ? id : 0;
+            const int at = (unsigned)id < (unsigned)num_pages ? id : 0;
             s.k[g] = k_scale[at * ks_sp];
             s.v[g] = v_scale[at * vs_sp];
         }
@@ -160,13 +163,17 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     int key0 = part.key_first;
     PrefillBytes<D> even, odd;
     Scales scales;
+    int id_next = 0;                                       // (ONE) the page of the block behind the next one
     if (key0 < most) {
+        look_scalar(key0);
         look(key0);
-        fetch(key0, even);
-        look(key0 + 64);
-        if (key0 + 64 < most) fetch(key0 + 64, odd);
-        look(key0 + 128);
+        fetch(key0, s_id[0], even);
         scales_of(key0, scales);
+        look_scalar(key0 + 64);
+        look(key0 + 64);
+        fetch(key0 + 64, s_id[0], odd);
+        look(key0 + 128);
+        if (ONE) id_next = table_s[column(key0 + 128)];
     }
     if (!part.whole) paged_open_ticket(p, paged_ticket(p, t), ticket_seen);
     __syncthreads();                                       // (the queries have been read)
@@ -174,23 +181,36 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     __syncthreads();
     auto block = [&](const char* now, char* then, PrefillBytes<D>& next, PrefillBytes<D>& after) __attribute__((always_inline)) {
         // `next` holds the bytes of the block behind this one, `after` takes those of the one behind that
-        if (key0 + 128 < most) fetch(key0 + 128, after);
-        look(key0 + 192);
-        if (key0 + 64 < most) store(next, then);
+        fetch(key0 + 128, id_next, after);
         const Scales sc = scales;
         scales_of(key0 + 64, scales);
+        if (ONE) s_id[0] = id_next;
+        else look_scalar(key0 + 128);
+        look(key0 + 192);
+        if (ONE) id_next = table_s[column(key0 + 192)];
+        store(next, then);
+        // The matrix pipe waits for no LDS read: four fragments are under way while the products of four others run.
         v16f s[2];
+        v8h kf[2][4];
+        const char* const kl = now + lq * S::K_ROW + 16 * lh;
+        auto read_k = [&](int quad, v8h (&f)[4]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+            for (int i = 0; i < 4; ++i) f[i] = *(const v8h*)(kl + 32 * (quad / (KS / 4)) * S::K_ROW + 32 * (4 * (quad % (KS / 4)) + i));
+        };
+        read_k(0, kf[0]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[half][r] = 0.f;
-            const char* const kl = now + (32 * half + lq) * S::K_ROW + 16 * lh;
+        for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const v8h kf = *(const v8h*)(kl + 32 * ks);
-                s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[ks], s[half], 0, 0, 0);
-                if (REST) s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q_rest[REST ? ks : 0], s[half], 0, 0, 0);
+        for (int quad = 0; quad < KS / 2; ++quad) {
+            if (quad + 1 < KS / 2) read_k(quad + 1, kf[(quad + 1) % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int half = quad / (KS / 4), ks = 4 * (quad % (KS / 4)) + i;
+                s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[quad % 2][i], q[ks], s[half], 0, 0, 0);
+                if (REST) s[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[quad % 2][i], q_rest[REST ? ks : 0], s[half], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         // ---- hidden keys
         bool masked = key0 + 64 > least;
@@ -260,11 +280,20 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
         l = fmaf(sum, v_back, l);
         // ---- O^T += V^T P^T
         if (v_top > 0.f) {
+            v8h vf[2][4];
+            const char* const vl = now + S::K_BYTES + lq * S::V_ROW + 16 * lh;
+            auto read_v = [&](int dt, v8h (&f)[4]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) f[g] = *(const v8h*)(vl + 32 * dt * S::V_ROW + 32 * g);
+            };
+            read_v(0, vf[0]);
 #pragma unroll
             for (int dt = 0; dt < DTILES; ++dt) {
-                const char* const vl = now + S::K_BYTES + (32 * dt + lq) * S::V_ROW + 16 * lh;
+                if (dt + 1 < DTILES) read_v(dt + 1, vf[(dt + 1) % 2]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const v8h*)(vl + 32 * g), pf[g], acc[dt], 0, 0, 0);
+                for (int g = 0; g < 4; ++g) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[dt % 2][g], pf[g], acc[dt], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         key0 += 64;
@@ -359,13 +388,10 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 
 template <int D> int launch_paged_prefill(const PagedParams& p, const PagedSel& sel, hipStream_t stream) {
     const dim3 grid((unsigned)p.grid), threads(PrefillShape<D>::THREADS);
-    const bool rest = p.rope.freqs != nullptr;
-#define INTFA_CALL(DT, REST, ONE) hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, ONE>), grid, threads, 0, stream, p)
-#define INTFA_CALL_DT(DT) do { \
-        if (rest) { if (sel.one_page) INTFA_CALL(DT, true, true); else INTFA_CALL(DT, true, false); } \
-        else { if (sel.one_page) INTFA_CALL(DT, false, true); else INTFA_CALL(DT, false, false); } } while (0)
-    if (sel.io_dt == 0) INTFA_CALL_DT(0); else INTFA_CALL_DT(1);
-#undef INTFA_CALL_DT
+#define INTFA_CALL(DT, REST) do { \
+        if (sel.one_page) hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, true>), grid, threads, 0, stream, p); \
+        else hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, false>), grid, threads, 0, stream, p); } while (0)
+    if (sel.io_dt == 1) INTFA_CALL(1, false); else if (p.rope.freqs != nullptr) INTFA_CALL(0, true); else INTFA_CALL(0, false);
 #undef INTFA_CALL
     return (int)hipGetLastError();
 }

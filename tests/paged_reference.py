@@ -90,11 +90,13 @@ def attend(q, cache, table, lens, causal, sm, fresh=None, rope=None):
     return out, lse, mean_v, size
 
 
-def bound(out, mean_v, size, dtype):
+def bound(out, mean_v, size, dtype, query_step=0.0):
     """How far the kernel may be from the above: half a step of the output's type; P rounded to 11 bits (half a step, 2^-11 of each weight, so at
     most 2^-11 of the mean of |v|); scores off by dS move a weight by dS and their sum as much: the products of a score are summed in
-    fp32 in at most 13 roundings, scaled and exponentiated in a few more, 2^-19 of the sum of |q k| in all; sums over keys 2^-14."""
-    return torch.finfo(dtype).eps / 2 * out.abs() + 1.05 * (2.0 ** -11 + 2.0 ** -14 + 2.0 * 2.0 ** -19 * size) * mean_v + 2.0 ** -24
+    fp32 in at most 13 roundings, scaled and exponentiated in a few more, 2^-19 of the sum of |q k| in all; sums over keys 2^-14.
+    query_step: where the queries are rounded after their rotation, half a step of theirs, which moves a score by as much of the sum of |q k| (each product
+    is off by at most half a step of its query's element): 2^-12 for the 11 bits that many rows of bf16 queries are held to."""
+    return torch.finfo(dtype).eps / 2 * out.abs() + 1.05 * (2.0 ** -11 + 2.0 ** -14 + 2.0 * (2.0 ** -19 + query_step) * size) * mean_v + 2.0 ** -24
 
 
 def make_cache(g, pages, Hkv, page, d, spread=0.0):

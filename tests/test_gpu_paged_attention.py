@@ -23,12 +23,14 @@ def run(q, cache, kv, sc, table, lens, causal, sm=None, fresh=None, freqs=None, 
     want, want_lse, mean_v, size = attend(q, cache, table, lens, causal, sm, fresh, rope)
     o, lse = o.cpu(), lse.cpu()
     assert o.isfinite().all()
-    far = (o.double() - want).abs() - bound(want, mean_v, size, q.dtype)
+    # rotated bf16 queries of more than 32 rows a K/V head are held to 11 bits
+    step = 2.0 ** -12 if freqs is not None and q.dtype == torch.bfloat16 and q.shape[1] // kv.shape[2] * q.shape[2] > 32 else 0.0
+    far = (o.double() - want).abs() - bound(want, mean_v, size, q.dtype, step)
     assert (far <= 0).all(), f"{far.max().item():.3g} past the bound"
     empty = want_lse == -float("inf")
     assert torch.equal(lse == -float("inf"), empty) and (o[empty] == 0).all()
     # lse: the scores' error and the sum's, in base 2
-    assert ((lse.double() - want_lse)[~empty].abs() <= (2.0 ** -12 + 2.0 * 2.0 ** -19 * size[..., 0] + 2.0 ** -23 * want_lse.abs())[~empty]).all()
+    assert ((lse.double() - want_lse)[~empty].abs() <= (2.0 ** -12 + 2.0 * (2.0 ** -19 + step) * size[..., 0] + 2.0 ** -23 * want_lse.abs())[~empty]).all()
     return o
 
 

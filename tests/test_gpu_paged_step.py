@@ -52,14 +52,15 @@ def test_prompts_then_steps(dtype, page, d):
         pool.append(k, v, fresh)
         o = pool.attend(q, fresh)
         want, _, mean_v, size = pool.want(q, fresh)
-        assert ((o.cpu().double() - want).abs() <= bound(want, mean_v, size, dtype)).all()
+        step = 2.0 ** -12 if dtype == torch.bfloat16 and H // Hkv * N > 32 else 0.0      # (many rows of bf16 queries: 11 bits)
+        assert ((o.cpu().double() - want).abs() <= bound(want, mean_v, size, dtype, step)).all()
         counts = [N] * Z if fresh is None else fresh.tolist()
         keys.append((k.cpu(), counts)); values.append((v.cpu(), counts))
         # the rotation as a call of its own: its rounding to the queries' type is all the difference
         first = pool.lens - (N if fresh is None else fresh)
         alone = pool.attend(M.rotary(q, first, pool.rope["freqs"]), fresh, rope=False)
         eps = torch.finfo(dtype).eps
-        assert ((alone.double() - o.double()).abs().cpu() <= 2 * bound(want, mean_v, size, dtype) + 2 * eps / 2 * size * mean_v).all()
+        assert ((alone.double() - o.double()).abs().cpu() <= 2 * bound(want, mean_v, size, dtype, step) + 2 * eps / 2 * size * mean_v).all()
         return q, o
 
     call(70, torch.tensor([70, 33, 1], dtype=torch.int32, device=DEV))
