@@ -59,15 +59,17 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     // ---- queries: through LDS into the waves that own them
     v8h q[KS], q_rest[REST ? KS : 1];
     float factor = 0.f;
+    Queries queries[R / S::PASS];
+#pragma unroll
+    for (int pass = 0; pass < R / S::PASS; ++pass) queries[pass].request(p, t, row0 + pass * S::PASS);
+#pragma unroll
     for (int pass = 0; pass < R / S::PASS; ++pass) {
-        Queries queries;
-        queries.request(p, t, row0 + pass * S::PASS);
         if (pass > 0) __syncthreads();
-        if (queries.rope) {
-            queries.turn_angles(p, t, (v2f*)(lds + ANGLES_AT));
+        if (queries[pass].rope) {
+            queries[pass].turn_angles(p, t, (v2f*)(lds + ANGLES_AT));
             __syncthreads();
         }
-        queries.template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
+        queries[pass].template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
         __syncthreads();
         if (32 * wave / S::PASS == pass) {
             const char* const mine = lds + (32 * wave % S::PASS + lq) * Queries::ROW + 16 * lh;
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
         for (int a = 0; a < D / 32; ++a)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mine.put((uint32_t)(32 * wave + lq), D, 4 * (8 * a + 4 * lh + i), value(a, i) * v_unit);
+            for (int i = 0; i < 4; ++i) mine.put((uint32_t)(32 * wave), D, 4 * (64 * (4 * a + i) + lane), value(a, i) * v_unit);      // (a wave's stores: 1 KB each)
         if (lh == 0) mine.put_stats((uint32_t)(32 * wave + lq), m, l);
         if (paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, part.pieces)) {
             // the pieces in their order, each wave its own rows in its own layout
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
                     for (int a = a0; a < a0 + 2; ++a)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            x[a - a0][i] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, (r0 * (uint32_t)D + (uint32_t)(4 * (8 * a + 4 * lh + i))) * 4u, 0, kSplitAux));
+                            x[a - a0][i] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(o, ((uint32_t)(32 * wave * D) + 4u * (uint32_t)(64 * (4 * a + i) + lane)) * 4u, 0, kSplitAux));
 #pragma unroll
                     for (int a = a0; a < a0 + 2; ++a)
 #pragma unroll
