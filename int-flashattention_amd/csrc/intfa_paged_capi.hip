@@ -80,7 +80,7 @@ int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream) {
     kp.part_stats = (float*)((char*)p->workspace + a.stats_at);
     kp.ticket = (uint64_t*)((char*)p->workspace + a.tickets_at);
     kp.epoch = next_epoch() << 8;
-    kp.d_group = make_fast_div(kp.group); kp.d_tiles = make_fast_div(kp.tiles); kp.d_heads_kv = make_fast_div(kp.heads_kv);
+    kp.d_group = make_fast_div(kp.group); kp.d_tiles = make_fast_div(kp.tiles); kp.d_pairs = make_fast_div(kp.rope.freqs != nullptr ? kp.rope.pairs : 1);
     const PagedSel& sel = a.sel;
     hipStream_t st = (hipStream_t)stream;
     if (sel.row_tiles == 0)

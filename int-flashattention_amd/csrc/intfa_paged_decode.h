@@ -177,9 +177,13 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
     static_assert(R * (D / 2) * 8 <= W * 16 * O_ROW * 4 && THREADS * 6 <= W * 16 * O_ROW, "the angles lie there first, and a merge's sums last");
     __shared__ float m_lds[W * R], l_lds[W * R];
     __shared__ uint32_t arrival_lds;
+    __shared__ double freq_lds[D / 2];
     PagedArgs p = paged_args_first();
     PagedItem t;
+    const double freq = paged_frequency(p);
     PagedPiece piece = paged_find(p, R, t);
+    if ((int)threadIdx.x < D / 2) freq_lds[threadIdx.x] = freq;
+    __syncthreads();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), x = lane & 15, c = lane >> 4;
   while (piece.start < piece.end) {
     const int row0 = t.tile * R;
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         for (int j = 0; j < DT16; ++j) o[rt][j] = (v4f){0.f, 0.f, 0.f, 0.f};
     }
     if (rope) {
-        queries.turn_angles(p, t, (v2f*)o_lds);
+        queries.turn_angles(p, t, freq_lds, (v2f*)o_lds);
         __syncthreads();
     }
     queries.template stage<true>(p, row0, (const v2f*)o_lds, q_lds, q_rest, factor_lds);

@@ -163,12 +163,16 @@ __device__ __forceinline__ int paged_token_keys(PagedArgs p, const PagedItem& t,
     return !p->causal || seen > t.n ? t.n : seen < 0 ? 0 : seen;
 }
 
+// The frequencies to LDS, once per workgroup: requested at the kernel's start, stored when its own place in the line is known.
+__device__ __forceinline__ double paged_frequency(PagedArgs p) {
+    return p->rope.freqs != nullptr && (int)threadIdx.x < p->rope.pairs ? p->rope.freqs[threadIdx.x] : 0.0;
+}
+
 // The rows of a tile on their way to LDS: requested first, ahead of the cache's (loads come back in order), then turned and stored.  A row is D / 16
 // units of sixteen elements, a lane each.
 template <int D, int DT, int R, int THREADS> struct PagedQueries {
     static constexpr int U = D / 16, N = (R * U + THREADS - 1) / THREADS, ROW = 2 * D + 16;      // ROW: bytes in LDS (16 more: sixteen rows in sixteen banks)
     v4i x[N][2];
-    double freq;
     int first_token, tokens;
     bool rope, interleaved;
     int pairs;
@@ -179,8 +183,6 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
         const int row_last = row0 + R < p->rows ? row0 + R - 1 : p->rows - 1;
         first_token = paged_div(row0 < p->rows ? row0 : p->rows - 1, p->d_group);
         tokens = paged_div(row_last, p->d_group) - first_token + 1;
-        freq = 0.0;
-        if ((int)threadIdx.x < pairs) freq = p->rope.freqs[threadIdx.x];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int i = (int)threadIdx.x + k * THREADS, r = i / U, u = i % U, row = row0 + r, token = paged_div(row, p->d_group);
@@ -194,14 +196,15 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
             }
         }
     }
-    // The angles of the tile's tokens, each once: angles[token * pairs + pair] = (cos, sin).  Threads beyond the pairs take further tokens.
-    __device__ __forceinline__ void turn_angles(PagedArgs p, const PagedItem& t, v2f* angles) const {
+    // The angles of the tile's tokens, each once: angles[token * pairs + pair] = (cos, sin).  freqs: a copy in LDS (from memory each further token's
+    // frequency was a trip of its own: 3 us a pass of 64 rows).
+    __device__ __forceinline__ void turn_angles(PagedArgs p, const PagedItem& t, const double* freqs, v2f* angles) const {
         const float magnitude = p->rope.magnitude;
         const int position = t.n - t.m + first_token;
         for (int i = threadIdx.x; i < tokens * pairs; i += THREADS) {
-            const int token = i / pairs, pair = i - token * pairs;
+            const int token = paged_div(i, p->d_pairs), pair = i - token * pairs;
             float c, s;
-            rope_angle(pair == (int)threadIdx.x ? freq : p->rope.freqs[pair], position + token, magnitude, c, s);
+            rope_angle(freqs[pair], position + token, magnitude, c, s);
             angles[i] = (v2f){c, s};
         }
     }

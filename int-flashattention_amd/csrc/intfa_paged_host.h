@@ -44,7 +44,7 @@ struct PagedParams {
     RopeArgs rope;
     float* parts; float* part_stats;                 // partial results: two slots per workgroup (intfa_paged_decode.h)
     uint64_t* ticket; uint64_t epoch;
-    FastDiv d_group, d_tiles, d_heads_kv;
+    FastDiv d_group, d_tiles, d_pairs;
 };
 
 struct PagedSel { int head_dim, io_dt, row_tiles; bool one_page; };      // row_tiles: of 16 rows, 0 for the prefill kernel; one_page: a page holds the keys that are taken at a time

@@ -46,9 +46,13 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     __shared__ __align__(16) char lds[2 * S::BLOCK];
     __shared__ float factor_lds[S::PASS];
     __shared__ uint32_t arrival_lds;
+    __shared__ double freq_lds[D / 2];
     PagedArgs p = paged_args_first();
     PagedItem t;
+    const double freq = paged_frequency(p);
     PagedPiece piece = paged_find(p, R, t);
+    if ((int)threadIdx.x < D / 2) freq_lds[threadIdx.x] = freq;
+    __syncthreads();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lq = lane & 31, lh = lane >> 5;
   while (piece.start < piece.end) {
     const PagedPart part = paged_part(p, t, piece);
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     for (int pass = 0; pass < R / S::PASS; ++pass) {
         if (pass > 0) __syncthreads();
         if (queries[pass].rope) {
-            queries[pass].turn_angles(p, t, (v2f*)(lds + ANGLES_AT));
+            queries[pass].turn_angles(p, t, freq_lds, (v2f*)(lds + ANGLES_AT));
             __syncthreads();
         }
         queries[pass].template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
@@ -219,13 +223,16 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
         for (int g = 0; g < G; ++g) masked = masked || !sc.has[g];
         if (masked) {
+            const int last = seen - key0 - 4 * lh;           // of the lane's keys: 16 g + 8 j + i is hidden from here on
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int g = 0; g < G; ++g) {
+                const int end = sc.has[g] ? last : 0;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = key0 + 32 * half + 8 * (r / 4) + 4 * lh + r % 4;
-                    s[half][r] = key < seen && sc.has[2 * half + r / 8] ? s[half][r] : -INFINITY;
+                for (int r = 0; r < 8; ++r) {
+                    const int e = 8 * (g % 2) + r;
+                    s[g / 2][e] = 16 * g + 8 * (r / 4) + r % 4 < end ? s[g / 2][e] : -INFINITY;
                 }
+            }
         }
         // ---- V's unit: the page's scale, or the largest of the block's
         float v_top = sc.has[0] ? sc.v[0] : 0.f;
@@ -242,7 +249,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[dt][r] *= scale;
         }
-        const float v_ratio = v_top > 0.f ? v_top / v_unit : 1.f, v_log = __builtin_amdgcn_logf(v_ratio), v_back = 1.f / v_ratio;
+        const float v_ratio = v_top > 0.f ? v_top * __builtin_amdgcn_rcpf(v_unit) : 1.f, v_log = __builtin_amdgcn_logf(v_ratio), v_back = __builtin_amdgcn_rcpf(v_ratio);
         // ---- softmax
         float f[G];
 #pragma unroll
@@ -270,7 +277,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
         v8h pf[4];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const float rel = ONE || v_top <= 0.f ? 1.f : (sc.has[g] ? sc.v[g] : 0.f) / v_top;
+            const float rel = ONE || v_top <= 0.f ? 1.f : (sc.has[g] ? sc.v[g] : 0.f) * __builtin_amdgcn_rcpf(v_top);
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 float e = fast_exp2(fmaf(s[g / 2][8 * (g % 2) + r], f[g], -frame));
