@@ -68,29 +68,44 @@ struct PagedAppendParams {
     const int32_t* table; int64_t bt_sb;
     const int32_t* seqlens_k; const int32_t* seqlens_new;
     RopeArgs rope;
-    int32_t heads, seqlen_new, page_log2, num_pages, table_width, units, slots;      // slots: pages that a sequence may reach
-    FastDiv d_slots, d_heads;
+    int32_t heads, seqlen_new, page_log2, num_pages, table_width, units;      // units: of sixteen elements per row
+    int32_t slots, head_groups, heads_each;      // pages that a sequence may reach; groups of heads_each heads
+    FastDiv d_slots, d_head_groups;
 };
 
 constexpr float kLeastScale = 0x1p-100f;
-constexpr int kAppendThreads = 256;
 
 __device__ __forceinline__ float finite_magnitude(float x) {
     const float a = fabsf(x);
     return a <= 3.402823466e38f ? a : 0.f;      // (false for NaN too)
 }
-// rint(x / scale) within +-127, 0 for NaN.  The quotient is the correctly rounded one (the scale is at least 2^-100, and not infinite
-// unless the cache held such a scale: then everything is 0).
+// rint(x / scale) within +-127, 0 for NaN, as a byte
 __device__ __forceinline__ uint32_t quantise(float x, float scale) {
     const float q = rintf(x / scale);
     return (uint32_t)(q >= 127.f ? 127 : q <= -127.f ? -127 : q == q ? (int)q : 0) & 0xffu;
 }
+// Four of them for finite x with |x| <= 127 scale (to rounding).  The quotient is the correctly rounded one, by Markstein's correction of the product with
+// the reciprocal (short of divisors whose significand is all ones, where it may be its neighbour); adding 1.5 * 2^23 rounds it to an integer
+// in the low byte.  NaN gives 0: its low byte is.
+__device__ __forceinline__ uint32_t quantise4(const float* x, float scale, float reciprocal) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = x[i] * reciprocal, e = __builtin_fmaf(-q, scale, x[i]);
+        b[i] = __builtin_bit_cast(uint32_t, __builtin_fmaf(e, reciprocal, q) + 12582912.0f);
+    }
+    return __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+}
 
-// One workgroup per page slot of a sequence, head, and K or V.
-template <int DT> __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const PagedAppendParams p) {
-    __shared__ float red[kAppendThreads / 64];
-    const int zh = fast_div((int)blockIdx.x, p.d_slots), slot = (int)blockIdx.x - zh * p.slots;
-    const int z = fast_div(zh, p.d_heads), h = zh - z * p.heads;
+// One workgroup per page slot of a sequence, K or V, and group of heads.  A page's scale needs all its new rows before the first is stored: a thread holds up
+// to HELD units of sixteen elements in registers in between (rows past that are read and turned a second time), and turns the same rows of all its
+// heads by the same angles, which take longer to form than all the rest.  The next head's rows are requested ahead of this one's work.
+// WAVES = 1, for few new rows: no wave waits for another.
+template <int DT, int WAVES, int HELD> __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendParams p) {
+    constexpr int THREADS = 64 * WAVES;
+    __shared__ float red[2][WAVES];
+    const int group = (int)blockIdx.x - fast_div((int)blockIdx.x, p.d_head_groups) * p.head_groups, zs = fast_div((int)blockIdx.x, p.d_head_groups);
+    const int z = fast_div(zs, p.d_slots), slot = zs - z * p.slots;
     const bool is_v = blockIdx.y != 0;
     const PagedSide& side = is_v ? p.v : p.k;
     const int page = 1 << p.page_log2;
@@ -108,64 +123,147 @@ template <int DT> __global__ void __launch_bounds__(kAppendThreads) paged_append
     const int row1 = past < page ? (int)past : page;
     if (row1 <= row0) return;
     const int id = p.table[z * p.bt_sb + column];
-    if ((unsigned)id >= (unsigned)p.num_pages) return;
-    const char* const src = side.src + z * side.n_sb + h * side.n_sh + (start + row0 - held) * side.n_sn;
-    char* const dst = side.cache + id * side.c_sp + h * side.c_sh;
-    float* const scale_at = side.scale + id * side.s_sp + h * side.s_sh;
+    const int h0 = group * p.heads_each, h1 = h0 + p.heads_each < p.heads ? h0 + p.heads_each : p.heads;
+    const char* const src0 = side.src + z * side.n_sb + (start + row0 - held) * side.n_sn;
     const bool rope = !is_v && p.rope.freqs != nullptr, interleaved = p.rope.interleaved != 0;
-    const int pairs = rope ? p.rope.pairs : 0, units = (row1 - row0) * p.units;
-    auto load = [&](int i, float (&x)[16], int& row, int& first, int& second) __attribute__((always_inline)) {
-        row = i / p.units;
-        const int u = i - row * p.units;
-        rope_unit(u, pairs, interleaved, first, second);
-        unpack8<DT>(*(const v4i*)(src + row * side.n_sn + 2 * first), x);
-        unpack8<DT>(*(const v4i*)(src + row * side.n_sn + 2 * second), x + 8);
-        if (8 * u < pairs) {
-            float c[8], s[8];
+    const int pairs = rope ? p.rope.pairs : 0, units = (row1 - row0) * p.units, units_log2 = __builtin_ctz(p.units);
+    // the thread's units: their rows, places and angles
+    int row[HELD], first[HELD], second[HELD];
+    v4i raw[HELD][2];
+    auto request = [&](int h) __attribute__((always_inline)) {
+        const char* const src = src0 + h * side.n_sh;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rope_angle(p.rope.freqs[8 * u + j], (int)(start + row0 + row), p.rope.magnitude, c[j], s[j]);
-            rope_turn_unit(x, c, s, interleaved);
+        for (int k = 0; k < HELD; ++k) {
+            raw[k][0] = raw[k][1] = (v4i){0, 0, 0, 0};
+            if ((int)threadIdx.x + k * THREADS < units) {
+                raw[k][0] = __builtin_nontemporal_load((const v4i*)(src + row[k] * side.n_sn + 2 * first[k]));
+                raw[k][1] = __builtin_nontemporal_load((const v4i*)(src + row[k] * side.n_sn + 2 * second[k]));
+            }
         }
     };
-    float top = 0.f;
-    for (int i = threadIdx.x; i < units; i += kAppendThreads) {
-        float x[16];
-        int row, first, second;
-        load(i, x, row, first, second);
+    float c[HELD][8], s[HELD][8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+    for (int k = 0; k < HELD; ++k) {
+        const int i = (int)threadIdx.x + k * THREADS;
+        row[k] = i >> units_log2;
+        rope_unit(i & (p.units - 1), pairs, interleaved, first[k], second[k]);
     }
-    for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    const float before = row0 > 0 ? *scale_at : 0.f;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float scale = fmaxf(fmaxf(top / 127.0f, kLeastScale), before);
-    if (scale != before) {
-        const float ratio = before / scale;
-        const int words = row0 * p.units * 4;
-        for (int i = threadIdx.x; i < words; i += kAppendThreads) {
-            const int row = i / (p.units * 4);
-            uint32_t* const at = (uint32_t*)(dst + row * side.c_sn) + (i - row * p.units * 4);
-            const uint32_t w = *at;
-            uint32_t r = 0;
+    request(h0);
+    if ((unsigned)id >= (unsigned)p.num_pages) return;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r |= ((uint32_t)(int)rintf((float)(int8_t)(w >> (8 * j)) * ratio) & 0xffu) << (8 * j);
-            *at = r;
+    for (int k = 0; k < HELD; ++k) {
+        const int i = (int)threadIdx.x + k * THREADS, u = i & (p.units - 1);
+        if (8 * u < pairs && i < units) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rope_angle(p.rope.freqs[8 * u + j], (int)(start + row0 + row[k]), p.rope.magnitude, c[k][j], s[k][j]);
         }
     }
-    for (int i = threadIdx.x; i < units; i += kAppendThreads) {
-        float x[16];
-        int row, first, second;
-        load(i, x, row, first, second);
-        uint32_t q[4];
+    // a unit past the held ones
+    auto read = [&](const char* src, int i, float (&x)[16], int& r, int& one, int& two) __attribute__((always_inline)) {
+        r = i >> units_log2;
+        const int u = i & (p.units - 1);
+        rope_unit(u, pairs, interleaved, one, two);
+        unpack8<DT>(*(const v4i*)(src + r * side.n_sn + 2 * one), x);
+        unpack8<DT>(*(const v4i*)(src + r * side.n_sn + 2 * two), x + 8);
+        if (8 * u < pairs) {
+            float cc[8], ss[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            q[j] = quantise(x[4 * j], scale) | quantise(x[4 * j + 1], scale) << 8 | quantise(x[4 * j + 2], scale) << 16 | quantise(x[4 * j + 3], scale) << 24;
-        *(v2i*)(dst + (row0 + row) * side.c_sn + first) = (v2i){(int)q[0], (int)q[1]};
-        *(v2i*)(dst + (row0 + row) * side.c_sn + second) = (v2i){(int)q[2], (int)q[3]};
+            for (int j = 0; j < 8; ++j) rope_angle(p.rope.freqs[8 * u + j], (int)(start + row0 + r), p.rope.magnitude, cc[j], ss[j]);
+            rope_turn_unit(x, cc, ss, interleaved);
+        }
+    };
+    for (int h = h0; h < h1; ++h) {
+        const char* const src = src0 + h * side.n_sh;
+        char* const dst = side.cache + id * side.c_sp + h * side.c_sh;
+        float* const scale_at = side.scale + id * side.s_sp + h * side.s_sh;
+        const float before = row0 > 0 ? *scale_at : 0.f;
+        float x[HELD][16], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+            unpack8<DT>(raw[k][0], x[k]);
+            unpack8<DT>(raw[k][1], x[k] + 8);
+            if (8 * (((int)threadIdx.x + k * THREADS) & (p.units - 1)) < pairs && (int)threadIdx.x + k * THREADS < units) rope_turn_unit(x[k], c[k], s[k], interleaved);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[k][j]));      // (no NaN gets through)
+        }
+        if (h + 1 < h1) request(h + 1);
+        for (int i = (int)threadIdx.x + HELD * THREADS; i < units; i += THREADS) {
+            float y[16];
+            int r, one, two;
+            read(src, i, y, r, one, two);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(y[j]));
+        }
+        auto of_all = [&](float v) __attribute__((always_inline)) {
+            for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+            if (WAVES > 1) {
+                float* const r = red[h & 1];
+                if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) v = fmaxf(v, r[w]);
+            }
+            return v;
+        };
+        top = of_all(top);
+        const bool infinite = top > 3.402823466e38f;      // some value is: it does not count, and quotients need their bounds
+        if (infinite) {
+            top = 0.f;
+#pragma unroll
+            for (int k = 0; k < HELD; ++k)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_magnitude(x[k][j]));
+            for (int i = (int)threadIdx.x + HELD * THREADS; i < units; i += THREADS) {
+                float y[16];
+                int r, one, two;
+                read(src, i, y, r, one, two);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_magnitude(y[j]));
+            }
+            if (WAVES > 1) __syncthreads();
+            top = of_all(top);
+        }
+        const float scale = fmaxf(fmaxf(top / 127.0f, kLeastScale), before), reciprocal = 1.0f / scale;
+        if (scale != before) {
+            const float ratio = before / scale;
+            for (int i = threadIdx.x; i < row0 * p.units; i += THREADS) {
+                v4i* const at = (v4i*)(dst + (i >> units_log2) * side.c_sn + 16 * (i & (p.units - 1)));
+                v4i w = *at;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t r = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r |= ((uint32_t)(int)rintf((float)(int8_t)((uint32_t)w[k] >> (8 * j)) * ratio) & 0xffu) << (8 * j);
+                    w[k] = (int)r;
+                }
+                *at = w;
+            }
+        }
+        auto put = [&](const float (&y)[16], int r, int one, int two) __attribute__((always_inline)) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                q[j] = !infinite ? quantise4(y + 4 * j, scale, reciprocal)
+                                 : quantise(y[4 * j], scale) | quantise(y[4 * j + 1], scale) << 8 | quantise(y[4 * j + 2], scale) << 16 | quantise(y[4 * j + 3], scale) << 24;
+            char* const d = dst + (row0 + r) * side.c_sn;
+            if (two == one + 8) {
+                *(v4i*)(d + one) = (v4i){(int)q[0], (int)q[1], (int)q[2], (int)q[3]};
+            } else {
+                *(v2i*)(d + one) = (v2i){(int)q[0], (int)q[1]};
+                *(v2i*)(d + two) = (v2i){(int)q[2], (int)q[3]};
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+            if ((int)threadIdx.x + k * THREADS < units) put(x[k], row[k], first[k], second[k]);
+        for (int i = (int)threadIdx.x + HELD * THREADS; i < units; i += THREADS) {
+            float y[16];
+            int r, one, two;
+            read(src, i, y, r, one, two);
+            put(y, r, one, two);
+        }
+        if (threadIdx.x == 0) *scale_at = scale;      // (`before` has been read by every thread: what it decides comes after the barrier)
     }
-    if (threadIdx.x == 0) *scale_at = scale;      // (every thread read it ahead of the barrier)
 }
 
 bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
@@ -230,12 +328,21 @@ int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream) {
     ap.units = c.head_dim / 16;
     ap.slots = (p->seqlen_new + c.page_size - 2) / c.page_size + 1;
     ap.slots = ap.slots < c.table_width ? ap.slots : c.table_width;
-    const int64_t grid = (int64_t)p->batch * c.heads_kv * ap.slots;
-    if (grid >= 1ll << 31) return INTFA_ERR_SHAPE;
-    ap.d_slots = make_fast_div(ap.slots); ap.d_heads = make_fast_div(c.heads_kv);
-    const dim3 g((unsigned)grid, 2);
-    if (p->dtype == INTFA_F16) hipLaunchKernelGGL(paged_append_kernel<0>, g, dim3(kAppendThreads), 0, (hipStream_t)stream, ap);
-    else hipLaunchKernelGGL(paged_append_kernel<1>, g, dim3(kAppendThreads), 0, (hipStream_t)stream, ap);
+    // Heads per workgroup: as many as leave a few workgroups per compute unit
+    const int64_t pages = (int64_t)p->batch * ap.slots;
+    const int rows = p->seqlen_new < c.page_size ? p->seqlen_new : c.page_size, units = rows * ap.units;
+    ap.heads_each = 1;
+    while (ap.heads_each < 8 && ap.heads_each < c.heads_kv && pages * c.heads_kv >= 2ll * ap.heads_each * 2 * kComputeUnits) ap.heads_each *= 2;
+    ap.head_groups = (c.heads_kv + ap.heads_each - 1) / ap.heads_each;
+    if (pages * ap.head_groups >= 1ll << 31) return INTFA_ERR_SHAPE;
+    ap.d_slots = make_fast_div(ap.slots); ap.d_head_groups = make_fast_div(ap.head_groups);
+    const dim3 g((unsigned)(pages * ap.head_groups), 2);
+#define INTFA_CALL(DT) do { \
+        if (units <= 64) hipLaunchKernelGGL((paged_append_kernel<DT, 1, 1>), g, dim3(64), 0, (hipStream_t)stream, ap); \
+        else if (units <= 512) hipLaunchKernelGGL((paged_append_kernel<DT, 4, 2>), g, dim3(256), 0, (hipStream_t)stream, ap); \
+        else hipLaunchKernelGGL((paged_append_kernel<DT, 4, 4>), g, dim3(256), 0, (hipStream_t)stream, ap); } while (0)
+    if (p->dtype == INTFA_F16) INTFA_CALL(0); else INTFA_CALL(1);
+#undef INTFA_CALL
     return (int)hipGetLastError();
 }
 
