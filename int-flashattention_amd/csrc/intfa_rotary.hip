@@ -19,8 +19,11 @@ struct RotaryParams {
     float sign;
 };
 
-// A thread takes one unit of one token and turns it in heads_each heads by the same eight angles.
-template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+// A thread takes one unit of one token and turns it in heads_each heads by the same eight angles, kRotaryHeads of them under way at a time.  Bound by memory
+// once a thread has a few heads (an angle costs as much as a dozen turned pairs); each line is touched once, so loads and stores pass by the caches.
+constexpr int kRotaryHeads = 4;
+template <int DT, bool MANY> __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+    constexpr int N = MANY ? kRotaryHeads : 1;
     const int64_t lin = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (lin >= p.threads) return;
     const int token = fast_div((int)lin, p.d_units), u = (int)lin - token * p.units;
@@ -28,6 +31,19 @@ template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(const Rot
     int first, second;
     const bool turns = 8 * u < p.rope.pairs, interleaved = p.rope.interleaved != 0;
     rope_unit(u, p.rope.pairs, interleaved, first, second);
+    const int h0 = (int)blockIdx.y * p.heads_each, h1 = h0 + p.heads_each < p.heads ? h0 + p.heads_each : p.heads;
+    const char* const src = p.x + b * p.x_sb + n * p.x_sn;
+    char* const dst = p.out + b * p.o_sb + n * p.o_sn;
+    v4i raw[N][2];
+    auto request = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const char* const at = src + (h + k < h1 ? h + k : h1 - 1) * p.x_sh;
+            raw[k][0] = __builtin_nontemporal_load((const v4i*)(at + 2 * first));
+            raw[k][1] = __builtin_nontemporal_load((const v4i*)(at + 2 * second));
+        }
+    };
+    request(h0);
     float c[8], s[8];
     if (turns) {
         const int position = p.positions == nullptr ? p.first + n : p.per_row ? p.positions[b * p.pos_sb + n * p.pos_sn] : p.positions[b * p.pos_sb] + n;
@@ -37,22 +53,29 @@ template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(const Rot
             s[i] *= p.sign;
         }
     }
-    const int h0 = (int)blockIdx.y * p.heads_each, h1 = h0 + p.heads_each < p.heads ? h0 + p.heads_each : p.heads;
-    for (int h = h0; h < h1; ++h) {
-        const char* src = p.x + b * p.x_sb + h * p.x_sh + n * p.x_sn;
-        char* dst = p.out + b * p.o_sb + h * p.o_sh + n * p.o_sn;
-        const v4i lo = *(const v4i*)(src + 2 * first), hi = *(const v4i*)(src + 2 * second);
-        if (!turns) {
-            *(v4i*)(dst + 2 * first) = lo;
-            *(v4i*)(dst + 2 * second) = hi;
-            continue;
+    for (int h = h0; h < h1; h += N) {
+        v4i y[N][2];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            y[k][0] = raw[k][0];
+            y[k][1] = raw[k][1];
+            if (turns) {
+                float x[16];
+                unpack8<DT>(raw[k][0], x);
+                unpack8<DT>(raw[k][1], x + 8);
+                rope_turn_unit(x, c, s, interleaved);
+                y[k][0] = pack8<DT>(x);
+                y[k][1] = pack8<DT>(x + 8);
+            }
         }
-        float x[16];
-        unpack8<DT>(lo, x);
-        unpack8<DT>(hi, x + 8);
-        rope_turn_unit(x, c, s, interleaved);
-        *(v4i*)(dst + 2 * first) = pack8<DT>(x);
-        *(v4i*)(dst + 2 * second) = pack8<DT>(x + 8);
+        if (h + N < h1) request(h + N);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (h + k >= h1) break;
+            char* const at = dst + (h + k) * p.o_sh;
+            __builtin_nontemporal_store(y[k][0], (v4i*)(at + 2 * first));
+            __builtin_nontemporal_store(y[k][1], (v4i*)(at + 2 * second));
+        }
     }
 }
 
@@ -296,11 +319,16 @@ int intfa_rotary(const intfa_rotary_params* p, void* stream) {
     rp.heads = p->heads; rp.seqlen = p->seqlen;
     rp.d_units = make_fast_div(rp.units); rp.d_seqlen = make_fast_div(p->seqlen);
     rp.sign = p->inverse ? -1.0f : 1.0f;
-    rp.heads_each = 1;
+    // Heads per thread: as many as leave a workgroup per compute unit, up to eight.  (4 x 4096 tokens, 32 heads of 128, us: one 59, four 47.7, eight 46.3, sixteen 46.0)
     const int blocks = (int)((rp.threads + 255) / 256);
-    const dim3 grid(blocks, p->heads);
-    if (p->dtype == INTFA_F16) hipLaunchKernelGGL(rotary_kernel<0>, grid, dim3(256), 0, (hipStream_t)stream, rp);
-    else hipLaunchKernelGGL(rotary_kernel<1>, grid, dim3(256), 0, (hipStream_t)stream, rp);
+    rp.heads_each = 1;
+    while (rp.heads_each < 8 && rp.heads_each < p->heads && (int64_t)blocks * p->heads >= 2ll * rp.heads_each * kComputeUnits) rp.heads_each *= 2;
+    const dim3 grid(blocks, (p->heads + rp.heads_each - 1) / rp.heads_each);
+#define INTFA_CALL(DT) do { \
+        if (rp.heads_each >= kRotaryHeads) hipLaunchKernelGGL((rotary_kernel<DT, true>), grid, dim3(256), 0, (hipStream_t)stream, rp); \
+        else hipLaunchKernelGGL((rotary_kernel<DT, false>), grid, dim3(256), 0, (hipStream_t)stream, rp); } while (0)
+    if (p->dtype == INTFA_F16) INTFA_CALL(0); else INTFA_CALL(1);
+#undef INTFA_CALL
     return (int)hipGetLastError();
 }
 
