@@ -374,7 +374,7 @@ int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream);
  * that position first where rope.freqs is given, and with causal seeing keys 0 .. n - m + i only.  Rows from m onward and rows that
  * see no key are zeros with lse = -infinity.  lse: as in intfa_fwd_params.
  * Keys and values enter as the numbers that the cache stands for: the int8 values go into 16-bit matrix products as they are, exactly, and
- * scales, which must not be negative, are applied in fp32.  Queries enter exactly, rotated ones to 22 bits (rotated bf16 queries of more than 32 rows a K/V
+ * scales, which must not be negative, are applied in fp32.  Queries enter exactly, rotated ones to 22 bits (rotated bf16 queries of more than 64 rows a K/V
  * head: to 11); probabilities are rounded to 11 bits; sums are fp32.
  * workspace: at least intfa_paged_attn_workspace_bytes(p) bytes of device memory, 16-byte aligned, nothing to clear; two launches that may
  * run at the same time must not share it. */

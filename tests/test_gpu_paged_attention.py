@@ -23,8 +23,8 @@ def run(q, cache, kv, sc, table, lens, causal, sm=None, fresh=None, freqs=None, 
     want, want_lse, mean_v, size = attend(q, cache, table, lens, causal, sm, fresh, rope)
     o, lse = o.cpu(), lse.cpu()
     assert o.isfinite().all()
-    # rotated bf16 queries of more than 32 rows a K/V head are held to 11 bits
-    step = 2.0 ** -12 if freqs is not None and q.dtype == torch.bfloat16 and q.shape[1] // kv.shape[2] * q.shape[2] > 32 else 0.0
+    # rotated bf16 queries of more than 64 rows a K/V head are held to 11 bits
+    step = 2.0 ** -12 if freqs is not None and q.dtype == torch.bfloat16 and q.shape[1] // kv.shape[2] * q.shape[2] > 64 else 0.0
     far = (o.double() - want).abs() - bound(want, mean_v, size, q.dtype, step)
     assert (far <= 0).all(), f"{far.max().item():.3g} past the bound"
     empty = want_lse == -float("inf")
