@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
                     v4f a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int w = 0; w < W; ++w) a += weight[w] * *(const v4f*)(o_lds + (w * 16 + r) * O_ROW + cols * DT16 + j);
+                    if (token >= t.m) a = (v4f){0.f, 0.f, 0.f, 0.f};      // (whatever the row holds: zero times what is not a number is none)
                     store_out4<DT>(dst + j * 2, a * inv);
                 }
                 if (p->lse != nullptr && cols == 0)

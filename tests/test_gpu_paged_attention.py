@@ -139,6 +139,16 @@ def test_a_query_that_is_not_a_number_stays_in_its_row():
     assert o.isfinite().all()
 
 
+@pytest.mark.parametrize("N,fresh,lens", [(4, [2, 0, 4], [100, 60, 9]), (4, [3, 1], [20000, 9000]), (90, [33, 90], [400, 90])])
+def test_what_pads_a_batch_may_be_anything(N, fresh, lens):
+    """Rows past a sequence's new tokens are zeros even where the padding is no number, in sequences of one piece and of many."""
+    q, cache, kv, sc, table = problem(84 + N, len(lens), 4, 2, N, 64, 64, lens, torch.bfloat16)
+    freqs, _ = M.rotary_frequencies(64, device=DEV)
+    for z, m in enumerate(fresh):
+        q[z, :, m:] = float("nan")
+    run(q, cache, kv, sc, table, lens, True, fresh=fresh, freqs=freqs)
+
+
 def test_strides():
     """Queries as [Z, N, H, d], pages as [page, head, (k, v), row]: any strides with a contiguous d."""
     lens = [77, 200]
