@@ -88,7 +88,7 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
         if (token >= t.m) acc = (v4f){0.f, 0.f, 0.f, 0.f};
         store_out4<DT>(p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + col * 2, acc * (empty ? 0.f : 1.f / l));
         if (p->lse != nullptr && col == 0)
-            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = empty ? -INFINITY : m + __builtin_log2f(l) - kPShift;
+            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : m + __builtin_log2f(l) - kPShift;
     }
 }
 
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
                     store_out4<DT>(dst + j * 2, a * inv);
                 }
                 if (p->lse != nullptr && cols == 0)
-                    p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = empty ? -INFINITY : top + __builtin_log2f(sum) - kPShift;
+                    p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : top + __builtin_log2f(sum) - kPShift;      // (no key: -infinity twice; no number in the row: the sum is none either)
             } else {
                 const PagedParts mine(p, R, D, (int)part.slot);
 #pragma unroll

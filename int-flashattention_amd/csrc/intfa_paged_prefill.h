@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
                 store_out4<DT>(dst + 64 * a + 8 * i, x);
             }
         if (p->lse != nullptr && lh == 0)
-            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = empty ? -INFINITY : m + __builtin_log2f(l) - kPrefillShift;
+            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : m + __builtin_log2f(l) - kPrefillShift;      // (as in intfa_paged_decode.h)
     }
     if (!paged_next(p, R, t, piece)) break;
     __syncthreads();

@@ -149,6 +149,19 @@ def test_what_pads_a_batch_may_be_anything(N, fresh, lens):
     run(q, cache, kv, sc, table, lens, True, fresh=fresh, freqs=freqs)
 
 
+@pytest.mark.parametrize("N,n", [(1, 90), (3, 20000), (70, 300)])
+def test_a_row_that_is_not_a_number_has_no_lse(N, n):
+    q, cache, kv, sc, table = problem(85, 1, 4, 2, N, 128, 32, [n], torch.float16)
+    q[0, 2, N // 2, 9] = float("nan")
+    kv_d, sc_d = kv.to(DEV), sc.to(DEV)
+    o, lse = M.attention_paged_int8(q.to(DEV), kv_d[:, 0], kv_d[:, 1], sc_d[:, 0], sc_d[:, 1], table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV),
+                                    True, 0.125, return_lse=True)
+    bad = torch.zeros((4, N), dtype=torch.bool, device=DEV)
+    bad[2, N // 2] = True
+    assert o[0][bad].isnan().all() and o[0][~bad].isfinite().all()
+    assert lse[0][bad].isnan().all() and lse[0][~bad].isfinite().all()
+
+
 def test_strides():
     """Queries as [Z, N, H, d], pages as [page, head, (k, v), row]: any strides with a contiguous d."""
     lens = [77, 200]
