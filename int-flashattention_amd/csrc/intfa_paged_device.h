@@ -247,7 +247,7 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
             }
             int e = (int)(top >> 23) - 127;
             e = e < -100 ? -100 : e > 100 ? 100 : e;
-            const float down = __builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23);
+            const float down = copysignf(__builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23), p->qk_scale_log2);
             uint32_t h[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -263,7 +263,7 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
                 *(v4i*)(q_rest + r * ROW + 2 * first) = (v4i){(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
                 *(v4i*)(q_rest + r * ROW + 2 * second) = (v4i){(int)h[4], (int)h[5], (int)h[6], (int)h[7]};
             }
-            if (u == 0) factor[r] = __builtin_bit_cast(float, (uint32_t)(127 + e - 8) << 23) * p->qk_scale_log2;
+            if (u == 0) factor[r] = __builtin_bit_cast(float, (uint32_t)(127 + e - 8) << 23) * fabsf(p->qk_scale_log2);
         }
     }
 };

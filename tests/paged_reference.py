@@ -85,7 +85,7 @@ def attend(q, cache, table, lens, causal, sm, fresh=None, rope=None):
         w = p / torch.where(total == 0, torch.ones_like(total), total)
         out[z, :, :m] = torch.einsum("hgmn,hnd->hgmd", w, v).reshape(H, m, d)
         mean_v[z, :, :m] = torch.einsum("hgmn,hnd->hgmd", w, v.abs()).reshape(H, m, d)
-        size[z, :, :m] = (torch.einsum("hgmd,hnd->hgmn", x.abs(), k.abs()) * sm * seen).amax(-1, keepdim=True).reshape(H, m, 1)
+        size[z, :, :m] = (torch.einsum("hgmd,hnd->hgmn", x.abs(), k.abs()) * abs(sm) * seen).amax(-1, keepdim=True).reshape(H, m, 1)
         lse[z, :, :m] = torch.where(any_key, ((top + total.log()) / math.log(2.0))[..., 0], torch.full((), -math.inf, dtype=torch.float64)).reshape(H, m)
     return out, lse, mean_v, size
 

@@ -162,6 +162,15 @@ def test_a_row_that_is_not_a_number_has_no_lse(N, n):
     assert lse[0][bad].isnan().all() and lse[0][~bad].isfinite().all()
 
 
+@pytest.mark.parametrize("N", [1, 9, 100])
+def test_a_negative_scale_of_scores(N):
+    """The sign goes to the queries, which are held to as many bits either way: the same as the positive scale with the queries' signs changed."""
+    lens = [N + 30, 500]
+    q, cache, kv, sc, table = problem(86, 2, 8, 2, N, 128, 64, lens, torch.float16)
+    assert torch.equal(run(-q, cache, kv, sc, table, lens, True, sm=0.1), run(q, cache, kv, sc, table, lens, True, sm=-0.1))
+    run(q, cache, kv, sc, table, lens, True, sm=0.0)
+
+
 def test_strides():
     """Queries as [Z, N, H, d], pages as [page, head, (k, v), row]: any strides with a contiguous d."""
     lens = [77, 200]
