@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
             for (int g = 1; g < G; ++g) v_top = fmaxf(v_top, sc.has[g] ? sc.v[g] : 0.f);
         }
+        v_top = v_top < 0x1p-120f ? 0.f : v_top;             // (its reciprocal would be none; the append leaves none under 2^-100)
         v_peak = fmaxf(v_peak, v_top);
         if (v_top > 2.f * v_unit || v_top < 0x1p-10f * v_unit) {
             const float unit = fmaxf(fmaxf(v_top, v_peak * 0x1p-60f), 0x1p-100f), scale = v_unit / unit;

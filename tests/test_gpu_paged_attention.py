@@ -171,6 +171,15 @@ def test_a_negative_scale_of_scores(N):
     run(q, cache, kv, sc, table, lens, True, sm=0.0)
 
 
+@pytest.mark.parametrize("N", [2, 100])
+def test_scales_of_values_near_nothing(N):
+    """Values of 2^-130 and less: below fp16's smallest, and no scale's reciprocal is formed that would not be a number."""
+    lens = [N + 100]
+    q, cache, kv, sc, table = problem(87, 1, 4, 2, N, 64, 16, lens, torch.float16)
+    sc[:, 1] = 2.0 ** -135
+    run(q, cache, kv, sc, table, lens, True)
+
+
 def test_strides():
     """Queries as [Z, N, H, d], pages as [page, head, (k, v), row]: any strides with a contiguous d."""
     lens = [77, 200]
