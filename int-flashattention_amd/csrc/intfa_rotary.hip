@@ -363,13 +363,14 @@ int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream) {
     ap.heads_each = 1;
     while (units > 64 && ap.heads_each < 8 && ap.heads_each < c.heads_kv && pages * c.heads_kv >= 2ll * ap.heads_each * kComputeUnits) ap.heads_each *= 2;
     ap.head_groups = (c.heads_kv + ap.heads_each - 1) / ap.heads_each;
-    if (pages * ap.head_groups >= 1ll << 31) return INTFA_ERR_SHAPE;
+    const int threads = units <= 64 ? 64 : 512;
+    if (pages * ap.head_groups * threads >= 1ll << 32) return INTFA_ERR_SHAPE;      // (threads of a launch are numbered in 32 bits)
     ap.d_slots = make_fast_div(ap.slots); ap.d_head_groups = make_fast_div(ap.head_groups);
     const dim3 g((unsigned)(pages * ap.head_groups), 2);
 #define INTFA_CALL(DT) do { \
-        if (units <= 64) hipLaunchKernelGGL((paged_append_kernel<DT, 1, 1>), g, dim3(64), 0, (hipStream_t)stream, ap); \
-        else if (units <= 512) hipLaunchKernelGGL((paged_append_kernel<DT, 8, 1>), g, dim3(512), 0, (hipStream_t)stream, ap); \
-        else hipLaunchKernelGGL((paged_append_kernel<DT, 8, 2>), g, dim3(512), 0, (hipStream_t)stream, ap); } while (0)
+        if (units <= 64) hipLaunchKernelGGL((paged_append_kernel<DT, 1, 1>), g, dim3(threads), 0, (hipStream_t)stream, ap); \
+        else if (units <= 512) hipLaunchKernelGGL((paged_append_kernel<DT, 8, 1>), g, dim3(threads), 0, (hipStream_t)stream, ap); \
+        else hipLaunchKernelGGL((paged_append_kernel<DT, 8, 2>), g, dim3(threads), 0, (hipStream_t)stream, ap); } while (0)
     if (p->dtype == INTFA_F16) INTFA_CALL(0); else INTFA_CALL(1);
 #undef INTFA_CALL
     return (int)hipGetLastError();

@@ -110,7 +110,7 @@ CACHE = [(dict(cache__k=None), -1), (dict(cache__v_scale=None), -1), (dict(cache
 
 @pytest.mark.parametrize("kw,code", CACHE + [(dict(k_new=None), -1), (dict(v_new=None), -1), (dict(seqlen_new=0), -3), (dict(seqlen_new=-1), -3),
                                              (dict(v_new=ADDRESS + 2), -4), (dict(kn_stride_n=68), -4), (dict(seqlens_new=ADDRESS + 2), -4),
-                                             (dict(batch=1 << 30), -7)])
+                                             (dict(batch=1 << 30), -7), (dict(batch=1 << 24, seqlen_new=256), -7)])
 def test_append_refusals(kw, code):
     assert _append(**kw) == code
 
