@@ -180,6 +180,24 @@ def test_scales_of_values_near_nothing(N):
     run(q, cache, kv, sc, table, lens, True)
 
 
+@pytest.mark.parametrize("H,Hkv,N,d", [(96, 1, 1, 128), (71, 1, 1, 64), (130, 2, 1, 256)])
+def test_many_query_heads_of_one_key_head(H, Hkv, N, d):
+    lens = [1, 777, 64]
+    q, cache, kv, sc, table = problem(88 + d, 3, H, Hkv, N, d, 32, lens, torch.bfloat16)
+    freqs, _ = M.rotary_frequencies(64, device=DEV)
+    run(q, cache, kv, sc, table, lens, False, freqs=freqs)
+
+
+def test_wide_tables_of_many_sequences():
+    """9600 items over tables of 320000 keys: more units of work than are numbered, so they are larger ones."""
+    Z, H, d, page, columns = 600, 16, 64, 16, 20000
+    lens = [1 + 7 * z % 50 for z in range(Z)]
+    q, cache, kv, sc, narrow = problem(89, Z, H, H, 1, d, page, lens, torch.float16)
+    table = torch.full((Z, columns), -1, dtype=torch.int32)
+    table[:, :narrow.shape[1]] = narrow
+    run(q, cache, kv, sc, table, lens, False)
+
+
 def test_strides():
     """Queries as [Z, N, H, d], pages as [page, head, (k, v), row]: any strides with a contiguous d."""
     lens = [77, 200]

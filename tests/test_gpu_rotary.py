@@ -100,3 +100,35 @@ def test_gradient(interleaved):
     check(leaf.grad, torch.ones_like(x), (4 + torch.arange(11)).expand(2, 11), freqs.cpu(), 1.0, interleaved, inverse=True)
     with torch.no_grad():
         assert not M.rotary(leaf, 4, freqs).requires_grad
+
+
+def test_a_captured_training_step():
+    """Forward and backward in one captured graph, replayed over new inputs with eager work in between."""
+    g = torch.Generator().manual_seed(9)
+    freqs, _ = M.rotary_frequencies(64, device=DEV)
+    x, y = (torch.zeros((2, 4, 50, 128), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    pos = torch.zeros((2,), dtype=torch.int32, device=DEV)
+    leaf = x.requires_grad_()
+
+    def step():
+        out = M.rotary(leaf, pos, freqs)
+        return out, *torch.autograd.grad(out, leaf, y)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()                                                # (nothing of its graph is kept)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, dx = step()
+    for k in range(4):
+        with torch.no_grad():
+            leaf.copy_(torch.randn(x.shape, generator=g))
+            y.copy_(torch.randn(x.shape, generator=g))
+            pos.copy_(torch.randint(0, 9000, (2,), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert torch.equal(out, M.rotary(leaf, pos, freqs)) and torch.equal(dx, M.rotary(y, pos, freqs, inverse=True))
