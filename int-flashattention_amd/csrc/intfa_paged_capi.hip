@@ -25,7 +25,7 @@ int check(const intfa_paged_attn_params* p) {
 }
 
 // How a call is dealt: rows per tile, keys per unit, workgroups; and the layout of its workspace.
-struct Plan { PagedSel sel; int rows, tiles, unit_log2, grid, slot_rows; size_t stats_at, tickets_at, bytes; };
+struct Plan { PagedSel sel; int rows, tiles, unit_log2, lead, grid, slot_rows; size_t stats_at, tickets_at, bytes; };
 Plan make_plan(const intfa_paged_attn_params* p) {
     const intfa_paged_cache& c = p->cache;
     Plan a{};
@@ -34,10 +34,13 @@ Plan make_plan(const intfa_paged_attn_params* p) {
     a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, prefill ? 0 : a.rows <= 16 ? 1 : 2, c.page_size >= (!prefill && c.head_dim == 256 ? 32 : 64)};
     a.slot_rows = prefill ? paged_prefill_rows(c.head_dim) : 16 * a.sel.row_tiles;
     a.tiles = (a.rows + a.slot_rows - 1) / a.slot_rows;
-    a.unit_log2 = !prefill && c.head_dim == 256 ? 7 : 8;
+    // (many rows, units of 256 keys with a lead of two -> of 64 with a lead of four, which is what beginning a part takes: two ragged chunks of 512 122.0 -> 118.4 us,
+    // sixteen chunks of 512 tokens of which fifteen have three 207 -> 172, a prompt of 2048 73.9 -> 72.8; a lead of three 121.2, 170, 77.5, of five 119.6, 177, 70.8)
+    a.lead = prefill ? 4 : 2;
+    a.unit_log2 = prefill ? 6 : c.head_dim == 256 ? 7 : 8;
     const int64_t items = (int64_t)p->batch * c.heads_kv * a.tiles, keys = (int64_t)c.table_width * c.page_size;
     const int slots = kComputeUnits * (prefill ? paged_prefill_wgs(c.head_dim) : c.head_dim == 256 || a.sel.row_tiles > 1 ? 1 : 2);
-    auto units = [&] { return items * (kPagedLead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
+    auto units = [&] { return items * (a.lead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
     a.grid = (int)(units() < slots ? units() : slots);
     while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)
     if (units() * a.grid >= 1ll << 32) a.grid = (int)(((1ll << 32) - 1) / units());
@@ -75,7 +78,7 @@ int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream) {
     kp.causal = p->causal != 0;
     kp.qk_scale_log2 = p->sm_scale * 1.4426950408889634f;
     kp.rope = {p->rope.freqs, p->rope.pairs, p->rope.interleaved, p->rope.magnitude};
-    kp.tiles = a.tiles; kp.unit_log2 = a.unit_log2; kp.grid = a.grid;
+    kp.tiles = a.tiles; kp.unit_log2 = a.unit_log2; kp.grid = a.grid; kp.lead = a.lead;
     kp.parts = (float*)p->workspace;
     kp.part_stats = (float*)((char*)p->workspace + a.stats_at);
     kp.ticket = (uint64_t*)((char*)p->workspace + a.tickets_at);

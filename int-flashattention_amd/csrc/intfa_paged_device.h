@@ -47,7 +47,7 @@ typedef const __attribute__((address_space(4))) float* PagedFloats;
 // ---- who works on what
 // The work is a line: the row tiles of all sequences, each with all K/V heads (an item: one tile and head), and each item's keys as units of
 // 2^unit_log2, at least one.  Every workgroup takes an equal piece of the line: whatever the lengths and the mask, all compute units end together.  An
-// item that lies in several pieces is merged by the workgroup that finishes its part last.  Ahead of its own units each item has kPagedLead
+// item that lies in several pieces is merged by the workgroup that finishes its part last.  Ahead of its own units each item has `lead`
 // without keys: beginning an item and ending one take a workgroup about as long as their keys would (decode-shaped: 8 us, where a unit takes 4 with the whole
 // card reading), and without them the workgroups that have parts of two items came in last (ragged batch of 16, 512 workgroups of 5.3 units: 42 -> 47 us).
 struct PagedItem {
@@ -69,7 +69,7 @@ __device__ __forceinline__ int paged_seen(PagedArgs p, int n, int m, int tile, i
 }
 __device__ __forceinline__ int paged_units(PagedArgs p, int keys) {
     const int u = (keys + (1 << p->unit_log2) - 1) >> p->unit_log2;
-    return (u > 1 ? u : 1) + kPagedLead;
+    return (u > 1 ? u : 1) + p->lead;
 }
 // The tile `pair` of the line's order (sequence, tile).
 template <typename Ints> __device__ __forceinline__ void paged_pair(PagedArgs p, int pair, int rows, PagedItem& t) {
@@ -139,7 +139,7 @@ __device__ __forceinline__ bool paged_next(PagedArgs p, int rows, PagedItem& t, 
 // A workgroup's part of an item.
 struct PagedPart { int key_first, key_end; bool none, whole; int one, pieces; bool first_is_first; uint32_t slot; };
 __device__ __forceinline__ PagedPart paged_part(PagedArgs p, const PagedItem& t, const PagedPiece& w) {
-    const uint32_t keys = w.start + (uint32_t)kPagedLead, item_end = w.start + (uint32_t)t.units;
+    const uint32_t keys = w.start + (uint32_t)p->lead, item_end = w.start + (uint32_t)t.units;
     PagedPart a;
     a.none = w.end <= keys;                                // (the piece ends in the item's lead)
     a.whole = w.first <= keys && item_end <= w.end;

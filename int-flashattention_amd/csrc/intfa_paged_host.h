@@ -26,7 +26,6 @@ inline int paged_cache_check(const intfa_paged_cache* c) {
     return INTFA_OK;
 }
 
-constexpr int kPagedLead = 2;          // units ahead of an item's keys (intfa_paged_decode.h)
 struct PagedParams {
     const char* q; char* out; float* lse;
     const char* k; const char* v; const float* k_scale; const float* v_scale;
@@ -40,6 +39,7 @@ struct PagedParams {
     int32_t tiles;                                   // row tiles of a K/V head
     int32_t unit_log2;                               // keys that are dealt together
     int32_t grid;                                    // workgroups of the launch
+    int32_t lead;                                    // units ahead of an item's keys (intfa_paged_device.h)
     float qk_scale_log2;
     RopeArgs rope;
     float* parts; float* part_stats;                 // partial results: two slots per workgroup (intfa_paged_decode.h)

@@ -11,6 +11,12 @@
 // A row's scale of scores and a page's go into one multiplier of the exponent's fused multiply-add (a page's scale is not negative: the maximum of the
 // products is that of the scores).  V's scale goes there too, as log2(scale / reference), the reference being the unit of the accumulators: it follows the
 // page's scale where that leaves 2^-10 .. 2 of it.  A row's maximum is followed where it grows by more than 2^6, so that most blocks rescale nothing.
+//
+// What bounds it (2 x 32 x 512 bf16 rows of 128 over up to 30720 keys: 953 TFLOP/s of the 1200 that a matrix product of 8192^3 reaches on the same card): per
+// block and SIMD 2050 clocks of products and 2400 of other vector work, two thirds of it the softmax, which hardly run beside each other - 4600 clocks
+// pass at 2.2 GHz.  P V under the exponentials of the granule behind (1 - 2 % and a fifth slower at head_dim 256), the next block's conversion under Q K,
+// a barrier every second block, scales by vector loads and 64 rows a wave changed nothing or spilled.  Short calls pay beginning and end besides: 13 us to
+// the first product (of which the queries take 9), 4 to 10 for the partial results and their merge.  (Ragged pair of chunks of 512 over 7680 keys: 118 us.)
 #pragma once
 #include "intfa_paged_device.h"
 
@@ -35,7 +41,7 @@ template <int D> struct PrefillBytes {
 };
 
 // REST: rotated fp16 queries, whose scores take a second product (PagedQueries::stage).  Rotated bf16 queries stay rounded to 11 bits here, three more than
-// they came with: a second product costs a third more matrix work and the registers for it (chunk 145 -> 187 us).  ONE: a page holds a block's keys.
+// they came with: a second product costs a third more matrix work and the registers for it (a ragged pair of chunks of 512 tokens over 7680 keys 145 -> 187 us).  ONE: a page holds a block's keys.
 template <int D, int DT, bool REST, bool ONE>
 __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS * PrefillShape<D>::WAVES / 4) paged_prefill_kernel(const PagedParams) {
     typedef PrefillShape<D> S;
@@ -63,26 +69,28 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     // ---- queries: through LDS into the waves that own them
     v8h q[KS], q_rest[REST ? KS : 1];
     float factor = 0.f;
-    Queries queries[R / S::PASS];
+    if (part.key_first < part.key_end) {                   // (rows that see no key are zeros without it)
+        Queries queries[R / S::PASS];
 #pragma unroll
-    for (int pass = 0; pass < R / S::PASS; ++pass) queries[pass].request(p, t, row0 + pass * S::PASS);
+        for (int pass = 0; pass < R / S::PASS; ++pass) queries[pass].request(p, t, row0 + pass * S::PASS);
 #pragma unroll
-    for (int pass = 0; pass < R / S::PASS; ++pass) {
-        if (pass > 0) __syncthreads();
-        if (queries[pass].rope) {
-            queries[pass].turn_angles(p, t, freq_lds, (v2f*)(lds + ANGLES_AT));
-            __syncthreads();
-        }
-        queries[pass].template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
-        __syncthreads();
-        if (32 * wave / S::PASS == pass) {
-            const char* const mine = lds + (32 * wave % S::PASS + lq) * Queries::ROW + 16 * lh;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                q[ks] = *(const v8h*)(mine + 32 * ks);
-                if (REST) q_rest[REST ? ks : 0] = *(const v8h*)(mine + S::PASS * Queries::ROW + 32 * ks);
+        for (int pass = 0; pass < R / S::PASS; ++pass) {
+            if (pass > 0) __syncthreads();
+            if (queries[pass].rope) {
+                queries[pass].turn_angles(p, t, freq_lds, (v2f*)(lds + ANGLES_AT));
+                __syncthreads();
             }
-            factor = factor_lds[32 * wave % S::PASS + lq];
+            queries[pass].template stage<REST>(p, row0 + pass * S::PASS, (const v2f*)(lds + ANGLES_AT), lds, lds + S::PASS * Queries::ROW, factor_lds);
+            __syncthreads();
+            if (32 * wave / S::PASS == pass) {
+                const char* const mine = lds + (32 * wave % S::PASS + lq) * Queries::ROW + 16 * lh;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    q[ks] = *(const v8h*)(mine + 32 * ks);
+                    if (REST) q_rest[REST ? ks : 0] = *(const v8h*)(mine + S::PASS * Queries::ROW + 32 * ks);
+                }
+                factor = factor_lds[32 * wave % S::PASS + lq];
+            }
         }
     }
     // ---- where the keys come from
