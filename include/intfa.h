@@ -353,8 +353,8 @@ typedef struct intfa_paged_cache {
  *     rows from before, if that is a larger scale than theirs: q = rint(q * (scale before / scale));
  *     new rows: q = rint(x / scale) within +-127.
  * A NaN becomes 0 and an infinity +-127, and neither counts for A: a page has one scale, which they would take from all its other tokens.
- * What lies behind the new rows in a page stays as it was.  A page that rows go to must belong to one sequence of the call only (two
- * would write it at once; the result of that is not defined, though inside the page). */
+ * What lies behind the new rows in a page stays as it was.  A page that rows go to must stand once in the table, in one sequence of the
+ * call (two writers at once: the result is not defined, though inside the page). */
 typedef struct intfa_paged_append_params {
     intfa_paged_cache cache;
     const void* k_new; const void* v_new;      /* fp16 or bf16 [batch, heads_kv, seqlen_new, head_dim], as for intfa_rotary */

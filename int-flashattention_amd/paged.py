@@ -18,7 +18,7 @@ def paged_kvcache_append(k_cache, k_scale, v_cache, v_scale, k_new, v_new, block
 
     A page's scale is the largest magnitude among its new rows over 127; a page that held rows of the sequence before keeps a larger scale,
     and where the new rows need a larger one its rows are requantised to it (rint(q * old / new)).  NaN becomes 0 and infinities +-127, and neither
-    counts for the scale.  A page that rows go to must belong to one sequence of the call."""
+    counts for the scale.  A page that rows go to must stand once in the table, in one sequence of the call."""
     return (_host._native or _host.native()).paged_kvcache_append(k_cache, k_scale, v_cache, v_scale, k_new, v_new, block_table, seqlens_k,
                                                                   freqs, interleaved, magnitude, seqlens_new)
 
@@ -32,7 +32,7 @@ def attention_paged_int8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq
     each sequence where they differ; rows past them are zeros.  Row i of m new tokens stands at position seqlens_k - m + i: with
     ``causal`` it sees the keys up to there, and with ``freqs`` the query is rotated by it first.  Rows that see no key are zeros with
     an lse of -inf; tokens of a page that the table does not name are hidden.
-    Page scales have to be finite: one that is not reaches the rows computed together with those that see its page.
+    Page scales must not be negative, and have to be finite: one that is not reaches the rows computed together with those that see its page.
     """
     return (_host._native or _host.native()).attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens_k, causal, sm_scale,
                                                              freqs, interleaved, magnitude, seqlens_q, return_lse)

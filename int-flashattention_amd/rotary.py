@@ -64,7 +64,7 @@ def rotary(x, positions, freqs, *, interleaved=False, inverse=False, magnitude=1
     ``positions``: an int (row n of every entry stands at positions + n), an int32 [Z] tensor (the first row's position of each
     entry) or an int32 [Z, N] tensor.  Angles are formed and reduced in fp64, so far positions keep theirs.
     ``inverse`` turns by the negative angle, times the same ``magnitude``: the transposed map.  Where x requires a gradient, it
-    goes back through that.
+    goes back through that; a captured backward pass is captured with its forward pass, while no eager graph of x's leaves is alive.
     """
     if x.requires_grad and torch.is_grad_enabled():
         return _Rotary.apply(x, positions, freqs, interleaved, inverse, magnitude)
