@@ -306,6 +306,7 @@ int intfa_rotary(const intfa_rotary_params* p, void* stream) {
     if (!rope_valid(&p->rope, d)) return INTFA_ERR_ROPE;
     if (!aligned(p->x, 16) || !aligned(p->out, 16) || !aligned(p->rope.freqs, 8) || !aligned(p->positions, 4) ||
         !strides16(p->x_stride_b, p->x_stride_h, p->x_stride_n) || !strides16(p->o_stride_b, p->o_stride_h, p->o_stride_n)) return INTFA_ERR_ALIGN;
+    if (p->positions == nullptr && (int64_t)p->position_first + p->seqlen > 1ll << 31) return INTFA_ERR_SHAPE;      // positions are 32-bit numbers
     RotaryParams rp{};
     rp.units = d / 16;
     rp.threads = (int64_t)p->batch * p->seqlen * rp.units;

@@ -115,3 +115,23 @@ def test_strided_new_rows():
     g = torch.Generator().manual_seed(34)
     qkv = torch.randn((2, 21, 3, 4, 128), generator=g).bfloat16()           # [Z, N, (q, k, v), H, d]
     run_both(32, qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2), [11, 0])
+
+
+def test_several_heads_a_workgroup():
+    """Enough pages that a workgroup takes several heads of one, and a number of heads that its share does not divide."""
+    g = torch.Generator().manual_seed(35)
+    k, v = (torch.randn((4, 11, 1030, 64), generator=g).half() for _ in range(2))
+    v[1, 7, 500, 3] = float("inf")
+    run_both(16, k, v, [0, 9, 16, 40], freqs=M.rotary_frequencies(64, device=DEV)[0])
+
+
+def test_pages_whose_heads_lie_side_by_side():
+    g = torch.Generator().manual_seed(36)
+    k, v = (torch.randn((2, 3, 50, 128), generator=g).bfloat16().to(DEV) for _ in range(2))
+    table, lens = torch.arange(8, dtype=torch.int32, device=DEV).reshape(2, 4), torch.tensor([5, 30], dtype=torch.int32, device=DEV)
+    side = torch.zeros((8, 32, 2, 3, 128), dtype=torch.int8, device=DEV)            # [page, row, (k, v), head, d]
+    plain = torch.zeros((8, 2, 3, 32, 128), dtype=torch.int8, device=DEV)
+    s1, s2 = (torch.full((8, 2, 3), 0.01, device=DEV) for _ in range(2))
+    M.paged_kvcache_append(side[:, :, 0].transpose(1, 2), s1[:, 0], side[:, :, 1].transpose(1, 2), s1[:, 1], k, v, table, lens)
+    M.paged_kvcache_append(plain[:, 0], s2[:, 0], plain[:, 1], s2[:, 1], k, v, table, lens)
+    assert torch.equal(side.permute(0, 2, 3, 1, 4), plain) and torch.equal(s1, s2) and plain.any()

@@ -210,6 +210,29 @@ def test_strides():
     assert torch.equal(o.cpu(), want)
 
 
+@pytest.mark.parametrize("N", [1, 30, 100])
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 128), (256, 16), (256, 32), (256, 256), (128, 16)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rotated_queries_of_all_head_dims(N, d, page, dtype):
+    """Both kernels of each head_dim, pages smaller and larger than the keys that they take at a time."""
+    lens = [N + 333, N, 1]
+    q, cache, kv, sc, table = problem(90 + d + page, 3, 4, 2, N, d, page, lens, dtype)
+    freqs, magnitude = M.rotary_frequencies(d, device=DEV, scaling="base", factor=2.0)
+    run(q, cache, kv, sc, table, lens, True, freqs=freqs, magnitude=magnitude, interleaved=page == 16)
+
+
+@pytest.mark.parametrize("N,d", [(1, 64), (1, 128), (20, 256), (150, 64), (150, 128), (150, 256)])
+def test_pages_whose_heads_lie_side_by_side(N, d):
+    """Pages as [page, row, head, d]: a row's next one is all heads further."""
+    lens = [N + 100, 300]
+    q, cache, kv, sc, table = problem(91, 2, 6, 3, N, d, 64, lens, torch.float16)
+    want = run(q, cache, kv, sc, table, lens, True)
+    k, v = (kv[:, i].transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for i in range(2))
+    sc_d = sc.to(DEV)
+    o = M.attention_paged_int8(q.to(DEV), k, v, sc_d[:, 0], sc_d[:, 1], table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), True, d ** -0.5)
+    assert torch.equal(o.cpu(), want)
+
+
 def test_offsets_past_32_bits():
     """Two pages at the ends of a pool of 4.3 GB."""
     page, Hkv, d = 256, 8, 256

@@ -94,7 +94,8 @@ NAN = float("nan")
     (dict(x=None), -1), (dict(out=None), -1), (dict(rope__freqs=None), -1), (dict(batch=0), -7), (dict(heads=0), -7), (dict(seqlen=0), -3),
     (dict(head_dim=48), -2), (dict(dtype=_capi.INTFA_F32), -5), (dict(rope__pairs=12), -12), (dict(rope__pairs=40), -12), (dict(rope__pairs=0), -12),
     (dict(rope__magnitude=0.0), -12), (dict(rope__magnitude=NAN), -12), (dict(rope__magnitude=math.inf), -12), (dict(x=ADDRESS + 8), -4),
-    (dict(o_stride_n=68), -4), (dict(positions=ADDRESS + 2), -4), (dict(rope__freqs=ADDRESS + 4), -4), (dict(batch=1 << 20, seqlen=1 << 20), -7)])
+    (dict(o_stride_n=68), -4), (dict(positions=ADDRESS + 2), -4), (dict(rope__freqs=ADDRESS + 4), -4), (dict(batch=1 << 20, seqlen=1 << 20), -7),
+    (dict(positions=None, position_first=(1 << 31) - 8, seqlen=9), -7)])
 def test_rotary_refusals(kw, code):
     assert _rotary(**kw) == code
     assert _capi.load().intfa_error_string(code).decode() not in ("", "ok", "unknown error")
