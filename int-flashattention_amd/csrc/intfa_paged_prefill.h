@@ -16,7 +16,7 @@
 // block and SIMD 2050 clocks of products and 2400 of other vector work, two thirds of it the softmax, which hardly run beside each other - 4600 clocks
 // pass at 2.2 GHz.  P V under the exponentials of the granule behind (1 - 2 % and a fifth slower at head_dim 256), the next block's conversion under Q K,
 // a barrier every second block, scales by vector loads and 64 rows a wave changed nothing or spilled.  Short calls pay beginning and end besides: 13 us to
-// the first product (of which the queries take 9), 4 to 10 for the partial results and their merge.  (Ragged pair of chunks of 512 over 7680 keys: 118 us.)
+// the first product (of which the queries take 9), 4 to 10 for the partial results and their merge.  (Ragged pair of chunks of 512 over 7680 keys: 118 - 123 us, by card.)
 #pragma once
 #include "intfa_paged_device.h"
 
@@ -41,7 +41,8 @@ template <int D> struct PrefillBytes {
 };
 
 // REST: rotated fp16 queries, whose scores take a second product (PagedQueries::stage).  Rotated bf16 queries stay rounded to 11 bits here, three more than
-// they came with: a second product costs a third more matrix work and the registers for it (a ragged pair of chunks of 512 tokens over 7680 keys 145 -> 187 us).  ONE: a page holds a block's keys.
+// they came with: a second product costs a third more matrix work and the registers for it (a
+// ragged pair of chunks of 512 tokens over 7680 keys 145 -> 187 us), which head_dim 256 does not have (make_plan).  ONE: a page holds a block's keys.
 template <int D, int DT, bool REST, bool ONE>
 __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS * PrefillShape<D>::WAVES / 4) paged_prefill_kernel(const PagedParams) {
     typedef PrefillShape<D> S;
@@ -409,7 +410,7 @@ template <int D> int launch_paged_prefill(const PagedParams& p, const PagedSel& 
 #define INTFA_CALL(DT, REST) do { \
         if (sel.one_page) hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, true>), grid, threads, 0, stream, p); \
         else hipLaunchKernelGGL((paged_prefill_kernel<D, DT, REST, false>), grid, threads, 0, stream, p); } while (0)
-    if (sel.io_dt == 1) INTFA_CALL(1, false); else if (p.rope.freqs != nullptr) INTFA_CALL(0, true); else INTFA_CALL(0, false);
+    if (sel.io_dt == 1) INTFA_CALL(1, false); else if (D < 256 && p.rope.freqs != nullptr) INTFA_CALL(0, (D < 256)); else INTFA_CALL(0, false);
 #undef INTFA_CALL
     return (int)hipGetLastError();
 }
