@@ -110,6 +110,44 @@ def test_a_captured_step_replays_like_eager_ones():
         torch.randn((512, 512), device=DEV).sum().item()
 
 
+def test_two_graphs_of_one_memory_pool():
+    """Attention steps of two lengths captured one after the other into graphs that share their memory, workspaces too, replayed in turn."""
+    d, H, Hkv = 128, 16, 2
+    g = torch.Generator().manual_seed(6)
+    pools = [Pool(2, Hkv, d, 32, 70) for _ in range(2)]
+    for pool, n in zip(pools, (2000, 130)):
+        pool.append(*(rows(g, 2, Hkv, n, d, torch.float16) for _ in range(2)))
+    qs = [rows(g, 2, H, n, d, torch.float16) for n in (1, 40)]                  # one kernel, the other
+    for pool, q in zip(pools, qs):
+        pool.attend(q)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for pool, q in zip(pools, qs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append([pool.attend(q), pool.attend(-q)])
+        graphs.append(graph)
+    for step in range(4):
+        for graph, pool, q, out in zip(graphs, pools, qs, outs):
+            q.copy_(torch.randn(q.shape, generator=g))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], pool.attend(q)) and torch.equal(out[1], pool.attend(-q))
+
+
+def test_sequences_that_share_pages():
+    """A prefix held once, named by both tables, and a page twice in one table."""
+    d, H, Hkv = 64, 8, 2
+    g = torch.Generator().manual_seed(7)
+    pool = Pool(2, Hkv, d, 16, 12)
+    pool.append(*(rows(g, 2, Hkv, 150, d, torch.float16) for _ in range(2)))
+    q = rows(g, 2, H, 3, d, torch.float16)
+    pool.table[1, :5] = pool.table[0, :5]
+    pool.table[0, 7] = pool.table[0, 2]
+    want, _, mean_v, size = pool.want(q)
+    assert ((pool.attend(q).cpu().double() - want).abs() <= bound(want, mean_v, size, torch.float16)).all()
+
+
 def test_two_streams_at_once():
     """Two requests' steps on streams of their own, many at a time, equal to the same ones in order."""
     d, H, Hkv = 64, 8, 8
