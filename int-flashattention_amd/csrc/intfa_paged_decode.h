@@ -16,7 +16,9 @@
 namespace intfa {
 
 constexpr int kPagedWaves = 4;
-constexpr float kPShift = 14.f;       // P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales
+// P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales.  The factor goes in with that ratio, p itself being
+// 2^(s - m) by a subtraction of its own: taken from m beforehand it would be lost to m's rounding, and p past fp16's range, from |m| = 2^25 on.
+constexpr float kPUnit = 0x1p14f;
 
 // Merges the rows of an item from its pieces: those of workgroups `one` onward, all of them first items of theirs but the one that the item begins in
 // the middle of (first_is_first: it begins at that workgroup's first unit).
@@ -86,9 +88,9 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
         const int row = row0 + r, token = paged_div(row, p->d_group), head = t.hk * p->group + row - token * p->group;
         const bool empty = m == -INFINITY || token >= t.m;
         if (token >= t.m) acc = (v4f){0.f, 0.f, 0.f, 0.f};
-        store_out4<DT>(p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + col * 2, acc * (empty ? 0.f : 1.f / l));
+        store_out4<DT>(p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + col * 2, acc * (empty ? 0.f : 1.f / (kPUnit * l)));
         if (p->lse != nullptr && col == 0)
-            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : m + __builtin_log2f(l) - kPShift;
+            p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : m + __builtin_log2f(l);
     }
 }
 
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         const float v_inv = __builtin_amdgcn_rcpf(v_top);
         float v_rel[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) v_rel[g] = now.has[g] ? now.vs[g] * v_inv : 0.f;
+        for (int g = 0; g < G; ++g) v_rel[g] = now.has[g] ? now.vs[g] * v_inv * kPUnit : 0.f;
         v4f scores[RT][G];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -287,6 +289,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         bool rescale = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+#pragma clang fp contract(off)                               // (what the maximum is taken from is what it was taken of)
             v4f (&s)[G] = scores[rt];
             float top = -INFINITY;
 #pragma unroll
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, s[g][i]);
             top = reduce_row_lanes(top, [](float a, float b) { return fmaxf(a, b); });
-            const float m_new = fmaxf(m[rt], top), frame = (m_new == -INFINITY ? 0.f : m_new) - kPShift;
+            const float m_new = fmaxf(m[rt], top), frame = m_new == -INFINITY ? 0.f : m_new;
             alpha[rt] = m_new == -INFINITY ? 1.f : fast_exp2(m[rt] - m_new);
             m[rt] = m_new;
             float sum = 0.f;
@@ -316,11 +319,11 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[g][i] = fast_exp2(s[g][i] - frame);
+                    s[g][i] = fast_exp2(s[g][i] - frame);      // (a score of the row's is the maximum, bit for bit: p is at most one)
                     sum += s[g][i];
                     s[g][i] *= v_rel[g];
                 }
-            l[rt] = l[rt] * alpha[rt] + sum;
+            l[rt] = fmaf(l[rt], alpha[rt], sum);
 #pragma unroll
             for (int h = 0; h < G / 2; ++h) {
                 v8h f;
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         const int head = t.hk * p->group + row - token * p->group;
         if (row < p->rows) {
             if (part.whole) {
-                const float inv = empty ? 0.f : 1.f / sum;
+                const float inv = empty ? 0.f : 1.f / (kPUnit * sum);
                 char* const dst = p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + cols * DT16 * 2;
 #pragma unroll
                 for (int j = 0; j < DT16; j += 4) {
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
                     store_out4<DT>(dst + j * 2, a * inv);
                 }
                 if (p->lse != nullptr && cols == 0)
-                    p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : top + __builtin_log2f(sum) - kPShift;      // (no key: -infinity twice; no number in the row: the sum is none either)
+                    p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : top + __builtin_log2f(sum);      // (no key: -infinity twice; no number in the row: the sum is none either)
             } else {
                 const PagedParts mine(p, R, D, (int)part.slot);
 #pragma unroll

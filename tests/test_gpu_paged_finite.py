@@ -1,0 +1,77 @@
+"""Attention over pages where the formula gives numbers and a step on the way to them could fail to: scores, queries and scales of values of any size
+that their types hold."""
+import math
+
+import pytest
+import torch
+
+import int_flashattention_amd as M
+from paged_reference import attend, bound, make_cache, make_table
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def call(q, kv, sc, table, lens, sm, causal=False, **kw):
+    kv_d, sc_d = kv.to(DEV), sc.to(DEV)
+    o, lse = M.attention_paged_int8(q.to(DEV), kv_d[:, 0], kv_d[:, 1], sc_d[:, 0], sc_d[:, 1], table.to(DEV),
+                                    torch.tensor(lens, dtype=torch.int32, device=DEV), causal, sm, return_lse=True, **kw)
+    torch.cuda.synchronize()
+    return o.cpu(), lse.cpu()
+
+
+def of_page(x, table, z, n):
+    """Rows [H, n, d] of sequence z."""
+    page = x.shape[2]
+    return x[table[z, :(n + page - 1) // page].long()].transpose(0, 1).reshape(x.shape[1], -1, x.shape[3])[:, :n]
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("N,d", [(1, 64), (3, 128), (20, 256)])
+@pytest.mark.parametrize("size", [16.0, 19.9, 20.1, 23.0, 24.3, 25.4, 25.8, 26.5, 27.5, 28.4, 30.0, 40.0, 100.0])
+def test_scores_of_any_size(N, d, page, size):
+    """Each query is a multiple of one key, whose score in base 2 is about 2^size and several times that of any other: the softmax is that key's, its value the
+    output to half a step and P's rounding.  (The scores of the others are behind by more than a tenth of 2^size, which exceeds every rounding of a score, 2^-18 of
+    it, and 30 from size 10 on.)"""
+    g = torch.Generator().manual_seed(int(10 * size) + N + d)
+    n = 4 * 64 + 7
+    cache, kv, sc = make_cache(g, n // page + 3, 1, page, d)
+    kv[:, 0] = torch.where(torch.rand(kv[:, 0].shape, generator=g) < 0.5, -1, 1).to(torch.int8) * torch.randint(60, 90, kv[:, 0].shape, generator=g, dtype=torch.int8)
+    sc[:, 0] = 0.5
+    table = make_table(g, [n], page, kv.shape[0])
+    keys, values = of_page(cache["k"], table, 0, n)[0], of_page(cache["v"].float() * cache["vs"][..., None, None], table, 0, n)[0]
+    winner = torch.randint(0, n, (N,), generator=g)
+    q = keys[winner].float()[None, None].bfloat16()                              # (whole numbers to 90: exact)
+    apart = keys.float() @ keys.float().T
+    norm = apart.diagonal().clone()
+    assert (apart - torch.diag(norm)).amax(0).div(norm.min()).max() < 0.85
+    sm = 2.0 ** size * math.log(2.0) / (0.5 * norm.mean().item())
+    o, lse = call(q, kv, sc, table, [n], sm)
+    assert o.isfinite().all() and lse.isfinite().all()
+    want = values[winner].double()
+    assert ((o[0, 0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11) * want.abs()).all()
+    top = norm[winner].double() * 0.5 * sm / math.log(2.0)
+    assert ((lse[0, 0].double() - top).abs() <= 2.0 ** -20 * top).all()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("size", [22.0, 23.0, 23.9, 24.6, 26.0, 27.3, 28.6])
+@pytest.mark.parametrize("N", [1])
+def test_large_scores_that_grow_slowly(N, page, size):
+    """Scores of about 2^size that grow by five in base 2 every 64 keys: a followed maximum may stay behind by as much, and the scales of values double with it."""
+    g = torch.Generator().manual_seed(int(10 * size) + page)
+    d, n = 64, 512
+    cache, kv, sc = make_cache(g, n // page, 1, page, d)
+    table = torch.arange(n // page, dtype=torch.int32)[None]
+    kv[:, 0] = 0
+    kv[:, 0, :, :, 0] = 127
+    kv[:, 0, 0, :, 1] = (torch.arange(n).reshape(-1, page) // 64).to(torch.int8)
+    sc[:, 0], sc[:, 1] = 1.0, 1.9 ** (torch.arange(n // page) * page // 64)[:, None]
+    q = torch.zeros((1, 1, N, d), dtype=torch.float16)
+    q[..., 0], q[..., 1] = 1.0, 127.0 * 5.0 / 2.0 ** size
+    sm = 2.0 ** size / 127.0 * math.log(2.0)
+    o, lse = call(q, kv, sc, table, [n], sm)
+    assert o.isfinite().all() and lse.isfinite().all()
+    want, want_lse, mean_v, extent = attend(q, cache, table, [n], False, sm)
+    assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -18 * extent[..., 0]).all()
