@@ -23,6 +23,7 @@
 namespace intfa {
 
 constexpr float kPrefillShift = 8.f, kPrefillSlack = 6.f;      // P is held as up to 2^(8 + 6 + 1) p, within fp16
+constexpr float kPrefillFar = 0x1p20f;      // a maximum of this size: scores are taken from it in a step of their own (its last place is 1/8 there)
 
 template <int D> struct PrefillShape {
     static constexpr int WAVES = D == 128 ? 8 : 4, ROWS = 32 * WAVES, THREADS = 64 * WAVES, KEYS = 64;
@@ -175,6 +176,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
     float m = -INFINITY, l = 0.f, v_unit = 1.f, v_peak = 0.f;
+    bool far = false;                                      // the wave's: some row's maximum is past kPrefillFar
     int key0 = part.key_first;
     PrefillBytes<D> even, odd;
     Scales scales;
@@ -273,16 +275,29 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
             top = fmaxf(top, raw * f[g]);
         }
         top = half_pair_max(top);
-        if (__any(top > m + kPrefillSlack)) {
+        if (__any(top - m > kPrefillSlack)) {                // (the difference is exact where it matters, m + 6 is not)
             const float grown = fmaxf(m, top), alpha = grown == -INFINITY ? 1.f : fast_exp2(m - grown);
             m = grown;
+            far = __any(m > kPrefillFar || (m < -kPrefillFar && m > -INFINITY));
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
         }
-        const float frame = (m == -INFINITY ? 0.f : m) - kPrefillShift - v_log;
+        // The exponent is one multiply-add of the score.  Far from zero its rounding, and that of the products which the maximum was taken of, would grow past
+        // what fp16 has room for: there the scores become differences from the maximum first, by the same products.
+        const float base = m == -INFINITY ? 0.f : m;
+        if (__builtin_expect(far, 0)) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int r = 0; r < 8; ++r) s[g / 2][8 * (g % 2) + r] = s[g / 2][8 * (g % 2) + r] * f[g] - base;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) f[g] = far ? 1.f : f[g];      // (chosen here and not in the branch: head_dim 256, 2 x 512 tokens over 30720 keys, 2060 -> 1729 us)
+        const float frame = (far ? 0.f : base) - kPrefillShift - v_log;
         float sum = 0.f;
         v8h pf[4];
 #pragma unroll

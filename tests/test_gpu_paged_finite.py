@@ -27,7 +27,7 @@ def of_page(x, table, z, n):
 
 
 @pytest.mark.parametrize("page", [16, 64])
-@pytest.mark.parametrize("N,d", [(1, 64), (3, 128), (20, 256)])
+@pytest.mark.parametrize("N,d", [(1, 64), (3, 128), (20, 256), (100, 64), (100, 128), (100, 256)])
 @pytest.mark.parametrize("size", [16.0, 19.9, 20.1, 23.0, 24.3, 25.4, 25.8, 26.5, 27.5, 28.4, 30.0, 40.0, 100.0])
 def test_scores_of_any_size(N, d, page, size):
     """Each query is a multiple of one key, whose score in base 2 is about 2^size and several times that of any other: the softmax is that key's, its value the
@@ -56,7 +56,7 @@ def test_scores_of_any_size(N, d, page, size):
 
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("size", [22.0, 23.0, 23.9, 24.6, 26.0, 27.3, 28.6])
-@pytest.mark.parametrize("N", [1])
+@pytest.mark.parametrize("N", [1, 100])
 def test_large_scores_that_grow_slowly(N, page, size):
     """Scores of about 2^size that grow by five in base 2 every 64 keys: a followed maximum may stay behind by as much, and the scales of values double with it."""
     g = torch.Generator().manual_seed(int(10 * size) + page)
