@@ -209,8 +209,9 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
         }
     }
     // To LDS as fp16 with a power of two of the row's own taken out (`factor` gets it back, with the softmax's scale in base 2): the row's largest element
-    // is brought to 2^8, so that neither the range of bf16 nor a rotation leaves fp16's, and what lies under fp16's smallest step is 2^-32 of it.
-    // 16-bit queries are held exactly that way; rotated ones are not 16-bit numbers, and what their rounding leaves goes to q_rest for a second product
+    // is brought to 2^8, so that neither the range of bf16 nor a rotation leaves fp16's at the upper end.  Elements from 2^-22 of the largest one on are held
+    // exactly, smaller ones in steps of 2^-32 of it (a row of less than 2^-100 is brought to less than 2^8: its scores are nothing, whatever the scale of its keys).
+    // Rotated queries are not 16-bit numbers, and what their rounding leaves goes to q_rest for a second product
     // (22 bits; one alone would put 2^-12 of each |q k| into the scores, more than P's rounding does to the result).  Without REST they stay rounded to 11 bits.
     template <bool REST> __device__ __forceinline__ void stage(PagedArgs p, int row0, const v2f* angles, char* q_lds, char* q_rest, float* factor) const {
 #pragma unroll
@@ -246,7 +247,7 @@ template <int D, int DT, int R, int THREADS> struct PagedQueries {
                 top = top > a ? top : a;
             }
             int e = (int)(top >> 23) - 127;
-            e = e < -100 ? -100 : e > 100 ? 100 : e;
+            e = e < -100 ? -100 : e;                       // (the factor below stays a normal number; 128, of a row that is none, leaves one too)
             const float down = copysignf(__builtin_bit_cast(float, (uint32_t)(127 + 8 - e) << 23), p->qk_scale_log2);
             uint32_t h[8];
 #pragma unroll

@@ -75,3 +75,20 @@ def test_large_scores_that_grow_slowly(N, page, size):
     want, want_lse, mean_v, extent = attend(q, cache, table, [n], False, sm)
     assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -18 * extent[..., 0]).all()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("N,d", [(1, 64), (5, 128), (30, 256), (100, 64), (100, 128), (100, 256)])
+@pytest.mark.parametrize("up", [90, 105, 110, 120])
+@pytest.mark.parametrize("rot", [0, 64])
+def test_queries_over_the_range_of_bf16(N, d, page, up, rot):
+    """Queries times 2^up with the softmax's scale by 2^-up: powers of two, so the same bits."""
+    g = torch.Generator().manual_seed(up + N)
+    lens = [N + 90]
+    cache, kv, sc = make_cache(g, 20, 2, page, d)
+    table = make_table(g, lens, page, 20)
+    q = torch.randn((1, 4, N, d), generator=g).bfloat16()
+    kw = dict(freqs=M.rotary_frequencies(rot, device=DEV)[0]) if rot else {}
+    o, lse = call(q, kv, sc, table, lens, d ** -0.5, True, **kw)
+    far, far_lse = call((q.float() * 2.0 ** up).bfloat16(), kv, sc, table, lens, d ** -0.5 * 2.0 ** -up, True, **kw)
+    assert o.isfinite().all() and torch.equal(far, o) and torch.equal(far_lse, lse)
