@@ -19,6 +19,9 @@ constexpr int kPagedWaves = 4;
 // P is held as 2^14 p: fp16 keeps its 11 bits down to p = 2^-28, times the ratio of two pages' scales.  The factor goes in with that ratio, p itself being
 // 2^(s - m) by a subtraction of its own: taken from m beforehand it would be lost to m's rounding, and p past fp16's range, from |m| = 2^25 on.
 constexpr float kPUnit = 0x1p14f;
+// Sums of p v are held as 2^-12 of themselves, so that those of 2^12 values fit fp32 wherever the values do, and the least scale that an append leaves
+// (2^-100) times all of that is a normal number.  Scales under it count as parts of it in P.
+constexpr float kSumUnit = 0x1p-12f, kLeastTop = 0x1p-100f;
 
 // Merges the rows of an item from its pieces: those of workgroups `one` onward, all of them first items of theirs but the one that the item begins in
 // the middle of (first_is_first: it begins at that workgroup's first unit).
@@ -88,7 +91,7 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
         const int row = row0 + r, token = paged_div(row, p->d_group), head = t.hk * p->group + row - token * p->group;
         const bool empty = m == -INFINITY || token >= t.m;
         if (token >= t.m) acc = (v4f){0.f, 0.f, 0.f, 0.f};
-        store_out4<DT>(p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + col * 2, acc * (empty ? 0.f : 1.f / (kPUnit * l)));
+        store_out4<DT>(p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + col * 2, acc * (empty ? 0.f : 1.f / (kSumUnit * l)));
         if (p->lse != nullptr && col == 0)
             p->lse[((int64_t)t.z * p->heads + head) * p->seqlen + token] = token >= t.m ? -INFINITY : m + __builtin_log2f(l);
     }
@@ -241,13 +244,13 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
 #pragma unroll
         for (int g = 0; g < G; ++g) masked = masked || !now.has[g];
         // V's scales relative to the largest of the step's go into P, that one into the sum
-        float v_top = 0x1p-120f;
+        float v_top = kLeastTop;
 #pragma unroll
         for (int g = 0; g < G; ++g) v_top = fmaxf(v_top, now.has[g] ? fabsf(now.vs[g]) : 0.f);
-        const float v_inv = __builtin_amdgcn_rcpf(v_top);
+        const float v_unit = v_top * (kSumUnit / kPUnit), v_inv = kSumUnit * __builtin_amdgcn_rcpf(v_unit);      // = kPUnit / v_top
         float v_rel[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) v_rel[g] = now.has[g] ? now.vs[g] * v_inv * kPUnit : 0.f;
+        for (int g = 0; g < G; ++g) v_rel[g] = now.has[g] ? now.vs[g] * v_inv : 0.f;
         v4f scores[RT][G];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
 #pragma unroll
                 for (int h = 0; h < G / 2; ++h) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[h], pf[rt][h], a, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[rt][j][i] = fmaf(a[i], v_top, o[rt][j][i]);
+                for (int i = 0; i < 4; ++i) o[rt][j][i] = fmaf(a[i], v_unit, o[rt][j][i]);
             }
         };
         static_for<DT16>(tile);
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(64 * kPagedWaves, RT == 1 && D < 256 ? 2 : 1) 
         const int head = t.hk * p->group + row - token * p->group;
         if (row < p->rows) {
             if (part.whole) {
-                const float inv = empty ? 0.f : 1.f / (kPUnit * sum);
+                const float inv = empty ? 0.f : 1.f / (kSumUnit * sum);
                 char* const dst = p->out + t.z * p->o_sb + head * p->o_sh + token * p->o_sn + cols * DT16 * 2;
 #pragma unroll
                 for (int j = 0; j < DT16; j += 4) {

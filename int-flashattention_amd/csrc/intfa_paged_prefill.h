@@ -23,6 +23,7 @@
 namespace intfa {
 
 constexpr float kPrefillShift = 8.f, kPrefillSlack = 6.f;      // P is held as up to 2^(8 + 6 + 1) p, within fp16
+constexpr float kPartUnit = 0x1p-26f;       // partial rows are held as so much of the sums, whose factor is 2^8 to 2^14: those of 2^12 values fit fp32 wherever the values do
 constexpr float kPrefillFar = 0x1p20f;      // a maximum of this size: scores are taken from it in a step of their own (its last place is 1/8 there)
 
 template <int D> struct PrefillShape {
@@ -354,13 +355,13 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
         for (int a = 0; a < D / 32; ++a)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mine.put((uint32_t)(32 * wave), D, 4 * (64 * (4 * a + i) + lane), value(a, i) * v_unit);      // (a wave's stores: 1 KB each)
+            for (int i = 0; i < 4; ++i) mine.put((uint32_t)(32 * wave), D, 4 * (64 * (4 * a + i) + lane), value(a, i) * (v_unit * kPartUnit));      // (a wave's stores: 1 KB each)
         if (lh == 0) mine.put_stats((uint32_t)(32 * wave + lq), m, l);
         if (paged_last_arrival(p, paged_ticket(p, t), &arrival_lds, part.pieces)) {
             // the pieces in their order, each wave its own rows in its own layout
             typedef unsigned v2u __attribute__((ext_vector_type(2)));
             done = true;
-            weight = 1.f;
+            weight = 1.f / kPartUnit;
             m = -INFINITY;
             l = 0.f;
 #pragma unroll

@@ -92,3 +92,22 @@ def test_queries_over_the_range_of_bf16(N, d, page, up, rot):
     o, lse = call(q, kv, sc, table, lens, d ** -0.5, True, **kw)
     far, far_lse = call((q.float() * 2.0 ** up).bfloat16(), kv, sc, table, lens, d ** -0.5 * 2.0 ** -up, True, **kw)
     assert o.isfinite().all() and torch.equal(far, o) and torch.equal(far_lse, lse)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("N,d", [(1, 64), (5, 128), (30, 256), (100, 64), (100, 128), (100, 256)])
+@pytest.mark.parametrize("up", [80, 100, 118])
+def test_values_over_the_range_of_bf16(N, d, page, up):
+    """Values of up to 2^(up + 7), thousands of them in a row with like weights: sums of them fit fp32 for as long as their mean does."""
+    g = torch.Generator().manual_seed(up)
+    lens = [5000, N]
+    pages = 2 * (5000 // page + 3)
+    cache, kv, sc = make_cache(g, pages, 1, page, d)
+    kv[:, 1] = kv[:, 1].abs()
+    sc[:, 1] = 2.0 ** up
+    table = make_table(g, lens, page, pages)
+    q = (0.1 * torch.randn((2, 2, N, d), generator=g)).bfloat16()
+    o, lse = call(q, kv, sc, table, lens, d ** -0.5, True)
+    assert o.isfinite().all() and lse.isfinite().all()
+    want, _, mean_v, extent = attend(q, cache, table, lens, True, d ** -0.5)
+    assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
