@@ -111,3 +111,24 @@ def test_values_over_the_range_of_bf16(N, d, page, up):
     assert o.isfinite().all() and lse.isfinite().all()
     want, _, mean_v, extent = attend(q, cache, table, lens, True, d ** -0.5)
     assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("N,d", [(1, 64), (5, 128), (100, 64), (100, 128), (100, 256)])
+@pytest.mark.parametrize("up,order", [(60, 0), (60, 1), (90, 0), (90, 1), (115, 0), (115, 1)])
+def test_pages_of_zeros_beside_large_values(N, d, page, up, order):
+    """Every other page holds zeros at the least scale that an append leaves, 2^-100; the others' scale is 2^up."""
+    g = torch.Generator().manual_seed(up + page)
+    lens = [700]
+    pages = 700 // page + 3
+    cache, kv, sc = make_cache(g, pages, 1, page, d)
+    table = make_table(g, lens, page, pages)
+    sc[:, 1] = 2.0 ** up
+    zeros = table[0, order::2].long()
+    kv[zeros, 1], sc[zeros, 1] = 0, 2.0 ** -100
+    q = (0.5 * torch.randn((1, 2, N, d), generator=g)).bfloat16()
+    o, lse = call(q, kv, sc, table, lens, d ** -0.5)
+    assert o.isfinite().all() and lse.isfinite().all()
+    want, want_lse, mean_v, extent = attend(q, cache, table, lens, False, d ** -0.5)
+    assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -18 * extent[..., 0]).all()
