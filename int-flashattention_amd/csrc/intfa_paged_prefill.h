@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[dt][r] *= scale;
         }
-        v_top = v_top < 0x1p-60f * v_unit ? 0.f : v_top;     // (under 2^-120 of the largest so far: pages of zeros, say.  The ratio's reciprocal would be none)
-        const float v_ratio = v_top > 0.f ? v_top * __builtin_amdgcn_rcpf(v_unit) : 1.f, v_log = __builtin_amdgcn_logf(v_ratio), v_back = __builtin_amdgcn_rcpf(v_ratio);
+        // (a ratio under 2^-100, of pages of zeros beside large values, say, counts as that: its reciprocal would be none)
+        const float v_ratio = v_top > 0.f ? fmaxf(v_top * __builtin_amdgcn_rcpf(v_unit), 0x1p-100f) : 1.f, v_log = __builtin_amdgcn_logf(v_ratio), v_back = __builtin_amdgcn_rcpf(v_ratio);
         // ---- softmax
         float f[G];
 #pragma unroll
