@@ -10,7 +10,7 @@
 //        tiles are four neighbouring columns.
 // A row's scale of scores and a page's go into one multiplier of the exponent's fused multiply-add (a page's scale is not negative: the maximum of the
 // products is that of the scores).  V's scale goes there too, as log2(scale / reference), the reference being the unit of the accumulators: it follows the
-// page's scale where that leaves 2^-10 .. 2 of it.  A row's maximum is followed where it grows by more than 2^6, so that most blocks rescale nothing.
+// page's scale where that leaves 2^-4 .. 2 of it.  A row's maximum is followed where it grows by more than 2^6, so that most blocks rescale nothing.
 //
 // What bounds it (2 x 32 x 512 bf16 rows of 128 over up to 30720 keys: 953 TFLOP/s of the 1200 that a matrix product of 8192^3 reaches on the same card): per
 // block and SIMD 2050 clocks of products and 2400 of other vector work, two thirds of it the softmax, which hardly run beside each other - 4600 clocks
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
     for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
-    float m = -INFINITY, l = 0.f, v_unit = 1.f, v_peak = 0.f;
+    float m = -INFINITY, l = 0.f, v_unit = 0.f, v_peak = 0.f;      // v_unit: of the accumulators, from the first scale of values on
     bool far = false;                                      // the wave's: some row's maximum is past kPrefillFar
     int key0 = part.key_first;
     PrefillBytes<D> even, odd;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS
         }
         v_top = v_top < 0x1p-120f ? 0.f : v_top;             // (its reciprocal would be none; the append leaves none under 2^-100)
         v_peak = fmaxf(v_peak, v_top);
-        if (v_top > 2.f * v_unit || v_top < 0x1p-10f * v_unit) {
+        if (v_top > 2.f * v_unit || v_top < 0x1p-4f * v_unit) {      // (P, within 2^-4 .. 2 of its own size, has 11 bits down to p = 2^-18)
             const float unit = fmaxf(fmaxf(v_top, v_peak * 0x1p-60f), 0x1p-100f), scale = v_unit / unit;
             v_unit = unit;
 #pragma unroll

@@ -132,3 +132,28 @@ def test_pages_of_zeros_beside_large_values(N, d, page, up, order):
     want, want_lse, mean_v, extent = attend(q, cache, table, lens, False, d ** -0.5)
     assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -12 + 2.0 ** -18 * extent[..., 0]).all()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("N", [1, 70])
+@pytest.mark.parametrize("scale,first", [(2.0 ** -5, 1.0), (2.0 ** -9.9, 1.0), (2.0 ** 9, 1.0), (2.0 ** -3, 2.0 ** 9.9), (2.0 ** -3, 2.0 ** 3.9)])
+def test_many_keys_of_small_weight(N, page, scale, first):
+    """32768 keys that each weigh 2^-14.6 of the first one, and together more than it: their weights keep 11 bits whatever the scale of the values, or one
+    of another page.  512 sequences of the same pages, so that no workgroup has only part of one.  (All weights are the same, so a rounding coarser than that does not average out; in steps of 2^-24 a weight of
+    2^(8 - 9.9 - 14.6033) is 180.6.)"""
+    g = torch.Generator().manual_seed(3)
+    Z, d, n = 512, 64, 1 << 15
+    cache, kv, sc = make_cache(g, n // page, 1, page, d)
+    table = torch.arange(n // page, dtype=torch.int32)[None]
+    kv[:, 0] = 0
+    kv[0, 0, 0, 0, 0] = 100
+    kv[:, 1] = torch.randint(100, 127, (1, 1, 1, d), generator=g, dtype=torch.int8)
+    kv[0, 1] = 0
+    sc[:, 0], sc[:, 1] = 1.0, scale
+    sc[0, 1] = scale * first                                 # (of the first key's page, whose values are zeros)
+    q = torch.zeros((1, 1, N, d), dtype=torch.float16)
+    q[..., 0] = 1.0
+    sm = 14.6033 / 100.0 * math.log(2.0)
+    o, _ = call(q.expand(Z, 1, N, d), kv, sc, table.expand(Z, -1), [n] * Z, sm)
+    want, _, mean_v, extent = attend(q, cache, table, [n], False, sm)
+    assert ((o.double() - want).abs() <= bound(want, mean_v, extent, q.dtype)).all()
