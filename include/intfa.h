@@ -318,7 +318,8 @@ typedef struct intfa_rotary_params {
     int64_t x_stride_b, x_stride_h, x_stride_n;
     int64_t o_stride_b, o_stride_h, o_stride_n;
     const int32_t* positions;          /* device memory: the first row's position of each batch entry, or with positions_per_row every
-                                          row's; NULL: position_first for all entries.  Positions may be negative. */
+                                          row's; NULL: position_first for all entries.  Positions may be negative; rows count on
+                                          from a first position past 32 bits (position_first: refused). */
     int64_t pos_stride_b, pos_stride_n;
     int32_t positions_per_row, position_first;
     intfa_rope rope;                   /* freqs required */

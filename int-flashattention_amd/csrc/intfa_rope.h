@@ -11,9 +11,10 @@ struct RopeArgs {
 };
 
 // magnitude * (cos, sin) of position * freq.  The angle is formed in turns and reduced in fp64: 2^31 positions at one radian each are
-// 3.4e8 turns, whose fp64 error is 4e-8 of a turn (fp32 would have lost the turn itself at 1.7e7).
-__device__ __forceinline__ void rope_angle(double freq, int position, float magnitude, float& c, float& s) {
-    double t = (double)position * freq * 0.15915494309189533577;      // 1 / (2 pi)
+// 3.4e8 turns, of which two products and the constant's rounding lose up to 1.1e-7 of a turn (fp32 would have lost the turn itself at 1.7e7).  position: a
+// whole number (rows count on from a first position of 32 bits, past those too).
+__device__ __forceinline__ void rope_angle(double freq, double position, float magnitude, float& c, float& s) {
+    double t = position * freq * 0.15915494309189533577;      // 1 / (2 pi)
     t -= __builtin_rint(t);
     sincospif(2.0f * (float)t, &s, &c);
     c *= magnitude;

@@ -46,7 +46,9 @@ template <int DT, bool MANY> __global__ void __launch_bounds__(256) rotary_kerne
     request(h0);
     float c[8], s[8];
     if (turns) {
-        const int position = p.positions == nullptr ? p.first + n : p.per_row ? p.positions[b * p.pos_sb + n * p.pos_sn] : p.positions[b * p.pos_sb] + n;
+        const double position = p.positions == nullptr ? (double)(p.first + n)
+                                : p.per_row           ? (double)p.positions[b * p.pos_sb + n * p.pos_sn]
+                                                      : (double)p.positions[b * p.pos_sb] + n;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             rope_angle(p.rope.freqs[8 * u + i], position, p.rope.magnitude, c[i], s[i]);

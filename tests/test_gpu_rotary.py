@@ -66,6 +66,15 @@ def test_far_positions_keep_their_angle():
     check(M.rotary(x.to(DEV), pos.to(DEV), freqs), x, pos, freqs.cpu())
 
 
+@pytest.mark.parametrize("first", [2 ** 31 - 1, 2 ** 31 - 3, -(2 ** 31)])
+def test_rows_count_on_past_32_bits(first):
+    """From a first position on the device that the last rows leave 32 bits behind."""
+    freqs, _ = M.rotary_frequencies(128, base=500000.0, device=DEV)
+    x = torch.randn((2, 2, 9, 128), generator=torch.Generator().manual_seed(10)).bfloat16()
+    out = M.rotary(x.to(DEV), torch.tensor([first, 5], dtype=torch.int32, device=DEV), freqs)
+    check(out, x, torch.tensor([[first], [5]]) + torch.arange(9), freqs.cpu())
+
+
 def test_values_that_are_not_finite_stay_in_their_pair():
     freqs, _ = M.rotary_frequencies(32, device=DEV)
     x = torch.randn((1, 1, 4, 64), generator=torch.Generator().manual_seed(7)).half()
