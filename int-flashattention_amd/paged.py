@@ -32,6 +32,7 @@ def attention_paged_int8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq
     each sequence where they differ; rows past them are zeros.  Row i of m new tokens stands at position seqlens_k - m + i: with
     ``causal`` it sees the keys up to there, and with ``freqs`` the query is rotated by it first.  Rows that see no key are zeros with
     an lse of -inf; tokens of a page that the table does not name are hidden.
+    Like the other attention entry points a forward pass alone: the result requires no gradient and carries no tangent, whatever q does.
     Page scales must not be negative, and have to be finite: one that is not reaches the rows computed together with those that see its page.
     """
     return (_host._native or _host.native()).attention_paged(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens_k, causal, sm_scale,

@@ -2,6 +2,7 @@
 import math
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _host
 
@@ -41,19 +42,31 @@ def rotary_frequencies(rot_dim, base=10000.0, *, scaling=None, factor=1.0, origi
 
 
 class _Rotary(torch.autograd.Function):
+    """The map is linear: its tangent goes through it, its gradient through the transposed one, and either of them may be differentiated again."""
+
     @staticmethod
-    def forward(ctx, x, positions, freqs, interleaved, inverse, magnitude):
-        ctx.save_for_backward(freqs, *([positions] if torch.is_tensor(positions) else []))
-        ctx.rest = (None if torch.is_tensor(positions) else positions, interleaved, inverse, magnitude)
+    def forward(x, positions, freqs, interleaved, inverse, magnitude):
         return _host.native().rotary(x, positions, freqs, interleaved, inverse, magnitude)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def setup_context(ctx, inputs, output):
+        _, positions, freqs, *rest = inputs
+        kept = (freqs, positions) if torch.is_tensor(positions) else (freqs,)
+        ctx.save_for_backward(*kept)
+        ctx.save_for_forward(*kept)
+        ctx.rest = (None if torch.is_tensor(positions) else positions, *rest)
+
+    @staticmethod
     def backward(ctx, grad):
         freqs, *positions = ctx.saved_tensors
         first, interleaved, inverse, magnitude = ctx.rest
-        dx = _host.native().rotary(grad, positions[0] if positions else first, freqs, interleaved, not inverse, magnitude)
-        return dx, None, None, None, None, None
+        return rotary(grad, positions[0] if positions else first, freqs, interleaved=interleaved, inverse=not inverse, magnitude=magnitude), *[None] * 5
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        freqs, *positions = ctx.saved_tensors
+        first, interleaved, inverse, magnitude = ctx.rest
+        return rotary(tangent, positions[0] if positions else first, freqs, interleaved=interleaved, inverse=inverse, magnitude=magnitude)
 
 
 def rotary(x, positions, freqs, *, interleaved=False, inverse=False, magnitude=1.0):
@@ -64,8 +77,9 @@ def rotary(x, positions, freqs, *, interleaved=False, inverse=False, magnitude=1
     ``positions``: an int (row n of every entry stands at positions + n), an int32 [Z] tensor (the first row's position of each
     entry) or an int32 [Z, N] tensor.  Angles are formed and reduced in fp64, so far positions keep theirs.
     ``inverse`` turns by the negative angle, times the same ``magnitude``: the transposed map.  Where x requires a gradient, it
-    goes back through that; a captured backward pass is captured with its forward pass, while no eager graph of x's leaves is alive.
+    goes back through that; tangents of forward mode go through the map itself, and both can be differentiated again (frequencies and positions
+    have neither).  A captured backward pass is captured with its forward pass, while no eager graph of x's leaves is alive.
     """
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or _forward_ad._current_level >= 0:
         return _Rotary.apply(x, positions, freqs, interleaved, inverse, magnitude)
     return (_host._native or _host.native()).rotary(x, positions, freqs, interleaved, inverse, magnitude)

@@ -1,6 +1,7 @@
 """Rotary positions against their formula in float64: layouts, parts of the head, strides, far positions, the gradient."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import int_flashattention_amd as M
 from paged_reference import rotate
@@ -109,6 +110,43 @@ def test_gradient(interleaved):
     check(leaf.grad, torch.ones_like(x), (4 + torch.arange(11)).expand(2, 11), freqs.cpu(), 1.0, interleaved, inverse=True)
     with torch.no_grad():
         assert not M.rotary(leaf, 4, freqs).requires_grad
+
+
+@pytest.mark.parametrize("first", [7, "tensor"])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_tangents(first, inverse):
+    """Forward mode: the map of the tangent, for inputs that require a gradient and for those that do not."""
+    g = torch.Generator().manual_seed(11)
+    freqs, magnitude = M.rotary_frequencies(32, device=DEV, scaling="parts", factor=4.0, original_length=512)
+    x, t = (torch.randn((2, 3, 9, 64), generator=g).half().to(DEV) for _ in range(2))
+    first = torch.tensor([3, 70], dtype=torch.int32, device=DEV) if first == "tensor" else first
+
+    def turn(a):
+        return M.rotary(a, first, freqs, inverse=inverse, interleaved=True, magnitude=magnitude)
+
+    want = turn(t)
+    for leaf in (x, x.clone().requires_grad_()):
+        with forward_ad.dual_level():
+            out, tangent = forward_ad.unpack_dual(turn(forward_ad.make_dual(leaf, t)))
+            assert torch.equal(out, turn(x)) and torch.equal(tangent, want)
+            assert forward_ad.unpack_dual(turn(x)).tangent is None
+    out, tangent = torch.func.jvp(turn, (x,), (t,))
+    assert torch.equal(out, turn(x)) and torch.equal(tangent, want)
+
+
+def test_gradients_of_gradients():
+    """d/dy <R^T y, t> = R t: the backward pass is differentiated, by reverse mode twice and by forward over reverse."""
+    g = torch.Generator().manual_seed(12)
+    freqs, _ = M.rotary_frequencies(64, device=DEV)
+    x, y, t = (torch.randn((1, 2, 5, 64), generator=g).bfloat16().to(DEV) for _ in range(3))
+    x.requires_grad_()
+    y.requires_grad_()
+    dx, = torch.autograd.grad(M.rotary(x, 6, freqs), x, y, create_graph=True)
+    dy, = torch.autograd.grad(dx, y, t)
+    assert torch.equal(dx, M.rotary(y, 6, freqs, inverse=True)) and torch.equal(dy, M.rotary(t, 6, freqs))
+    _, tangent = torch.func.jvp(torch.func.grad(lambda a: (M.rotary(a, 6, freqs).float() ** 2).sum() / 2), (x.detach(),), (t,))
+    want = M.rotary(M.rotary(t, 6, freqs), 6, freqs, inverse=True)
+    assert torch.equal(tangent, want)
 
 
 def test_a_captured_training_step():
