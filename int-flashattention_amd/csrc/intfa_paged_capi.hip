@@ -20,7 +20,7 @@ int check(const intfa_paged_attn_params* p) {
     if (p->rope.freqs != nullptr && !rope_valid(&p->rope, c.head_dim)) return INTFA_ERR_ROPE;
     if (!rows16(p->q, p->q_stride_b, p->q_stride_h, p->q_stride_n) || !rows16(p->out, p->o_stride_b, p->o_stride_h, p->o_stride_n) ||
         !aligned(p->lse, 4) || !aligned(p->seqlens_k, 4) || !aligned(p->seqlens_q, 4) || !aligned(p->rope.freqs, 8)) return INTFA_ERR_ALIGN;
-    if ((int64_t)p->batch * p->heads * p->seqlen >= 1ll << 30) return INTFA_ERR_SHAPE;
+    if (size_product((int64_t)p->batch * p->heads, p->seqlen) >= 1ll << 30) return INTFA_ERR_SHAPE;
     return INTFA_OK;
 }
 

@@ -6,6 +6,12 @@
 
 namespace intfa {
 
+// a * b of sizes that are not negative, the largest number where it does not fit
+inline int64_t size_product(int64_t a, int64_t b) {
+    int64_t c;
+    return __builtin_mul_overflow(a, b, &c) ? INT64_MAX : c;
+}
+
 inline bool rope_valid(const intfa_rope* r, int head_dim) {
     return r->pairs > 0 && r->pairs % 8 == 0 && 2 * (int64_t)r->pairs <= head_dim && r->magnitude > 0.f && r->magnitude <= 3.402823466e38f;
 }

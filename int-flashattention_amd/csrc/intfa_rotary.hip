@@ -311,7 +311,7 @@ int intfa_rotary(const intfa_rotary_params* p, void* stream) {
     if (p->positions == nullptr && (int64_t)p->position_first + p->seqlen > 1ll << 31) return INTFA_ERR_SHAPE;      // positions are 32-bit numbers
     RotaryParams rp{};
     rp.units = d / 16;
-    rp.threads = (int64_t)p->batch * p->seqlen * rp.units;
+    rp.threads = size_product((int64_t)p->batch * p->seqlen, rp.units);
     if (rp.threads >= (1ll << 31) - 256 || p->heads > 65535) return INTFA_ERR_SHAPE;
     rp.x = (const char*)p->x; rp.out = (char*)p->out;
     rp.x_sb = p->x_stride_b * 2; rp.x_sh = p->x_stride_h * 2; rp.x_sn = p->x_stride_n * 2;
@@ -364,10 +364,10 @@ int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream) {
     const int64_t pages = (int64_t)p->batch * ap.slots;
     const int rows = p->seqlen_new < c.page_size ? p->seqlen_new : c.page_size, units = rows * ap.units;
     ap.heads_each = 1;
-    while (units > 64 && ap.heads_each < 8 && ap.heads_each < c.heads_kv && pages * c.heads_kv >= 2ll * ap.heads_each * kComputeUnits) ap.heads_each *= 2;
+    while (units > 64 && ap.heads_each < 8 && ap.heads_each < c.heads_kv && size_product(pages, c.heads_kv) >= 2ll * ap.heads_each * kComputeUnits) ap.heads_each *= 2;
     ap.head_groups = (c.heads_kv + ap.heads_each - 1) / ap.heads_each;
     const int threads = units <= 64 ? 64 : 512;
-    if (pages * ap.head_groups * threads >= 1ll << 32) return INTFA_ERR_SHAPE;      // (threads of a launch are numbered in 32 bits)
+    if (size_product(size_product(pages, ap.head_groups), threads) >= 1ll << 32) return INTFA_ERR_SHAPE;      // (threads of a launch are numbered in 32 bits)
     ap.d_slots = make_fast_div(ap.slots); ap.d_head_groups = make_fast_div(ap.head_groups);
     const dim3 g((unsigned)(pages * ap.head_groups), 2);
 #define INTFA_CALL(DT) do { \

@@ -123,6 +123,14 @@ def test_attention_refusals(kw, code):
     assert _attn(**kw) == code
 
 
+def test_sizes_whose_products_pass_64_bits():
+    assert _rotary(batch=1 << 30, seqlen=1 << 30, head_dim=256) == -7
+    assert _rotary(batch=(1 << 31) - 1, seqlen=(1 << 31) - 1, head_dim=256) == -7
+    assert _append(batch=1 << 30, seqlen_new=1 << 30, cache__page_size=16, cache__table_width=1 << 25, cache__heads_kv=1 << 9) == -7
+    assert _attn(batch=1 << 20, heads=1 << 22, seqlen=1 << 22) == -7
+    assert _capi.load().intfa_paged_attn_workspace_bytes(ctypes.byref(_attn_block(batch=1 << 20, heads=1 << 22, seqlen=1 << 22))) == 0
+
+
 def test_null_blocks():
     lib = _capi.load()
     assert lib.intfa_rotary(None, None) == lib.intfa_paged_append_int8(None, None) == lib.intfa_paged_attn_int8(None, None) == -1
