@@ -1,9 +1,12 @@
 """Rotary positions against their formula in float64: layouts, parts of the head, strides, far positions, the gradient."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import int_flashattention_amd as M
+from int_flashattention_amd import _capi
 from paged_reference import rotate
 
 pytestmark = pytest.mark.gpu
@@ -58,6 +61,50 @@ def test_strides_and_one_position_for_all_rows():
     check(out, x, pos.expand(2, 37), freqs.cpu())
     odd = torch.randn((2, 3, 9, 130), generator=g).bfloat16()[..., 1:129]       # rows that are not 16-byte aligned
     check(M.rotary(odd.to(DEV), 3, freqs), odd.contiguous(), (3 + torch.arange(9)).expand(2, 9), freqs.cpu())
+
+
+MANY_HEADS = [          # (two, four, four, eight and eight heads a thread; the last thread's share is smaller)
+    (1, 5, 4000, 128, 128, False, False, torch.float16),
+    (1, 5, 8000, 128, 64, True, True, torch.bfloat16),
+    (4, 9, 1500, 128, 128, True, False, torch.float16),
+    (4, 13, 3000, 128, 64, False, True, torch.bfloat16),
+    (2, 13, 2100, 256, 80, True, False, torch.float16),
+]
+
+
+@pytest.mark.parametrize("Z,H,N,d,rot,interleaved,inverse,dtype", MANY_HEADS)
+def test_several_heads_a_thread(Z, H, N, d, rot, interleaved, inverse, dtype):
+    g = torch.Generator().manual_seed(N)
+    y = torch.randn((Z, N, H, d), generator=g).to(dtype)                       # (heads side by side)
+    freqs, magnitude = M.rotary_frequencies(rot, device=DEV, scaling="parts", factor=4.0, original_length=2048)
+    first = torch.randint(0, 5000, (Z,), generator=g, dtype=torch.int32)
+    kw = dict(interleaved=interleaved, inverse=inverse, magnitude=magnitude)
+    out = M.rotary(y.to(DEV).transpose(1, 2), first.to(DEV), freqs, **kw)
+    check(out, y.transpose(1, 2), first[:, None] + torch.arange(N), freqs.cpu(), magnitude, interleaved, inverse)
+    leaf = y.transpose(1, 2).contiguous().to(DEV).requires_grad_()
+    grad = torch.randn((Z, H, N, d), generator=g).to(dtype).to(DEV)
+    M.rotary(leaf, first.to(DEV), freqs, **kw).backward(grad)
+    kw["inverse"] = not inverse
+    assert torch.equal(leaf.grad, M.rotary(grad, first.to(DEV), freqs, **kw))
+    check(leaf.grad, grad.cpu(), first[:, None] + torch.arange(N), freqs.cpu(), magnitude, interleaved, not inverse)
+
+
+@pytest.mark.parametrize("Z,H,N,d,rot,interleaved,inverse,dtype", MANY_HEADS + [(2, 3, 7, 64, 32, False, False, torch.float16), (1, 32, 1, 128, 128, True, False, torch.bfloat16)])
+def test_in_place(Z, H, N, d, rot, interleaved, inverse, dtype):
+    """The C entry with out = x gives the bits of a result of its own."""
+    x = torch.randn((Z, H, N, d), generator=torch.Generator().manual_seed(d)).to(dtype).to(DEV)
+    freqs, _ = M.rotary_frequencies(rot, device=DEV)
+    want = M.rotary(x, 11, freqs, interleaved=interleaved, inverse=inverse)
+    p = _capi.RotaryParams()
+    p.x = p.out = x.data_ptr()
+    for t in "xo":
+        setattr(p, f"{t}_stride_b", x.stride(0)); setattr(p, f"{t}_stride_h", x.stride(1)); setattr(p, f"{t}_stride_n", x.stride(2))
+    p.position_first, p.inverse = 11, int(inverse)
+    p.rope.freqs, p.rope.pairs, p.rope.interleaved, p.rope.magnitude = freqs.data_ptr(), freqs.numel(), int(interleaved), 1.0
+    p.batch, p.heads, p.seqlen, p.head_dim, p.dtype = Z, H, N, d, _capi.INTFA_F16 if dtype == torch.float16 else _capi.INTFA_BF16
+    assert _capi.load().intfa_rotary(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(x, want)
 
 
 def test_far_positions_keep_their_angle():
