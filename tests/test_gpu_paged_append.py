@@ -135,3 +135,47 @@ def test_pages_whose_heads_lie_side_by_side():
     M.paged_kvcache_append(side[:, :, 0].transpose(1, 2), s1[:, 0], side[:, :, 1].transpose(1, 2), s1[:, 1], k, v, table, lens)
     M.paged_kvcache_append(plain[:, 0], s2[:, 0], plain[:, 1], s2[:, 1], k, v, table, lens)
     assert torch.equal(side.permute(0, 2, 3, 1, 4), plain) and torch.equal(s1, s2) and plain.any()
+
+
+@pytest.mark.parametrize("rot", [False, True])
+@pytest.mark.parametrize("Z,Hkv,N,d,page,lens,dtype", [
+    (4, 5, 1030, 64, 32, [0, 9, 31, 40], torch.float16),                # two heads a workgroup, then four and eight: the last one's share is smaller
+    (4, 11, 1030, 64, 32, [0, 9, 31, 40], torch.bfloat16),
+    (4, 17, 1030, 64, 32, [3, 0, 64, 100], torch.float16),
+    (2, 7, 4500, 256, 64, [0, 50], torch.bfloat16),                     # two units a thread
+    (2, 2, 520, 256, 256, [0, 100], torch.float16),                     # pages of more units than the threads hold
+    (2, 3, 300, 256, 128, [77, 0], torch.bfloat16),
+    (2, 1, 700, 128, 256, [255, 3], torch.float16),
+])
+def test_large_launches(Z, Hkv, N, d, page, lens, dtype, rot):
+    """Workgroups of several heads, and of pages that the threads read again; values that are not numbers in a middle head and in the last rows of a page."""
+    g = torch.Generator().manual_seed(N + Hkv)
+    k, v = (torch.randn((Z, Hkv, N, d), generator=g).to(dtype) for _ in range(2))
+    last = page - lens[0] % page - 1                                    # the first sequence's last row of its first page
+    for x in (v,) if rot else (k, v):
+        x[0, Hkv // 2, last, 5], x[0, Hkv // 2, last - 1, d - 1] = float("inf"), float("nan")
+        x[1, Hkv - 1, N - 1, 0] = float("-inf")
+    run_both(page, k, v, lens, freqs=M.rotary_frequencies(d, device=DEV)[0] if rot else None)
+
+
+@pytest.mark.parametrize("Z,Hkv,N,d,page", [(4, 11, 1030, 64, 32), (1, 2, 300, 256, 256), (1, 2, 20, 64, 16)])
+def test_rotated_keys_that_are_not_finite(Z, Hkv, N, d, page):
+    """A pair with a NaN becomes zeros, one with an infinity +-127 twice, and the others keep the scale of the finite ones."""
+    g = torch.Generator().manual_seed(37)
+    k = torch.randn((Z, Hkv, N, d), generator=g).half()
+    at = min(page, N) - 1
+    k[0, Hkv // 2, at, 5], k[0, Hkv // 2, at - 2, 9] = float("nan"), float("inf")
+    freqs = M.rotary_frequencies(d, device=DEV)[0]
+    pages = Z * -(-N // page)
+    table = torch.arange(pages, dtype=torch.int32).reshape(Z, -1)
+    kv, sc = torch.zeros((pages, 2, Hkv, page, d), dtype=torch.int8), torch.zeros((pages, 2, Hkv))
+    kv_d, sc_d = kv.to(DEV), sc.to(DEV)
+    M.paged_kvcache_append(kv_d[:, 0], sc_d[:, 0], kv_d[:, 1], sc_d[:, 1], k.to(DEV), k.to(DEV), table.to(DEV), torch.zeros((Z,), dtype=torch.int32, device=DEV), freqs)
+    turned = rotate(k, torch.arange(N).expand(Z, N), freqs.cpu())
+    append(kv[:, 0], sc[:, 0], turned.float(), table, [0] * Z, [N] * Z)
+    got, scale = kv_d[:, 0].cpu(), sc_d[:, 0].cpu()
+    assert scale.isfinite().all() and torch.allclose(scale, sc[:, 0], rtol=3e-6, atol=0.0)
+    off = (got.int() - kv[:, 0].int()).abs()
+    assert off.max() <= 1 and off.float().mean() <= 1e-3
+    first = got[0, Hkv // 2]
+    assert (first[at, [5, 5 + d // 2]] == 0).all() and (first[at - 2, [9, 9 + d // 2]].abs() == 127).all()
