@@ -30,10 +30,12 @@ Plan make_plan(const intfa_paged_attn_params* p) {
     const intfa_paged_cache& c = p->cache;
     Plan a{};
     a.rows = p->heads / c.heads_kv * p->seqlen;
-    // 64 rows of 16 x 8 heads over 8192 keys, us, as tiles of 32 in the decode kernel / in the one for many rows: d64 70 / 73, d128 101 / 161, d256 131 / 211; 128 rows 134 / 76,
-    // 195 / 168, 203 / 214.  Rotated fp16 queries of 256 elements, whose second part (PagedQueries::stage) has no room in the registers of the latter, stay in tiles
-    // of 32: 2 x 512 tokens of 32 heads over 7680 keys 995 us, there 1512 with 740 registers spilled.
-    const bool prefill = a.rows > 64 && !(c.head_dim == 256 && p->dtype == INTFA_F16 && p->rope.freqs != nullptr);
+    // Rows of 16 x 8 heads over 8192 keys, us, as tiles of 32 in the decode kernel / in the one for many rows: 64 rows d64 68 / 68, d128 92 / 151, d256 210 / 315;
+    // 72 rows 108 / 68, 155 / 151, 360 / 315; 128 rows 133 / 70, 184 / 156, 416 / 319.  Rotated fp16 queries take a second product there (PagedQueries::stage), which
+    // puts head_dim 128 behind until 128 rows (72 rows 172 / 204, 128 rows 205 / 209, 160 rows 290 / 215) and has no room in head_dim 256's registers: those
+    // stay in tiles of 32 (2 x 512 tokens of 32 heads over 7680 keys 975 us, there 1512 with 740 registers spilled).
+    const bool two_products = p->dtype == INTFA_F16 && p->rope.freqs != nullptr;
+    const bool prefill = a.rows > (two_products && c.head_dim == 128 ? 128 : 64) && !(two_products && c.head_dim == 256);
     a.sel = {c.head_dim, p->dtype == INTFA_BF16 ? 1 : 0, prefill ? 0 : a.rows <= 16 ? 1 : 2, c.page_size >= (!prefill && c.head_dim == 256 ? 32 : 64)};
     a.slot_rows = prefill ? paged_prefill_rows(c.head_dim) : 16 * a.sel.row_tiles;
     a.tiles = (a.rows + a.slot_rows - 1) / a.slot_rows;

@@ -76,6 +76,17 @@ def test_queries_are_rotated_on_the_way(N, rot, interleaved, dtype):
     run(q, cache, kv, sc, table, lens, True, freqs=freqs, magnitude=magnitude, interleaved=interleaved)
 
 
+@pytest.mark.parametrize("N", [32, 33, 64, 65])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rotated_queries_where_the_kernels_take_turns(N, d, dtype):
+    """64, 66, 128 and 130 rows a K/V head."""
+    lens = [N + 70, N]
+    q, cache, kv, sc, table = problem(92 + N, 2, 4, 2, N, d, 32, lens, dtype)
+    freqs, _ = M.rotary_frequencies(d, device=DEV)
+    run(q, cache, kv, sc, table, lens, True, freqs=freqs)
+
+
 @pytest.mark.parametrize("N,fresh,lens", [(4, [4, 0, 1, 9, -3], [100, 50, 1, 70, 20]), (200, [200, 7, 0, 129], [260, 7, 100, 129]),
                                           (80, [3, 80, 1], [500, 80, 3])])
 def test_new_tokens_of_each_sequence(N, fresh, lens):
