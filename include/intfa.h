@@ -375,8 +375,11 @@ int intfa_paged_append_int8(const intfa_paged_append_params* p, void* stream);
  * that position first where rope.freqs is given, and with causal seeing keys 0 .. n - m + i only.  Rows from m onward and rows that
  * see no key are zeros with lse = -infinity.  lse: as in intfa_fwd_params.
  * Keys and values enter as the numbers that the cache stands for: the int8 values go into 16-bit matrix products as they are, exactly, and
- * scales, which must not be negative, are applied in fp32.  Queries enter exactly, rotated ones to 22 bits (rotated bf16 queries of more than 64 rows a K/V
- * head: to 11); probabilities are rounded to 11 bits; sums are fp32.
+ * scales, which must not be negative, are applied in fp32.  Queries enter exactly down to 2^-22 of their row's largest element and in steps of 2^-32 of it
+ * below; rotated ones to 22 bits (rotated bf16 queries of more than 64 rows a K/V head: to 11).  Scores and sums are fp32 (a score past 2^128 is no number).
+ * Probabilities are rounded to 11 bits, those under 2^-28 of the row's largest one to steps of 2^-38 of it; with more than 64 rows a K/V head under 2^-18, to
+ * steps of 2^-28.  Pages that share 64 keys share these steps: what they are for the one with the largest scale of values, they are times the ratio of the
+ * scales for another.
  * workspace: at least intfa_paged_attn_workspace_bytes(p) bytes of device memory, 16-byte aligned, nothing to clear; two launches that may
  * run at the same time must not share it. */
 typedef struct intfa_paged_attn_params {

@@ -41,7 +41,7 @@ __device__ __forceinline__ void paged_merge(PagedArgs p, const PagedItem& t, int
         const int r = r0 + group % side, rr = r < nrows ? r : nrows - 1;
         v4f acc = {0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
-        auto add = [&](auto many) __attribute__((always_inline)) {      // (so many loads under way together: each takes a microsecond)
+        auto add = [&](auto many) __attribute__((always_inline)) {
             constexpr int U = decltype(many)::value;
             for (int i0 = share; i0 < pieces; i0 += U * shares) {      // (U loads under way together: each takes a microsecond)
                 v4f x[U];

@@ -12,11 +12,11 @@
 // products is that of the scores).  V's scale goes there too, as log2(scale / reference), the reference being the unit of the accumulators: it follows the
 // page's scale where that leaves 2^-4 .. 2 of it.  A row's maximum is followed where it grows by more than 2^6, so that most blocks rescale nothing.
 //
-// What bounds it (2 x 32 x 512 bf16 rows of 128 over up to 30720 keys: 953 TFLOP/s of the 1200 that a matrix product of 8192^3 reaches on the same card): per
+// What bounds it (2 x 32 x 512 bf16 rows of 128 over up to 30720 keys: 534 - 560 us by card, 910 - 955 TFLOP/s of the 1200 that a matrix product of 8192^3 reaches): per
 // block and SIMD 2050 clocks of products and 2400 of other vector work, two thirds of it the softmax, which hardly run beside each other - 4600 clocks
 // pass at 2.2 GHz.  P V under the exponentials of the granule behind (1 - 2 % and a fifth slower at head_dim 256), the next block's conversion under Q K,
 // a barrier every second block, scales by vector loads and 64 rows a wave changed nothing or spilled.  Short calls pay beginning and end besides: 13 us to
-// the first product (of which the queries take 9), 4 to 10 for the partial results and their merge.  (Ragged pair of chunks of 512 over 7680 keys: 118 - 123 us, by card.)
+// the first product (of which the queries take 9), 4 to 10 for the partial results and their merge.  (Ragged pair of chunks of 512 over 7680 keys: 116 - 127 us, by card.)
 #pragma once
 #include "intfa_paged_device.h"
 
@@ -43,8 +43,8 @@ template <int D> struct PrefillBytes {
 };
 
 // REST: rotated fp16 queries, whose scores take a second product (PagedQueries::stage).  Rotated bf16 queries stay rounded to 11 bits here, three more than
-// they came with: a second product costs a third more matrix work and the registers for it (a
-// ragged pair of chunks of 512 tokens over 7680 keys 145 -> 187 us), which head_dim 256 does not have (make_plan).  ONE: a page holds a block's keys.
+// they came with: a second product doubles Q K, which is half more matrix work, and its fragments have no room in the registers (head_dim 128: 73 spilled, or 59
+// with small pages; 2 x 512 tokens over 30720 keys 554 us without it, 742 with it.  head_dim 256: make_plan).  ONE: a page holds a block's keys.
 template <int D, int DT, bool REST, bool ONE>
 __global__ void __launch_bounds__(PrefillShape<D>::THREADS, PrefillShape<D>::WGS * PrefillShape<D>::WAVES / 4) paged_prefill_kernel(const PagedParams) {
     typedef PrefillShape<D> S;

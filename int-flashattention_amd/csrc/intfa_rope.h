@@ -20,10 +20,10 @@ __device__ __forceinline__ void rope_angle(double freq, double position, float m
     c *= magnitude;
     s *= magnitude;
 }
-// (a, b) turned, each product rounded by itself as in the formula
+// (a, b) turned (the compiler fuses one product of each sum into it: at most two roundings)
 __device__ __forceinline__ void rope_turn(float& a, float& b, float c, float s) {
-    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-    b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+    const float x = a * c - b * s;
+    b = b * c + a * s;
     a = x;
 }
 
