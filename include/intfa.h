@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define INTFA_VERSION 9
+#define INTFA_VERSION 10
 
 /* forward variants (one entry point each, below) */
 enum { INTFA_VARIANT_FULL_INT8 = 0, INTFA_VARIANT_HALF_INT8 = 1, INTFA_VARIANT_FP16 = 2 };
@@ -64,7 +64,8 @@ enum {
     INTFA_ERR_SCRATCH = -10,      /* intfa_fwd_full_int8_static: the call's split-KV partials exceed
                                      INTFA_STATIC_SCRATCH_BYTES, or the device index is beyond the table of 64 devices */
     INTFA_ERR_PAGE = -11,         /* page_size not 16, 32, 64, 128 or 256, no page, or a block table without a column */
-    INTFA_ERR_ROPE = -12          /* rotated pairs not a multiple of 8 or more than half of head_dim, or a magnitude that is not a positive number */
+    INTFA_ERR_ROPE = -12,         /* rotated pairs not a multiple of 8 or more than half of head_dim, or a magnitude that is not a positive number */
+    INTFA_ERR_POOL = -13          /* pools of pages: none where some are needed, more than INTFA_MAX_POOLS, or a page of no or negative size */
 };
 
 /*
@@ -398,6 +399,92 @@ typedef struct intfa_paged_attn_params {
 } intfa_paged_attn_params;
 size_t intfa_paged_attn_workspace_bytes(const intfa_paged_attn_params* p);
 int intfa_paged_attn_int8(const intfa_paged_attn_params* p, void* stream);
+
+/* ---- Attention whose keys and values come from one latent vector a token, over pages. */
+
+/* A cache of pages for it: a token is latent_dim int8 numbers followed by rope_dim ones (the rotary key that all heads share), and two fp32 scales, of
+ * its latent part and of its rotary part (a value is its int8 number times the scale of its part).  Pages and block table as in intfa_paged_cache. */
+typedef struct intfa_latent_cache {
+    void* rows;                        /* int8 [num_pages, page_size, latent_dim + rope_dim], a row's numbers contiguous, 16-byte aligned */
+    int64_t r_stride_p, r_stride_n;
+    float* scale;                      /* [num_pages, page_size, 2], a token's two side by side, 8-byte aligned */
+    int64_t s_stride_p, s_stride_n;
+    const int32_t* block_table;        /* device memory [batch, table_width], columns contiguous */
+    int64_t bt_stride_b;
+    int32_t num_pages, page_size, table_width;
+    int32_t latent_dim, rope_dim;      /* 128, 256 or 512; 32 or 64 */
+    int32_t reserved;                  /* set to 0 */
+} intfa_latent_cache;
+
+/* Appends new tokens.  Sequence b holds n = seqlens_k[b] tokens (device memory; negative counts as 0) and its row i goes to position n + i, which is also the
+ * position that its rotary part is turned by (where rope.freqs is given; elements behind the pairs pass unchanged).  With norm_weight the latent part c is
+ * normalised first: c * w / sqrt(mean(c^2) + norm_eps).  All of it in fp32 and without a rounding in between; then for either part x
+ *     scale = max(A / 127, 2^-100), A the part's largest magnitude;   q = rint(x / scale) within +-127.
+ * A NaN becomes 0 and an infinity +-127, and neither counts for A.  Rows past the table's last column, of a page that it does not name, or from
+ * seqlens_new[b] onward (optional; clamped to [0, seqlen_new]) are dropped.  The lengths are the caller's to advance.  No other token of a page is touched. */
+typedef struct intfa_latent_append_params {
+    intfa_latent_cache cache;
+    const void* c_new;                 /* fp16 or bf16 [batch, seqlen_new, latent_dim] and [batch, seqlen_new, rope_dim], rows contiguous, 16-byte aligned */
+    const void* k_new;
+    int64_t cn_stride_b, cn_stride_n;
+    int64_t kn_stride_b, kn_stride_n;
+    const void* norm_weight;           /* optional [latent_dim] of the same type, 16-byte aligned */
+    float norm_eps;                    /* positive and finite where norm_weight is given */
+    int32_t batch, seqlen_new, dtype;
+    const int32_t* seqlens_k;
+    const int32_t* seqlens_new;
+    intfa_rope rope;
+} intfa_latent_append_params;
+int intfa_latent_append_int8(const intfa_latent_append_params* p, void* stream);
+
+/* ---- The pages themselves: which are in use, and by how many sequences.
+ * refs [num_pages] counts the entries of the block table that name a page; one with a count of 0 (or less) is free.  Counts, table and lengths are on the
+ * device and change there, so that captured calls follow them; nothing is read back.  pools: the tensors whose first axis is pages (keys, values, scales, of any
+ * number of layers that share the table): what is copied of a page is page_bytes bytes of each. */
+typedef struct intfa_page_pool {
+    void* data;
+    int64_t page_stride;               /* bytes from page to page */
+    int64_t page_bytes;
+} intfa_page_pool;
+#define INTFA_MAX_POOLS 4096
+
+typedef struct intfa_page_table {
+    int32_t* refs;                     /* [num_pages] */
+    int32_t* block_table;              /* [batch, table_width], columns contiguous */
+    int64_t bt_stride_b;
+    int32_t* seqlens_k;                /* [batch]; not used by intfa_pages_compact */
+    int32_t num_pages, page_size, table_width, batch;      /* page_size: not used by intfa_pages_fork and intfa_pages_compact; positive */
+} intfa_page_table;
+
+/* Copies page src[i] over page dst[i], i < n, in every pool.  Pairs with either outside [0, num_pages) are left out.  A page that is copied to must not stand
+ * in dst twice, nor in src (the result would depend on the order). */
+int intfa_pages_copy(const intfa_page_pool* pools, int32_t num_pools, int32_t num_pages, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
+/* Sequence children[i] becomes what sequence parents[i] is: its row of the table and its length, the counts of its pages one up; what the child named before goes
+ * one down.  All parents are read before any child is written (beams may be exchanged); of equal children the last one counts; pairs with either outside
+ * [0, batch) are left out.  n is at most 4096. */
+int intfa_pages_fork(const intfa_page_table* t, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
+
+/* Sequence sequences[i] (outside [0, batch): left out) keeps its first keep[i] tokens (NULL: none; clamped to [0, its length]): entries of the table behind
+ * them become -1, the counts of their pages one down.  A sequence that stands there twice keeps the least. */
+int intfa_pages_free(const intfa_page_table* t, const int32_t* sequences, const int32_t* keep, int32_t n, void* stream);
+
+/* Room for fresh[b] tokens (or fresh_all, where fresh is NULL) behind the seqlens_k[b] of each sequence.  Columns that these tokens reach and that name no page
+ * get a free one; a page among them that others hold too is replaced by a copy (in every pool) of the sequence's own, unless all others that hold it in the same column get
+ * copies in this call: the last one keeps it.  Free pages are dealt in their order, to sequence 0 first.  granted[b]: tokens that there is room for now, fewer
+ * than asked where the pages ran out or the table ends; pass it to the append as seqlens_new.  (Once the pages have run out, sequences behind are granted
+ * nothing in a page that had to be shared out.)  Lengths are not changed.  batch is at most 8192.
+ * workspace: intfa_pages_reserve_workspace_bytes(t), 16-byte aligned, nothing to clear. */
+size_t intfa_pages_reserve_workspace_bytes(const intfa_page_table* t);
+int intfa_pages_reserve(const intfa_page_table* t, const intfa_page_pool* pools, int32_t num_pools, const int32_t* fresh, int32_t fresh_all, int32_t* granted,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Moves the used pages to the first places, as few as that takes: of U used ones those from place U onward, in their order, to the free places before U, in
+ * theirs.  Counts and table follow (an entry that names a free page becomes -1).  new_index [num_pages]: where each page is now, -1 for those that were free.
+ * workspace: intfa_pages_compact_workspace_bytes(t), 16-byte aligned, nothing to clear. */
+size_t intfa_pages_compact_workspace_bytes(const intfa_page_table* t);
+int intfa_pages_compact(const intfa_page_table* t, const intfa_page_pool* pools, int32_t num_pools, int32_t* new_index, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }

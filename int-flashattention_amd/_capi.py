@@ -11,7 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libintfa.so")
 
-ABI_VERSION = 9          # INTFA_VERSION of include/intfa.h this mirror was written against
+ABI_VERSION = 10         # INTFA_VERSION of include/intfa.h this mirror was written against
 INTFA_F16, INTFA_BF16, INTFA_F32 = 0, 1, 2
 PROUND_REFERENCE, PROUND_RNE = 0, 1
 STATIC_SCRATCH_BYTES = 32 << 20      # INTFA_STATIC_SCRATCH_BYTES
@@ -95,6 +95,34 @@ class PagedAttnParams(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("causal", "batch", "heads", "seqlen", "dtype")])
 
 
+class LatentCache(ctypes.Structure):
+    """Mirror of ``intfa_latent_cache``."""
+    _fields_ = ([("rows", ctypes.c_void_p), ("r_stride_p", ctypes.c_int64), ("r_stride_n", ctypes.c_int64),
+                 ("scale", ctypes.c_void_p), ("s_stride_p", ctypes.c_int64), ("s_stride_n", ctypes.c_int64),
+                 ("block_table", ctypes.c_void_p), ("bt_stride_b", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "table_width", "latent_dim", "rope_dim", "reserved")])
+
+
+class LatentAppendParams(ctypes.Structure):
+    """Mirror of ``intfa_latent_append_params``."""
+    _fields_ = ([("cache", LatentCache), ("c_new", ctypes.c_void_p), ("k_new", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in ("cn", "kn") for a in "bn"]
+                + [("norm_weight", ctypes.c_void_p), ("norm_eps", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("batch", "seqlen_new", "dtype")]
+                + [("seqlens_k", ctypes.c_void_p), ("seqlens_new", ctypes.c_void_p), ("rope", Rope)])
+
+
+class PagePool(ctypes.Structure):
+    """Mirror of ``intfa_page_pool``."""
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("page_bytes", ctypes.c_int64)]
+
+
+class PageTable(ctypes.Structure):
+    """Mirror of ``intfa_page_table``."""
+    _fields_ = ([("refs", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("bt_stride_b", ctypes.c_int64), ("seqlens_k", ctypes.c_void_p)]
+                + [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "table_width", "batch")])
+
+
 VARIANT_FULL_INT8, VARIANT_HALF_INT8, VARIANT_FP16 = 0, 1, 2
 
 EXPORTS = ("intfa_version", "intfa_error_string", "intfa_fwd_block_n", "intfa_fwd_workspace_bytes",
@@ -102,7 +130,9 @@ EXPORTS = ("intfa_version", "intfa_error_string", "intfa_fwd_block_n", "intfa_fw
            "intfa_fwd_full_int8", "intfa_fwd_half_int8", "intfa_fwd_fp16", "intfa_fwd_full_int8_static", "intfa_debug_qk_int32",
            "intfa_quant_pertoken", "intfa_quant_pertensor_workspace_bytes",
            "intfa_quant_pertensor_parts_workspace_bytes", "intfa_quant_pertensor", "intfa_quant_perblock_channel", "intfa_kvcache_append_int8",
-           "intfa_rotary", "intfa_paged_append_int8", "intfa_paged_attn_workspace_bytes", "intfa_paged_attn_int8")
+           "intfa_rotary", "intfa_paged_append_int8", "intfa_paged_attn_workspace_bytes", "intfa_paged_attn_int8",
+           "intfa_latent_append_int8", "intfa_pages_copy", "intfa_pages_fork", "intfa_pages_free", "intfa_pages_reserve_workspace_bytes", "intfa_pages_reserve",
+           "intfa_pages_compact_workspace_bytes", "intfa_pages_compact")
 
 _lib = None
 
@@ -151,12 +181,23 @@ def load():
     lib.intfa_quant_perblock_channel.argtypes = [vp, i64, i64, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp]
     lib.intfa_kvcache_append_int8.restype = ctypes.c_int
     lib.intfa_kvcache_append_int8.argtypes = [ctypes.POINTER(AppendParams), vp]
-    for name, block in (("intfa_rotary", RotaryParams), ("intfa_paged_append_int8", PagedAppendParams), ("intfa_paged_attn_int8", PagedAttnParams)):
+    for name, block in (("intfa_rotary", RotaryParams), ("intfa_paged_append_int8", PagedAppendParams), ("intfa_paged_attn_int8", PagedAttnParams),
+                        ("intfa_latent_append_int8", LatentAppendParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(block), vp]
     lib.intfa_paged_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.intfa_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
+    table, pools, size = ctypes.POINTER(PageTable), ctypes.POINTER(PagePool), ctypes.c_size_t
+    for name, args in (("copy", [pools, i32, i32, vp, vp, i32, vp]), ("fork", [table, vp, vp, i32, vp]), ("free", [table, vp, vp, i32, vp]),
+                       ("reserve", [table, pools, i32, vp, i32, vp, vp, size, vp]), ("compact", [table, pools, i32, vp, vp, size, vp])):
+        fn = getattr(lib, "intfa_pages_" + name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = args
+    for name in ("reserve", "compact"):
+        fn = getattr(lib, f"intfa_pages_{name}_workspace_bytes")
+        fn.restype = size
+        fn.argtypes = [table]
     if lib.intfa_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI version {lib.intfa_version()}, this package expects {ABI_VERSION}: rebuild it")
     _lib = lib

@@ -1,0 +1,482 @@
+// The pages of a cache: copies, and the bookkeeping of who holds which.  See include/intfa.h.
+//
+// Counts, table and lengths stay on the device.  What has an order (free pages are dealt by their index, sequences served by theirs) is done by one workgroup, which
+// walks the counts 4096 at a time; it leaves the pages to copy as a list, and a second launch copies them with the whole card.  Bound by latency: the walk
+// takes about 1.2 us per 4096 counts.  The copies move 16 bytes a lane, four at a time, past the caches.
+#include "intfa_paged_host.h"
+
+using namespace intfa;
+
+namespace {
+
+constexpr int kPoolsEach = 96;                 // pools of a launch (the argument block holds them)
+constexpr int kChunk = 16384;                  // bytes of a page that a workgroup copies at a time
+constexpr int kWalk = 1024;                    // threads that keep the books
+constexpr int kLeastBlocks = 4 * kComputeUnits;
+
+struct PoolArgs {
+    char* data[kPoolsEach];
+    int64_t stride[kPoolsEach], bytes[kPoolsEach];
+    int32_t first[kPoolsEach + 1];             // chunk at which each pool begins within a page
+    int32_t width[kPoolsEach];                 // bytes of a lane's access
+    int32_t pools, num_pages;
+    FastDiv d_chunks;
+};
+struct MoveArgs {
+    const int32_t* src; const int32_t* dst;
+    const int32_t* count;                      // on the device, or nullptr: n of them
+    int32_t n;
+    // compaction: the table's entries follow
+    int32_t* table; const int32_t* new_index; int64_t bt_sb;
+    int32_t batch, table_width;
+};
+
+template <typename W> __device__ __forceinline__ void copy_chunk(const char* src, char* dst, int64_t bytes) {
+    constexpr int B = sizeof(W), MANY = 4;
+    const int n = (int)(bytes / B);
+    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * MANY) {
+        W w[MANY];
+#pragma unroll
+        for (int k = 0; k < MANY; ++k)
+            if (i0 + 256 * k < n) w[k] = __builtin_nontemporal_load((const W*)src + i0 + 256 * k);
+#pragma unroll
+        for (int k = 0; k < MANY; ++k)
+            if (i0 + 256 * k < n) __builtin_nontemporal_store(w[k], (W*)dst + i0 + 256 * k);
+    }
+}
+
+__global__ void __launch_bounds__(256) pages_move_kernel(const PoolArgs a, const MoveArgs m) {
+    const int count = m.count != nullptr ? *m.count : m.n, chunks = a.first[a.pools];
+    const int64_t work = (int64_t)count * chunks;
+    for (int64_t i = blockIdx.x; i < work; i += gridDim.x) {
+        const int pair = work < 1ll << 31 ? fast_div((int)i, a.d_chunks) : (int)(i / chunks), chunk = (int)(i - (int64_t)pair * chunks);
+        const int src = m.src[pair], dst = m.dst[pair];
+        if ((unsigned)src >= (unsigned)a.num_pages || (unsigned)dst >= (unsigned)a.num_pages || src == dst) continue;
+        int p = 0;
+        while (chunk >= a.first[p + 1]) ++p;
+        const int64_t at = (int64_t)(chunk - a.first[p]) * kChunk, left = a.bytes[p] - at, bytes = left < kChunk ? left : kChunk;
+        const char* const from = a.data[p] + src * a.stride[p] + at;
+        char* const to = a.data[p] + dst * a.stride[p] + at;
+        if (a.width[p] == 16) copy_chunk<v4i>(from, to, bytes);
+        else if (a.width[p] == 4) copy_chunk<int32_t>(from, to, bytes);
+        else copy_chunk<int8_t>(from, to, bytes);
+    }
+    if (m.table == nullptr) return;
+    const int64_t entries = (int64_t)m.batch * m.table_width;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
+        const int64_t z = i / m.table_width;
+        int32_t* const at = m.table + z * m.bt_sb + (i - z * m.table_width);
+        const int id = *at;
+        if ((unsigned)id < (unsigned)a.num_pages) *at = m.new_index[id];
+    }
+}
+
+// ---- books
+// Exclusive sum over the workgroup in thread order, and its total.
+__device__ __forceinline__ int scan_all(int mine, int* lds, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    __syncthreads();                           // (the words of the scan before have been read)
+    if (lane == 63) lds[wave] = upto;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWalk / 64; ++w) {
+        const int v = lds[w];
+        before += w < wave ? v : 0;
+        total += v;
+    }
+    return before + upto - mine;
+}
+// Four counts of a thread (those behind the last page: 0 or 1 as `pad` says)
+__device__ __forceinline__ v4i four_counts(const int32_t* refs, int at, int pages, int pad) {
+    v4i r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = at + k < pages ? refs[at + k] : pad;
+    return r;
+}
+
+struct CompactArgs { int32_t* refs; int32_t* new_index; int32_t* src; int32_t* dst; int32_t* count; int32_t num_pages; };
+
+__global__ void __launch_bounds__(kWalk) pages_compact_kernel(const CompactArgs a) {
+    __shared__ int lds[kWalk / 64];
+    const int pages = a.num_pages;
+    int mine = 0, used;
+    for (int at = threadIdx.x; at < pages; at += kWalk) mine += a.refs[at] > 0;
+    scan_all(mine, lds, used);
+    // the used pages from place `used` onward, and the free places before it: as many of both
+    int from = 0, to = 0;
+    for (int at0 = 0; at0 < pages; at0 += 4 * kWalk) {
+        const int at = at0 + 4 * (int)threadIdx.x;
+        const v4i r = four_counts(a.refs, at, pages, 0);
+        int moves = 0, places = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            moves += r[k] > 0 && at + k >= used;
+            places += r[k] <= 0 && at + k < used;
+        }
+        // (at most 4096 of either: both in one word)
+        int both;
+        const int before = scan_all(moves | places << 16, lds, both);
+        int f = from + (before & 0xffff), t = to + (before >> 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (at + k >= pages) break;
+            const bool is_used = r[k] > 0;
+            if (is_used && at + k >= used) a.src[f++] = at + k;
+            else a.new_index[at + k] = is_used ? at + k : -1;
+            if (!is_used && at + k < used) a.dst[t++] = at + k;
+        }
+        from += both & 0xffff;
+        to += both >> 16;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int i = threadIdx.x; i < from; i += kWalk) {
+        const int s = a.src[i], d = a.dst[i];
+        a.new_index[s] = d;
+        a.refs[d] = a.refs[s];
+        a.refs[s] = 0;
+    }
+    if (threadIdx.x == 0) *a.count = from;
+}
+
+struct TableArgs {
+    int32_t* refs; int32_t* table; int64_t bt_sb; int32_t* lens;
+    int32_t num_pages, page_log2, table_width, batch;
+};
+
+__global__ void __launch_bounds__(256) pages_free_kernel(const TableArgs a, const int32_t* sequences, const int32_t* keep) {
+    const int z = sequences[blockIdx.y];
+    if ((unsigned)z >= (unsigned)a.batch) return;
+    int kept = keep != nullptr ? keep[blockIdx.y] : 0;
+    const int held = a.lens[z];                // (it may be shortened by another pair of the same sequence: that one takes what is more then)
+    kept = kept < held ? kept : held;
+    kept = kept < 0 ? 0 : kept;
+    const int column = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    if (column == 0) atomicMin(a.lens + z, kept);
+    // (an entry is taken by one thread, however often the sequence is listed)
+    if (column < a.table_width && (int64_t)column << a.page_log2 >= kept) {
+        const int id = atomicExch(a.table + z * a.bt_sb + column, -1);
+        if ((unsigned)id < (unsigned)a.num_pages) atomicSub(a.refs + id, 1);
+    }
+}
+
+// A workgroup takes some columns of all pairs: it reads the parents' entries to LDS before it writes the children's.
+__global__ void __launch_bounds__(256) pages_fork_kernel(const TableArgs a, const int32_t* parents, const int32_t* children, int n, int columns) {
+    extern __shared__ int32_t fork_lds[];
+    int32_t* const child = fork_lds;           // -1: left out
+    int32_t* const parent = fork_lds + n;
+    int32_t* const entry = fork_lds + 2 * n;   // [n][columns]; the last workgroup's: the lengths
+    const int column0 = (int)blockIdx.x * columns;
+    const bool lengths = blockIdx.x == gridDim.x - 1;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int c = children[i], p = parents[i];
+        const bool ok = (unsigned)c < (unsigned)a.batch && (unsigned)p < (unsigned)a.batch;
+        child[i] = ok ? c : -1;
+        parent[i] = ok ? p : 0;
+    }
+    __syncthreads();
+    const int wide = lengths ? 1 : columns;
+    for (int i = threadIdx.x; i < n * wide; i += 256) {
+        const int k = i / wide, column = column0 + i - k * wide;
+        entry[i] = lengths ? a.lens[parent[k]] : column < a.table_width ? a.table[parent[k] * a.bt_sb + column] : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * wide; i += 256) {
+        const int k = i / wide, column = column0 + i - k * wide, c = child[k];
+        if (c < 0) continue;
+        bool again = false;                    // (the last of equal children counts)
+        for (int o = k + 1; o < n; ++o) again = again || child[o] == c;
+        if (again) continue;
+        if (lengths) {
+            a.lens[c] = entry[i];
+        } else if (column < a.table_width) {
+            int32_t* const at = a.table + c * a.bt_sb + column;
+            const int was = *at, now = entry[i];
+            if (was == now) continue;
+            if ((unsigned)now < (unsigned)a.num_pages) atomicAdd(a.refs + now, 1);
+            if ((unsigned)was < (unsigned)a.num_pages) atomicSub(a.refs + was, 1);
+            *at = now;
+        }
+    }
+}
+
+struct ReserveArgs {
+    TableArgs t;
+    const int32_t* fresh; int32_t fresh_all;
+    int32_t* granted;
+    int32_t* free_list; int32_t* src; int32_t* dst; int32_t* count;      // src, dst: as long as the free list
+};
+
+// The columns that a sequence's fresh tokens reach: [first, end), end at most the table's width.
+__device__ __forceinline__ void reserve_span(const ReserveArgs& a, int z, int& held, int& fresh, int& first, int& end) {
+    held = a.t.lens[z];
+    held = held < 0 ? 0 : held;
+    fresh = a.fresh != nullptr ? a.fresh[z] : a.fresh_all;
+    fresh = fresh < 0 ? 0 : fresh;
+    const int64_t last = ((int64_t)held + fresh + (1ll << a.t.page_log2) - 1) >> a.t.page_log2;
+    first = held >> a.t.page_log2;
+    first = first < a.t.table_width ? first : a.t.table_width;
+    end = fresh == 0 ? first : last < a.t.table_width ? (int)last : a.t.table_width;
+}
+
+// Every sequence needs so many pages: those that it lacks, and copies of those that others hold.  Its page of the first column, which holds its last tokens, is the one that
+// forked sequences share: of all that want a copy of it in this call, the last takes none if nobody else is left.
+__global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs a) {
+    extern __shared__ int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
+    int32_t* const plan_lds = head_lds + a.t.batch;      // [batch]: what becomes of it
+    enum { kKeep = 0, kCopy = 1, kNone = 2 };
+    __shared__ int lds[kWalk / 64];
+    __shared__ int moves_lds;
+    const int pages = a.t.num_pages, Z = a.t.batch;
+    if (threadIdx.x == 0) moves_lds = 0;
+    for (int z = threadIdx.x; z < Z; z += kWalk) {
+        int held, fresh, first, end, head = -1;
+        reserve_span(a, z, held, fresh, first, end);
+        if (first < end) {
+            const int id = a.t.table[z * a.t.bt_sb + first];
+            if ((unsigned)id < (unsigned)pages && a.t.refs[id] > 1) head = id;
+        }
+        head_lds[z] = head;
+    }
+    __syncthreads();
+    auto copies_head = [&](int z, int& before) __attribute__((always_inline)) {
+        const int head = head_lds[z];
+        before = 0;
+        if (head < 0) return false;
+        for (int o = 0; o < z; ++o) before += head_lds[o] == head;
+        return a.t.refs[head] - before > 1;
+    };
+    // needs, in the order of the sequences: granted[z] holds the pages that were dealt before it until its own are
+    int dealt = 0;
+    for (int z0 = 0; z0 < Z; z0 += kWalk) {
+        const int z = z0 + (int)threadIdx.x;
+        int needs = 0, before;
+        if (z < Z) {
+            int held, fresh, first, end;
+            reserve_span(a, z, held, fresh, first, end);
+            for (int c = first; c < end; ++c) {
+                const int id = a.t.table[z * a.t.bt_sb + c];
+                if ((unsigned)id >= (unsigned)pages) ++needs;
+                else if (c == first) needs += copies_head(z, before);
+                else needs += a.t.refs[id] > 1;
+            }
+        }
+        int total;
+        const int ahead = scan_all(needs, lds, total);
+        if (z < Z) a.granted[z] = dealt + ahead;
+        dealt += total;
+    }
+    // as many free pages, in their order
+    int found = 0;
+    for (int at0 = 0; at0 < pages && found < dealt; at0 += 4 * kWalk) {
+        const int at = at0 + 4 * (int)threadIdx.x;
+        const v4i r = four_counts(a.t.refs, at, pages, 1);
+        int mine = 0, total;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine += r[k] <= 0;
+        int f = found + scan_all(mine, lds, total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r[k] <= 0) {
+                if (f < dealt) a.free_list[f] = at + k;
+                ++f;
+            }
+        found += total;
+    }
+    found = found < dealt ? found : dealt;
+    __threadfence_block();
+    __syncthreads();
+    for (int z = threadIdx.x; z < Z; z += kWalk) {
+        int before;
+        const bool copies = copies_head(z, before);
+        plan_lds[z] = copies ? kCopy : before > 0 && a.granted[z] > found ? kNone : kKeep;      // (none: another was to leave it and could not)
+    }
+    for (int z = threadIdx.x; z < Z; z += kWalk) {
+        int held, fresh, first, end;
+        reserve_span(a, z, held, fresh, first, end);
+        int rank = a.granted[z], room = end;                 // columns before `room` can be written
+        const int plan = plan_lds[z];
+        if (plan == kNone) room = first;
+        for (int c = first; c < room; ++c) {
+            int32_t* const at = a.t.table + z * a.t.bt_sb + c;
+            const int id = *at;
+            const bool named = (unsigned)id < (unsigned)pages;
+            const bool copy = named && (c == first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
+            if (named && !copy) continue;
+            if (rank >= found) {
+                room = c;
+                break;
+            }
+            const int page = a.free_list[rank++];
+            a.t.refs[page] = 1;
+            if (copy) {
+                const int m = atomicAdd(&moves_lds, 1);
+                a.src[m] = id;
+                a.dst[m] = page;
+            }
+            *at = page;
+        }
+        const int64_t places = ((int64_t)room << a.t.page_log2) - held;
+        a.granted[z] = places <= 0 ? 0 : places < fresh ? (int)places : fresh;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int m = threadIdx.x; m < moves_lds; m += kWalk) atomicSub(a.t.refs + a.src[m], 1);
+    if (threadIdx.x == 0) *a.count = moves_lds;
+}
+
+// ---- host
+int check_pools(const intfa_page_pool* pools, int32_t n) {
+    if (n < 0 || n > INTFA_MAX_POOLS || (n > 0 && pools == nullptr)) return INTFA_ERR_POOL;
+    for (int i = 0; i < n; ++i) {
+        if (pools[i].data == nullptr) return INTFA_ERR_NULL;
+        if (pools[i].page_bytes <= 0 || pools[i].page_bytes > 1ll << 40) return INTFA_ERR_POOL;
+    }
+    return INTFA_OK;
+}
+int check_table(const intfa_page_table* t, bool lens, bool page) {
+    if (t == nullptr || t->refs == nullptr || t->block_table == nullptr || (lens && t->seqlens_k == nullptr)) return INTFA_ERR_NULL;
+    if (t->num_pages <= 0 || t->num_pages >= 1 << 30 || t->table_width <= 0 || t->table_width >= 1 << 30) return INTFA_ERR_PAGE;
+    if (t->batch <= 0) return INTFA_ERR_SHAPE;
+    if (page && (t->page_size < 16 || t->page_size > 256 || (t->page_size & (t->page_size - 1)))) return INTFA_ERR_PAGE;
+    if ((reinterpret_cast<uintptr_t>(t->refs) | reinterpret_cast<uintptr_t>(t->block_table) | reinterpret_cast<uintptr_t>(t->seqlens_k)) & 3u) return INTFA_ERR_ALIGN;
+    return INTFA_OK;
+}
+TableArgs table_args(const intfa_page_table* t) {
+    return {t->refs, t->block_table, t->bt_stride_b, t->seqlens_k, t->num_pages, t->page_size > 0 ? __builtin_ctz((unsigned)t->page_size) : 0, t->table_width, t->batch};
+}
+// The copies of the list in all pools, kPoolsEach of them a launch; the table follows in the last one.  most: of the list.
+int launch_moves(const intfa_page_pool* pools, int num_pools, int num_pages, MoveArgs m, int most, hipStream_t stream) {
+    int32_t* const table = m.table;
+    for (int at = 0; at < num_pools || (at == 0 && table != nullptr); at += kPoolsEach) {
+        PoolArgs a{};
+        a.pools = num_pools - at < kPoolsEach ? num_pools - at : kPoolsEach;
+        a.num_pages = num_pages;
+        int64_t chunks = 0;
+        for (int i = 0; i < a.pools; ++i) {
+            const intfa_page_pool& p = pools[at + i];
+            a.data[i] = (char*)p.data; a.stride[i] = p.page_stride; a.bytes[i] = p.page_bytes;
+            const uint64_t all = (uint64_t)reinterpret_cast<uintptr_t>(p.data) | (uint64_t)p.page_stride | (uint64_t)p.page_bytes;
+            a.width[i] = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+            a.first[i] = (int32_t)chunks;
+            chunks += (p.page_bytes + kChunk - 1) / kChunk;
+            if (chunks >= 1ll << 31) return INTFA_ERR_POOL;
+        }
+        a.first[a.pools] = (int32_t)chunks;
+        a.d_chunks = make_fast_div(chunks > 0 ? (int)chunks : 1);
+        m.table = at + kPoolsEach >= num_pools ? table : nullptr;
+        const int64_t work = size_product(most, chunks), entries = m.table != nullptr ? ((int64_t)m.batch * m.table_width + 255) / 256 : 0;
+        // Workgroups: one a chunk while that is few, and not so many that those which find the list short cost more than the list
+        int64_t grid = work > entries ? work : entries;
+        grid = grid < 1 ? 1 : grid < 8 * kLeastBlocks ? grid : 8 * kLeastBlocks;
+        hipLaunchKernelGGL(pages_move_kernel, dim3((unsigned)grid), dim3(256), 0, stream, a, m);
+        const int rc = (int)hipGetLastError();
+        if (rc != 0) return rc;
+    }
+    return INTFA_OK;
+}
+int64_t reserve_most(const intfa_page_table* t) {       // pages that a call can deal at most
+    const int64_t entries = size_product(t->batch, t->table_width);
+    return entries < t->num_pages ? entries : t->num_pages;
+}
+
+}  // namespace
+
+extern "C" {
+
+int intfa_pages_copy(const intfa_page_pool* pools, int32_t num_pools, int32_t num_pages, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+    if (num_pools <= 0) return INTFA_ERR_POOL;
+    const int rc = check_pools(pools, num_pools);
+    if (rc != INTFA_OK) return rc;
+    if (src == nullptr || dst == nullptr) return INTFA_ERR_NULL;
+    if (num_pages <= 0) return INTFA_ERR_PAGE;
+    if (n <= 0) return INTFA_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3u) return INTFA_ERR_ALIGN;
+    MoveArgs m{};
+    m.src = src; m.dst = dst; m.n = n;
+    return launch_moves(pools, num_pools, num_pages, m, n, (hipStream_t)stream);
+}
+
+int intfa_pages_fork(const intfa_page_table* t, const int32_t* parents, const int32_t* children, int32_t n, void* stream) {
+    const int rc = check_table(t, true, false);
+    if (rc != INTFA_OK) return rc;
+    if (parents == nullptr || children == nullptr) return INTFA_ERR_NULL;
+    if (n <= 0 || n > 4096) return INTFA_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(parents) | reinterpret_cast<uintptr_t>(children)) & 3u) return INTFA_ERR_ALIGN;
+    // Columns of a workgroup: 1024 entries in four rounds, or one column
+    const int columns = n >= 1024 ? 1 : 1024 / n < 64 ? 1024 / n : 64;
+    const unsigned groups = (unsigned)((t->table_width + columns - 1) / columns);
+    hipLaunchKernelGGL(pages_fork_kernel, dim3(groups + 1), dim3(256), (size_t)(2 + columns) * n * 4, (hipStream_t)stream, table_args(t), parents, children, n, columns);
+    return (int)hipGetLastError();
+}
+
+int intfa_pages_free(const intfa_page_table* t, const int32_t* sequences, const int32_t* keep, int32_t n, void* stream) {
+    const int rc = check_table(t, true, true);
+    if (rc != INTFA_OK) return rc;
+    if (sequences == nullptr) return INTFA_ERR_NULL;
+    if (n <= 0 || n > 65535) return INTFA_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(sequences) | reinterpret_cast<uintptr_t>(keep)) & 3u) return INTFA_ERR_ALIGN;
+    const unsigned groups = (unsigned)((t->table_width + 255) / 256);
+    if (size_product((int64_t)groups * 256, n) >= 1ll << 32) return INTFA_ERR_SHAPE;
+    hipLaunchKernelGGL(pages_free_kernel, dim3(groups, (unsigned)n), dim3(256), 0, (hipStream_t)stream, table_args(t), sequences, keep);
+    return (int)hipGetLastError();
+}
+
+size_t intfa_pages_reserve_workspace_bytes(const intfa_page_table* t) {
+    return check_table(t, true, true) == INTFA_OK ? (size_t)(16 + 12 * reserve_most(t)) : 0;
+}
+
+int intfa_pages_reserve(const intfa_page_table* t, const intfa_page_pool* pools, int32_t num_pools, const int32_t* fresh, int32_t fresh_all, int32_t* granted,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_table(t, true, true);
+    if (rc != INTFA_OK) return rc;
+    rc = check_pools(pools, num_pools);
+    if (rc != INTFA_OK) return rc;
+    if (granted == nullptr) return INTFA_ERR_NULL;
+    if (t->batch > 8192 || size_product(t->batch, t->table_width) >= 1ll << 31) return INTFA_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(fresh) | reinterpret_cast<uintptr_t>(granted)) & 3u) return INTFA_ERR_ALIGN;
+    const int64_t most = reserve_most(t);
+    if (workspace == nullptr || workspace_bytes < (size_t)(16 + 12 * most) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return INTFA_ERR_WORKSPACE;
+    int32_t* const words = (int32_t*)workspace;
+    ReserveArgs a{table_args(t), fresh, fresh_all, granted, words + 4, words + 4 + most, words + 4 + 2 * most, words};
+    hipLaunchKernelGGL(pages_reserve_kernel, dim3(1), dim3(kWalk), (size_t)t->batch * 8, (hipStream_t)stream, a);
+    rc = (int)hipGetLastError();
+    if (rc != 0 || num_pools == 0) return rc;
+    MoveArgs m{};
+    m.src = a.src; m.dst = a.dst; m.count = a.count;
+    return launch_moves(pools, num_pools, t->num_pages, m, (int)most < t->batch ? (int)most : t->batch, (hipStream_t)stream);
+}
+
+size_t intfa_pages_compact_workspace_bytes(const intfa_page_table* t) {
+    return check_table(t, false, false) == INTFA_OK ? 16 + 8 * (size_t)t->num_pages : 0;
+}
+
+int intfa_pages_compact(const intfa_page_table* t, const intfa_page_pool* pools, int32_t num_pools, int32_t* new_index, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+    int rc = check_table(t, false, false);
+    if (rc != INTFA_OK) return rc;
+    rc = check_pools(pools, num_pools);
+    if (rc != INTFA_OK) return rc;
+    if (new_index == nullptr) return INTFA_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(new_index) & 3u) return INTFA_ERR_ALIGN;
+    if (workspace == nullptr || workspace_bytes < 16 + 8 * (size_t)t->num_pages || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return INTFA_ERR_WORKSPACE;
+    int32_t* const words = (int32_t*)workspace;
+    const CompactArgs a{t->refs, new_index, words + 4, words + 4 + t->num_pages, words, t->num_pages};
+    hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(kWalk), 0, (hipStream_t)stream, a);
+    rc = (int)hipGetLastError();
+    if (rc != 0) return rc;
+    MoveArgs m{};
+    m.src = a.src; m.dst = a.dst; m.count = a.count;
+    m.table = t->block_table; m.new_index = new_index; m.bt_sb = t->bt_stride_b; m.batch = t->batch; m.table_width = t->table_width;
+    return launch_moves(pools, num_pools, t->num_pages, m, t->num_pages / 2 + 1, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -21,6 +21,7 @@
 #include <atomic>
 #include <climits>
 #include <string>
+#include <vector>
 
 #include "../../include/intfa.h"
 
@@ -619,10 +620,266 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the latent cache
+// Rows, scales and the block table of a latent cache, checked against [Z] sequences.
+intfa_latent_cache latent_cache_arg(const Tensor& rows, const Tensor& scale, const Tensor& table, int64_t Z, int64_t dc, int64_t dr, const Tensor& like) {
+    if (dc != 128 && dc != 256 && dc != 512) fail(PyExc_AssertionError, "the latent part must have 128, 256 or 512 elements, got " + std::to_string(dc));
+    if (dr != 32 && dr != 64) fail(PyExc_AssertionError, "the rotary part must have 32 or 64 elements, got " + std::to_string(dr));
+    if (rows.scalar_type() != ScalarType::Char || rows.dim() != 3 || rows.size(2) != dc + dr)
+        fail(PyExc_ValueError, "cache must be an int8 [pages, page_size, " + std::to_string(dc + dr) + "] tensor (latent and rotary part)");
+    const int64_t pages = rows.size(0), page = rows.size(1);
+    if (scale.scalar_type() != ScalarType::Float || scale.dim() != 3 || scale.size(0) != pages || scale.size(1) != page || scale.size(2) != 2)
+        fail(PyExc_ValueError, "scale must be a float32 [pages, page_size, 2] tensor");
+    if (table.scalar_type() != ScalarType::Int || table.dim() != 2 || table.size(0) != Z || (table.size(1) > 1 && table.stride(1) != 1))
+        fail(PyExc_ValueError, "block_table must be an int32 [Z, columns] tensor with contiguous columns");
+    require_on(rows, like, "cache"); require_on(scale, like, "scale"); require_on(table, like, "block_table");
+    if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256) fail(PyExc_ValueError, "page_size must be 16, 32, 64, 128 or 256, got " + std::to_string(page));
+    if (pages == 0 || pages > INT_MAX || table.size(1) == 0 || table.size(1) > INT_MAX) fail(PyExc_ValueError, "a paged cache needs at least one page and one column of block_table");
+    if (rows.stride(2) != 1 || reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 != 0 || rows.stride(0) % 16 != 0 || rows.stride(1) % 16 != 0)
+        fail(PyExc_ValueError, "rows of cache must be contiguous, and pages and rows 16-byte aligned (the cache is used in place)");
+    if (scale.stride(2) != 1 || reinterpret_cast<uintptr_t>(scale.data_ptr()) % 8 != 0 || scale.stride(0) % 2 != 0 || scale.stride(1) % 2 != 0)
+        fail(PyExc_ValueError, "the two scales of a token must lie side by side, 8-byte aligned (the cache is used in place)");
+    intfa_latent_cache c{};
+    c.rows = rows.data_ptr(); c.r_stride_p = rows.stride(0); c.r_stride_n = rows.stride(1);
+    c.scale = scale.data_ptr<float>(); c.s_stride_p = scale.stride(0); c.s_stride_n = scale.stride(1);
+    c.block_table = table.data_ptr<int32_t>(); c.bt_stride_b = table.stride(0);
+    c.num_pages = (int)pages; c.page_size = (int)page; c.table_width = (int)table.size(1); c.latent_dim = (int)dc; c.rope_dim = (int)dr;
+    return c;
+}
+
+// paged_latent_append(cache, scale, c_new, k_new, block_table, seqlens_k, freqs, interleaved, magnitude, seqlens_new, norm_weight, norm_eps)
+PyObject* paged_latent_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 12, "paged_latent_append");
+    const Tensor &rows = tensor_arg(a[0], "cache"), &scale = tensor_arg(a[1], "scale"), &c_new = tensor_arg(a[2], "c_new"), &k_new = tensor_arg(a[3], "k_new");
+    const Tensor &table = tensor_arg(a[4], "block_table"), &lens = tensor_arg(a[5], "seqlens_k"), &freqs = optional_tensor_arg(a[6], "freqs");
+    const Tensor &fresh = optional_tensor_arg(a[9], "seqlens_new"), &weight = optional_tensor_arg(a[10], "norm_weight");
+    if (!c_new.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd.paged_latent_append runs on the GPU only; got a CPU tensor");
+    if (quant_dtype(c_new) < 0 || k_new.scalar_type() != c_new.scalar_type()) fail(PyExc_TypeError, "new latent vectors and rotary keys must both be fp16 or both bf16");
+    if (c_new.dim() != 3 || k_new.dim() != 3 || k_new.size(0) != c_new.size(0) || k_new.size(1) != c_new.size(1))
+        fail(PyExc_ValueError, "c_new and k_new must be [Z, N_new, latent_dim] and [Z, N_new, rope_dim]");
+    require_on(k_new, c_new, "k_new");
+    const int64_t Z = c_new.size(0), dc = c_new.size(2), dr = k_new.size(2);
+    intfa_latent_append_params p{};
+    p.cache = latent_cache_arg(rows, scale, table, Z, dc, dr, c_new);
+    const CallDevice dev(c_new);
+    const Tensor cn = row_major(c_new, dc, 2), kn = row_major(k_new, dr, 2);
+    Tensor freqs_, fresh_, weight_;
+    const Tensor lens_ = lengths_arg(lens, Z, c_new, "seqlens_k");
+    if (fresh.defined()) fresh_ = lengths_arg(fresh, Z, c_new, "seqlens_new");
+    p.rope = rope_arg(freqs, bool_arg(a[7]), float_arg(a[8]), c_new, dr, &freqs_);
+    if (weight.defined()) {
+        if (weight.scalar_type() != c_new.scalar_type() || weight.dim() != 1 || weight.size(0) != dc)
+            fail(PyExc_ValueError, "norm_weight must have c_new's dtype and shape (" + std::to_string(dc) + ",)");
+        require_on(weight, c_new, "norm_weight");
+        weight_ = row_major(weight, dc, 2);
+        p.norm_weight = weight_.data_ptr();
+        p.norm_eps = (float)float_arg(a[11]);
+        if (!(p.norm_eps > 0.f) || p.norm_eps > 3.402823466e38f) fail(PyExc_ValueError, "norm_eps must be a positive number");
+    }
+    if (cn.numel() == 0) Py_RETURN_NONE;
+    p.c_new = cn.data_ptr(); p.cn_stride_b = cn.stride(0); p.cn_stride_n = cn.stride(1);
+    p.k_new = kn.data_ptr(); p.kn_stride_b = kn.stride(0); p.kn_stride_n = kn.stride(1);
+    p.seqlens_k = lens_.data_ptr<int32_t>();
+    p.seqlens_new = fresh_.defined() ? fresh_.data_ptr<int32_t>() : nullptr;
+    p.batch = (int)Z; p.seqlen_new = (int)cn.size(1); p.dtype = quant_dtype(cn);
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_latent_append_int8(&p, st); }), "intfa_latent_append_int8");
+    for (const Tensor* t : {&rows, &scale, &table, &cn, &kn, &lens_, const_cast<const Tensor*>(&fresh_), const_cast<const Tensor*>(&freqs_), const_cast<const Tensor*>(&weight_)})
+        dev.used(*t);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- pages
+// A sequence of tensors whose first axis is pages.
+std::vector<Tensor> pools_arg(PyObject* o, std::vector<intfa_page_pool>* pools) {
+    PyObject* const fast = PySequence_Fast(o, "caches must be a sequence of tensors");
+    if (fast == nullptr) throw python_error();
+    std::vector<Tensor> held;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
+    bool tensors = true;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* const item = PySequence_Fast_GET_ITEM(fast, i);
+        tensors = tensors && THPVariable_Check(item);
+        if (tensors) held.push_back(THPVariable_Unpack(item));
+    }
+    Py_DECREF(fast);
+    if (!tensors) fail(PyExc_TypeError, "caches must be a sequence of tensors");
+    if (n > INTFA_MAX_POOLS) fail(PyExc_ValueError, "at most " + std::to_string(INTFA_MAX_POOLS) + " caches, got " + std::to_string(n));
+    for (const Tensor& t : held) {
+        if (t.dim() < 1 || t.size(0) == 0 || t.size(0) > INT_MAX || t.numel() == 0) fail(PyExc_ValueError, "caches must be tensors of pages: [pages, ...], none of them empty");
+        if (!t.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd kernels run on the GPU only; got a CPU tensor");
+        require_on(t, held[0], "every cache");
+        if (t.size(0) != held[0].size(0)) fail(PyExc_ValueError, "caches must have one number of pages");
+        if (!t.select(0, 0).is_contiguous()) fail(PyExc_ValueError, "a page of a cache must be contiguous (pages may lie apart)");
+        pools->push_back({t.data_ptr(), t.stride(0) * (int64_t)t.element_size(), t.numel() / t.size(0) * (int64_t)t.element_size()});
+    }
+    return held;
+}
+// int32 on the device of `like`, changed in place
+void books_arg(const Tensor& t, int64_t dims, const Tensor& like, const char* name) {
+    if (!t.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd kernels run on the GPU only; got a CPU tensor");
+    if (t.scalar_type() != ScalarType::Int || t.dim() != dims) fail(PyExc_ValueError, std::string(name) + " must be an int32 tensor of " + std::to_string(dims) + (dims == 1 ? " dimension" : " dimensions"));
+    require_on(t, like, name);
+    if (t.size(-1) > 1 && t.stride(-1) != 1) fail(PyExc_ValueError, std::string(name) + " must be contiguous along its last dimension (it is changed in place)");
+}
+intfa_page_table page_table_arg(const Tensor& refs, const Tensor& table, const Tensor& lens) {
+    books_arg(refs, 1, refs, "refs");
+    books_arg(table, 2, refs, "block_table");
+    if (refs.size(0) == 0 || refs.size(0) >= 1 << 30) fail(PyExc_ValueError, "refs must hold a count for each page, at least one and fewer than 2^30");
+    if (table.size(1) >= 1 << 30 || table.size(0) > INT_MAX) fail(PyExc_ValueError, "block_table has too many columns or rows");
+    intfa_page_table t{};
+    if (lens.defined()) {
+        books_arg(lens, 1, refs, "seqlens_k");
+        if (lens.size(0) != table.size(0)) fail(PyExc_ValueError, "seqlens_k must hold a length for each row of block_table");
+        t.seqlens_k = lens.data_ptr<int32_t>();
+    }
+    t.refs = refs.data_ptr<int32_t>(); t.block_table = table.data_ptr<int32_t>(); t.bt_stride_b = table.stride(0);
+    t.num_pages = (int)refs.size(0); t.table_width = (int)table.size(1); t.batch = (int)table.size(0);
+    return t;
+}
+int32_t page_size_arg(PyObject* o) {
+    const int page = int32_arg(o, "page_size");
+    if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256) fail(PyExc_ValueError, "page_size must be 16, 32, 64, 128 or 256, got " + std::to_string(page));
+    return page;
+}
+// int32 [n] on the device of `like` (read only: copied where it is not contiguous)
+Tensor indices_arg(const Tensor& t, const Tensor& like, const char* name) {
+    if (t.scalar_type() != ScalarType::Int || t.dim() != 1 || t.size(0) > INT_MAX) fail(PyExc_ValueError, std::string(name) + " must be a one-dimensional int32 tensor");
+    require_on(t, like, name);
+    return t.contiguous();
+}
+
+// paged_copy(caches, src, dst)
+PyObject* paged_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 3, "paged_copy");
+    std::vector<intfa_page_pool> pools;
+    const std::vector<Tensor> held = pools_arg(a[0], &pools);
+    if (held.empty()) fail(PyExc_ValueError, "caches must hold at least one tensor");
+    const CallDevice dev(held[0]);
+    const Tensor src = indices_arg(tensor_arg(a[1], "src"), held[0], "src"), dst = indices_arg(tensor_arg(a[2], "dst"), held[0], "dst");
+    if (src.size(0) != dst.size(0)) fail(PyExc_ValueError, "src and dst must hold as many pages");
+    if (src.size(0) == 0) Py_RETURN_NONE;
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_pages_copy(pools.data(), (int)pools.size(), (int)held[0].size(0), src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), (int)src.size(0), st); }),
+             "intfa_pages_copy");
+    for (const Tensor& t : held) dev.used(t);
+    dev.used(src); dev.used(dst);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_fork(refs, block_table, seqlens_k, parents, children)
+PyObject* paged_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 5, "paged_fork");
+    const Tensor &refs = tensor_arg(a[0], "refs"), &table = tensor_arg(a[1], "block_table"), &lens = tensor_arg(a[2], "seqlens_k");
+    const intfa_page_table t = page_table_arg(refs, table, lens);
+    const CallDevice dev(refs);
+    const Tensor parents = indices_arg(tensor_arg(a[3], "parents"), refs, "parents"), children = indices_arg(tensor_arg(a[4], "children"), refs, "children");
+    if (parents.size(0) != children.size(0)) fail(PyExc_ValueError, "parents and children must hold as many sequences");
+    if (parents.size(0) > 4096) fail(PyExc_ValueError, "at most 4096 sequences are forked in a call, got " + std::to_string(parents.size(0)));
+    if (parents.size(0) == 0 || table.numel() == 0) Py_RETURN_NONE;
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_pages_fork(&t, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), (int)parents.size(0), st); }), "intfa_pages_fork");
+    for (const Tensor* x : {&refs, &table, &lens, &parents, &children}) dev.used(*x);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_free(refs, block_table, seqlens_k, sequences, page_size, keep)
+PyObject* paged_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 6, "paged_free");
+    const Tensor &refs = tensor_arg(a[0], "refs"), &table = tensor_arg(a[1], "block_table"), &lens = tensor_arg(a[2], "seqlens_k"), &keep = optional_tensor_arg(a[5], "keep");
+    intfa_page_table t = page_table_arg(refs, table, lens);
+    t.page_size = page_size_arg(a[4]);
+    const CallDevice dev(refs);
+    const Tensor sequences = indices_arg(tensor_arg(a[3], "sequences"), refs, "sequences");
+    Tensor keep_;
+    if (keep.defined()) {
+        keep_ = indices_arg(keep, refs, "keep");
+        if (keep_.size(0) != sequences.size(0)) fail(PyExc_ValueError, "sequences and keep must hold as many numbers");
+    }
+    if (sequences.size(0) > 65535) fail(PyExc_ValueError, "at most 65535 sequences are freed in a call, got " + std::to_string(sequences.size(0)));
+    if (sequences.size(0) == 0 || table.numel() == 0) Py_RETURN_NONE;
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_pages_free(&t, sequences.data_ptr<int32_t>(), keep_.defined() ? keep_.data_ptr<int32_t>() : nullptr, (int)sequences.size(0), st); }),
+             "intfa_pages_free");
+    for (const Tensor* x : {&refs, &table, &lens, &sequences, const_cast<const Tensor*>(&keep_)}) dev.used(*x);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_reserve(caches, refs, block_table, seqlens_k, seqlens_new, page_size) -> granted
+PyObject* paged_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 6, "paged_reserve");
+    std::vector<intfa_page_pool> pools;
+    const std::vector<Tensor> held = pools_arg(a[0], &pools);
+    const Tensor &refs = tensor_arg(a[1], "refs"), &table = tensor_arg(a[2], "block_table"), &lens = tensor_arg(a[3], "seqlens_k");
+    intfa_page_table t = page_table_arg(refs, table, lens);
+    t.page_size = page_size_arg(a[5]);
+    if (!held.empty()) {
+        require_on(held[0], refs, "every cache");
+        if (held[0].size(0) != refs.size(0)) fail(PyExc_ValueError, "refs must hold a count for each page of the caches");
+    }
+    if (t.batch > 8192) fail(PyExc_ValueError, "at most 8192 sequences, got " + std::to_string(t.batch));
+    const CallDevice dev(refs);
+    Tensor fresh, granted = dev.empty({(int64_t)t.batch}, ScalarType::Int);
+    int fresh_all = 0;
+    if (PyLong_Check(a[4])) {
+        fresh_all = int32_arg(a[4], "seqlens_new");
+    } else {
+        fresh = lengths_arg(tensor_arg(a[4], "seqlens_new"), t.batch, refs, "seqlens_new");
+    }
+    if (t.batch == 0) return THPVariable_Wrap(std::move(granted));
+    if (t.table_width == 0) fail(PyExc_ValueError, "block_table needs at least one column");
+    const size_t bytes = intfa_pages_reserve_workspace_bytes(&t);
+    const Tensor ws = dev.empty({(int64_t)bytes}, ScalarType::Byte);
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] {
+        return intfa_pages_reserve(&t, pools.data(), (int)pools.size(), fresh.defined() ? fresh.data_ptr<int32_t>() : nullptr, fresh_all, granted.data_ptr<int32_t>(),
+                                   ws.data_ptr(), bytes, st);
+    }), "intfa_pages_reserve");
+    for (const Tensor& x : held) dev.used(x);
+    for (const Tensor* x : {&refs, &table, &lens, const_cast<const Tensor*>(&fresh)}) dev.used(*x);
+    return THPVariable_Wrap(std::move(granted));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_compact(caches, refs, block_table) -> new_index
+PyObject* paged_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 3, "paged_compact");
+    std::vector<intfa_page_pool> pools;
+    const std::vector<Tensor> held = pools_arg(a[0], &pools);
+    const Tensor &refs = tensor_arg(a[1], "refs"), &table = tensor_arg(a[2], "block_table");
+    const intfa_page_table t = page_table_arg(refs, table, Tensor());
+    if (!held.empty()) {
+        require_on(held[0], refs, "every cache");
+        if (held[0].size(0) != refs.size(0)) fail(PyExc_ValueError, "refs must hold a count for each page of the caches");
+    }
+    if (table.numel() == 0) fail(PyExc_ValueError, "block_table needs at least one row and one column");
+    const CallDevice dev(refs);
+    Tensor index = dev.empty({refs.size(0)}, ScalarType::Int);
+    const size_t bytes = intfa_pages_compact_workspace_bytes(&t);
+    const Tensor ws = dev.empty({(int64_t)bytes}, ScalarType::Byte);
+    void* const st = dev.raw_stream();
+    check_rc(unlocked([&] { return intfa_pages_compact(&t, pools.data(), (int)pools.size(), index.data_ptr<int32_t>(), ws.data_ptr(), bytes, st); }), "intfa_pages_compact");
+    for (const Tensor& x : held) dev.used(x);
+    for (const Tensor* x : {&refs, &table}) dev.used(*x);
+    return THPVariable_Wrap(std::move(index));
+    END_HANDLE_TH_ERRORS
+}
+
 #define INTFA_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     INTFA_FAST(forward), INTFA_FAST(check_head_dims), INTFA_FAST(debug_qk_int32), INTFA_FAST(quant_perblock_channel), INTFA_FAST(kvcache_append),
     INTFA_FAST(rotary), INTFA_FAST(paged_kvcache_append), INTFA_FAST(attention_paged),
+    INTFA_FAST(paged_latent_append), INTFA_FAST(paged_copy), INTFA_FAST(paged_fork), INTFA_FAST(paged_free), INTFA_FAST(paged_reserve), INTFA_FAST(paged_compact),
     {"quant_pertoken", quant_pertoken, METH_O, nullptr}, {"quant_pertensor", quant_pertensor, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "host side of the entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,21 @@
+"""Attention whose keys and values come from one latent vector a token.
+
+The cache is a pool of pages, ``cache`` int8 [pages, page_size, latent_dim + rope_dim]: a token's latent vector (128, 256 or 512 numbers) and the rotary key (32 or 64) that all heads
+share, with two fp32 scales a token, ``scale`` [pages, page_size, 2].  Pages and ``block_table`` are those of the other paged cache.
+"""
+from . import _host
+
+
+def paged_latent_append(cache, scale, c_new, k_new, block_table, seqlens_k, freqs=None, *, interleaved=False, magnitude=1.0, seqlens_new=None,
+                        norm_weight=None, norm_eps=1e-6):
+    """Appends new tokens, ``c_new`` [Z, N_new, latent_dim] and ``k_new`` [Z, N_new, rope_dim] (both fp16 or both bf16), to the pages of their sequences, in place.
+
+    Sequence z holds ``seqlens_k[z]`` tokens (int32 [Z] on the device); its new rows go to the positions from there on.  With ``norm_weight`` ([latent_dim] of the same type)
+    the latent vectors are normalised on the way, c * weight / sqrt(mean(c^2) + norm_eps), and with ``freqs`` the rotary keys are rotated by their positions as ``rotary``
+    does; neither is rounded to 16 bits in between.  ``seqlens_new`` (int32 [Z]): new rows of each sequence where they differ.  Rows past the table's last column, or
+    of a page that the table does not name, are dropped.  The lengths are not advanced here.
+
+    Each part of a token is rounded to its own scale, its largest magnitude over 127 (at least 2^-100).  NaN becomes 0 and infinities +-127, and neither counts for the scale.
+    No other token of a page is touched."""
+    return (_host._native or _host.native()).paged_latent_append(cache, scale, c_new, k_new, block_table, seqlens_k, freqs, interleaved, magnitude, seqlens_new,
+                                                                 norm_weight, norm_eps)
