@@ -437,6 +437,34 @@ typedef struct intfa_latent_append_params {
 } intfa_latent_append_params;
 int intfa_latent_append_int8(const intfa_latent_append_params* p, void* stream);
 
+/* Attention of new tokens over a latent cache, with queries that are in the latent space already (the absorbed form): the key of a token is its latent part
+ * followed by its rotary part, its value the latent part, for all heads.  q_latent [batch, heads, seqlen, latent_dim], q_rope [batch, heads, seqlen, rope_dim]
+ * and out [batch, heads, seqlen, latent_dim] are fp16 or bf16 (dtype, all alike).  Lengths, positions (q_rope is turned by them where rope.freqs is given), causal, rows
+ * without keys and lse as in intfa_paged_attn_params.
+ * Keys and values enter as the numbers that the cache stands for; scales must be finite and not negative, and count as 2^-100 for the values where they are less.
+ * A query row (after its turn) enters in whole steps of 1/32512 of its largest element, so that a score is off by at most half of that times the sum of its key's
+ * magnitudes times sm_scale; a row that holds no number gives none.  Products are exact in integers, scores and sums fp32 (a score past 2^128 is no number; so are scores of keys past
+ * 2^124 or queries past 2^120).  Probabilities times their token's scale are rounded to 11 bits, those under 2^-25 of the row's largest to steps of 2^-35 of it.
+ * workspace: at least intfa_latent_attn_workspace_bytes(p) bytes of device memory, 16-byte aligned, nothing to clear; two launches that may run at the same
+ * time must not share it. */
+typedef struct intfa_latent_attn_params {
+    intfa_latent_cache cache;
+    const void* q_latent; const void* q_rope; void* out;
+    int64_t ql_stride_b, ql_stride_h, ql_stride_n;
+    int64_t qr_stride_b, qr_stride_h, qr_stride_n;
+    int64_t o_stride_b, o_stride_h, o_stride_n;
+    float* lse;                                /* optional [batch, heads, seqlen] contiguous */
+    const int32_t* seqlens_k;
+    const int32_t* seqlens_q;
+    intfa_rope rope;
+    void* workspace; size_t workspace_bytes;
+    float sm_scale;
+    int32_t causal;
+    int32_t batch, heads, seqlen, dtype;
+} intfa_latent_attn_params;
+size_t intfa_latent_attn_workspace_bytes(const intfa_latent_attn_params* p);
+int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream);
+
 /* ---- The pages themselves: which are in use, and by how many sequences.
  * refs [num_pages] counts the entries of the block table that name a page; one with a count of 0 (or less) is free.  Counts, table and lengths are on the
  * device and change there, so that captured calls follow them; nothing is read back.  pools: the tensors whose first axis is pages (keys, values, scales, of any

@@ -112,6 +112,15 @@ class LatentAppendParams(ctypes.Structure):
                 + [("seqlens_k", ctypes.c_void_p), ("seqlens_new", ctypes.c_void_p), ("rope", Rope)])
 
 
+class LatentAttnParams(ctypes.Structure):
+    """Mirror of ``intfa_latent_attn_params``."""
+    _fields_ = ([("cache", LatentCache), ("q_latent", ctypes.c_void_p), ("q_rope", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t in ("ql", "qr", "o") for a in "bhn"]
+                + [("lse", ctypes.c_void_p), ("seqlens_k", ctypes.c_void_p), ("seqlens_q", ctypes.c_void_p), ("rope", Rope),
+                   ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("sm_scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("causal", "batch", "heads", "seqlen", "dtype")])
+
+
 class PagePool(ctypes.Structure):
     """Mirror of ``intfa_page_pool``."""
     _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("page_bytes", ctypes.c_int64)]
@@ -131,7 +140,7 @@ EXPORTS = ("intfa_version", "intfa_error_string", "intfa_fwd_block_n", "intfa_fw
            "intfa_quant_pertoken", "intfa_quant_pertensor_workspace_bytes",
            "intfa_quant_pertensor_parts_workspace_bytes", "intfa_quant_pertensor", "intfa_quant_perblock_channel", "intfa_kvcache_append_int8",
            "intfa_rotary", "intfa_paged_append_int8", "intfa_paged_attn_workspace_bytes", "intfa_paged_attn_int8",
-           "intfa_latent_append_int8", "intfa_pages_copy", "intfa_pages_fork", "intfa_pages_free", "intfa_pages_reserve_workspace_bytes", "intfa_pages_reserve",
+           "intfa_latent_append_int8", "intfa_latent_attn_workspace_bytes", "intfa_latent_attn_int8", "intfa_pages_copy", "intfa_pages_fork", "intfa_pages_free", "intfa_pages_reserve_workspace_bytes", "intfa_pages_reserve",
            "intfa_pages_compact_workspace_bytes", "intfa_pages_compact")
 
 _lib = None
@@ -182,12 +191,14 @@ def load():
     lib.intfa_kvcache_append_int8.restype = ctypes.c_int
     lib.intfa_kvcache_append_int8.argtypes = [ctypes.POINTER(AppendParams), vp]
     for name, block in (("intfa_rotary", RotaryParams), ("intfa_paged_append_int8", PagedAppendParams), ("intfa_paged_attn_int8", PagedAttnParams),
-                        ("intfa_latent_append_int8", LatentAppendParams)):
+                        ("intfa_latent_append_int8", LatentAppendParams), ("intfa_latent_attn_int8", LatentAttnParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(block), vp]
     lib.intfa_paged_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.intfa_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnParams)]
+    lib.intfa_latent_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.intfa_latent_attn_workspace_bytes.argtypes = [ctypes.POINTER(LatentAttnParams)]
     table, pools, size = ctypes.POINTER(PageTable), ctypes.POINTER(PagePool), ctypes.c_size_t
     for name, args in (("copy", [pools, i32, i32, vp, vp, i32, vp]), ("fork", [table, vp, vp, i32, vp]), ("free", [table, vp, vp, i32, vp]),
                        ("reserve", [table, pools, i32, vp, i32, vp, vp, size, vp]), ("compact", [table, pools, i32, vp, vp, size, vp])):

@@ -1,0 +1,2 @@
+#include "intfa_latent_attn.h"
+namespace intfa { INTFA_DECL_LATENT(launch_latent_c512_r32_f16) { return launch_latent<512, 32, 0>(p, rows, stream); } }

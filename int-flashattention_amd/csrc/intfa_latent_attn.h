@@ -1,0 +1,633 @@
+// Attention over a paged cache of latent vectors (absorbed queries): keys are the whole rows of the cache, values their latent part, for all heads.
+//
+// A workgroup takes a tile of 32 or 64 query rows and a range of keys in blocks of 64, which come into a ring of four LDS stages by asynchronous copies, as int8, once.
+// Of its eight waves four form scores and weights (one a SIMD), and four multiply the weights of the block before with its values, so that one half's
+// exponentials run under the other's products.
+//   S^T = K Q^T    in int8.  A query row is held as whole steps of 1/32512 of its largest element, in two bytes: two products, whose sums 256 hi + lo are exact in
+//                  32 bits (512 x 128 x 32640 < 2^31).  That takes the time of one fp16 product, leaves the keys as they are, and halves what is read from LDS.
+//   O^T = V^T P^T  in fp16: P has a range that eight bits have not.  V's bytes are read transposed (ds_read_b64_tr_b8) and converted exactly; each wave has a quarter of
+//                  the columns for all rows, so that no byte is converted twice.  P goes through LDS in the operand's own layout.
+// A token's value scale s goes into the exponent: rows follow the maximum of t = score + log2 s, P = 2^(t - frame), and the sum of weights is that of P / s.  Whatever the
+// scales' sizes, P is within fp16 and the accumulators are plain sums of int8 numbers times P; the output is their quotient.
+#pragma once
+#include "intfa_latent_host.h"
+#include "intfa_paged_device.h"
+
+namespace intfa {
+
+typedef const __attribute__((address_space(4))) LatentParams* LatentArgs;
+__device__ __forceinline__ LatentArgs latent_args() {
+    LatentArgs p = (LatentArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
+// P = 2^(t - m + kLatentShift), and up to 2^kLatentSlack more before a row's m follows: at most 2^15, and 11 bits down to 2^-25 of the row's largest.
+constexpr float kLatentShift = 11.f, kLatentSlack = 4.f;
+// Scales enter scores as 2^-20 of themselves and the query's step as 2^20 of itself: products of up to 2^31 with scales of up to 2^117 fit.
+constexpr float kScoreUnit = 0x1p-20f;
+// Weights are summed as 2^-5 of themselves: 1 / s of scales of 2^121 is a normal number then, and sums of 2^21 of 2^-100 fit.
+constexpr float kWeightUnit = 0x1p-5f;
+constexpr float kQuerySteps = 32512.f;         // 127 * 256: the high byte of a step count rounds to at most 127
+
+// What the scale of a token on a page that the table does not name is read from
+static __device__ const float kHiddenScale[32] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+
+template <int DC, int DR, int ROWS> struct LatentShape {
+    static constexpr int ROW = DC + DR, UNITS = ROW / 16, LATENT_UNITS = DC / 16, KEYS = 64, THREADS = 512;
+    static constexpr int RG = ROWS / 32, KG = 4 / RG;          // groups of 32 rows; waves that share a group's keys
+    static constexpr int STAGE = KEYS * ROW, STAGES = 4;
+    static constexpr int COPIES = (UNITS + 3) / 4 + 1;         // asynchronous copies of a wave and stage: its 16 rows, and their scales
+    static constexpr int ANGLES_AT = (STAGES - 1) * STAGE, ANGLES_END = ANGLES_AT + ROWS * (DR / 2) * 8;
+    static constexpr int P_AT = STAGES * STAGE > ANGLES_END ? STAGES * STAGE : ANGLES_END, P_BYTES = ROWS * KEYS * 2;
+    static constexpr int SCALES_AT = P_AT + P_BYTES, SCALE_STAGE = KEYS * 8;
+    static constexpr int ALPHA_AT = SCALES_AT + STAGES * SCALE_STAGE;      // [ROWS] factor of a row's accumulators; then what the waves tell each other
+    static constexpr int TOPS_AT = ALPHA_AT + ROWS * 4;                    // [KG][ROWS]
+    static constexpr int FLAGS_AT = TOPS_AT + KG * ROWS * 4;               // [4]
+    static constexpr int FREQS_AT = FLAGS_AT + 16, LDS = FREQS_AT + (DR / 2) * 8;
+    static_assert(LDS <= 160 * 1024, "");
+    static constexpr int CT = DC / 32, NT = CT / 4;            // column tiles of 32; of a wave
+    // Where unit u of sixteen bytes of row m lies in its row.  Bank by bank: rows are 16 (rotary part of 64) or 8 words (of 32) past a multiple of 64, or such multiples that as few
+    // consecutive rows meet; reads take one unit of sixteen consecutive rows (keys), or two neighbouring ones of rows 0 - 3 and 8 - 11 (+ 4) (values).
+    static __device__ __forceinline__ int place(int u, int m) {
+        if (DR == 64) return u ^ ((m >> 2) & 3);
+        const int b = (m >> 3) & 1;
+        return u ^ (u < LATENT_UNITS && LATENT_UNITS >= 16 ? 9 * b : b);
+    }
+};
+
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// 64 x 16 bytes (or 64 x 4) from base + each lane's offset to LDS at lds + 16 (4) * lane.  (As the copies of intfa_device.h: M0 is nobody else's.)
+__device__ __forceinline__ void copy_units(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void copy_words(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" :: "i"(N) : "memory"); }
+
+// Sixteen step counts x * steps, rounded, as their high bytes and what is left of them (-128 .. 127) as low bytes
+__device__ __forceinline__ void split_steps(const float (&x)[16], float steps, v4i& hi, v4i& lo) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = __builtin_bit_cast(uint32_t, fmaf(x[4 * w + i], steps, 12582912.f + 128.f));      // count + 128 in the low 16 bits
+        hi[w] = (int)(__builtin_amdgcn_perm(u[1], u[0], 0x0c0c0501u) | __builtin_amdgcn_perm(u[3], u[2], 0x05010c0cu));
+        lo[w] = (int)((__builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u) | __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu)) ^ 0x80808080u);
+    }
+}
+
+// A query row's operand fragments.  A lane has sixteen elements of every STEP: those from 16 * part on (STEP 32: of the two lanes l, l ^ 32; 64: of the four of equal l % 16).
+template <int DC, int DR, int DT, int STEP> struct LatentQuery {
+    static constexpr int KC = DC / STEP, KR = (DR + STEP - 1) / STEP, KS = KC + KR;
+    v4i hi[KS], lo[KS];
+    float factor;                              // of the integer sums times kScoreUnit * scale: the score in base 2; NaN for a row that holds no number
+    v4i raw[KS][2], partner[KR][2];
+    // Element `at` of the rotary part begins eight that turn alike (pairs are a multiple of eight): where their partners are, and the first one's angle
+    struct Turn { bool turned, second; int partner, angle; };
+    static __device__ __forceinline__ Turn turn_of(int at, int pairs, bool interleaved) {
+        Turn x;
+        x.turned = at < 2 * pairs;
+        x.second = at >= pairs && !interleaved;
+        x.partner = !x.turned || interleaved ? at : x.second ? at - pairs : at + pairs;
+        x.angle = !x.turned ? 0 : interleaved ? at / 2 : x.second ? at - pairs : at;
+        return x;
+    }
+    __device__ __forceinline__ void request(LatentArgs p, const PagedItem& t, int row, int part) {
+        const auto& d = p->deal;
+        row = row < d.rows ? row : d.rows - 1;
+        const int token = paged_div(row, d.d_group), head = row - token * d.group, pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
+        const char* const c = d.q + t.z * d.q_sb + head * d.q_sh + token * d.q_sn;
+        const char* const r = p->q_rope + t.z * p->qr_sb + head * p->qr_sh + token * p->qr_sn;
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = STEP * k + 16 * part + 8 * h, in = at < DR ? at : 0;
+                raw[KC + k][h] = *(const v4i*)(r + 2 * in);
+                partner[k][h] = *(const v4i*)(r + 2 * turn_of(in, pairs, d.rope.interleaved != 0).partner);
+            }
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) raw[k][h] = *(const v4i*)(c + 2 * (STEP * k + 16 * part + 8 * h));
+    }
+    // angles: of the tile's tokens, (cos, sin) of pair i at token * pairs + i
+    __device__ __forceinline__ void form(LatentArgs p, int row, int part, const v2f* angles, int first_token) {
+        const auto& d = p->deal;
+        row = row < d.rows ? row : d.rows - 1;
+        const int token = paged_div(row, d.d_group), pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
+        const bool interleaved = d.rope.interleaved != 0;
+        float rope[KR][16];
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = STEP * k + 16 * part + 8 * h;
+                float* const x = &rope[k][8 * h];
+                unpack8<DT>(raw[KC + k][h], x);
+                if (pairs > 0) {
+                    const Turn turn = turn_of(at < DR ? at : 0, pairs, interleaved);
+                    const v2f* const mine = angles + (token - first_token) * pairs + turn.angle;
+                    float y[8];
+                    if (interleaved) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = x[i];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rope_turn(y[2 * i], y[2 * i + 1], mine[i][0], mine[i][1]);
+                    } else {
+                        unpack8<DT>(partner[k][h], y);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = x[i] * mine[i][0] + y[i] * (turn.second ? mine[i][1] : -mine[i][1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = turn.turned ? y[i] : x[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = at < DR ? x[i] : 0.f;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        // (magnitudes of 16-bit numbers are ordered as their bits are)
+        typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+        v2us most = {0, 0};
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, raw[k][h][i] & 0x7fff7fff));
+        float two[8];
+        unpack8<DT>((v4i){__builtin_bit_cast(int, most), 0, 0, 0}, two);
+        uint32_t top = __builtin_bit_cast(uint32_t, two[0]), other_top = __builtin_bit_cast(uint32_t, two[1]);
+        top = top > other_top ? top : other_top;
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t a = __builtin_bit_cast(uint32_t, rope[k][i]) & 0x7fffffffu;
+                top = top > a ? top : a;
+            }
+#pragma unroll
+        for (int w = STEP == 32 ? 32 : 16; w < 64; w <<= 1) {
+            const uint32_t a = (uint32_t)__shfl_xor((int)top, w);
+            top = top > a ? top : a;
+        }
+        const float size = fmaxf(__builtin_bit_cast(float, top), 0x1p-100f);      // (a row under it: its scores are nothing)
+        const float steps = copysignf(kQuerySteps / size, d.qk_scale_log2);
+        factor = top < 0x7f800000u ? size * (1.f / kQuerySteps) * (fabsf(d.qk_scale_log2) * (1.f / kScoreUnit)) : __builtin_nanf("");
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            float x[16];
+            unpack8<DT>(raw[k][0], x);
+            unpack8<DT>(raw[k][1], x + 8);
+            split_steps(x, steps, hi[k], lo[k]);
+            __builtin_amdgcn_sched_barrier(0);     // (in place of the raw elements, one after the other: all of them at once have no room)
+        }
+#pragma unroll
+        for (int k = 0; k < KR; ++k) split_steps(rope[k], steps, hi[KC + k], lo[KC + k]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// A lane's scales of one key: of scores (latent and rotary part, times kScoreUnit), log2 of the value's, and its reciprocal times kWeightUnit
+struct LatentScale { float c, r, log, inv; };
+__device__ __forceinline__ LatentScale latent_scale(float c, float r, bool beyond) {
+    LatentScale s;
+    const bool hidden = beyond || c < 0.f;
+    const float v = fmaxf(c, 0x1p-100f);
+    s.c = hidden ? 0.f : c * kScoreUnit;
+    s.r = hidden ? 0.f : r * kScoreUnit;
+    s.log = hidden ? -INFINITY : __builtin_amdgcn_logf(v);
+    s.inv = hidden ? 0.f : kWeightUnit * __builtin_amdgcn_rcpf(v);
+    return s;
+}
+
+// V's bytes of eight keys as fp16
+__device__ __forceinline__ v8h bytes_to_f16(v2i b) {
+    uint32_t w[4];
+    i8x4_to_f16((uint32_t)b[0], w[0], w[1]);
+    i8x4_to_f16((uint32_t)b[1], w[2], w[3]);
+    return __builtin_bit_cast(v8h, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
+}
+
+// QT: tiles of 16 rows that the scores of a tile of 32 are formed for (the second one may be empty)
+template <int DC, int DR, int DT, int ROWS, int QT>
+__global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams) {
+    typedef LatentShape<DC, DR, ROWS> S;
+    constexpr int RG = S::RG, KG = S::KG, NT = S::NT, KEYS = S::KEYS, STAGES = S::STAGES;
+    constexpr bool SMALL = ROWS == 32;         // scores in tiles of 16 keys by 16 rows: a wave has 16 keys of a block; else of 32 by 32
+    constexpr int STEP = SMALL ? 64 : 32;
+    static_assert(SMALL || (QT == 1 && RG == 2), "");
+    typedef LatentQuery<DC, DR, DT, STEP> Query;
+    __shared__ __align__(16) char lds[S::LDS];
+    LatentArgs p = latent_args();
+    PagedArgs deal = paged_args_first();
+    PagedItem t;
+    const double freq = paged_frequency(deal);
+    PagedPiece piece = paged_find(deal, ROWS, t);
+    if ((int)threadIdx.x < DR / 2) ((double*)(lds + S::FREQS_AT))[threadIdx.x] = freq;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & 3;      // (of its half)
+    const bool scoring = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) < 4;
+    const int lq = lane & 31, lh = lane >> 5, x16 = lane & 15, c16 = lane >> 4;
+    const int rg = SMALL ? 0 : wave % RG, kg = SMALL ? wave : wave / RG;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    float* const tops = (float*)(lds + S::TOPS_AT);
+    float* const alphas = (float*)(lds + S::ALPHA_AT);
+    int* const flags = (int*)(lds + S::FLAGS_AT);
+    v4i open = {0, 0, 0, 0};
+    __syncthreads();
+  while (piece.start < piece.end) {
+    const PagedPart part = paged_part(deal, t, piece);
+    if (part.none) break;
+    const int row0 = t.tile * ROWS, most = part.key_end, key_first = part.key_first;
+    const int blocks = most > key_first ? (most - key_first + KEYS - 1) / KEYS : 0;
+    if (scoring) {
+        // ======== scores and weights
+        Query query[QT];
+        int seen[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const int row = row0 + (SMALL ? 16 * q + x16 : 32 * rg + lq);
+            query[q].request(p, t, row, SMALL ? c16 : lh);
+            seen[q] = paged_token_keys(deal, t, paged_div(row < deal->rows ? row : deal->rows - 1, deal->d_group));
+        }
+        const int first_token = paged_div(row0, deal->d_group), least = paged_token_keys(deal, t, t.first_token);
+        if (deal->rope.freqs != nullptr) {
+            const int last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
+            const int tokens = paged_div(last_row, deal->d_group) - first_token + 1;
+            for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
+                const int token = paged_div(i, deal->d_pairs), pair = i - token * pairs;
+                float c, s;
+                rope_angle(((const double*)(lds + S::FREQS_AT))[pair], t.n - t.m + first_token + token, deal->rope.magnitude, c, s);
+                ((v2f*)(lds + S::ANGLES_AT))[i] = (v2f){c, s};
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int q = 0; q < QT; ++q) query[q].form(p, row0 + (SMALL ? 16 * q + x16 : 32 * rg + lq), SMALL ? c16 : lh, (const v2f*)(lds + S::ANGLES_AT), first_token);
+        // Reads of the tiles: a fragment's place is one of two lane addresses and a constant (the permutation flips low bits of the unit's number, and for a rotary part
+        // of 32 bit 3 as well).
+        constexpr bool FLIP = DR == 32 && S::LATENT_UNITS >= 16;
+        int key_at[2], key_rope_at;
+        {
+            const int key_row = SMALL ? 16 * wave + x16 : 32 * kg + lq, unit = SMALL ? c16 : lh;
+            key_at[0] = key_row * S::ROW + 16 * S::place(unit, key_row);
+            key_at[1] = key_row * S::ROW + 16 * S::place(unit + (DR == 32 ? 8 : 2), key_row);
+            key_rope_at = key_row * S::ROW + 16 * S::place(S::LATENT_UNITS + unit, key_row);
+        }
+        auto key_offset = [&](int k) __attribute__((always_inline)) {
+            constexpr int UPF = SMALL ? 4 : 2;     // units of a fragment
+            if (DR == 64) return SMALL ? key_at[0] + 64 * k : key_at[k & 1] + 64 * (k >> 1);
+            if (k >= Query::KC) return key_rope_at + 16 * UPF * (k - Query::KC);
+            const int bit = FLIP ? UPF * k >> 3 & 1 : 0;
+            return key_at[bit] + 16 * (UPF * k - 8 * bit);
+        };
+        float m[QT], l[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            m[q] = -INFINITY;
+            l[q] = 0.f;
+        }
+        lds_barrier();                         // (the first block is there)
+        for (int block = 0; block < blocks; ++block) {
+            const int key0 = key_first + KEYS * block, tile = (block % STAGES) * S::STAGE;
+            const float* const scales = (const float*)(lds + S::SCALES_AT + (block % STAGES) * S::SCALE_STAGE);
+            // ---- scores, as t = score + log2 of the value's scale
+            constexpr int PER = SMALL ? 4 : 16;    // a lane's keys
+            constexpr int KS = Query::KS, KC = Query::KC;
+            typedef typename std::conditional<SMALL, v4i, v16i>::type Sums;
+            float s[QT][PER];
+            // (lane i of a row of sixteen has the scales of the row's i-th key, from where all of the row take them)
+            const int tile_key = SMALL ? 16 * wave : 32 * kg, lane_key = tile_key + (SMALL ? 4 * c16 + (x16 & 3) : (int)scale_lane_key(lane));
+            const v2f two = *(const v2f*)(scales + 2 * lane_key);
+            // the rotary part first, then the latent one, two fragments ahead of the products
+            auto fragment = [&](int i) __attribute__((always_inline)) {
+                const int k = i < KS - KC ? KC + i : i - (KS - KC);
+                return *(const v4i*)(lds + tile + key_offset(k));
+            };
+            Sums hi[QT], lo[QT];
+            auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int q = 0; q < QT; ++q)
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) hi[q][i] = lo[q][i] = 0;
+            };
+            v4i f[4];
+            f[0] = fragment(0);
+            f[1] = fragment(1);
+            const LatentScale sc = latent_scale(two[0], two[1], key0 + lane_key >= most);
+            clear();
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                if (i + 2 < KS) f[(i + 2) % 4] = fragment(i + 2);
+                const int k = i < KS - KC ? KC + i : i - (KS - KC);
+                if (i == KS - KC) {
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) s[q][e] = (float)(hi[q][e] * 256 + lo[q][e]) * lane_scale(sc.r, e);
+                    clear();
+                }
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    if constexpr (SMALL) {
+                        hi[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query[q].hi[k], hi[q], 0, 0, 0);
+                        lo[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query[q].lo[k], lo[q], 0, 0, 0);
+                    } else {
+                        hi[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query[q].hi[k], hi[q], 0, 0, 0);
+                        lo[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query[q].lo[k], lo[q], 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float top[QT];
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    s[q][i] = ((float)(hi[q][i] * 256 + lo[q][i]) * lane_scale(sc.c, i) + s[q][i]) * query[q].factor + lane_scale(sc.log, i);
+                if (key0 + KEYS > least) {
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) {
+                        const int key = key0 + tile_key + (SMALL ? 4 * c16 + i : 8 * (i / 4) + 4 * lh + i % 4);
+                        s[q][i] = key < seen[q] ? s[q][i] : -INFINITY;
+                    }
+                }
+                // ---- the rows' maxima: of the lanes that share a row, and of the waves that share its keys
+                top[q] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) top[q] = fmaxf(top[q], s[q][i]);
+                if constexpr (SMALL) top[q] = reduce_row_lanes(top[q], [](float a, float b) { return fmaxf(a, b); });
+                else top[q] = half_pair_max(top[q]);
+                if (SMALL ? c16 == 0 : lh == 0) tops[kg * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)] = top[q];
+            }
+            lds_barrier();                     // A: the maxima are there, and P of the block before has been read
+            bool grows = false;
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+#pragma unroll
+                for (int k = 0; k < KG; ++k) top[q] = fmaxf(top[q], tops[k * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)]);
+                grows = grows || top[q] - m[q] > kLatentSlack;
+            }
+            const bool follow = __any(grows);  // (of a row group's waves alike)
+            if (follow) {
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    const float grown = fmaxf(m[q], top[q]), alpha = grown == -INFINITY ? 1.f : fast_exp2(m[q] - grown);
+                    m[q] = grown;
+                    l[q] *= alpha;
+                    if (kg == 0 && (SMALL ? c16 == 0 : lh == 0)) alphas[SMALL ? 16 * q + x16 : 32 * rg + lq] = alpha;
+                }
+            }
+            if (kg == 0 && lane == 0) flags[rg] = follow;
+            // ---- P, in the layout of the second product's operand: lane (row, h) has keys 16 t + 8 j + 4 h + i of step t at byte 8 j + 2 i of its sixteen
+#pragma unroll
+            for (int q = 0; q < QT; ++q) {
+                const float frame = (m[q] == -INFINITY ? 0.f : m[q]) - kLatentShift;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    s[q][i] = fast_exp2(s[q][i] - frame);
+                    l[q] += s[q][i] * lane_scale(sc.inv, i);
+                }
+                uint32_t w[PER / 2];
+#pragma unroll
+                for (int h = 0; h < PER / 2; ++h) w[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){s[q][2 * h], s[q][2 * h + 1]}, v2h));
+                if constexpr (SMALL) {
+                    *(v2i*)(lds + S::P_AT + (64 * wave + 16 * q + x16 + 32 * (c16 & 1)) * 16 + 8 * (c16 >> 1)) = (v2i){(int)w[0], (int)w[1]};
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        *(v4i*)(lds + S::P_AT + ((rg * 4 + 2 * kg + half) * 64 + lane) * 16) = (v4i){(int)w[4 * half], (int)w[4 * half + 1], (int)w[4 * half + 2], (int)w[4 * half + 3]};
+                }
+            }
+            lds_barrier();                     // B: P is there, and so is the next block
+        }
+        lds_barrier();                         // (A and B of the other half's last block)
+        lds_barrier();
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            if constexpr (SMALL) l[q] = reduce_row_lanes(l[q], [](float a, float b) { return a + b; });
+            else l[q] = half_pair_sum(l[q]);
+            if (SMALL ? c16 == 0 : lh == 0) {
+                const int r = SMALL ? 16 * q + x16 : 32 * rg + lq;
+                tops[kg * ROWS + r] = l[q];
+                if (kg == 0) alphas[r] = m[q];
+            }
+        }
+        lds_barrier();
+    } else {
+        // ======== copies, and the values' product: wave w copies rows 16 w .. 16 w + 15 of every block
+        uint32_t copy_off[S::COPIES - 1];
+#pragma unroll
+        for (int i = 0; i < S::COPIES - 1; ++i) {
+            const int unit = 64 * i + lane, r = unit / S::UNITS < 16 ? unit / S::UNITS : 15, u = unit % S::UNITS;
+            copy_off[i] = (uint32_t)(r * deal->k_sn + 16 * S::place(u, r));      // (the permutation is its own inverse)
+        }
+        const uint32_t scale_off = (uint32_t)(((lane & 31) >> 1) * (int)deal->ks_sh * 4 + (lane & 1) * 4);
+        const PagedInts table = (PagedInts)(deal->table + t.z * deal->bt_sb);
+        const int page_log2 = deal->page_log2, page_mask = (1 << page_log2) - 1, last_column = deal->table_width - 1;
+        auto look = [&](int block) __attribute__((always_inline)) {
+            const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
+            return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
+        };
+        auto copy = [&](int block, int id) __attribute__((always_inline)) {
+            const bool named = (unsigned)id < (unsigned)deal->num_pages;
+            const int at = named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
+            const char* const rows = deal->k + at * deal->k_sp + row * deal->k_sn;
+            const uint32_t to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
+#pragma unroll
+            for (int i = 0; i < S::COPIES - 1; ++i)
+                if (64 * i + 64 <= 16 * S::UNITS || lane < 32) copy_units(rows, copy_off[i], to + 1024u * i);
+            const char* const scales = (const char*)(deal->k_scale + at * deal->ks_sp + row * deal->ks_sh);
+            if (lane < 32)
+                copy_words(named ? scales : (const char*)kHiddenScale, named ? scale_off : (uint32_t)lane * 4, lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128));
+        };
+        if (blocks > 0) copy(0, look(0));
+        if (blocks > 1) copy(1, look(1));
+        int id_next = look(2);
+        int value_at[2];
+        {
+            const int j = x16 >> 1, value_row = 8 * (j >> 2) + 4 * lh + (j & 3), u = 2 * NT * wave + (c16 & 1);
+            value_at[0] = value_row * S::ROW + 16 * S::place(u, value_row) + 8 * (x16 & 1);
+            value_at[1] = value_row * S::ROW + 16 * S::place(u ^ 2, value_row) + 8 * (x16 & 1);
+        }
+        // (the tile's units 2 (NT w + ct) + ..: their bit 1 is that of ct where a wave has several tiles)
+        auto value_offset = [&](int ct) __attribute__((always_inline)) { return DR == 64 ? value_at[ct & 1] + 64 * (ct >> 1) : value_at[0] + 32 * ct; };
+        v16f acc[RG][NT];
+#pragma unroll
+        for (int g = 0; g < RG; ++g)
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[g][ct][r] = 0.f;
+        lds_barrier();                         // (the angles are there)
+        if (blocks > 1) wait_copies<S::COPIES>(); else wait_copies<0>();
+        lds_barrier();
+        for (int i = 0; i <= blocks; ++i) {
+            if (i + 2 < blocks) {
+                copy(i + 2, id_next);
+                id_next = look(i + 3);
+            }
+            const int tile = ((i + STAGES - 1) % STAGES) * S::STAGE;      // of block i - 1
+            v8h pf[KEYS / 16][RG];
+            auto product = [&](int step) __attribute__((always_inline)) {
+                v2i vb[NT];
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct)
+                    vb[ct] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)INTFA_LDS(lds + tile + value_offset(ct) + 16 * step * S::ROW));
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct) {
+                    const v8h vf = bytes_to_f16(vb[ct]);
+#pragma unroll
+                    for (int g = 0; g < RG; ++g) acc[g][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[step][g], acc[g][ct], 0, 0, 0);
+                }
+            };
+            if (i > 0) {
+#pragma unroll
+                for (int step = 0; step < KEYS / 16; ++step)
+#pragma unroll
+                    for (int g = 0; g < RG; ++g) pf[step][g] = *(const v8h*)(lds + S::P_AT + ((g * 4 + step) * 64 + lane) * 16);
+                // accumulators follow the maxima
+#pragma unroll
+                for (int g = 0; g < RG; ++g)
+                    if (__builtin_amdgcn_readfirstlane(flags[g])) {
+                        const float alpha = alphas[32 * g + lq];
+#pragma unroll
+                        for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) acc[g][ct][r] *= alpha;
+                    }
+                product(0);
+                product(1);
+            }
+            lds_barrier();                     // A
+            if (i > 0) {
+                product(2);
+                product(3);
+            }
+            if (i + 2 < blocks) wait_copies<S::COPIES>(); else wait_copies<0>();
+            lds_barrier();                     // B
+        }
+        lds_barrier();                         // (the rows' sums are there)
+        p = latent_args();
+#pragma unroll
+        for (int g = 0; g < RG; ++g) {
+            const int r = 32 * g + lq, row = row0 + r;
+            if (row >= p->deal.rows) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < KG; ++k) sum += tops[k * ROWS + r];
+            const float top = alphas[r];
+            if (part.whole) {
+                const int token = paged_div(row, p->deal.d_group), head = row - token * p->deal.group;
+                const bool empty = top == -INFINITY || token >= t.m;
+                const float weight = empty ? 0.f : kWeightUnit / sum;
+                char* const dst = p->deal.out + t.z * p->deal.o_sb + head * p->deal.o_sh + token * p->deal.o_sn + 2 * (32 * NT * wave + 4 * lh);
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        v4f o = {acc[g][ct][4 * k], acc[g][ct][4 * k + 1], acc[g][ct][4 * k + 2], acc[g][ct][4 * k + 3]};
+                        o *= weight;
+                        if (token >= t.m) o = (v4f){0.f, 0.f, 0.f, 0.f};
+                        store_out4<DT>(dst + 2 * (32 * ct + 8 * k), o);
+                    }
+                if (p->deal.lse != nullptr && wave == 0 && lh == 0)
+                    p->deal.lse[((int64_t)t.z * p->deal.heads + head) * p->deal.seqlen + token] =
+                        token >= t.m ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+            } else {
+                float* const slot = p->deal.parts + (int64_t)part.slot * ROWS * DC;
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *(v4f*)(slot + (((g * S::CT + NT * wave + ct) * 4 + k) * 64 + lane) * 4) = (v4f){acc[g][ct][4 * k], acc[g][ct][4 * k + 1], acc[g][ct][4 * k + 2], acc[g][ct][4 * k + 3]};
+                if (wave == 0 && lh == 0) *(v2f*)(p->deal.part_stats + ((int64_t)part.slot * ROWS + r) * 2) = (v2f){top, sum};
+            }
+        }
+    }
+    if (!part.whole && part.one == (int)blockIdx.x) open = (v4i){part.pieces, t.z, t.tile, (int)part.slot};
+    if (!paged_next(deal, ROWS, t, piece)) break;
+    lds_barrier();
+  }
+    if (threadIdx.x == 0) latent_args()->open_items[blockIdx.x] = open;
+}
+
+// The items that lie in several pieces, a launch later: a thread has four neighbouring columns of a row, in all pieces.
+template <int DC, int DT, int ROWS>
+__global__ void __launch_bounds__(256) latent_merge_kernel(const LatentParams) {
+    LatentArgs p = latent_args();
+    const v4i open = p->open_items[blockIdx.y];
+    const int pieces = open[0];
+    if (pieces == 0) return;
+    constexpr int CT = DC / 32;
+    const int i = (int)blockIdx.x * 256 + (int)threadIdx.x, lane = i & 63, k = (i >> 6) & 3, ct = (i >> 8) % CT, g = (i >> 8) / CT;
+    const int r = 32 * g + (lane & 31), row = open[2] * ROWS + r, col = 32 * ct + 8 * k + 4 * (lane >> 5), z = open[1];
+    const auto& d = p->deal;
+    if (row >= d.rows) return;
+    const int token = paged_div(row, d.d_group), head = row - token * d.group;
+    int m = d.seqlen;
+    if (d.seqlens_q != nullptr) {
+        const int n = d.seqlens_q[z];
+        m = n < 0 ? 0 : n < m ? n : m;
+    }
+    // the pieces: the first in its workgroup's own slot, the others first items of theirs
+    auto slot_of = [&](int j) __attribute__((always_inline)) { return (int64_t)(j == 0 ? open[3] : 2 * ((open[3] >> 1) + j)); };
+    constexpr int MANY = 8;
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.f;
+    for (int j0 = 0; j0 < pieces; j0 += MANY) {
+        v4f x[MANY];
+        v2f st[MANY];
+#pragma unroll
+        for (int u = 0; u < MANY; ++u) {
+            const int64_t slot = slot_of(j0 + u < pieces ? j0 + u : j0);
+            st[u] = *(const v2f*)(d.part_stats + (slot * ROWS + r) * 2);
+            x[u] = *(const v4f*)(d.parts + slot * ROWS * DC + (int64_t)i * 4);
+        }
+        float grown = top;
+#pragma unroll
+        for (int u = 0; u < MANY; ++u) {
+            if (j0 + u >= pieces) st[u][0] = -INFINITY;
+            grown = fmaxf(grown, st[u][0]);
+        }
+        const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
+        acc *= a;
+        sum *= a;
+        top = grown;
+#pragma unroll
+        for (int u = 0; u < MANY; ++u) {
+            const float w = fast_exp2(st[u][0] - frame);
+            if (j0 + u < pieces) {
+                acc += w * x[u];
+                sum = fmaf(w, st[u][1], sum);
+            }
+        }
+    }
+    const bool empty = top == -INFINITY || token >= m;
+    acc *= empty ? 0.f : kWeightUnit / sum;
+    if (token >= m) acc = (v4f){0.f, 0.f, 0.f, 0.f};
+    char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * col;
+    store_out4<DT>(dst, acc);
+    if (d.lse != nullptr && col == 0)
+        d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = token >= m ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+}
+
+template <int DC, int DR, int DT, int ROWS, int QT> int launch_latent_rows(const LatentParams& p, hipStream_t stream) {
+    hipLaunchKernelGGL((latent_attn_kernel<DC, DR, DT, ROWS, QT>), dim3((unsigned)p.deal.grid), dim3(512), 0, stream, p);
+    const int rc = (int)hipGetLastError();
+    if (rc != 0) return rc;
+    hipLaunchKernelGGL((latent_merge_kernel<DC, DT, ROWS>), dim3(ROWS * DC / 1024, (unsigned)p.deal.grid), dim3(256), 0, stream, p);
+    return (int)hipGetLastError();
+}
+template <int DC, int DR, int DT> int launch_latent(const LatentParams& p, int rows, hipStream_t stream) {
+    if (rows == 64) return launch_latent_rows<DC, DR, DT, 64, 1>(p, stream);
+    return p.deal.rows <= 16 ? launch_latent_rows<DC, DR, DT, 32, 1>(p, stream) : launch_latent_rows<DC, DR, DT, 32, 2>(p, stream);
+}
+
+}  // namespace intfa

@@ -1,0 +1,86 @@
+// C entry of the attention over a latent cache: argument checks, kernel selection and launch.  See include/intfa.h.
+#include "intfa_latent_host.h"
+
+using namespace intfa;
+
+namespace {
+
+bool rows16(const void* p, int64_t a, int64_t b, int64_t c) { return aligned_to(p, 16) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }
+
+int check(const intfa_latent_attn_params* p) {
+    if (p == nullptr || p->q_latent == nullptr || p->q_rope == nullptr || p->out == nullptr || p->seqlens_k == nullptr) return INTFA_ERR_NULL;
+    const int rc = latent_cache_check(&p->cache);
+    if (rc != INTFA_OK) return rc;
+    if (p->batch <= 0 || p->heads <= 0) return INTFA_ERR_SHAPE;
+    if (p->seqlen <= 0) return INTFA_ERR_SEQLEN;
+    if (p->dtype != INTFA_F16 && p->dtype != INTFA_BF16) return INTFA_ERR_DTYPE;
+    if (p->rope.freqs != nullptr && !rope_valid(&p->rope, p->cache.rope_dim)) return INTFA_ERR_ROPE;
+    if (!rows16(p->q_latent, p->ql_stride_b, p->ql_stride_h, p->ql_stride_n) || !rows16(p->q_rope, p->qr_stride_b, p->qr_stride_h, p->qr_stride_n) ||
+        !rows16(p->out, p->o_stride_b, p->o_stride_h, p->o_stride_n) || !aligned_to(p->lse, 4) || !aligned_to(p->seqlens_k, 4) || !aligned_to(p->seqlens_q, 4) ||
+        !aligned_to(p->rope.freqs, 8)) return INTFA_ERR_ALIGN;
+    if (size_product((int64_t)p->batch * p->heads, p->seqlen) >= 1ll << 30) return INTFA_ERR_SHAPE;
+    return INTFA_OK;
+}
+
+// How a call is dealt: rows of a tile, keys of a unit, workgroups (one a compute unit: the ring of stages takes its LDS); and the layout of its workspace.
+struct Plan { int rows, tiles, unit_log2, lead, grid; size_t stats_at, items_at, bytes; };
+Plan make_plan(const intfa_latent_attn_params* p) {
+    Plan a{};
+    const int rows = p->heads * p->seqlen;
+    a.rows = rows <= 32 ? 32 : 64;
+    a.tiles = (rows + a.rows - 1) / a.rows;
+    a.lead = 2;
+    a.unit_log2 = 6;
+    const int64_t items = (int64_t)p->batch * a.tiles, keys = (int64_t)p->cache.table_width * p->cache.page_size;
+    auto units = [&] { return items * (a.lead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
+    a.grid = (int)(units() < kComputeUnits ? units() : kComputeUnits);
+    while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)
+    if (units() * a.grid >= 1ll << 32) a.grid = (int)(((1ll << 32) - 1) / units());
+    const size_t slot_rows = (size_t)a.grid * 2 * a.rows;
+    a.stats_at = slot_rows * p->cache.latent_dim * sizeof(float);
+    a.items_at = a.stats_at + slot_rows * 2 * sizeof(float);
+    a.bytes = a.items_at + (size_t)a.grid * 16;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t intfa_latent_attn_workspace_bytes(const intfa_latent_attn_params* p) { return check(p) == INTFA_OK ? make_plan(p).bytes : 0; }
+
+int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream) {
+    const int rc = check(p);
+    if (rc != INTFA_OK) return rc;
+    const intfa_latent_cache& c = p->cache;
+    const Plan a = make_plan(p);
+    if (p->workspace == nullptr || p->workspace_bytes < a.bytes || !aligned_to(p->workspace, 16)) return INTFA_ERR_WORKSPACE;
+    LatentParams lp{};
+    PagedParams& kp = lp.deal;
+    kp.q = (const char*)p->q_latent; kp.out = (char*)p->out; kp.lse = p->lse;
+    kp.k = (const char*)c.rows; kp.k_scale = c.scale;
+    kp.table = c.block_table; kp.seqlens_k = p->seqlens_k; kp.seqlens_q = p->seqlens_q;
+    kp.q_sb = p->ql_stride_b * 2; kp.q_sh = p->ql_stride_h * 2; kp.q_sn = p->ql_stride_n * 2;
+    kp.o_sb = p->o_stride_b * 2; kp.o_sh = p->o_stride_h * 2; kp.o_sn = p->o_stride_n * 2;
+    kp.k_sp = c.r_stride_p; kp.k_sn = (int)c.r_stride_n; kp.ks_sp = c.s_stride_p; kp.ks_sh = c.s_stride_n; kp.bt_sb = c.bt_stride_b;
+    kp.batch = p->batch; kp.heads = p->heads; kp.heads_kv = 1; kp.group = p->heads;
+    kp.seqlen = p->seqlen; kp.rows = p->heads * p->seqlen;
+    kp.page_log2 = __builtin_ctz((unsigned)c.page_size); kp.num_pages = c.num_pages; kp.table_width = c.table_width;
+    kp.causal = p->causal != 0;
+    kp.qk_scale_log2 = p->sm_scale * 1.4426950408889634f;
+    kp.rope = {p->rope.freqs, p->rope.pairs, p->rope.interleaved, p->rope.magnitude};
+    kp.tiles = a.tiles; kp.unit_log2 = a.unit_log2; kp.grid = a.grid; kp.lead = a.lead;
+    kp.parts = (float*)p->workspace;
+    kp.part_stats = (float*)((char*)p->workspace + a.stats_at);
+    kp.d_group = make_fast_div(kp.group); kp.d_tiles = make_fast_div(kp.tiles); kp.d_pairs = make_fast_div(kp.rope.freqs != nullptr ? kp.rope.pairs : 1);
+    lp.q_rope = (const char*)p->q_rope; lp.qr_sb = p->qr_stride_b * 2; lp.qr_sh = p->qr_stride_h * 2; lp.qr_sn = p->qr_stride_n * 2;
+    lp.open_items = (v4i*)((char*)p->workspace + a.items_at);
+    hipStream_t st = (hipStream_t)stream;
+#define INTFA_CALL(name) (p->dtype == INTFA_BF16 ? name##_bf16(lp, a.rows, st) : name##_f16(lp, a.rows, st))
+    if (c.latent_dim == 128) return c.rope_dim == 32 ? INTFA_CALL(launch_latent_c128_r32) : INTFA_CALL(launch_latent_c128_r64);
+    if (c.latent_dim == 256) return c.rope_dim == 32 ? INTFA_CALL(launch_latent_c256_r32) : INTFA_CALL(launch_latent_c256_r64);
+    return c.rope_dim == 32 ? INTFA_CALL(launch_latent_c512_r32) : INTFA_CALL(launch_latent_c512_r64);
+#undef INTFA_CALL
+}
+
+}  // extern "C"

@@ -18,4 +18,15 @@ inline int latent_cache_check(const intfa_latent_cache* c) {
     return INTFA_OK;
 }
 
+struct LatentParams {
+    PagedParams deal;                          // (k: the rows, k_scale: their scales, ks_sh: elements from token to token; one head)
+    const char* q_rope; int64_t qr_sb, qr_sh, qr_sn;      // bytes
+    v4i* open_items;                           // [workgroups]: the item that begins in a workgroup's piece and goes on in others (pieces, sequence, tile, its slot there); pieces 0: none
+};
+
+#define INTFA_DECL_LATENT(name) int name(const LatentParams& p, int rows, hipStream_t stream)
+INTFA_DECL_LATENT(launch_latent_c128_r32_f16); INTFA_DECL_LATENT(launch_latent_c128_r32_bf16); INTFA_DECL_LATENT(launch_latent_c128_r64_f16); INTFA_DECL_LATENT(launch_latent_c128_r64_bf16);
+INTFA_DECL_LATENT(launch_latent_c256_r32_f16); INTFA_DECL_LATENT(launch_latent_c256_r32_bf16); INTFA_DECL_LATENT(launch_latent_c256_r64_f16); INTFA_DECL_LATENT(launch_latent_c256_r64_bf16);
+INTFA_DECL_LATENT(launch_latent_c512_r32_f16); INTFA_DECL_LATENT(launch_latent_c512_r32_bf16); INTFA_DECL_LATENT(launch_latent_c512_r64_f16); INTFA_DECL_LATENT(launch_latent_c512_r64_bf16);
+
 }  // namespace intfa

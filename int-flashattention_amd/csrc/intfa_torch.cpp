@@ -691,6 +691,52 @@ PyObject* paged_latent_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// attention_latent_paged(q_latent, q_rope, cache, scale, block_table, seqlens_k, causal, sm_scale, freqs, interleaved, magnitude, seqlens_q, return_lse)
+PyObject* attention_latent_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 13, "attention_latent_paged");
+    const Tensor &ql_in = tensor_arg(a[0], "q_latent"), &qr_in = tensor_arg(a[1], "q_rope"), &cache = tensor_arg(a[2], "cache"), &scale = tensor_arg(a[3], "scale");
+    const Tensor &table = tensor_arg(a[4], "block_table"), &lens = tensor_arg(a[5], "seqlens_k"), &freqs = optional_tensor_arg(a[8], "freqs");
+    const Tensor& rows = optional_tensor_arg(a[11], "seqlens_q");
+    require_gpu(ql_in);
+    if (quant_dtype(ql_in) < 0 || qr_in.scalar_type() != ql_in.scalar_type()) fail(PyExc_TypeError, "q_latent and q_rope must both be fp16 or both bf16");
+    require_4d(ql_in, "q_latent"); require_4d(qr_in, "q_rope");
+    require_on(qr_in, ql_in, "q_rope");
+    const int64_t Z = ql_in.size(0), H = ql_in.size(1), N = ql_in.size(2), dc = ql_in.size(3), dr = qr_in.size(3);
+    if (qr_in.size(0) != Z || qr_in.size(1) != H || qr_in.size(2) != N) fail(PyExc_ValueError, "q_latent and q_rope must be [Z, H, N, latent_dim] and [Z, H, N, rope_dim]");
+    intfa_latent_attn_params p{};
+    p.cache = latent_cache_arg(cache, scale, table, Z, dc, dr, ql_in);
+    const CallDevice dev(ql_in);
+    const Tensor ql = row_major(ql_in, dc, 2), qr = row_major(qr_in, dr, 2);
+    Tensor freqs_, rows_, lse, ws, out = dev.empty({Z, H, N, dc}, ql.scalar_type());
+    const bool return_lse = bool_arg(a[12]);
+    if (return_lse) lse = dev.empty({Z, H, N}, ScalarType::Float);
+    const Tensor lens_ = lengths_arg(lens, Z, ql, "seqlens_k");
+    if (rows.defined()) rows_ = lengths_arg(rows, Z, ql, "seqlens_q");
+    p.rope = rope_arg(freqs, bool_arg(a[9]), float_arg(a[10]), ql, dr, &freqs_);
+    p.causal = bool_arg(a[6]) ? 1 : 0;
+    p.sm_scale = (float)float_arg(a[7]);
+    if (out.numel() != 0) {
+        p.q_latent = ql.data_ptr(); p.q_rope = qr.data_ptr(); p.out = out.data_ptr();
+        p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+        set_strides(&p.ql_stride_b, ql); set_strides(&p.qr_stride_b, qr); set_strides(&p.o_stride_b, out);
+        p.seqlens_k = lens_.data_ptr<int32_t>();
+        p.seqlens_q = rows_.defined() ? rows_.data_ptr<int32_t>() : nullptr;
+        p.batch = (int)Z; p.heads = (int)H; p.seqlen = (int)N; p.dtype = quant_dtype(ql);
+        p.workspace_bytes = intfa_latent_attn_workspace_bytes(&p);
+        if (p.workspace_bytes > 0) {
+            ws = dev.empty({(int64_t)p.workspace_bytes}, ScalarType::Byte);
+            p.workspace = ws.data_ptr();
+        }
+        void* const st = dev.raw_stream();
+        check_rc(unlocked([&] { return intfa_latent_attn_int8(&p, st); }), "intfa_latent_attn_int8");
+        for (const Tensor* t : {&ql, &qr, &cache, &scale, &table, &lens_, const_cast<const Tensor*>(&rows_), const_cast<const Tensor*>(&freqs_)}) dev.used(*t);
+    }
+    if (!return_lse) return THPVariable_Wrap(std::move(out));
+    return tensor_pair(std::move(out), std::move(lse));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- pages
 // A sequence of tensors whose first axis is pages.
 std::vector<Tensor> pools_arg(PyObject* o, std::vector<intfa_page_pool>* pools) {
@@ -879,7 +925,7 @@ PyObject* paged_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     INTFA_FAST(forward), INTFA_FAST(check_head_dims), INTFA_FAST(debug_qk_int32), INTFA_FAST(quant_perblock_channel), INTFA_FAST(kvcache_append),
     INTFA_FAST(rotary), INTFA_FAST(paged_kvcache_append), INTFA_FAST(attention_paged),
-    INTFA_FAST(paged_latent_append), INTFA_FAST(paged_copy), INTFA_FAST(paged_fork), INTFA_FAST(paged_free), INTFA_FAST(paged_reserve), INTFA_FAST(paged_compact),
+    INTFA_FAST(paged_latent_append), INTFA_FAST(attention_latent_paged), INTFA_FAST(paged_copy), INTFA_FAST(paged_fork), INTFA_FAST(paged_free), INTFA_FAST(paged_reserve), INTFA_FAST(paged_compact),
     {"quant_pertoken", quant_pertoken, METH_O, nullptr}, {"quant_pertensor", quant_pertensor, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "host side of the entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -19,3 +19,17 @@ def paged_latent_append(cache, scale, c_new, k_new, block_table, seqlens_k, freq
     No other token of a page is touched."""
     return (_host._native or _host.native()).paged_latent_append(cache, scale, c_new, k_new, block_table, seqlens_k, freqs, interleaved, magnitude, seqlens_new,
                                                                  norm_weight, norm_eps)
+
+
+def attention_paged_latent_int8(q_latent, q_rope, cache, scale, block_table, seqlens_k, causal, sm_scale, *, freqs=None, interleaved=False,
+                                magnitude=1.0, seqlens_q=None, return_lse=False):
+    """Attention of new tokens over the pages of their sequences, with queries taken into the latent space (the absorbed form): ``q_latent`` [Z, H, N, latent_dim] is what
+    a head's query becomes by the matrix that would expand its keys, ``q_rope`` [Z, H, N, rope_dim] its rotary part, fp16 or bf16.  Every head's key is the whole row of the cache, its
+    value the latent part.  Returns [Z, H, N, latent_dim] of the same type, to be taken through the matrix that would expand the values, and with ``return_lse`` also
+    m + log2(l) of each row, fp32 [Z, H, N].
+
+    ``seqlens_k``, ``causal``, ``freqs`` (for ``q_rope``), ``seqlens_q`` and rows that see no key: as in ``attention_paged_int8``; a forward pass alone, like it.
+    Scales must be finite and not negative.  A query row enters in steps of 1/32512 of its largest element, keys and values as the numbers that the cache stands for.
+    """
+    return (_host._native or _host.native()).attention_latent_paged(q_latent, q_rope, cache, scale, block_table, seqlens_k, causal, sm_scale, freqs, interleaved,
+                                                                    magnitude, seqlens_q, return_lse)

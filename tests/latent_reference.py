@@ -45,8 +45,8 @@ def make_pool(g, pages, page, dc, dr, spread=0.0):
 
 
 def attend(q_latent, q_rope, cache, scale, table, lens, causal, sm, fresh=None, rope=None):
-    """q_latent [Z, H, N, dc], q_rope [Z, H, N, dr].  Returns the output, lse (base 2), and for the bound on errors: the mean of |v| under the row's weights,
-    the largest sum of |q k| of a visible key, and the largest error of a visible key's score that half a step of the row's queries makes."""
+    """q_latent [Z, H, N, dc], q_rope [Z, H, N, dr].  Returns the output, lse (base 2), and for the bound on errors (as a part of 2^-11, the steps of weights): the mean of |v| under the row's weights and what steps of
+    small weights add, the largest sum of |q k| of a visible key, and the largest error of a visible key's score that half a step of the row's queries makes."""
     Z, H, N, dc = q_latent.shape
     pages, page, _ = cache.shape
     out, lse = torch.zeros(q_latent.shape, dtype=torch.float64), torch.full((Z, H, N), -math.inf, dtype=torch.float64)
@@ -78,6 +78,8 @@ def attend(q_latent, q_rope, cache, scale, table, lens, causal, sm, fresh=None, 
         w = p / torch.where(total == 0, torch.ones_like(total), total)
         v = k[:, :dc]
         out[z, :, :m], mean_v[z, :, :m] = w @ v, w @ v.abs()
+        # weights that are far under the row's largest one, times its token's scale, are held in steps of 2^-35 of that: half a step of it for every token's int8 numbers
+        mean_v[z, :, :m] += 2.0 ** 11 * 2.0 ** -36 * (w * sc[:, 0].clamp(min=LEAST_SCALE)).amax(-1, keepdim=True) * (rows[:, :dc].abs() * there[:, None]).sum(0)
         size[z, :, :m] = (x.abs() @ k.abs().T * abs(sm) * seen).amax(-1, keepdim=True)
         step[z, :, :m] = (k.abs().sum(-1) * abs(sm) * seen).amax(-1, keepdim=True) * (x.abs().amax(-1, keepdim=True) / 32512.0 / 2.0)
         lse[z, :, :m] = torch.where(seen.any(-1), ((top + total.log()) / math.log(2.0))[..., 0], torch.full((), -math.inf, dtype=torch.float64))
