@@ -465,6 +465,31 @@ typedef struct intfa_latent_attn_params {
 size_t intfa_latent_attn_workspace_bytes(const intfa_latent_attn_params* p);
 int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream);
 
+/* The same attention with keys and values expanded for every head, which prompts are cheaper with: q_nope, k_nope [batch, heads, seqlen (seqlen_k), nope_dim], q_rope
+ * [batch, heads, seqlen, rope_dim], k_rope [batch, seqlen_k, rope_dim] (one for all heads, turned already like q_rope), v [batch, heads, seqlen_k, v_dim],
+ * out [batch, heads, seqlen, v_dim], all fp16 or all bf16 (dtype).  Dimensions (nope, rope, v): (128, 64, 128) or (64, 32, 64).
+ *     score = sm_scale * (q_nope . k_nope + q_rope . k_rope)
+ * Sequence b has m = seqlens_q[b] queries (optional; clamped to [0, seqlen]; NULL: seqlen) and n = seqlens_k[b] keys (optional; clamped to [0, seqlen_k]; NULL: seqlen_k); with causal row i
+ * sees keys 0 .. n - m + i.  Rows from m onward and rows that see no key are zeros with lse = -infinity; lse as in intfa_fwd_params.
+ * Scores and sums are fp32, probabilities are rounded to the type of v; values that are not finite reach the rows that are computed together with those that see them (at
+ * most 128 rows, and 64 keys behind a row's last).  Nothing behind a sequence's n keys is read. */
+typedef struct intfa_latent_expanded_params {
+    const void* q_nope; const void* q_rope; const void* k_nope; const void* k_rope; const void* v; void* out;
+    int64_t qn_stride_b, qn_stride_h, qn_stride_n;
+    int64_t qr_stride_b, qr_stride_h, qr_stride_n;
+    int64_t kn_stride_b, kn_stride_h, kn_stride_n;
+    int64_t kr_stride_b, kr_stride_n;
+    int64_t v_stride_b, v_stride_h, v_stride_n;
+    int64_t o_stride_b, o_stride_h, o_stride_n;
+    float* lse;                                /* optional [batch, heads, seqlen] contiguous */
+    const int32_t* seqlens_q;
+    const int32_t* seqlens_k;
+    float sm_scale;
+    int32_t causal;
+    int32_t batch, heads, seqlen, seqlen_k, nope_dim, rope_dim, v_dim, dtype;
+} intfa_latent_expanded_params;
+int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream);
+
 /* ---- The pages themselves: which are in use, and by how many sequences.
  * refs [num_pages] counts the entries of the block table that name a page; one with a count of 0 (or less) is free.  Counts, table and lengths are on the
  * device and change there, so that captured calls follow them; nothing is read back.  pools: the tensors whose first axis is pages (keys, values, scales, of any

@@ -121,6 +121,14 @@ class LatentAttnParams(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("causal", "batch", "heads", "seqlen", "dtype")])
 
 
+class LatentExpandedParams(ctypes.Structure):
+    """Mirror of ``intfa_latent_expanded_params``."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q_nope", "q_rope", "k_nope", "k_rope", "v", "out")]
+                + [(f"{t}_stride_{a}", ctypes.c_int64) for t, axes in (("qn", "bhn"), ("qr", "bhn"), ("kn", "bhn"), ("kr", "bn"), ("v", "bhn"), ("o", "bhn")) for a in axes]
+                + [("lse", ctypes.c_void_p), ("seqlens_q", ctypes.c_void_p), ("seqlens_k", ctypes.c_void_p), ("sm_scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("causal", "batch", "heads", "seqlen", "seqlen_k", "nope_dim", "rope_dim", "v_dim", "dtype")])
+
+
 class PagePool(ctypes.Structure):
     """Mirror of ``intfa_page_pool``."""
     _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("page_bytes", ctypes.c_int64)]
@@ -140,7 +148,7 @@ EXPORTS = ("intfa_version", "intfa_error_string", "intfa_fwd_block_n", "intfa_fw
            "intfa_quant_pertoken", "intfa_quant_pertensor_workspace_bytes",
            "intfa_quant_pertensor_parts_workspace_bytes", "intfa_quant_pertensor", "intfa_quant_perblock_channel", "intfa_kvcache_append_int8",
            "intfa_rotary", "intfa_paged_append_int8", "intfa_paged_attn_workspace_bytes", "intfa_paged_attn_int8",
-           "intfa_latent_append_int8", "intfa_latent_attn_workspace_bytes", "intfa_latent_attn_int8", "intfa_pages_copy", "intfa_pages_fork", "intfa_pages_free", "intfa_pages_reserve_workspace_bytes", "intfa_pages_reserve",
+           "intfa_latent_append_int8", "intfa_latent_attn_workspace_bytes", "intfa_latent_attn_int8", "intfa_latent_expanded", "intfa_pages_copy", "intfa_pages_fork", "intfa_pages_free", "intfa_pages_reserve_workspace_bytes", "intfa_pages_reserve",
            "intfa_pages_compact_workspace_bytes", "intfa_pages_compact")
 
 _lib = None
@@ -191,7 +199,8 @@ def load():
     lib.intfa_kvcache_append_int8.restype = ctypes.c_int
     lib.intfa_kvcache_append_int8.argtypes = [ctypes.POINTER(AppendParams), vp]
     for name, block in (("intfa_rotary", RotaryParams), ("intfa_paged_append_int8", PagedAppendParams), ("intfa_paged_attn_int8", PagedAttnParams),
-                        ("intfa_latent_append_int8", LatentAppendParams), ("intfa_latent_attn_int8", LatentAttnParams)):
+                        ("intfa_latent_append_int8", LatentAppendParams), ("intfa_latent_attn_int8", LatentAttnParams),
+                        ("intfa_latent_expanded", LatentExpandedParams)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(block), vp]

@@ -1,0 +1,2 @@
+#include "intfa_latent_expanded.h"
+namespace intfa { INTFA_DECL_EXPANDED(launch_expanded_n128_bf16) { return launch_expanded<128, 64, 128, 1>(p, causal, stream); } }

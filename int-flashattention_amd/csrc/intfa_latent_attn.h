@@ -367,19 +367,20 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 if (SMALL ? c16 == 0 : lh == 0) tops[kg * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)] = top[q];
             }
             lds_barrier();                     // A: the maxima are there, and P of the block before has been read
-            bool grows = false;
+            bool grows[QT], any = false;
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
 #pragma unroll
                 for (int k = 0; k < KG; ++k) top[q] = fmaxf(top[q], tops[k * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)]);
-                grows = grows || top[q] - m[q] > kLatentSlack;
+                grows[q] = top[q] - m[q] > kLatentSlack;
+                any = any || grows[q];
             }
-            const bool follow = __any(grows);  // (of a row group's waves alike)
+            const bool follow = __any(any);    // (of a row group's waves alike; rows that do not need it stay: what a row gets does not depend on the others)
             if (follow) {
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
-                    const float grown = fmaxf(m[q], top[q]), alpha = grown == -INFINITY ? 1.f : fast_exp2(m[q] - grown);
-                    m[q] = grown;
+                    const float alpha = grows[q] ? fast_exp2(m[q] - top[q]) : 1.f;
+                    m[q] = grows[q] ? top[q] : m[q];
                     l[q] *= alpha;
                     if (kg == 0 && (SMALL ? c16 == 0 : lh == 0)) alphas[SMALL ? 16 * q + x16 : 32 * rg + lq] = alpha;
                 }

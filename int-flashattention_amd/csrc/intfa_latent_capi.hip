@@ -1,5 +1,6 @@
 // C entry of the attention over a latent cache: argument checks, kernel selection and launch.  See include/intfa.h.
 #include "intfa_latent_host.h"
+#include "intfa_latent_expanded_host.h"
 
 using namespace intfa;
 
@@ -81,6 +82,45 @@ int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream) {
     if (c.latent_dim == 256) return c.rope_dim == 32 ? INTFA_CALL(launch_latent_c256_r32) : INTFA_CALL(launch_latent_c256_r64);
     return c.rope_dim == 32 ? INTFA_CALL(launch_latent_c512_r32) : INTFA_CALL(launch_latent_c512_r64);
 #undef INTFA_CALL
+}
+
+int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream) {
+    if (p == nullptr || p->q_nope == nullptr || p->q_rope == nullptr || p->k_nope == nullptr || p->k_rope == nullptr || p->v == nullptr || p->out == nullptr)
+        return INTFA_ERR_NULL;
+    if (p->batch <= 0 || p->heads <= 0) return INTFA_ERR_SHAPE;
+    if (p->seqlen <= 0 || p->seqlen_k < 0) return INTFA_ERR_SEQLEN;
+    const bool wide = p->nope_dim == 128 && p->rope_dim == 64 && p->v_dim == 128;
+    if (!wide && !(p->nope_dim == 64 && p->rope_dim == 32 && p->v_dim == 64)) return INTFA_ERR_HEAD_DIM;
+    if (p->dtype != INTFA_F16 && p->dtype != INTFA_BF16) return INTFA_ERR_DTYPE;
+    if (!rows16(p->q_nope, p->qn_stride_b, p->qn_stride_h, p->qn_stride_n) || !rows16(p->q_rope, p->qr_stride_b, p->qr_stride_h, p->qr_stride_n) ||
+        !rows16(p->k_nope, p->kn_stride_b, p->kn_stride_h, p->kn_stride_n) || !rows16(p->k_rope, p->kr_stride_b, 0, p->kr_stride_n) ||
+        !rows16(p->v, p->v_stride_b, p->v_stride_h, p->v_stride_n) || !rows16(p->out, p->o_stride_b, p->o_stride_h, p->o_stride_n) || !aligned_to(p->lse, 4) ||
+        !aligned_to(p->seqlens_q, 4) || !aligned_to(p->seqlens_k, 4)) return INTFA_ERR_ALIGN;
+    // the keys of a (sequence, head) are addressed with 32 bits, those of a block behind the last one among them
+    auto fits = [&](int64_t row, int64_t dim) { return row >= dim && size_product((int64_t)p->seqlen_k + 64, row) < 1ll << 31; };
+    if (!fits(p->kn_stride_n, p->nope_dim) || !fits(p->kr_stride_n, p->rope_dim) || !fits(p->v_stride_n, p->v_dim)) return INTFA_ERR_SHAPE;
+    if (p->seqlen > 1 << 30 || p->seqlen_k > 1 << 30) return INTFA_ERR_SHAPE;
+    ExpandedParams ep{};
+    ep.tiles = (p->seqlen + 127) / 128;
+    ep.pairs = (ep.tiles + 1) / 2;
+    const int64_t units = size_product(p->batch, p->heads), groups = size_product(units, ep.pairs);
+    if (groups * 512 >= 1ll << 32 || groups >= 1ll << 31) return INTFA_ERR_SHAPE;
+    ep.qn = (const char*)p->q_nope; ep.qr = (const char*)p->q_rope; ep.kn = (const char*)p->k_nope; ep.kr = (const char*)p->k_rope; ep.v = (const char*)p->v;
+    ep.out = (char*)p->out; ep.lse = p->lse; ep.seqlens_q = p->seqlens_q; ep.seqlens_k = p->seqlens_k;
+    ep.qn_sb = p->qn_stride_b * 2; ep.qn_sh = p->qn_stride_h * 2; ep.qn_sn = p->qn_stride_n * 2;
+    ep.qr_sb = p->qr_stride_b * 2; ep.qr_sh = p->qr_stride_h * 2; ep.qr_sn = p->qr_stride_n * 2;
+    ep.kn_sb = p->kn_stride_b * 2; ep.kn_sh = p->kn_stride_h * 2; ep.kn_sn = (uint32_t)(p->kn_stride_n * 2);
+    ep.kr_sb = p->kr_stride_b * 2; ep.kr_sn = (uint32_t)(p->kr_stride_n * 2);
+    ep.v_sb = p->v_stride_b * 2; ep.v_sh = p->v_stride_h * 2; ep.v_sn = (uint32_t)(p->v_stride_n * 2);
+    ep.o_sb = p->o_stride_b * 2; ep.o_sh = p->o_stride_h * 2; ep.o_sn = p->o_stride_n * 2;
+    ep.batch = p->batch; ep.heads = p->heads; ep.seqlen = p->seqlen; ep.seqlen_k = p->seqlen_k;
+    ep.whole = (int)(units / kXcds) * kXcds * ep.pairs;
+    ep.qk_scale_log2 = p->sm_scale * 1.4426950408889634f;
+    ep.d_pairs = make_fast_div(ep.pairs); ep.d_heads = make_fast_div(p->heads);
+    hipStream_t st = (hipStream_t)stream;
+    const bool causal = p->causal != 0;
+    if (wide) return p->dtype == INTFA_BF16 ? launch_expanded_n128_bf16(ep, causal, st) : launch_expanded_n128_f16(ep, causal, st);
+    return p->dtype == INTFA_BF16 ? launch_expanded_n64_bf16(ep, causal, st) : launch_expanded_n64_f16(ep, causal, st);
 }
 
 }  // extern "C"

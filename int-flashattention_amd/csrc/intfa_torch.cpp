@@ -20,6 +20,7 @@
 
 #include <atomic>
 #include <climits>
+#include <limits>
 #include <string>
 #include <vector>
 
@@ -737,6 +738,58 @@ PyObject* attention_latent_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// attention_latent(q_nope, q_rope, k_nope, k_rope, v, causal, sm_scale, seqlens_q, seqlens_k, return_lse)
+PyObject* attention_latent(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect_args(n, 10, "attention_latent");
+    static const char* const names[5] = {"q_nope", "q_rope", "k_nope", "k_rope", "v"};
+    const Tensor* in[5];
+    for (int i = 0; i < 5; ++i) {
+        in[i] = &tensor_arg(a[i], names[i]);
+        require_gpu(*in[i]);
+        require_4d(*in[i], names[i]);
+        require_on(*in[i], *in[0], names[i]);
+        if (quant_dtype(*in[i]) < 0 || in[i]->scalar_type() != in[0]->scalar_type()) fail(PyExc_TypeError, "queries, keys and values must all be fp16 or all bf16");
+    }
+    const int64_t Z = in[0]->size(0), H = in[0]->size(1), N = in[0]->size(2), dn = in[0]->size(3), dr = in[1]->size(3), Nk = in[2]->size(2), dv = in[4]->size(3);
+    if (!(dn == 128 && dr == 64 && dv == 128) && !(dn == 64 && dr == 32 && dv == 64))
+        fail(PyExc_AssertionError, "the parts of queries and keys and the values must have 128, 64 and 128 elements, or 64, 32 and 64");
+    const auto is = [&](int i, int64_t h, int64_t rows, int64_t d) { return in[i]->size(0) == Z && in[i]->size(1) == h && in[i]->size(2) == rows && in[i]->size(3) == d; };
+    if (!is(1, H, N, dr) || !is(2, H, Nk, dn) || !is(3, 1, Nk, dr) || !is(4, H, Nk, dv))
+        fail(PyExc_ValueError, "q_nope and q_rope must be [Z, H, N, d], k_nope and v [Z, H, N_k, d], k_rope [Z, 1, N_k, d]");
+    const CallDevice dev(*in[0]);
+    Tensor x[5];
+    for (int i = 0; i < 5; ++i) x[i] = row_major(*in[i], in[i]->size(3), 2);
+    const Tensor &lens_q = optional_tensor_arg(a[7], "seqlens_q"), &lens_k = optional_tensor_arg(a[8], "seqlens_k");
+    Tensor lens_q_, lens_k_, lse, out = dev.empty({Z, H, N, dv}, x[0].scalar_type());
+    const bool return_lse = bool_arg(a[9]);
+    if (return_lse) lse = dev.empty({Z, H, N}, ScalarType::Float);
+    if (lens_q.defined()) lens_q_ = lengths_arg(lens_q, Z, x[0], "seqlens_q");
+    if (lens_k.defined()) lens_k_ = lengths_arg(lens_k, Z, x[0], "seqlens_k");
+    intfa_latent_expanded_params p{};
+    p.causal = bool_arg(a[5]) ? 1 : 0;
+    p.sm_scale = (float)float_arg(a[6]);
+    if (out.numel() != 0 && Nk == 0) {
+        out.zero_();
+        if (return_lse) lse.fill_(-std::numeric_limits<float>::infinity());
+    } else if (out.numel() != 0) {
+        p.q_nope = x[0].data_ptr(); p.q_rope = x[1].data_ptr(); p.k_nope = x[2].data_ptr(); p.k_rope = x[3].data_ptr(); p.v = x[4].data_ptr(); p.out = out.data_ptr();
+        p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+        set_strides(&p.qn_stride_b, x[0]); set_strides(&p.qr_stride_b, x[1]); set_strides(&p.kn_stride_b, x[2]); set_strides(&p.v_stride_b, x[4]); set_strides(&p.o_stride_b, out);
+        p.kr_stride_b = x[3].stride(0); p.kr_stride_n = x[3].stride(2);
+        p.seqlens_q = lens_q_.defined() ? lens_q_.data_ptr<int32_t>() : nullptr;
+        p.seqlens_k = lens_k_.defined() ? lens_k_.data_ptr<int32_t>() : nullptr;
+        p.batch = (int)Z; p.heads = (int)H; p.seqlen = (int)N; p.seqlen_k = (int)Nk; p.nope_dim = (int)dn; p.rope_dim = (int)dr; p.v_dim = (int)dv; p.dtype = quant_dtype(x[0]);
+        void* const st = dev.raw_stream();
+        check_rc(unlocked([&] { return intfa_latent_expanded(&p, st); }), "intfa_latent_expanded");
+        for (const Tensor& t : x) dev.used(t);
+        dev.used(lens_q_); dev.used(lens_k_);
+    }
+    if (!return_lse) return THPVariable_Wrap(std::move(out));
+    return tensor_pair(std::move(out), std::move(lse));
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- pages
 // A sequence of tensors whose first axis is pages.
 std::vector<Tensor> pools_arg(PyObject* o, std::vector<intfa_page_pool>* pools) {
@@ -925,7 +978,7 @@ PyObject* paged_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     INTFA_FAST(forward), INTFA_FAST(check_head_dims), INTFA_FAST(debug_qk_int32), INTFA_FAST(quant_perblock_channel), INTFA_FAST(kvcache_append),
     INTFA_FAST(rotary), INTFA_FAST(paged_kvcache_append), INTFA_FAST(attention_paged),
-    INTFA_FAST(paged_latent_append), INTFA_FAST(attention_latent_paged), INTFA_FAST(paged_copy), INTFA_FAST(paged_fork), INTFA_FAST(paged_free), INTFA_FAST(paged_reserve), INTFA_FAST(paged_compact),
+    INTFA_FAST(paged_latent_append), INTFA_FAST(attention_latent_paged), INTFA_FAST(attention_latent), INTFA_FAST(paged_copy), INTFA_FAST(paged_fork), INTFA_FAST(paged_free), INTFA_FAST(paged_reserve), INTFA_FAST(paged_compact),
     {"quant_pertoken", quant_pertoken, METH_O, nullptr}, {"quant_pertensor", quant_pertensor, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", "host side of the entry points", -1, methods, nullptr, nullptr, nullptr, nullptr};
