@@ -37,12 +37,17 @@ template <int DC, int DR, int ROWS> struct LatentShape {
     static constexpr int ROW = DC + DR, UNITS = ROW / 16, LATENT_UNITS = DC / 16, KEYS = 64, THREADS = 512;
     static constexpr int RG = ROWS / 32, KG = 4 / RG;          // groups of 32 rows; waves that share a group's keys
     static constexpr int STAGE = KEYS * ROW, STAGES = 4;
-    static constexpr int COPIES = (UNITS + 3) / 4 + 1;         // asynchronous copies of a wave and stage: its 16 rows, and their scales
-    static constexpr int ANGLES_AT = (STAGES - 1) * STAGE, ANGLES_END = ANGLES_AT + ROWS * (DR / 2) * 8;
-    static constexpr int P_AT = STAGES * STAGE > ANGLES_END ? STAGES * STAGE : ANGLES_END, P_BYTES = ROWS * KEYS * 2;
+    static constexpr int WHOLE = UNITS / 4, HALF = UNITS % 4 / 2;      // asynchronous copies of a wave and stage, of 64 and of 32 lanes: its 16 rows
+    static constexpr int COPIES = WHOLE + HALF + 1;            // ... and their scales
+    static_assert(UNITS % 4 == 0 || UNITS % 4 == 2, "");
+    // The first block comes into the first stage while the queries are in the last two and the angles in the second one (or behind them, where stages are small).
+    static constexpr int QUERY_AT = 2 * STAGE, QUERY_END = QUERY_AT + ROWS * 2 * ROW, ANGLES = ROWS * (DR / 2) * 8;
+    static constexpr bool ANGLES_IN = ANGLES <= STAGE;
+    static constexpr int TILES_END = STAGES * STAGE > QUERY_END ? STAGES * STAGE : QUERY_END, ANGLES_AT = ANGLES_IN ? STAGE : TILES_END;
+    static constexpr int P_AT = ANGLES_IN ? TILES_END : TILES_END + ANGLES, P_BYTES = ROWS * KEYS * 2;
     static constexpr int SCALES_AT = P_AT + P_BYTES, SCALE_STAGE = KEYS * 8;
-    static constexpr int ALPHA_AT = SCALES_AT + STAGES * SCALE_STAGE;      // [ROWS] factor of a row's accumulators; then what the waves tell each other
-    static constexpr int TOPS_AT = ALPHA_AT + ROWS * 4;                    // [KG][ROWS]
+    static constexpr int ALPHA_AT = SCALES_AT + STAGES * SCALE_STAGE;      // [2][ROWS] factor of a row's accumulators, by the block's parity; then what the waves tell each other
+    static constexpr int TOPS_AT = ALPHA_AT + 2 * ROWS * 4;                    // [KG][ROWS]
     static constexpr int FLAGS_AT = TOPS_AT + KG * ROWS * 4;               // [4]
     static constexpr int FREQS_AT = FLAGS_AT + 16, LDS = FREQS_AT + (DR / 2) * 8;
     static_assert(LDS <= 160 * 1024, "");
@@ -61,7 +66,29 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-// 64 x 16 bytes (or 64 x 4) from base + each lane's offset to LDS at lds + 16 (4) * lane.  (As the copies of intfa_device.h: M0 is nobody else's.)
+// A wave's copies of a stage: N times 64 x 16 bytes from base + each lane's offset to consecutive KB of LDS from `lds` on (the last one of 32 lanes, if HALF), without a register on the
+// way.  (As the copies of intfa_device.h: M0 is nobody else's.  One statement, which counts M0 on: with one each, the compiler keeps a scalar for every place of every stage, in lanes
+// of vector registers.)
+#define INTFA_COPY(o) "\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 " o ", %1"
+#define INTFA_FIRST "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1"
+template <int N> __device__ __forceinline__ void copy_rows(const char* base, const uint32_t (&o)[N], uint32_t lds) {
+    static_assert(N == 2 || N == 3 || N == 4 || N == 5 || N == 8 || N == 9, "");
+    if constexpr (N == 2) asm volatile(INTFA_FIRST INTFA_COPY("%3") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]) : "memory", "scc");
+    else if constexpr (N == 3) asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]) : "memory", "scc");
+    else if constexpr (N == 4) asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]) : "memory", "scc");
+    else if constexpr (N == 5)
+        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6")
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]) : "memory", "scc");
+    else if constexpr (N == 8)
+        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6") INTFA_COPY("%7") INTFA_COPY("%8") INTFA_COPY("%9")
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]) : "memory", "scc");
+    else
+        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6") INTFA_COPY("%7") INTFA_COPY("%8") INTFA_COPY("%9") INTFA_COPY("%10")
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]), "v"(o[8]) : "memory", "scc");
+}
+#undef INTFA_COPY
+#undef INTFA_FIRST
+// 64 x 16 bytes and 64 x 4 alone
 __device__ __forceinline__ void copy_units(const char* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
@@ -82,58 +109,56 @@ __device__ __forceinline__ void split_steps(const float (&x)[16], float steps, v
     }
 }
 
+// A tile's query rows on their way: rows of latent and rotary part side by side (16-bit, 2 (DC + DR) bytes) are copied to LDS, units of sixteen bytes permuted so that
+// sixteen neighbouring rows are read in one unit, and taken from there by the lanes that hold them as operands.  (From memory straight to the lanes each load would touch 64
+// lines, eight times over: 64 rows 18 us.)
+template <int DC, int DR, int ROWS> struct LatentQueryTile {
+    static constexpr int ROW = 2 * (DC + DR), UNITS = ROW / 16, BYTES = ROWS * ROW, COPIES = BYTES / 1024;
+    static_assert(BYTES % 1024 == 0, "");
+    static __device__ __forceinline__ int place(int u, int r) { return u ^ (DR == 64 ? (r >> 1) & 7 : (r >> 2) & 3); }
+    static __device__ __forceinline__ void copy(LatentArgs p, const PagedItem& t, int row0, int wave, int lane, uint32_t to) {
+        const auto& d = p->deal;
+        const char* latent = d.q + t.z * d.q_sb;
+        const char* rotary = p->q_rope + t.z * p->qr_sb;
+        int64_t l_sh = d.q_sh, l_sn = d.q_sn, r_sh = p->qr_sh, r_sn = p->qr_sn;
+        int rows = d.rows, group = d.group;
+        FastDiv by_group = {d.d_group.m, d.d_group.s};
+        asm volatile("" : "+s"(latent), "+s"(rotary), "+s"(l_sh), "+s"(l_sn), "+s"(r_sh), "+s"(r_sn), "+s"(rows), "+s"(group), "+s"(by_group.m), "+s"(by_group.s));      // (held: else they are loaded lane by lane, behind a choice of address)
+#pragma clang loop unroll(disable)
+        for (int i = wave; i < COPIES; i += 4) {             // (rolled: eighteen addresses at once have no room beside what the loop over the blocks keeps)
+            const int at = 64 * i + lane, r = at / UNITS, u = place(at % UNITS, r);      // (the permutation is its own inverse)
+            const int row = row0 + r < rows ? row0 + r : rows - 1, token = fast_div(row, by_group), head = row - token * group;
+            const bool rope = u >= DC / 8;
+            const char* const src = (rope ? rotary : latent) + head * (rope ? r_sh : l_sh) + token * (rope ? r_sn : l_sn) + 16 * (rope ? u - DC / 8 : u);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(__builtin_amdgcn_readfirstlane((int)(to + 1024u * i))), "v"(src) : "memory");
+        }
+    }
+};
 // A query row's operand fragments.  A lane has sixteen elements of every STEP: those from 16 * part on (STEP 32: of the two lanes l, l ^ 32; 64: of the four of equal l % 16).
-template <int DC, int DR, int DT, int STEP> struct LatentQuery {
+template <int DC, int DR, int DT, int STEP, int ROWS> struct LatentQuery {
+    typedef LatentQueryTile<DC, DR, ROWS> Tile;
     static constexpr int KC = DC / STEP, KR = (DR + STEP - 1) / STEP, KS = KC + KR;
     v4i hi[KS], lo[KS];
     float factor;                              // of the integer sums times kScoreUnit * scale: the score in base 2; NaN for a row that holds no number
-    v4i raw[KS][2], partner[KR][2];
-    // Element `at` of the rotary part begins eight that turn alike (pairs are a multiple of eight): where their partners are, and the first one's angle
-    struct Turn { bool turned, second; int partner, angle; };
-    static __device__ __forceinline__ Turn turn_of(int at, int pairs, bool interleaved) {
-        Turn x;
-        x.turned = at < 2 * pairs;
-        x.second = at >= pairs && !interleaved;
-        x.partner = !x.turned || interleaved ? at : x.second ? at - pairs : at + pairs;
-        x.angle = !x.turned ? 0 : interleaved ? at / 2 : x.second ? at - pairs : at;
-        return x;
-    }
-    __device__ __forceinline__ void request(LatentArgs p, const PagedItem& t, int row, int part) {
+    // r: the row in the tile.  angles: (cos, sin) of the pairs of its token
+    __device__ __forceinline__ void form(LatentArgs p, const char* tile, int r, int part, const v2f* angles) {
         const auto& d = p->deal;
-        row = row < d.rows ? row : d.rows - 1;
-        const int token = paged_div(row, d.d_group), head = row - token * d.group, pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
-        const char* const c = d.q + t.z * d.q_sb + head * d.q_sh + token * d.q_sn;
-        const char* const r = p->q_rope + t.z * p->qr_sb + head * p->qr_sh + token * p->qr_sn;
-#pragma unroll
-        for (int k = 0; k < KR; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = STEP * k + 16 * part + 8 * h, in = at < DR ? at : 0;
-                raw[KC + k][h] = *(const v4i*)(r + 2 * in);
-                partner[k][h] = *(const v4i*)(r + 2 * turn_of(in, pairs, d.rope.interleaved != 0).partner);
-            }
-#pragma unroll
-        for (int k = 0; k < KC; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) raw[k][h] = *(const v4i*)(c + 2 * (STEP * k + 16 * part + 8 * h));
-    }
-    // angles: of the tile's tokens, (cos, sin) of pair i at token * pairs + i
-    __device__ __forceinline__ void form(LatentArgs p, int row, int part, const v2f* angles, int first_token) {
-        const auto& d = p->deal;
-        row = row < d.rows ? row : d.rows - 1;
-        const int token = paged_div(row, d.d_group), pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
+        const int pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
         const bool interleaved = d.rope.interleaved != 0;
+        // eight elements from `at` on, of the row's latent and rotary part side by side
+        auto eight = [&](int at) __attribute__((always_inline)) { return *(const v4i*)(tile + r * Tile::ROW + 16 * Tile::place(at / 8, r)); };
         float rope[KR][16];
 #pragma unroll
         for (int k = 0; k < KR; ++k)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int at = STEP * k + 16 * part + 8 * h;
+                const int at = STEP * k + 16 * part + 8 * h, in = at < DR ? at : 0;
                 float* const x = &rope[k][8 * h];
-                unpack8<DT>(raw[KC + k][h], x);
+                unpack8<DT>(eight(DC + in), x);
                 if (pairs > 0) {
-                    const Turn turn = turn_of(at < DR ? at : 0, pairs, interleaved);
-                    const v2f* const mine = angles + (token - first_token) * pairs + turn.angle;
+                    // (pairs are a multiple of eight: eight elements turn alike)
+                    const bool turned = in < 2 * pairs, second = in >= pairs && !interleaved;
+                    const v2f* const mine = angles + (!turned ? 0 : interleaved ? in / 2 : second ? in - pairs : in);
                     float y[8];
                     if (interleaved) {
 #pragma unroll
@@ -141,12 +166,12 @@ template <int DC, int DR, int DT, int STEP> struct LatentQuery {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) rope_turn(y[2 * i], y[2 * i + 1], mine[i][0], mine[i][1]);
                     } else {
-                        unpack8<DT>(partner[k][h], y);
+                        unpack8<DT>(eight(DC + (!turned ? in : second ? in - pairs : in + pairs)), y);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = x[i] * mine[i][0] + y[i] * (turn.second ? mine[i][1] : -mine[i][1]);
+                        for (int i = 0; i < 8; ++i) y[i] = x[i] * mine[i][0] + y[i] * (second ? mine[i][1] : -mine[i][1]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = turn.turned ? y[i] : x[i];
+                    for (int i = 0; i < 8; ++i) x[i] = turned ? y[i] : x[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = at < DR ? x[i] : 0.f;
@@ -158,9 +183,11 @@ template <int DC, int DR, int DT, int STEP> struct LatentQuery {
 #pragma unroll
         for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                const v4i raw = eight(STEP * k + 16 * part + 8 * h);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, raw[k][h][i] & 0x7fff7fff));
+                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, raw[i] & 0x7fff7fff));
+            }
         float two[8];
         unpack8<DT>((v4i){__builtin_bit_cast(int, most), 0, 0, 0}, two);
         uint32_t top = __builtin_bit_cast(uint32_t, two[0]), other_top = __builtin_bit_cast(uint32_t, two[1]);
@@ -181,16 +208,16 @@ template <int DC, int DR, int DT, int STEP> struct LatentQuery {
         const float steps = copysignf(kQuerySteps / size, d.qk_scale_log2);
         factor = top < 0x7f800000u ? size * (1.f / kQuerySteps) * (fabsf(d.qk_scale_log2) * (1.f / kScoreUnit)) : __builtin_nanf("");
 #pragma unroll
+        for (int k = 0; k < KR; ++k) split_steps(rope[k], steps, hi[KC + k], lo[KC + k]);
+        asm volatile("" ::: "memory");         // (the elements once more, and not kept since the maximum)
+#pragma unroll
         for (int k = 0; k < KC; ++k) {
             float x[16];
-            unpack8<DT>(raw[k][0], x);
-            unpack8<DT>(raw[k][1], x + 8);
+            unpack8<DT>(eight(STEP * k + 16 * part), x);
+            unpack8<DT>(eight(STEP * k + 16 * part + 8), x + 8);
             split_steps(x, steps, hi[k], lo[k]);
-            __builtin_amdgcn_sched_barrier(0);     // (in place of the raw elements, one after the other: all of them at once have no room)
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int k = 0; k < KR; ++k) split_steps(rope[k], steps, hi[KC + k], lo[KC + k]);
-        __builtin_amdgcn_sched_barrier(0);
     }
 };
 
@@ -205,6 +232,26 @@ __device__ __forceinline__ LatentScale latent_scale(float c, float r, bool beyon
     s.log = hidden ? -INFINITY : __builtin_amdgcn_logf(v);
     s.inv = hidden ? 0.f : kWeightUnit * __builtin_amdgcn_rcpf(v);
     return s;
+}
+
+// Scales that come as lanes of a register (scale_lane_key), in the instruction that uses them: c = f * scale, c += scale of the lane's i-th key.  (Hand-written as fmac_lane_scale:
+// the compiler takes sixteen copies of the register first, which have no room here.)
+__device__ __forceinline__ float mul_lane_scale(float f, float scales, int i) {
+    float c;
+    asm("v_mul_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "=v"(c) : "v"(scales), "v"(f), "i"(i));
+    return c;
+}
+__device__ __forceinline__ float add_lane_scale(float f, float scales, int i) {
+    float c;
+    asm("v_add_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "=v"(c) : "v"(scales), "v"(f), "i"(i));
+    return c;
+}
+__device__ __forceinline__ void fmac_lane_scale_f(float& c, float scales, float f, int i) {
+    asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(c) : "v"(scales), "v"(f), "i"(i));
+}
+// (f: of an exponential just ahead, which needs a wait state to its first reader; the compiler does not see a reader here)
+__device__ __forceinline__ void fmac_lane_scale_exp(float& c, float scales, float f, int i) {
+    asm("s_nop 0\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(c) : "v"(scales), "v"(f), "i"(i));
 }
 
 // V's bytes of eight keys as fp16
@@ -223,7 +270,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     constexpr bool SMALL = ROWS == 32;         // scores in tiles of 16 keys by 16 rows: a wave has 16 keys of a block; else of 32 by 32
     constexpr int STEP = SMALL ? 64 : 32;
     static_assert(SMALL || (QT == 1 && RG == 2), "");
-    typedef LatentQuery<DC, DR, DT, STEP> Query;
+    typedef LatentQuery<DC, DR, DT, STEP, ROWS> Query;
     __shared__ __align__(16) char lds[S::LDS];
     LatentArgs p = latent_args();
     PagedArgs deal = paged_args_first();
@@ -250,26 +297,14 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         // ======== scores and weights
         Query query[QT];
         int seen[QT];
+        const int first_token = paged_div(row0, deal->d_group), least = paged_token_keys(deal, t, t.first_token);
+        lds_barrier();                         // (queries and angles are there)
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
-            const int row = row0 + (SMALL ? 16 * q + x16 : 32 * rg + lq);
-            query[q].request(p, t, row, SMALL ? c16 : lh);
-            seen[q] = paged_token_keys(deal, t, paged_div(row < deal->rows ? row : deal->rows - 1, deal->d_group));
+            const int r = SMALL ? 16 * q + x16 : 32 * rg + lq, row = row0 + r < deal->rows ? row0 + r : deal->rows - 1, token = paged_div(row, deal->d_group);
+            seen[q] = paged_token_keys(deal, t, token);
+            query[q].form(p, lds + S::QUERY_AT, r, SMALL ? c16 : lh, (const v2f*)(lds + S::ANGLES_AT) + (deal->rope.freqs != nullptr ? (token - first_token) * deal->rope.pairs : 0));
         }
-        const int first_token = paged_div(row0, deal->d_group), least = paged_token_keys(deal, t, t.first_token);
-        if (deal->rope.freqs != nullptr) {
-            const int last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
-            const int tokens = paged_div(last_row, deal->d_group) - first_token + 1;
-            for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
-                const int token = paged_div(i, deal->d_pairs), pair = i - token * pairs;
-                float c, s;
-                rope_angle(((const double*)(lds + S::FREQS_AT))[pair], t.n - t.m + first_token + token, deal->rope.magnitude, c, s);
-                ((v2f*)(lds + S::ANGLES_AT))[i] = (v2f){c, s};
-            }
-        }
-        lds_barrier();
-#pragma unroll
-        for (int q = 0; q < QT; ++q) query[q].form(p, row0 + (SMALL ? 16 * q + x16 : 32 * rg + lq), SMALL ? c16 : lh, (const v2f*)(lds + S::ANGLES_AT), first_token);
         // Reads of the tiles: a fragment's place is one of two lane addresses and a constant (the permutation flips low bits of the unit's number, and for a rotary part
         // of 32 bit 3 as well).
         constexpr bool FLIP = DR == 32 && S::LATENT_UNITS >= 16;
@@ -294,6 +329,119 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             l[q] = 0.f;
         }
         lds_barrier();                         // (the first block is there)
+        if constexpr (!SMALL)
+        {
+            // A step forms the scores of block i + 1 while it takes the exponentials of block i: the first fragments' products run while the rows' maxima are settled, and with each of
+            // the others come one or two of a lane's sixteen weights.
+            constexpr int KC = Query::KC, KS = Query::KS, AHEAD = 3, EARLY = KC / 8 > 1 ? KC / 8 : 1;      // fragments ahead of the products; of the latent part ahead of the weights
+            static_assert(KC >= 4, "");
+            float s[16], inv = 0.f, e_last = 0.f;
+            uint32_t w[4];
+            auto element = [&](int j, float frame, int ln) __attribute__((always_inline)) {
+                const float e = fast_exp2(s[j] - frame);
+                fmac_lane_scale_exp(l[0], inv, e, j);
+                if (j & 1) w[j % 8 / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){e_last, e}, v2h));
+                else e_last = e;
+                if (j % 8 == 7) *(v4i*)(lds + S::P_AT + ((rg * 4 + 2 * kg + j / 8) * 64 + ln) * 16) = (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+            };
+            // scores of block `next` (QK) beside the weights of the block before it (E)
+            auto step = [&](auto qk_tag, auto e_tag, int next, int parity) __attribute__((always_inline)) {
+                constexpr bool QK = decltype(qk_tag)::value, E = decltype(e_tag)::value;
+                int ln = lane;
+                asm volatile("" : "+v"(ln));   // (places that follow from it are found again in each step: kept, they push operands out of the registers)
+                const int lq = ln & 31, lh = ln >> 5;
+                const int tile = (next % STAGES) * S::STAGE, key0 = key_first + KEYS * next;
+                v4i f[4];
+                v16i hi, lo;
+                auto fetch = [&](int k) __attribute__((always_inline)) {
+                    if (QK && k < KS) f[k % 4] = *(const v4i*)(lds + tile + key_offset(k));
+                };
+                auto product = [&](int k) __attribute__((always_inline)) {
+                    fetch(k + AHEAD);
+                    if (!QK) return;
+                    const bool first = k == 0 || k == KC;
+                    hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query[0].hi[k], first ? (v16i){0} : hi, 0, 0, 0);
+                    lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query[0].lo[k], first ? (v16i){0} : lo, 0, 0, 0);
+                };
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) fetch(k);
+                float theirs[2];
+                if (E) {                       // the rows' maxima: of the two waves that share a row's keys
+                    theirs[0] = tops[32 * rg + lq];
+                    theirs[1] = tops[ROWS + 32 * rg + lq];
+                }
+#pragma unroll
+                for (int k = 0; k < EARLY; ++k) {
+                    product(k);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float frame = 0.f;
+                if (E) {
+                    const float top = fmaxf(theirs[0], theirs[1]);
+                    const bool grows = top - m[0] > kLatentSlack, follow = __any(grows);      // (rows that do not need it stay: what a row gets does not depend on the others)
+                    if (follow) {
+                        const float alpha = grows ? fast_exp2(m[0] - top) : 1.f;
+                        m[0] = grows ? top : m[0];
+                        l[0] *= alpha;
+                        if (kg == 0 && lh == 0) alphas[parity * ROWS + 32 * rg + lq] = alpha;
+                    }
+                    if (kg == 0 && ln == 0) flags[2 * parity + rg] = follow;
+                    frame = (m[0] == -INFINITY ? 0.f : m[0]) - kLatentShift;
+                    lds_barrier();             // A: P of the block before has been read
+                }
+#pragma unroll
+                for (int k = EARLY; k < KC; ++k) {
+                    product(k);
+                    if (E) {
+#pragma unroll
+                        for (int j = 16 * (k - EARLY) / (KC - EARLY); j < 16 * (k - EARLY + 1) / (KC - EARLY); ++j) element(j, frame, ln);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (QK) {
+                    const v2f two = *(const v2f*)(lds + S::SCALES_AT + (next % STAGES) * S::SCALE_STAGE + 8 * (32 * kg + (int)scale_lane_key(ln)));
+                    LatentScale sc = latent_scale(two[0], two[1], key0 + 32 * kg + (int)scale_lane_key(ln) >= most);
+                    inv = sc.inv;
+                    asm volatile("s_nop 1" : "+v"(sc.c), "+v"(sc.r), "+v"(sc.log), "+v"(inv));      // (two wait states to other lanes' reads)
+                    wait_for_product(hi);
+                    wait_for_product(lo);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = mul_lane_scale((float)(hi[i] * 256 + lo[i]), sc.c, i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = KC; k < KS; ++k) product(k);
+                    wait_for_product(hi);
+                    wait_for_product(lo);
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        fmac_lane_scale_f(s[i], sc.r, (float)(hi[i] * 256 + lo[i]), i);
+                        s[i] = add_lane_scale(s[i] * query[0].factor, sc.log, i);
+                    }
+                    if (key0 + KEYS > least) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[i] = key0 + 32 * kg + 8 * (i / 4) + 4 * lh + i % 4 < seen[0] ? s[i] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+                    top = half_pair_max(top);
+                    if (lh == 0) tops[kg * ROWS + 32 * rg + lq] = top;
+                }
+            };
+            constexpr BoolTag<false> F{};
+            constexpr BoolTag<true> T{};
+            if (blocks > 0) step(T, F, 0, 0);
+#pragma clang loop unroll(disable)
+            for (int i = 0; i + 1 < blocks; ++i) {
+                lds_barrier();                 // B: the next block is there
+                step(T, T, i + 1, i & 1);
+            }
+            if (blocks > 0) {
+                lds_barrier();
+                step(F, T, blocks, (blocks - 1) & 1);
+            }
+        }
+        else
         for (int block = 0; block < blocks; ++block) {
             const int key0 = key_first + KEYS * block, tile = (block % STAGES) * S::STAGE;
             const float* const scales = (const float*)(lds + S::SCALES_AT + (block % STAGES) * S::SCALE_STAGE);
@@ -408,7 +556,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             }
             lds_barrier();                     // B: P is there, and so is the next block
         }
-        lds_barrier();                         // (A and B of the other half's last block)
+        lds_barrier();                         // (the other half's last block)
         lds_barrier();
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
@@ -423,33 +571,43 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         lds_barrier();
     } else {
         // ======== copies, and the values' product: wave w copies rows 16 w .. 16 w + 15 of every block
-        uint32_t copy_off[S::COPIES - 1];
-#pragma unroll
-        for (int i = 0; i < S::COPIES - 1; ++i) {
+        const int k_sn = deal->k_sn;
+        auto offset_of = [&](int i) __attribute__((always_inline)) {
             const int unit = 64 * i + lane, r = unit / S::UNITS < 16 ? unit / S::UNITS : 15, u = unit % S::UNITS;
-            copy_off[i] = (uint32_t)(r * deal->k_sn + 16 * S::place(u, r));      // (the permutation is its own inverse)
-        }
+            return (uint32_t)(r * k_sn + 16 * S::place(u, r));      // (the permutation is its own inverse)
+        };
+        uint32_t copy_off[S::WHOLE], copy_half = S::HALF ? offset_of(S::WHOLE) : 0u;
+#pragma unroll
+        for (int i = 0; i < S::WHOLE; ++i) copy_off[i] = offset_of(i);
         const uint32_t scale_off = (uint32_t)(((lane & 31) >> 1) * (int)deal->ks_sh * 4 + (lane & 1) * 4);
-        const PagedInts table = (PagedInts)(deal->table + t.z * deal->bt_sb);
-        const int page_log2 = deal->page_log2, page_mask = (1 << page_log2) - 1, last_column = deal->table_width - 1;
+        // (what a copy needs of the arguments, held: loaded anew for each one, they are a chain of trips to the scalar cache)
+        PagedInts table = (PagedInts)(deal->table + t.z * deal->bt_sb);
+        const char* all_rows = deal->k;
+        const float* all_scales = deal->k_scale;
+        int64_t k_sp = deal->k_sp, ks_sp = deal->ks_sp;
+        int page_log2 = deal->page_log2, last_column = deal->table_width - 1, num_pages = deal->num_pages, ks_sh = (int)deal->ks_sh;
+        asm volatile("" : "+s"(table), "+s"(all_rows), "+s"(all_scales), "+s"(k_sp), "+s"(ks_sp), "+s"(page_log2), "+s"(last_column), "+s"(num_pages), "+s"(ks_sh));
+        const int page_mask = (1 << page_log2) - 1;
         auto look = [&](int block) __attribute__((always_inline)) {
             const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
             return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
         };
         auto copy = [&](int block, int id) __attribute__((always_inline)) {
-            const bool named = (unsigned)id < (unsigned)deal->num_pages;
+            const bool named = (unsigned)id < (unsigned)num_pages;
             const int at = named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
-            const char* const rows = deal->k + at * deal->k_sp + row * deal->k_sn;
+            const char* const rows = all_rows + at * k_sp + row * k_sn;
             const uint32_t to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
-#pragma unroll
-            for (int i = 0; i < S::COPIES - 1; ++i)
-                if (64 * i + 64 <= 16 * S::UNITS || lane < 32) copy_units(rows, copy_off[i], to + 1024u * i);
-            const char* const scales = (const char*)(deal->k_scale + at * deal->ks_sp + row * deal->ks_sh);
+            copy_rows(rows, copy_off, to);
+            if (S::HALF && lane < 32) copy_units(rows, copy_half, to + 1024u * S::WHOLE);
+            const char* const scales = (const char*)(all_scales + at * ks_sp + row * ks_sh);
             if (lane < 32)
                 copy_words(named ? scales : (const char*)kHiddenScale, named ? scale_off : (uint32_t)lane * 4, lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128));
         };
-        if (blocks > 0) copy(0, look(0));
-        if (blocks > 1) copy(1, look(1));
+        if (blocks > 0) {
+            LatentQueryTile<DC, DR, ROWS>::copy(p, t, row0, wave, lane, lds0 + S::QUERY_AT);
+            copy(0, look(0));
+        }
+        const int id_second = look(1);
         int id_next = look(2);
         int value_at[2];
         {
@@ -466,53 +624,91 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[g][ct][r] = 0.f;
-        lds_barrier();                         // (the angles are there)
-        if (blocks > 1) wait_copies<S::COPIES>(); else wait_copies<0>();
-        lds_barrier();
-        for (int i = 0; i <= blocks; ++i) {
-            if (i + 2 < blocks) {
-                copy(i + 2, id_next);
-                id_next = look(i + 3);
+        if (blocks > 0 && deal->rope.freqs != nullptr) {      // the angles of the tile's tokens, each once
+            const int first_token = paged_div(row0, deal->d_group), last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
+            const int tokens = paged_div(last_row, deal->d_group) - first_token + 1;
+            for (int i = (int)threadIdx.x - 256; i < tokens * pairs; i += 256) {
+                const int token = paged_div(i, deal->d_pairs), pair = i - token * pairs;
+                float c, s;
+                rope_angle(((const double*)(lds + S::FREQS_AT))[pair], t.n - t.m + first_token + token, deal->rope.magnitude, c, s);
+                ((v2f*)(lds + S::ANGLES_AT))[i] = (v2f){c, s};
             }
-            const int tile = ((i + STAGES - 1) % STAGES) * S::STAGE;      // of block i - 1
+        }
+        wait_copies<S::COPIES>();
+        lds_barrier();
+        wait_copies<0>();
+        lds_barrier();
+        if (blocks > 1) copy(1, id_second);
+        for (int i = 0; i <= blocks; ++i) {
+            if (!SMALL) {
+                wait_copies<0>();
+                lds_barrier();                 // B: the scores' next block, P of block i - 1 and its factors are there
+            }
+            auto copy_next = [&]() __attribute__((always_inline)) {
+                if (i + 2 < blocks) {
+                    copy(i + 2, id_next);
+                    id_next = look(i + 3);
+                }
+            };
+            const int tile = ((i + STAGES - 1) % STAGES) * S::STAGE, parity = SMALL ? 0 : (i & 1) ^ 1;      // of block i - 1
             v8h pf[KEYS / 16][RG];
-            auto product = [&](int step) __attribute__((always_inline)) {
-                v2i vb[NT];
+            float alpha[RG];
+            bool follow[RG];
+            // (values two steps ahead of their products)
+            v2i vb[2][NT];
+            auto fetch = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
                 for (int ct = 0; ct < NT; ++ct)
-                    vb[ct] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)INTFA_LDS(lds + tile + value_offset(ct) + 16 * step * S::ROW));
+                    vb[step % 2][ct] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)INTFA_LDS(lds + tile + value_offset(ct) + 16 * step * S::ROW));
+            };
+            auto product = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
                 for (int ct = 0; ct < NT; ++ct) {
-                    const v8h vf = bytes_to_f16(vb[ct]);
+                    const v8h vf = bytes_to_f16(vb[step % 2][ct]);
 #pragma unroll
                     for (int g = 0; g < RG; ++g) acc[g][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[step][g], acc[g][ct], 0, 0, 0);
                 }
+                if (step + 2 < KEYS / 16) fetch(step + 2);
+                __builtin_amdgcn_sched_barrier(0);
             };
             if (i > 0) {
 #pragma unroll
                 for (int step = 0; step < KEYS / 16; ++step)
 #pragma unroll
                     for (int g = 0; g < RG; ++g) pf[step][g] = *(const v8h*)(lds + S::P_AT + ((g * 4 + step) * 64 + lane) * 16);
+#pragma unroll
+                for (int g = 0; g < RG; ++g) {
+                    follow[g] = flags[2 * parity + g] != 0;
+                    alpha[g] = alphas[parity * ROWS + 32 * g + lq];
+                }
+                fetch(0);
+                fetch(1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            copy_next();
+            if (!SMALL) lds_barrier();         // A: P has been read
+            if (i > 0) {
                 // accumulators follow the maxima
 #pragma unroll
                 for (int g = 0; g < RG; ++g)
-                    if (__builtin_amdgcn_readfirstlane(flags[g])) {
-                        const float alpha = alphas[32 * g + lq];
+                    if (__builtin_amdgcn_readfirstlane((int)follow[g])) {
 #pragma unroll
                         for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) acc[g][ct][r] *= alpha;
+                            for (int r = 0; r < 16; ++r) acc[g][ct][r] *= alpha[g];
                     }
                 product(0);
                 product(1);
             }
-            lds_barrier();                     // A
+            if (SMALL) lds_barrier();          // A
             if (i > 0) {
                 product(2);
                 product(3);
             }
-            if (i + 2 < blocks) wait_copies<S::COPIES>(); else wait_copies<0>();
-            lds_barrier();                     // B
+            if (SMALL) {
+                if (i + 2 < blocks) wait_copies<S::COPIES>(); else wait_copies<0>();
+                lds_barrier();                 // B
+            }
         }
         lds_barrier();                         // (the rows' sums are there)
         p = latent_args();
