@@ -97,10 +97,10 @@ __device__ __forceinline__ void copy_words(const char* base, uint32_t off, uint3
 }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" :: "i"(N) : "memory"); }
 
-// Sixteen step counts x * steps, rounded, as their high bytes and what is left of them (-128 .. 127) as low bytes
-__device__ __forceinline__ void split_steps(const float (&x)[16], float steps, v4i& hi, v4i& lo) {
+// Eight step counts x * steps, rounded, as their high bytes and what is left of them (-128 .. 127) as low bytes
+__device__ __forceinline__ void split_steps(const float (&x)[8], float steps, v2i& hi, v2i& lo) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < 2; ++w) {
         uint32_t u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = __builtin_bit_cast(uint32_t, fmaf(x[4 * w + i], steps, 12582912.f + 128.f));      // count + 128 in the low 16 bits
@@ -109,115 +109,93 @@ __device__ __forceinline__ void split_steps(const float (&x)[16], float steps, v
     }
 }
 
-// A tile's query rows on their way: rows of latent and rotary part side by side (16-bit, 2 (DC + DR) bytes) are copied to LDS, units of sixteen bytes permuted so that
-// sixteen neighbouring rows are read in one unit, and taken from there by the lanes that hold them as operands.  (From memory straight to the lanes each load would touch 64
-// lines, eight times over: 64 rows 18 us.)
-template <int DC, int DR, int ROWS> struct LatentQueryTile {
-    static constexpr int ROW = 2 * (DC + DR), UNITS = ROW / 16, BYTES = ROWS * ROW, COPIES = BYTES / 1024;
-    static_assert(BYTES % 1024 == 0, "");
-    static __device__ __forceinline__ int place(int u, int r) { return u ^ (DR == 64 ? (r >> 1) & 7 : (r >> 2) & 3); }
-    static __device__ __forceinline__ void copy(LatentArgs p, const PagedItem& t, int row0, int wave, int lane, uint32_t to) {
+// A tile's query rows on their way: all threads take part, 512 / ROWS of them a row, each with units of eight elements.  Their bytes go to LDS, from where the scoring waves take them
+// as operands.  (Formed by the lanes that hold them, from rows copied to LDS, the code was 1300 instructions of straight line, read from memory in each launch: 64 rows of 576 elements
+// took 35 000 clocks until their first product, and 13 000 so.)
+template <int DC, int DR, int DT, int ROWS> struct LatentQueries {
+    typedef LatentShape<DC, DR, ROWS> S;
+    static constexpr int T = S::THREADS / ROWS, N = DC / 8 / T, RU = DR / 8;
+    static_assert(RU <= T && DC % (8 * T) == 0, "");
+    v4i x[N], rope, other;
+    int row, unit, token;
+    __device__ __forceinline__ void load(LatentArgs p, const PagedItem& t, int row0, int tid) {
         const auto& d = p->deal;
-        const char* latent = d.q + t.z * d.q_sb;
-        const char* rotary = p->q_rope + t.z * p->qr_sb;
-        int64_t l_sh = d.q_sh, l_sn = d.q_sn, r_sh = p->qr_sh, r_sn = p->qr_sn;
-        int rows = d.rows, group = d.group;
-        FastDiv by_group = {d.d_group.m, d.d_group.s};
-        asm volatile("" : "+s"(latent), "+s"(rotary), "+s"(l_sh), "+s"(l_sn), "+s"(r_sh), "+s"(r_sn), "+s"(rows), "+s"(group), "+s"(by_group.m), "+s"(by_group.s));      // (held: else they are loaded lane by lane, behind a choice of address)
-#pragma clang loop unroll(disable)
-        for (int i = wave; i < COPIES; i += 4) {             // (rolled: eighteen addresses at once have no room beside what the loop over the blocks keeps)
-            const int at = 64 * i + lane, r = at / UNITS, u = place(at % UNITS, r);      // (the permutation is its own inverse)
-            const int row = row0 + r < rows ? row0 + r : rows - 1, token = fast_div(row, by_group), head = row - token * group;
-            const bool rope = u >= DC / 8;
-            const char* const src = (rope ? rotary : latent) + head * (rope ? r_sh : l_sh) + token * (rope ? r_sn : l_sn) + 16 * (rope ? u - DC / 8 : u);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(__builtin_amdgcn_readfirstlane((int)(to + 1024u * i))), "v"(src) : "memory");
+        row = tid / T;
+        unit = tid % T;
+        const int r = row0 + row < d.rows ? row0 + row : d.rows - 1;
+        token = paged_div(r, d.d_group);
+        const int head = r - token * d.group, u = unit % RU;
+        const char* const latent = d.q + t.z * d.q_sb + head * d.q_sh + token * d.q_sn + 16 * unit;
+        const char* const rotary = p->q_rope + t.z * p->qr_sb + head * p->qr_sh + token * p->qr_sn;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = *(const v4i*)(latent + 16 * T * i);
+        rope = *(const v4i*)(rotary + 16 * u);
+        other = rope;
+        if (d.rope.freqs != nullptr && !d.rope.interleaved) {
+            const int half = d.rope.pairs / 8;
+            other = *(const v4i*)(rotary + 16 * (u >= 2 * half ? u : u >= half ? u - half : u + half));
         }
     }
-};
-// A query row's operand fragments.  A lane has sixteen elements of every STEP: those from 16 * part on (STEP 32: of the two lanes l, l ^ 32; 64: of the four of equal l % 16).
-template <int DC, int DR, int DT, int STEP, int ROWS> struct LatentQuery {
-    typedef LatentQueryTile<DC, DR, ROWS> Tile;
-    static constexpr int KC = DC / STEP, KR = (DR + STEP - 1) / STEP, KS = KC + KR;
-    v4i hi[KS], lo[KS];
-    float factor;                              // of the integer sums times kScoreUnit * scale: the score in base 2; NaN for a row that holds no number
-    // r: the row in the tile.  angles: (cos, sin) of the pairs of its token
-    __device__ __forceinline__ void form(LatentArgs p, const char* tile, int r, int part, const v2f* angles) {
+    // angles: (cos, sin) of the pairs, of the tokens from first_token on.  The row's factor: of the integer sums times kScoreUnit * scale; NaN for a row that holds no number.
+    __device__ __forceinline__ void form(LatentArgs p, char* lds, const v2f* angles, int first_token, float* factors) {
         const auto& d = p->deal;
-        const int pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
-        const bool interleaved = d.rope.interleaved != 0;
-        // eight elements from `at` on, of the row's latent and rotary part side by side
-        auto eight = [&](int at) __attribute__((always_inline)) { return *(const v4i*)(tile + r * Tile::ROW + 16 * Tile::place(at / 8, r)); };
-        float rope[KR][16];
+        const int u = unit % RU, pairs = d.rope.freqs != nullptr ? d.rope.pairs : 0;
+        float turned[8];
+        unpack8<DT>(rope, turned);
+        if (8 * u < 2 * pairs) {               // (pairs are a multiple of eight: eight elements turn alike)
+            const bool second = 8 * u >= pairs;
+            const v2f* const mine = angles + (token - first_token) * pairs;
+            if (d.rope.interleaved) {
 #pragma unroll
-        for (int k = 0; k < KR; ++k)
+                for (int i = 0; i < 4; ++i) rope_turn(turned[2 * i], turned[2 * i + 1], mine[4 * u + i][0], mine[4 * u + i][1]);
+            } else {
+                float y[8];
+                unpack8<DT>(other, y);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = STEP * k + 16 * part + 8 * h, in = at < DR ? at : 0;
-                float* const x = &rope[k][8 * h];
-                unpack8<DT>(eight(DC + in), x);
-                if (pairs > 0) {
-                    // (pairs are a multiple of eight: eight elements turn alike)
-                    const bool turned = in < 2 * pairs, second = in >= pairs && !interleaved;
-                    const v2f* const mine = angles + (!turned ? 0 : interleaved ? in / 2 : second ? in - pairs : in);
-                    float y[8];
-                    if (interleaved) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = x[i];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) rope_turn(y[2 * i], y[2 * i + 1], mine[i][0], mine[i][1]);
-                    } else {
-                        unpack8<DT>(eight(DC + (!turned ? in : second ? in - pairs : in + pairs)), y);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = x[i] * mine[i][0] + y[i] * (second ? mine[i][1] : -mine[i][1]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = turned ? y[i] : x[i];
+                for (int i = 0; i < 8; ++i) {
+                    const v2f a = mine[8 * u - (second ? pairs : 0) + i];
+                    turned[i] = turned[i] * a[0] + y[i] * (second ? a[1] : -a[1]);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = at < DR ? x[i] : 0.f;
-                __builtin_amdgcn_sched_barrier(0);
             }
-        // (magnitudes of 16-bit numbers are ordered as their bits are)
+        }
+        // (magnitudes of numbers are ordered as their bits are)
         typedef unsigned short v2us __attribute__((ext_vector_type(2)));
         v2us most = {0, 0};
 #pragma unroll
-        for (int k = 0; k < KC; ++k)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v4i raw = eight(STEP * k + 16 * part + 8 * h);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, raw[i] & 0x7fff7fff));
-            }
-        float two[8];
-        unpack8<DT>((v4i){__builtin_bit_cast(int, most), 0, 0, 0}, two);
-        uint32_t top = __builtin_bit_cast(uint32_t, two[0]), other_top = __builtin_bit_cast(uint32_t, two[1]);
+            for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, x[i][w] & 0x7fff7fff));
+        float y[8];
+        unpack8<DT>((v4i){__builtin_bit_cast(int, most), 0, 0, 0}, y);
+        uint32_t top = __builtin_bit_cast(uint32_t, y[0]), other_top = __builtin_bit_cast(uint32_t, y[1]);
         top = top > other_top ? top : other_top;
 #pragma unroll
-        for (int k = 0; k < KR; ++k)
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t a = __builtin_bit_cast(uint32_t, turned[i]) & 0x7fffffffu;
+            top = top > a ? top : a;
+        }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t a = __builtin_bit_cast(uint32_t, rope[k][i]) & 0x7fffffffu;
-                top = top > a ? top : a;
-            }
-#pragma unroll
-        for (int w = STEP == 32 ? 32 : 16; w < 64; w <<= 1) {
+        for (int w = 1; w < T; w <<= 1) {
             const uint32_t a = (uint32_t)__shfl_xor((int)top, w);
             top = top > a ? top : a;
         }
         const float size = fmaxf(__builtin_bit_cast(float, top), 0x1p-100f);      // (a row under it: its scores are nothing)
         const float steps = copysignf(kQuerySteps / size, d.qk_scale_log2);
-        factor = top < 0x7f800000u ? size * (1.f / kQuerySteps) * (fabsf(d.qk_scale_log2) * (1.f / kScoreUnit)) : __builtin_nanf("");
+        if (unit == 0) factors[row] = top < 0x7f800000u ? size * (1.f / kQuerySteps) * (fabsf(d.qk_scale_log2) * (1.f / kScoreUnit)) : __builtin_nanf("");
+        char* const to = lds + S::QUERY_AT + row * S::ROW;
+        auto put = [&](int at, const float (&e)[8]) __attribute__((always_inline)) {       // at: unit of eight
+            v2i hi, lo;
+            split_steps(e, steps, hi, lo);
+            char* const dst = to + 16 * S::place(at / 2, row) + 8 * (at & 1);
+            *(v2i*)dst = hi;
+            *(v2i*)(dst + ROWS * S::ROW) = lo;
+        };
 #pragma unroll
-        for (int k = 0; k < KR; ++k) split_steps(rope[k], steps, hi[KC + k], lo[KC + k]);
-        asm volatile("" ::: "memory");         // (the elements once more, and not kept since the maximum)
-#pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            float x[16];
-            unpack8<DT>(eight(STEP * k + 16 * part), x);
-            unpack8<DT>(eight(STEP * k + 16 * part + 8), x + 8);
-            split_steps(x, steps, hi[k], lo[k]);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < N; ++i) {
+            unpack8<DT>(x[i], y);
+            put(unit + T * i, y);
         }
+        if (unit < RU) put(DC / 8 + unit, turned);
     }
 };
 
@@ -270,7 +248,8 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     constexpr bool SMALL = ROWS == 32;         // scores in tiles of 16 keys by 16 rows: a wave has 16 keys of a block; else of 32 by 32
     constexpr int STEP = SMALL ? 64 : 32;
     static_assert(SMALL || (QT == 1 && RG == 2), "");
-    typedef LatentQuery<DC, DR, DT, STEP, ROWS> Query;
+    constexpr int KC = DC / STEP, KR = (DR + STEP - 1) / STEP, KS = KC + KR;      // steps of the score's products: latent part, rotary part
+    typedef LatentQueries<DC, DR, DT, ROWS> Queries;
     __shared__ __align__(16) char lds[S::LDS];
     LatentArgs p = latent_args();
     PagedArgs deal = paged_args_first();
@@ -278,9 +257,8 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     const double freq = paged_frequency(deal);
     PagedPiece piece = paged_find(deal, ROWS, t);
     if ((int)threadIdx.x < DR / 2) ((double*)(lds + S::FREQS_AT))[threadIdx.x] = freq;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & 3;      // (of its half)
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) & 3;      // (of its half)
     const bool scoring = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) < 4;
-    const int lq = lane & 31, lh = lane >> 5, x16 = lane & 15, c16 = lane >> 4;
     const int rg = SMALL ? 0 : wave % RG, kg = SMALL ? wave : wave / RG;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     float* const tops = (float*)(lds + S::TOPS_AT);
@@ -289,51 +267,115 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     v4i open = {0, 0, 0, 0};
     __syncthreads();
   while (piece.start < piece.end) {
+    int tid = (int)threadIdx.x;
+    asm volatile("" : "+v"(tid));              // (the lanes' many places are found again for each item: held beside each other from the kernel's start, they spill)
+    const int lane = tid & 63, lq = lane & 31, lh = lane >> 5, x16 = lane & 15, c16 = lane >> 4;
     const PagedPart part = paged_part(deal, t, piece);
     if (part.none) break;
     const int row0 = t.tile * ROWS, most = part.key_end, key_first = part.key_first;
     const int blocks = most > key_first ? (most - key_first + KEYS - 1) / KEYS : 0;
+    // Reads of rows of the tiles as operands: a fragment's place is one of two lane addresses and a constant (the permutation flips low bits of the unit's number, and for a
+    // rotary part of 32 bit 3 as well).
+    struct RowAt { int at[2], rope; };
+    auto row_at = [&](int r, int unit) __attribute__((always_inline)) {
+        return RowAt{{r * S::ROW + 16 * S::place(unit, r), r * S::ROW + 16 * S::place(unit + (DR == 32 ? 8 : 2), r)}, r * S::ROW + 16 * S::place(S::LATENT_UNITS + unit, r)};
+    };
+    auto fragment_at = [&](const RowAt& w, int k) __attribute__((always_inline)) {
+        constexpr int UPF = SMALL ? 4 : 2;     // units of a fragment
+        if (DR == 64) return SMALL ? w.at[0] + 64 * k : w.at[k & 1] + 64 * (k >> 1);
+        if (k >= KC) return w.rope + 16 * UPF * (k - KC);
+        const int bit = DR == 32 && S::LATENT_UNITS >= 16 ? UPF * k >> 3 & 1 : 0;
+        return w.at[bit] + 16 * (UPF * k - 8 * bit);
+    };
+    // ======== copies: wave w of the second half copies rows 16 w .. 16 w + 15 of every block
+    const int k_sn = deal->k_sn;
+    auto offset_of = [&](int i) __attribute__((always_inline)) {
+        const int unit = 64 * i + lane, r = unit / S::UNITS < 16 ? unit / S::UNITS : 15, u = unit % S::UNITS;
+        return (uint32_t)(r * k_sn + 16 * S::place(u, r));      // (the permutation is its own inverse)
+    };
+    uint32_t copy_off[S::WHOLE], copy_half = S::HALF ? offset_of(S::WHOLE) : 0u;
+#pragma unroll
+    for (int i = 0; i < S::WHOLE; ++i) copy_off[i] = offset_of(i);
+    const uint32_t scale_off = (uint32_t)(((lane & 31) >> 1) * (int)deal->ks_sh * 4 + (lane & 1) * 4);
+    // (what a copy needs of the arguments, held: loaded anew for each one, they are a chain of trips to the scalar cache)
+    PagedInts table = (PagedInts)(deal->table + t.z * deal->bt_sb);
+    const char* all_rows = deal->k;
+    const float* all_scales = deal->k_scale;
+    int64_t k_sp = deal->k_sp, ks_sp = deal->ks_sp;
+    int page_log2 = deal->page_log2, last_column = deal->table_width - 1, num_pages = deal->num_pages, ks_sh = (int)deal->ks_sh;
+    asm volatile("" : "+s"(table), "+s"(all_rows), "+s"(all_scales), "+s"(k_sp), "+s"(ks_sp), "+s"(page_log2), "+s"(last_column), "+s"(num_pages), "+s"(ks_sh));
+    const int page_mask = (1 << page_log2) - 1;
+    auto look = [&](int block) __attribute__((always_inline)) {
+        const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
+        return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
+    };
+    auto copy = [&](int block, int id) __attribute__((always_inline)) {
+        const bool named = (unsigned)id < (unsigned)num_pages;
+        const int at = named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
+        const char* const rows = all_rows + at * k_sp + row * k_sn;
+        const uint32_t to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
+        copy_rows(rows, copy_off, to);
+        if (S::HALF && lane < 32) copy_units(rows, copy_half, to + 1024u * S::WHOLE);
+        const char* const scales = (const char*)(all_scales + at * ks_sp + row * ks_sh);
+        if (lane < 32)
+            copy_words(named ? scales : (const char*)kHiddenScale, named ? scale_off : (uint32_t)lane * 4, lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128));
+    };
+    // ======== the queries, by all waves, while the first block comes
+    {
+        Queries queries;
+        if (blocks > 0) {
+            queries.load(p, t, row0, tid);
+            if (!scoring) copy(0, look(0));
+            const int first_token = paged_div(row0, deal->d_group);
+            if (deal->rope.freqs != nullptr) {     // the angles of the tile's tokens, each once
+                const int last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
+                const int angles = (paged_div(last_row, deal->d_group) - first_token + 1) * pairs;
+                for (int i = tid; i < angles; i += S::THREADS) {
+                    const int token = paged_div(i, deal->d_pairs), pair = i - token * pairs;
+                    float c, s;
+                    rope_angle(((const double*)(lds + S::FREQS_AT))[pair], t.n - t.m + first_token + token, deal->rope.magnitude, c, s);
+                    ((v2f*)(lds + S::ANGLES_AT))[i] = (v2f){c, s};
+                }
+                lds_barrier();
+            }
+            queries.form(p, lds, (const v2f*)(lds + S::ANGLES_AT), first_token, alphas);
+        }
+        if (!scoring) wait_copies<0>();
+        lds_barrier();                         // queries and first block are there
+    }
     if (scoring) {
         // ======== scores and weights
-        Query query[QT];
+        v4i query_hi[QT][KS], query_lo[QT][KS];
+        float factor[QT];
         int seen[QT];
-        const int first_token = paged_div(row0, deal->d_group), least = paged_token_keys(deal, t, t.first_token);
-        lds_barrier();                         // (queries and angles are there)
+        const int least = paged_token_keys(deal, t, t.first_token);
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
             const int r = SMALL ? 16 * q + x16 : 32 * rg + lq, row = row0 + r < deal->rows ? row0 + r : deal->rows - 1, token = paged_div(row, deal->d_group);
+            const RowAt at = row_at(r, SMALL ? c16 : lh);
             seen[q] = paged_token_keys(deal, t, token);
-            query[q].form(p, lds + S::QUERY_AT, r, SMALL ? c16 : lh, (const v2f*)(lds + S::ANGLES_AT) + (deal->rope.freqs != nullptr ? (token - first_token) * deal->rope.pairs : 0));
+            factor[q] = alphas[r];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const bool in = DR % STEP == 0 || k < KC || c16 < DR / 16;      // (else the row's last step reaches behind it)
+                query_hi[q][k] = *(const v4i*)(lds + S::QUERY_AT + fragment_at(at, k));
+                query_lo[q][k] = *(const v4i*)(lds + S::QUERY_AT + ROWS * S::ROW + fragment_at(at, k));
+                if (!in) query_hi[q][k] = query_lo[q][k] = (v4i){0, 0, 0, 0};
+            }
         }
-        // Reads of the tiles: a fragment's place is one of two lane addresses and a constant (the permutation flips low bits of the unit's number, and for a rotary part
-        // of 32 bit 3 as well).
-        constexpr bool FLIP = DR == 32 && S::LATENT_UNITS >= 16;
-        int key_at[2], key_rope_at;
-        {
-            const int key_row = SMALL ? 16 * wave + x16 : 32 * kg + lq, unit = SMALL ? c16 : lh;
-            key_at[0] = key_row * S::ROW + 16 * S::place(unit, key_row);
-            key_at[1] = key_row * S::ROW + 16 * S::place(unit + (DR == 32 ? 8 : 2), key_row);
-            key_rope_at = key_row * S::ROW + 16 * S::place(S::LATENT_UNITS + unit, key_row);
-        }
-        auto key_offset = [&](int k) __attribute__((always_inline)) {
-            constexpr int UPF = SMALL ? 4 : 2;     // units of a fragment
-            if (DR == 64) return SMALL ? key_at[0] + 64 * k : key_at[k & 1] + 64 * (k >> 1);
-            if (k >= Query::KC) return key_rope_at + 16 * UPF * (k - Query::KC);
-            const int bit = FLIP ? UPF * k >> 3 & 1 : 0;
-            return key_at[bit] + 16 * (UPF * k - 8 * bit);
-        };
+        const RowAt key_at = row_at(SMALL ? 16 * wave + x16 : 32 * kg + lq, SMALL ? c16 : lh);
         float m[QT], l[QT];
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
             m[q] = -INFINITY;
             l[q] = 0.f;
         }
-        lds_barrier();                         // (the first block is there)
+        if (SMALL) lds_barrier();              // (the queries have been read)
         if constexpr (!SMALL)
         {
             // A step forms the scores of block i + 1 while it takes the exponentials of block i: the first fragments' products run while the rows' maxima are settled, and with each of
             // the others come one or two of a lane's sixteen weights.
-            constexpr int KC = Query::KC, KS = Query::KS, AHEAD = 3, EARLY = KC / 8 > 1 ? KC / 8 : 1;      // fragments ahead of the products; of the latent part ahead of the weights
+            constexpr int AHEAD = 3, EARLY = KC / 8 > 1 ? KC / 8 : 1;      // fragments ahead of the products; of the latent part ahead of the weights
             static_assert(KC >= 4, "");
             float s[16], inv = 0.f, e_last = 0.f;
             uint32_t w[4];
@@ -354,14 +396,14 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 v4i f[4];
                 v16i hi, lo;
                 auto fetch = [&](int k) __attribute__((always_inline)) {
-                    if (QK && k < KS) f[k % 4] = *(const v4i*)(lds + tile + key_offset(k));
+                    if (QK && k < KS) f[k % 4] = *(const v4i*)(lds + tile + fragment_at(key_at, k));
                 };
                 auto product = [&](int k) __attribute__((always_inline)) {
                     fetch(k + AHEAD);
                     if (!QK) return;
                     const bool first = k == 0 || k == KC;
-                    hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query[0].hi[k], first ? (v16i){0} : hi, 0, 0, 0);
-                    lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query[0].lo[k], first ? (v16i){0} : lo, 0, 0, 0);
+                    hi = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query_hi[0][k], first ? (v16i){0} : hi, 0, 0, 0);
+                    lo = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k % 4], query_lo[0][k], first ? (v16i){0} : lo, 0, 0, 0);
                 };
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) fetch(k);
@@ -416,7 +458,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         fmac_lane_scale_f(s[i], sc.r, (float)(hi[i] * 256 + lo[i]), i);
-                        s[i] = add_lane_scale(s[i] * query[0].factor, sc.log, i);
+                        s[i] = add_lane_scale(s[i] * factor[0], sc.log, i);
                     }
                     if (key0 + KEYS > least) {
 #pragma unroll
@@ -447,7 +489,6 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             const float* const scales = (const float*)(lds + S::SCALES_AT + (block % STAGES) * S::SCALE_STAGE);
             // ---- scores, as t = score + log2 of the value's scale
             constexpr int PER = SMALL ? 4 : 16;    // a lane's keys
-            constexpr int KS = Query::KS, KC = Query::KC;
             typedef typename std::conditional<SMALL, v4i, v16i>::type Sums;
             float s[QT][PER];
             // (lane i of a row of sixteen has the scales of the row's i-th key, from where all of the row take them)
@@ -456,7 +497,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             // the rotary part first, then the latent one, two fragments ahead of the products
             auto fragment = [&](int i) __attribute__((always_inline)) {
                 const int k = i < KS - KC ? KC + i : i - (KS - KC);
-                return *(const v4i*)(lds + tile + key_offset(k));
+                return *(const v4i*)(lds + tile + fragment_at(key_at, k));
             };
             Sums hi[QT], lo[QT];
             auto clear = [&]() __attribute__((always_inline)) {
@@ -484,11 +525,11 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
                     if constexpr (SMALL) {
-                        hi[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query[q].hi[k], hi[q], 0, 0, 0);
-                        lo[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query[q].lo[k], lo[q], 0, 0, 0);
+                        hi[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_hi[q][k], hi[q], 0, 0, 0);
+                        lo[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_lo[q][k], lo[q], 0, 0, 0);
                     } else {
-                        hi[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query[q].hi[k], hi[q], 0, 0, 0);
-                        lo[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query[q].lo[k], lo[q], 0, 0, 0);
+                        hi[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query_hi[q][k], hi[q], 0, 0, 0);
+                        lo[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query_lo[q][k], lo[q], 0, 0, 0);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -498,7 +539,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             for (int q = 0; q < QT; ++q) {
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    s[q][i] = ((float)(hi[q][i] * 256 + lo[q][i]) * lane_scale(sc.c, i) + s[q][i]) * query[q].factor + lane_scale(sc.log, i);
+                    s[q][i] = ((float)(hi[q][i] * 256 + lo[q][i]) * lane_scale(sc.c, i) + s[q][i]) * factor[q] + lane_scale(sc.log, i);
                 if (key0 + KEYS > least) {
 #pragma unroll
                     for (int i = 0; i < PER; ++i) {
@@ -570,43 +611,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         }
         lds_barrier();
     } else {
-        // ======== copies, and the values' product: wave w copies rows 16 w .. 16 w + 15 of every block
-        const int k_sn = deal->k_sn;
-        auto offset_of = [&](int i) __attribute__((always_inline)) {
-            const int unit = 64 * i + lane, r = unit / S::UNITS < 16 ? unit / S::UNITS : 15, u = unit % S::UNITS;
-            return (uint32_t)(r * k_sn + 16 * S::place(u, r));      // (the permutation is its own inverse)
-        };
-        uint32_t copy_off[S::WHOLE], copy_half = S::HALF ? offset_of(S::WHOLE) : 0u;
-#pragma unroll
-        for (int i = 0; i < S::WHOLE; ++i) copy_off[i] = offset_of(i);
-        const uint32_t scale_off = (uint32_t)(((lane & 31) >> 1) * (int)deal->ks_sh * 4 + (lane & 1) * 4);
-        // (what a copy needs of the arguments, held: loaded anew for each one, they are a chain of trips to the scalar cache)
-        PagedInts table = (PagedInts)(deal->table + t.z * deal->bt_sb);
-        const char* all_rows = deal->k;
-        const float* all_scales = deal->k_scale;
-        int64_t k_sp = deal->k_sp, ks_sp = deal->ks_sp;
-        int page_log2 = deal->page_log2, last_column = deal->table_width - 1, num_pages = deal->num_pages, ks_sh = (int)deal->ks_sh;
-        asm volatile("" : "+s"(table), "+s"(all_rows), "+s"(all_scales), "+s"(k_sp), "+s"(ks_sp), "+s"(page_log2), "+s"(last_column), "+s"(num_pages), "+s"(ks_sh));
-        const int page_mask = (1 << page_log2) - 1;
-        auto look = [&](int block) __attribute__((always_inline)) {
-            const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
-            return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
-        };
-        auto copy = [&](int block, int id) __attribute__((always_inline)) {
-            const bool named = (unsigned)id < (unsigned)num_pages;
-            const int at = named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
-            const char* const rows = all_rows + at * k_sp + row * k_sn;
-            const uint32_t to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
-            copy_rows(rows, copy_off, to);
-            if (S::HALF && lane < 32) copy_units(rows, copy_half, to + 1024u * S::WHOLE);
-            const char* const scales = (const char*)(all_scales + at * ks_sp + row * ks_sh);
-            if (lane < 32)
-                copy_words(named ? scales : (const char*)kHiddenScale, named ? scale_off : (uint32_t)lane * 4, lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128));
-        };
-        if (blocks > 0) {
-            LatentQueryTile<DC, DR, ROWS>::copy(p, t, row0, wave, lane, lds0 + S::QUERY_AT);
-            copy(0, look(0));
-        }
+        // ======== copies, and the values' product
         const int id_second = look(1);
         int id_next = look(2);
         int value_at[2];
@@ -624,20 +629,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[g][ct][r] = 0.f;
-        if (blocks > 0 && deal->rope.freqs != nullptr) {      // the angles of the tile's tokens, each once
-            const int first_token = paged_div(row0, deal->d_group), last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
-            const int tokens = paged_div(last_row, deal->d_group) - first_token + 1;
-            for (int i = (int)threadIdx.x - 256; i < tokens * pairs; i += 256) {
-                const int token = paged_div(i, deal->d_pairs), pair = i - token * pairs;
-                float c, s;
-                rope_angle(((const double*)(lds + S::FREQS_AT))[pair], t.n - t.m + first_token + token, deal->rope.magnitude, c, s);
-                ((v2f*)(lds + S::ANGLES_AT))[i] = (v2f){c, s};
-            }
-        }
-        wait_copies<S::COPIES>();
-        lds_barrier();
-        wait_copies<0>();
-        lds_barrier();
+        if (SMALL) lds_barrier();
         if (blocks > 1) copy(1, id_second);
         for (int i = 0; i <= blocks; ++i) {
             if (!SMALL) {
@@ -724,7 +716,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 const int token = paged_div(row, p->deal.d_group), head = row - token * p->deal.group;
                 const bool empty = top == -INFINITY || token >= t.m;
                 const float weight = empty ? 0.f : kWeightUnit / sum;
-                char* const dst = p->deal.out + t.z * p->deal.o_sb + head * p->deal.o_sh + token * p->deal.o_sn + 2 * (32 * NT * wave + 4 * lh);
+                // (through LDS: a lane has eight bytes of each of its units, and 32 rows are as many lines)
 #pragma unroll
                 for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
@@ -732,7 +724,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                         v4f o = {acc[g][ct][4 * k], acc[g][ct][4 * k + 1], acc[g][ct][4 * k + 2], acc[g][ct][4 * k + 3]};
                         o *= weight;
                         if (token >= t.m) o = (v4f){0.f, 0.f, 0.f, 0.f};
-                        store_out4<DT>(dst + 2 * (32 * ct + 8 * k), o);
+                        store_out4<DT>(lds + r * (2 * DC) + 16 * ((4 * (NT * wave + ct) + k) ^ (r & 15)) + 8 * lh, o);
                     }
                 if (p->deal.lse != nullptr && wave == 0 && lh == 0)
                     p->deal.lse[((int64_t)t.z * p->deal.heads + head) * p->deal.seqlen + token] =
@@ -746,6 +738,15 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                         *(v4f*)(slot + (((g * S::CT + NT * wave + ct) * 4 + k) * 64 + lane) * 4) = (v4f){acc[g][ct][4 * k], acc[g][ct][4 * k + 1], acc[g][ct][4 * k + 2], acc[g][ct][4 * k + 3]};
                 if (wave == 0 && lh == 0) *(v2f*)(p->deal.part_stats + ((int64_t)part.slot * ROWS + r) * 2) = (v2f){top, sum};
             }
+        }
+    }
+    if (part.whole) {
+        lds_barrier();
+        for (int i = tid; i < ROWS * (DC / 8); i += S::THREADS) {
+            const int r = i / (DC / 8), u = i % (DC / 8), row = row0 + r;
+            if (row >= p->deal.rows) break;
+            const int token = paged_div(row, p->deal.d_group), head = row - token * p->deal.group;
+            *(v4i*)(p->deal.out + t.z * p->deal.o_sb + head * p->deal.o_sh + token * p->deal.o_sn + 16 * u) = *(const v4i*)(lds + r * (2 * DC) + 16 * (u ^ (r & 15)));
         }
     }
     if (!part.whole && part.one == (int)blockIdx.x) open = (v4i){part.pieces, t.z, t.tile, (int)part.slot};
