@@ -756,71 +756,146 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     if (threadIdx.x == 0) latent_args()->open_items[blockIdx.x] = open;
 }
 
-// The items that lie in several pieces, a launch later: a thread has four neighbouring columns of a row, in all pieces.
+// The items that lie in several pieces, a launch later.  A slice is 32 rows by 32 columns; a wave takes one, or, of an item of many pieces, an eighth of the pieces of one, and the
+// eight join theirs.  The workgroups deal the open items' slices among themselves (a grid over all items would be mostly workgroups without work).
 template <int DC, int DT, int ROWS>
-__global__ void __launch_bounds__(256) latent_merge_kernel(const LatentParams) {
+__global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
+    constexpr int SLICES = ROWS / 32 * (DC / 32), MANY = 8, WAVES = 8;
+    constexpr int SETS = (SLICES + WAVES - 1) / WAVES;         // of slices, an eight of waves each
+    __shared__ __align__(16) float joined[WAVES - 1][64][18];
+    __shared__ int items[512 + 1], first[512 + 1], count;      // the open items; their first unit of work
     LatentArgs p = latent_args();
-    const v4i open = p->open_items[blockIdx.y];
-    const int pieces = open[0];
-    if (pieces == 0) return;
-    constexpr int CT = DC / 32;
-    const int i = (int)blockIdx.x * 256 + (int)threadIdx.x, lane = i & 63, k = (i >> 6) & 3, ct = (i >> 8) % CT, g = (i >> 8) / CT;
-    const int r = 32 * g + (lane & 31), row = open[2] * ROWS + r, col = 32 * ct + 8 * k + 4 * (lane >> 5), z = open[1];
     const auto& d = p->deal;
-    if (row >= d.rows) return;
-    const int token = paged_div(row, d.d_group), head = row - token * d.group;
-    int m = d.seqlen;
-    if (d.seqlens_q != nullptr) {
-        const int n = d.seqlens_q[z];
-        m = n < 0 ? 0 : n < m ? n : m;
-    }
-    // the pieces: the first in its workgroup's own slot, the others first items of theirs
-    auto slot_of = [&](int j) __attribute__((always_inline)) { return (int64_t)(j == 0 ? open[3] : 2 * ((open[3] >> 1) + j)); };
-    constexpr int MANY = 8;
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    float top = -INFINITY, sum = 0.f;
-    for (int j0 = 0; j0 < pieces; j0 += MANY) {
-        v4f x[MANY];
-        v2f st[MANY];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (wave == 0) {
+        int found = 0, units = 0;
+        for (int i0 = 0; i0 < d.grid; i0 += 64) {
+            const int pieces = i0 + lane < d.grid ? p->open_items[i0 + lane][0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
+            int upto = mine;
 #pragma unroll
-        for (int u = 0; u < MANY; ++u) {
-            const int64_t slot = slot_of(j0 + u < pieces ? j0 + u : j0);
-            st[u] = *(const v2f*)(d.part_stats + (slot * ROWS + r) * 2);
-            x[u] = *(const v4f*)(d.parts + slot * ROWS * DC + (int64_t)i * 4);
-        }
-        float grown = top;
-#pragma unroll
-        for (int u = 0; u < MANY; ++u) {
-            if (j0 + u >= pieces) st[u][0] = -INFINITY;
-            grown = fmaxf(grown, st[u][0]);
-        }
-        const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
-        acc *= a;
-        sum *= a;
-        top = grown;
-#pragma unroll
-        for (int u = 0; u < MANY; ++u) {
-            const float w = fast_exp2(st[u][0] - frame);
-            if (j0 + u < pieces) {
-                acc += w * x[u];
-                sum = fmaf(w, st[u][1], sum);
+            for (int w = 1; w < 64; w <<= 1) {
+                const int o = __shfl_up(upto, w);
+                if (lane >= w) upto += o;
             }
+            const uint64_t open = __ballot(pieces != 0);
+            const int at = found + __popcll(open & ((1ull << lane) - 1));
+            if (pieces != 0) {
+                items[at] = i0 + lane;
+                first[at] = units + upto - mine;
+            }
+            found += __popcll(open);
+            units += __shfl(upto, 63);
+        }
+        if (lane == 0) {
+            count = found;
+            first[found] = units;
         }
     }
-    const bool empty = top == -INFINITY || token >= m;
-    acc *= empty ? 0.f : kWeightUnit / sum;
-    if (token >= m) acc = (v4f){0.f, 0.f, 0.f, 0.f};
-    char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * col;
-    store_out4<DT>(dst, acc);
-    if (d.lse != nullptr && col == 0)
-        d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = token >= m ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+    __syncthreads();
+    const int found = count, total = first[found];
+    for (int unit = (int)blockIdx.x; unit < total; unit += (int)gridDim.x) {
+        int lo = 0, hi = found;                // the item that has it: first[lo] <= unit < first[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first[mid] <= unit) lo = mid; else hi = mid;
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        const v4i open = ((const __attribute__((address_space(4))) v4i*)p->open_items)[__builtin_amdgcn_readfirstlane(items[lo])];
+        const int pieces = open[0], z = open[1], part = unit - __builtin_amdgcn_readfirstlane(first[lo]);
+        const bool share = pieces > MANY;      // the waves share a slice's pieces
+        const int slice = share ? part : part * WAVES + wave, g = slice / (DC / 32), ct = slice % (DC / 32);
+        const int r = 32 * g + (lane & 31), row = open[2] * ROWS + r;
+        const bool valid = row < d.rows && slice < SLICES;
+        const int token = paged_div(valid ? row : 0, d.d_group), head = (valid ? row : 0) - token * d.group;
+        const int64_t slot0 = open[3];
+        float acc[16], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        const int step = share ? WAVES : 1;
+        if (valid)
+            for (int j0 = share ? wave : 0; j0 < pieces; j0 += MANY / 2 * step) {
+                v4f x[MANY / 2][4];
+                v2f st[MANY / 2];
+#pragma unroll
+                for (int u = 0; u < MANY / 2; ++u) {
+                    const int j = j0 + u * step;
+                    st[u] = (v2f){-INFINITY, 0.f};
+                    if (j >= pieces) continue;
+                    // the pieces: the first in its workgroup's own slot, the others first items of theirs
+                    const int64_t slot = j == 0 ? slot0 : 2 * ((slot0 >> 1) + j);
+                    st[u] = *(const v2f*)(d.part_stats + (slot * ROWS + r) * 2);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[u][k] = *(const v4f*)(d.parts + slot * ROWS * DC + ((slice * 4 + k) * 64 + lane) * 4);
+                }
+                float grown = top;
+#pragma unroll
+                for (int u = 0; u < MANY / 2; ++u) grown = fmaxf(grown, st[u][0]);
+                const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] *= a;
+                sum *= a;
+                top = grown;
+#pragma unroll
+                for (int u = 0; u < MANY / 2; ++u) {
+                    if (j0 + u * step >= pieces) continue;
+                    const float w = fast_exp2(st[u][0] - frame);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[i] = fmaf(w, x[u][i / 4][i % 4], acc[i]);
+                    sum = fmaf(w, st[u][1], sum);
+                }
+            }
+        if (share) {
+            if (wave > 0) {
+                float* const to = joined[wave - 1][lane];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[i] = acc[i];
+                to[16] = top;
+                to[17] = sum;
+            }
+            __syncthreads();
+            if (wave == 0) {
+#pragma unroll 1
+                for (int w = 0; w < WAVES - 1; ++w) {
+                    const float* const from = joined[w][lane];
+                    const float grown = fmaxf(top, from[16]), frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame), b = fast_exp2(from[16] - frame);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[i] = fmaf(b, from[i], a * acc[i]);
+                    sum = fmaf(b, from[17], a * sum);
+                    top = grown;
+                }
+            }
+            __syncthreads();
+        }
+        if (valid && (!share || wave == 0)) {
+            int m = d.seqlen;
+            if (d.seqlens_q != nullptr) {
+                const int n = d.seqlens_q[z];
+                m = n < 0 ? 0 : n < m ? n : m;
+            }
+            const bool beyond = token >= m;
+            const float weight = beyond || top == -INFINITY ? 0.f : kWeightUnit / sum;
+            char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * (32 * ct + 4 * (lane >> 5));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v4f o = {acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]};
+                o *= weight;
+                if (beyond) o = (v4f){0.f, 0.f, 0.f, 0.f};
+                store_out4<DT>(dst + 16 * k, o);
+            }
+            if (d.lse != nullptr && ct == 0 && lane < 32)
+                d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = beyond ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+        }
+    }
 }
 
 template <int DC, int DR, int DT, int ROWS, int QT> int launch_latent_rows(const LatentParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((latent_attn_kernel<DC, DR, DT, ROWS, QT>), dim3((unsigned)p.deal.grid), dim3(512), 0, stream, p);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
-    hipLaunchKernelGGL((latent_merge_kernel<DC, DT, ROWS>), dim3(ROWS * DC / 1024, (unsigned)p.deal.grid), dim3(256), 0, stream, p);
+    // (an item of few pieces is SLICES / 8 units of work, one of nine or more SLICES)
+    constexpr int SLICES = ROWS / 32 * (DC / 32);
+    const int units = p.deal.grid * SLICES / 8 + SLICES;
+    hipLaunchKernelGGL((latent_merge_kernel<DC, DT, ROWS>), dim3((unsigned)(units < 2 * kComputeUnits ? units : 2 * kComputeUnits)), dim3(512), 0, stream, p);
     return (int)hipGetLastError();
 }
 template <int DC, int DR, int DT> int launch_latent(const LatentParams& p, int rows, hipStream_t stream) {
