@@ -92,6 +92,11 @@ template <int N> __device__ __forceinline__ void copy_rows(const char* base, con
 __device__ __forceinline__ void copy_units(const char* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
+// 64 x 16 bytes to lds + at, if `wanted`.  (The branch is the statement's own: among the products, a branch of the compiler's costs it its schedule.)
+__device__ __forceinline__ void copy_units_if(int wanted, const char* base, uint32_t off, uint32_t lds, int at) {
+    asm volatile("s_cmp_eq_u32 %4, 0\n\ts_cbranch_scc1 .Lskip_copy%=\n\ts_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n.Lskip_copy%=:"
+                 :: "s"(lds), "v"(off), "s"(base), "i"(at), "s"(wanted) : "memory", "scc");
+}
 __device__ __forceinline__ void copy_words(const char* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
@@ -232,14 +237,6 @@ __device__ __forceinline__ void fmac_lane_scale_exp(float& c, float scales, floa
     asm("s_nop 0\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(c) : "v"(scales), "v"(f), "i"(i));
 }
 
-// V's bytes of eight keys as fp16
-__device__ __forceinline__ v8h bytes_to_f16(v2i b) {
-    uint32_t w[4];
-    i8x4_to_f16((uint32_t)b[0], w[0], w[1]);
-    i8x4_to_f16((uint32_t)b[1], w[2], w[3]);
-    return __builtin_bit_cast(v8h, (v4i){(int)w[0], (int)w[1], (int)w[2], (int)w[3]});
-}
-
 // QT: tiles of 16 rows that the scores of a tile of 32 are formed for (the second one may be empty)
 template <int DC, int DR, int DT, int ROWS, int QT>
 __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams) {
@@ -309,16 +306,25 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
         return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
     };
+    struct BlockCopy { const char* rows; const char* scales; uint32_t to, scales_to; bool named; };
+    auto block_copy = [&](int block, int id) __attribute__((always_inline)) {
+        BlockCopy c;
+        c.named = (unsigned)id < (unsigned)num_pages;
+        const int at = c.named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
+        c.rows = all_rows + at * k_sp + row * k_sn;
+        c.to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
+        c.scales = c.named ? (const char*)(all_scales + at * ks_sp + row * ks_sh) : (const char*)kHiddenScale;
+        c.scales_to = lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128);
+        return c;
+    };
+    auto copy_rest = [&](const BlockCopy& c) __attribute__((always_inline)) {      // what is not copied 64 lanes at a time
+        if (S::HALF && lane < 32) copy_units(c.rows, copy_half, c.to + 1024u * S::WHOLE);
+        if (lane < 32) copy_words(c.scales, c.named ? scale_off : (uint32_t)lane * 4, c.scales_to);
+    };
     auto copy = [&](int block, int id) __attribute__((always_inline)) {
-        const bool named = (unsigned)id < (unsigned)num_pages;
-        const int at = named ? id : 0, row = (key_first + KEYS * block + 16 * wave) & page_mask, stage = block % STAGES;
-        const char* const rows = all_rows + at * k_sp + row * k_sn;
-        const uint32_t to = lds0 + (uint32_t)(stage * S::STAGE + wave * 16 * S::ROW);
-        copy_rows(rows, copy_off, to);
-        if (S::HALF && lane < 32) copy_units(rows, copy_half, to + 1024u * S::WHOLE);
-        const char* const scales = (const char*)(all_scales + at * ks_sp + row * ks_sh);
-        if (lane < 32)
-            copy_words(named ? scales : (const char*)kHiddenScale, named ? scale_off : (uint32_t)lane * 4, lds0 + (uint32_t)(S::SCALES_AT + stage * S::SCALE_STAGE + wave * 128));
+        const BlockCopy c = block_copy(block, id);
+        copy_rows(c.rows, copy_off, c.to);
+        copy_rest(c);
     };
     // ======== the queries, by all waves, while the first block comes
     {
@@ -646,22 +652,40 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             v8h pf[KEYS / 16][RG];
             float alpha[RG];
             bool follow[RG];
-            // (values two steps ahead of their products)
+            const bool more = !SMALL && i > 0 && i + 2 < blocks;
+            int wanted = __builtin_amdgcn_readfirstlane(more ? 1 : 0);
+            asm volatile("" : "+s"(wanted));
+            BlockCopy next{};
+            // (values two steps ahead of their products; a copy of block i + 2 behind each column tile's products)
             v2i vb[2][NT];
             auto fetch = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
                 for (int ct = 0; ct < NT; ++ct)
                     vb[step % 2][ct] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)INTFA_LDS(lds + tile + value_offset(ct) + 16 * step * S::ROW));
             };
+            // Products of step `step`, the conversion of the next column tile's values between them: half of it in the shadow of each product (all of it ahead of both, the matrix
+            // unit waited for it: 64 rows 2.9 us a block).
+            uint32_t vf[2][4];
+            auto convert = [&](int at, int half) __attribute__((always_inline)) {
+                i8x4_to_f16((uint32_t)vb[at / NT % 2][at % NT][half], vf[at % 2][2 * half], vf[at % 2][2 * half + 1]);
+            };
             auto product = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
                 for (int ct = 0; ct < NT; ++ct) {
-                    const v8h vf = bytes_to_f16(vb[step % 2][ct]);
+                    const int at = NT * step + ct;
+                    const v8h v = __builtin_bit_cast(v8h, (v4i){(int)vf[at % 2][0], (int)vf[at % 2][1], (int)vf[at % 2][2], (int)vf[at % 2][3]});
 #pragma unroll
-                    for (int g = 0; g < RG; ++g) acc[g][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[step][g], acc[g][ct], 0, 0, 0);
+                    for (int g = 0; g < RG; ++g) {
+                        acc[g][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[step][g], acc[g][ct], 0, 0, 0);
+                        if (g == 0 && !SMALL && at < S::WHOLE) copy_units_if(wanted, next.rows, copy_off[at < S::WHOLE ? at : 0], next.to, 1024 * at);
+                        if (at + 1 < NT * (KEYS / 16)) {
+                            if (RG == 1) convert(at + 1, 0);
+                            convert(at + 1, RG == 1 ? 1 : g);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
                 if (step + 2 < KEYS / 16) fetch(step + 2);
-                __builtin_amdgcn_sched_barrier(0);
             };
             if (i > 0) {
 #pragma unroll
@@ -677,8 +701,15 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 fetch(1);
             }
             __builtin_amdgcn_sched_barrier(0);
-            copy_next();
-            if (!SMALL) lds_barrier();         // A: P has been read
+            if (SMALL) copy_next();
+            else {
+                if (more) {
+                    next = block_copy(i + 2, id_next);
+                    id_next = look(i + 3);
+                    copy_rest(next);
+                }
+                lds_barrier();                 // A: P has been read
+            }
             if (i > 0) {
                 // accumulators follow the maxima
 #pragma unroll
@@ -689,11 +720,17 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) acc[g][ct][r] *= alpha[g];
                     }
+                convert(0, 0);
+                convert(0, 1);
                 product(0);
                 product(1);
-            }
+                if (!SMALL) {
+                    product(2);
+                    product(3);
+                }
+            } else if (!SMALL) copy_next();
             if (SMALL) lds_barrier();          // A
-            if (i > 0) {
+            if (SMALL && i > 0) {
                 product(2);
                 product(3);
             }
