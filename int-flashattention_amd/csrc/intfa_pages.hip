@@ -1,8 +1,8 @@
 // The pages of a cache: copies, and the bookkeeping of who holds which.  See include/intfa.h.
 //
 // Counts, table and lengths stay on the device.  What has an order (free pages are dealt by their index, sequences served by theirs) is done by one workgroup, which
-// walks the counts 4096 at a time; it leaves the pages to copy as a list, and a second launch copies them with the whole card.  Bound by latency: the walk
-// takes about 1.2 us per 4096 counts.  The copies move 16 bytes a lane, four at a time, past the caches.
+// walks the counts 16384 at a time; it leaves the pages to copy as a list, and a second launch copies them with the whole card.  Bound by latency: the walk
+// takes about 2 us per 16384 counts.  The copies move 16 bytes a lane, four at a time, past the caches.
 #include "intfa_paged_host.h"
 
 using namespace intfa;
@@ -94,12 +94,24 @@ __device__ __forceinline__ int scan_all(int mine, int* lds, int& total) {
     }
     return before + upto - mine;
 }
-// Four counts of a thread (those behind the last page: 0 or 1 as `pad` says)
-__device__ __forceinline__ v4i four_counts(const int32_t* refs, int at, int pages, int pad) {
-    v4i r;
+// The counts that a thread has of a stretch of the pool (behind the last page: 0 or 1 as `pad` says)
+constexpr int kEach = 16, kStretch = kEach * kWalk;
+struct Counts { int32_t r[kEach]; };
+__device__ __forceinline__ Counts load_counts(const int32_t* refs, int at, int pages, int pad) {
+    typedef int32_t Four __attribute__((ext_vector_type(4), aligned(4)));
+    Counts c;
+    if (at + kEach <= pages) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = at + k < pages ? refs[at + k] : pad;
-    return r;
+        for (int k = 0; k < kEach / 4; ++k) {
+            const Four f = *(const Four*)(refs + at + 4 * k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c.r[4 * k + i] = f[i];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) c.r[k] = at + k < pages ? refs[at + k] : pad;
+    }
+    return c;
 }
 
 struct CompactArgs { int32_t* refs; int32_t* new_index; int32_t* src; int32_t* dst; int32_t* count; int32_t num_pages; };
@@ -108,27 +120,34 @@ __global__ void __launch_bounds__(kWalk) pages_compact_kernel(const CompactArgs 
     __shared__ int lds[kWalk / 64];
     const int pages = a.num_pages;
     int mine = 0, used;
-    for (int at = threadIdx.x; at < pages; at += kWalk) mine += a.refs[at] > 0;
+    const Counts first = load_counts(a.refs, kEach * (int)threadIdx.x, pages, 0);      // (kept for the walk: most pools are no longer)
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) mine += first.r[k] > 0;
+    for (int at0 = kStretch; at0 < pages; at0 += kStretch) {
+        const Counts c = load_counts(a.refs, at0 + kEach * (int)threadIdx.x, pages, 0);
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) mine += c.r[k] > 0;
+    }
     scan_all(mine, lds, used);
     // the used pages from place `used` onward, and the free places before it: as many of both
     int from = 0, to = 0;
-    for (int at0 = 0; at0 < pages; at0 += 4 * kWalk) {
-        const int at = at0 + 4 * (int)threadIdx.x;
-        const v4i r = four_counts(a.refs, at, pages, 0);
+    for (int at0 = 0; at0 < pages; at0 += kStretch) {
+        const int at = at0 + kEach * (int)threadIdx.x;
+        const Counts c = at0 == 0 ? first : load_counts(a.refs, at, pages, 0);
         int moves = 0, places = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            moves += r[k] > 0 && at + k >= used;
-            places += r[k] <= 0 && at + k < used;
+        for (int k = 0; k < kEach; ++k) {
+            moves += c.r[k] > 0 && at + k >= used;
+            places += c.r[k] <= 0 && at + k < used;
         }
-        // (at most 4096 of either: both in one word)
+        // (at most 16384 of either: both in one word)
         int both;
         const int before = scan_all(moves | places << 16, lds, both);
         int f = from + (before & 0xffff), t = to + (before >> 16);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kEach; ++k) {
             if (at + k >= pages) break;
-            const bool is_used = r[k] > 0;
+            const bool is_used = c.r[k] > 0;
             if (is_used && at + k >= used) a.src[f++] = at + k;
             else a.new_index[at + k] = is_used ? at + k : -1;
             if (!is_used && at + k < used) a.dst[t++] = at + k;
@@ -168,12 +187,15 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const TableArgs a, cons
     }
 }
 
-// A workgroup takes some columns of all pairs: it reads the parents' entries to LDS before it writes the children's.
-__global__ void __launch_bounds__(256) pages_fork_kernel(const TableArgs a, const int32_t* parents, const int32_t* children, int n, int columns) {
+// A workgroup takes some columns of all pairs: it reads the parents' entries to LDS before it writes the children's.  Of equal children the last pair counts: each child's last pair
+// stands in a table of `slots` places (a power of two, 3 / 2 of the pairs or more), found by the child's number.  (Looked for by each entry among the pairs behind its own, 224 pairs of
+// 95 columns took 47 us.)
+__global__ void __launch_bounds__(256) pages_fork_kernel(const TableArgs a, const int32_t* parents, const int32_t* children, int n, int columns, int slots) {
     extern __shared__ int32_t fork_lds[];
-    int32_t* const child = fork_lds;           // -1: left out
-    int32_t* const parent = fork_lds + n;
-    int32_t* const entry = fork_lds + 2 * n;   // [n][columns]; the last workgroup's: the lengths
+    int32_t* const child = fork_lds;           // [n]: -1: left out
+    int32_t* const entry = child + n;          // [n][columns]; the last workgroup's: the lengths
+    int32_t* const parent = entry + n * columns;      // [n], and then
+    int32_t* const last = parent;              // [slots]: a child's last pair, or -1
     const int column0 = (int)blockIdx.x * columns;
     const bool lengths = blockIdx.x == gridDim.x - 1;
     for (int i = threadIdx.x; i < n; i += 256) {
@@ -189,12 +211,40 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(const TableArgs a, cons
         entry[i] = lengths ? a.lens[parent[k]] : column < a.table_width ? a.table[parent[k] * a.bt_sb + column] : -1;
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < slots; i += 256) last[i] = -1;
+    __syncthreads();
+    // (linear probing: ends, since there are more places than children)
+    auto place = [&](int c) __attribute__((always_inline)) { return (int)((uint32_t)c * 2654435769u >> 16) & (slots - 1); };
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int c = child[i];
+        if (c < 0) continue;
+        int at = place(c);
+        while (true) {
+            const int was = atomicCAS(last + at, -1, i);
+            if (was == -1) break;
+            if (child[was] == c) {             // (a place stays its child's)
+                atomicMax(last + at, i);
+                break;
+            }
+            at = (at + 1) & (slots - 1);
+        }
+    }
+    __syncthreads();
+    uint32_t out = 0;                          // (of up to 4096 pairs a thread has sixteen)
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int c = child[i];
+        if (c < 0) continue;
+        int at = place(c);
+        while (child[last[at]] != c) at = (at + 1) & (slots - 1);
+        if (last[at] != i) out |= 1u << (i >> 8);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 256)
+        if (out >> (i >> 8) & 1) child[i] = -1;
+    __syncthreads();
     for (int i = threadIdx.x; i < n * wide; i += 256) {
         const int k = i / wide, column = column0 + i - k * wide, c = child[k];
         if (c < 0) continue;
-        bool again = false;                    // (the last of equal children counts)
-        for (int o = k + 1; o < n; ++o) again = again || child[o] == c;
-        if (again) continue;
         if (lengths) {
             a.lens[c] = entry[i];
         } else if (column < a.table_width) {
@@ -216,57 +266,76 @@ struct ReserveArgs {
 };
 
 // The columns that a sequence's fresh tokens reach: [first, end), end at most the table's width.
-__device__ __forceinline__ void reserve_span(const ReserveArgs& a, int z, int& held, int& fresh, int& first, int& end) {
-    held = a.t.lens[z];
-    held = held < 0 ? 0 : held;
-    fresh = a.fresh != nullptr ? a.fresh[z] : a.fresh_all;
-    fresh = fresh < 0 ? 0 : fresh;
-    const int64_t last = ((int64_t)held + fresh + (1ll << a.t.page_log2) - 1) >> a.t.page_log2;
-    first = held >> a.t.page_log2;
-    first = first < a.t.table_width ? first : a.t.table_width;
-    end = fresh == 0 ? first : last < a.t.table_width ? (int)last : a.t.table_width;
+struct Span { int held, fresh, first, end; };
+__device__ __forceinline__ Span reserve_span(const ReserveArgs& a, int z) {
+    Span s;
+    s.held = a.t.lens[z];
+    s.held = s.held < 0 ? 0 : s.held;
+    s.fresh = a.fresh != nullptr ? a.fresh[z] : a.fresh_all;
+    s.fresh = s.fresh < 0 ? 0 : s.fresh;
+    const int64_t last = ((int64_t)s.held + s.fresh + (1ll << a.t.page_log2) - 1) >> a.t.page_log2;
+    s.first = s.held >> a.t.page_log2;
+    s.first = s.first < a.t.table_width ? s.first : a.t.table_width;
+    s.end = s.fresh == 0 ? s.first : last < a.t.table_width ? (int)last : a.t.table_width;
+    return s;
 }
 
 // Every sequence needs so many pages: those that it lacks, and copies of those that others hold.  Its page of the first column, which holds its last tokens, is the one that
-// forked sequences share: of all that want a copy of it in this call, the last takes none if nobody else is left.
+// forked sequences share: of all that want a copy of it in this call, the last takes none if nobody else is left.  (A thread keeps what it knows of its first sequence; of
+// batches over 1024 it reads the others' again.)
 __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs a) {
-    extern __shared__ int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
-    int32_t* const plan_lds = head_lds + a.t.batch;      // [batch]: what becomes of it
-    enum { kKeep = 0, kCopy = 1, kNone = 2 };
+    extern __shared__ __align__(16) int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
+    int32_t* const plan_lds = head_lds + a.t.batch;      // [batch]: what becomes of its first column
+    enum { kLacks, kKeep, kCopy, kLeft, kNone };      // (left: kept if all that share it and come earlier get their copies, else kNone)
     __shared__ int lds[kWalk / 64];
     __shared__ int moves_lds;
     const int pages = a.t.num_pages, Z = a.t.batch;
     if (threadIdx.x == 0) moves_lds = 0;
+    const Counts stretch = load_counts(a.t.refs, kEach * (int)threadIdx.x, pages, 1);      // (asked for ahead of its use)
+    Span own = {0, 0, 0, 0};
+    int own_head = -1, own_holders = 0;
     for (int z = threadIdx.x; z < Z; z += kWalk) {
-        int held, fresh, first, end, head = -1;
-        reserve_span(a, z, held, fresh, first, end);
-        if (first < end) {
-            const int id = a.t.table[z * a.t.bt_sb + first];
-            if ((unsigned)id < (unsigned)pages && a.t.refs[id] > 1) head = id;
+        const Span s = reserve_span(a, z);
+        int head = -1, holders = 0, plan = kLacks;
+        if (s.first < s.end) {
+            const int id = a.t.table[z * a.t.bt_sb + s.first];
+            if ((unsigned)id < (unsigned)pages) {
+                holders = a.t.refs[id];
+                plan = kKeep;
+                if (holders > 1) head = id;
+            }
         }
         head_lds[z] = head;
+        plan_lds[z] = plan;
+        if (z < kWalk) {
+            own = s;
+            own_head = head;
+            own_holders = holders;
+        }
     }
     __syncthreads();
-    auto copies_head = [&](int z, int& before) __attribute__((always_inline)) {
-        const int head = head_lds[z];
-        before = 0;
-        if (head < 0) return false;
-        for (int o = 0; o < z; ++o) before += head_lds[o] == head;
-        return a.t.refs[head] - before > 1;
-    };
     // needs, in the order of the sequences: granted[z] holds the pages that were dealt before it until its own are
     int dealt = 0;
     for (int z0 = 0; z0 < Z; z0 += kWalk) {
         const int z = z0 + (int)threadIdx.x;
-        int needs = 0, before;
+        int needs = 0;
         if (z < Z) {
-            int held, fresh, first, end;
-            reserve_span(a, z, held, fresh, first, end);
-            for (int c = first; c < end; ++c) {
+            const Span s = z < kWalk ? own : reserve_span(a, z);
+            const int head = z < kWalk ? own_head : head_lds[z];
+            if (head >= 0) {
+                const int holders = z < kWalk ? own_holders : a.t.refs[head];
+                int before = 0, o = 0;
+                for (; o + 4 <= z; o += 4) {
+                    const v4i h = *(const v4i*)(head_lds + o);
+                    before += (h[0] == head) + (h[1] == head) + (h[2] == head) + (h[3] == head);
+                }
+                for (; o < z; ++o) before += head_lds[o] == head;
+                plan_lds[z] = holders - before > 1 ? kCopy : before > 0 ? kLeft : kKeep;
+            }
+            needs = s.first < s.end && (plan_lds[z] == kLacks || plan_lds[z] == kCopy);
+            for (int c = s.first + 1; c < s.end; ++c) {
                 const int id = a.t.table[z * a.t.bt_sb + c];
-                if ((unsigned)id >= (unsigned)pages) ++needs;
-                else if (c == first) needs += copies_head(z, before);
-                else needs += a.t.refs[id] > 1;
+                needs += (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
             }
         }
         int total;
@@ -276,16 +345,16 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
     }
     // as many free pages, in their order
     int found = 0;
-    for (int at0 = 0; at0 < pages && found < dealt; at0 += 4 * kWalk) {
-        const int at = at0 + 4 * (int)threadIdx.x;
-        const v4i r = four_counts(a.t.refs, at, pages, 1);
+    for (int at0 = 0; at0 < pages && found < dealt; at0 += kStretch) {
+        const int at = at0 + kEach * (int)threadIdx.x;
+        const Counts c = at0 == 0 ? stretch : load_counts(a.t.refs, at, pages, 1);
         int mine = 0, total;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mine += r[k] <= 0;
+        for (int k = 0; k < kEach; ++k) mine += c.r[k] <= 0;
         int f = found + scan_all(mine, lds, total);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (r[k] <= 0) {
+        for (int k = 0; k < kEach; ++k)
+            if (c.r[k] <= 0) {
                 if (f < dealt) a.free_list[f] = at + k;
                 ++f;
             }
@@ -295,21 +364,15 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
     __threadfence_block();
     __syncthreads();
     for (int z = threadIdx.x; z < Z; z += kWalk) {
-        int before;
-        const bool copies = copies_head(z, before);
-        plan_lds[z] = copies ? kCopy : before > 0 && a.granted[z] > found ? kNone : kKeep;      // (none: another was to leave it and could not)
-    }
-    for (int z = threadIdx.x; z < Z; z += kWalk) {
-        int held, fresh, first, end;
-        reserve_span(a, z, held, fresh, first, end);
-        int rank = a.granted[z], room = end;                 // columns before `room` can be written
-        const int plan = plan_lds[z];
-        if (plan == kNone) room = first;
-        for (int c = first; c < room; ++c) {
+        const Span s = z < kWalk ? own : reserve_span(a, z);
+        int rank = a.granted[z], room = s.end, plan = plan_lds[z];       // columns before `room` can be written
+        if (plan == kLeft && rank > found) plan = kNone;
+        if (plan == kNone) room = s.first;
+        for (int c = s.first; c < room; ++c) {
             int32_t* const at = a.t.table + z * a.t.bt_sb + c;
             const int id = *at;
             const bool named = (unsigned)id < (unsigned)pages;
-            const bool copy = named && (c == first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
+            const bool copy = named && (c == s.first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
             if (named && !copy) continue;
             if (rank >= found) {
                 room = c;
@@ -324,8 +387,8 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
             }
             *at = page;
         }
-        const int64_t places = ((int64_t)room << a.t.page_log2) - held;
-        a.granted[z] = places <= 0 ? 0 : places < fresh ? (int)places : fresh;
+        const int64_t places = ((int64_t)room << a.t.page_log2) - s.held;
+        a.granted[z] = places <= 0 ? 0 : places < s.fresh ? (int)places : s.fresh;
     }
     __threadfence_block();
     __syncthreads();
@@ -414,7 +477,10 @@ int intfa_pages_fork(const intfa_page_table* t, const int32_t* parents, const in
     // Columns of a workgroup: 1024 entries in four rounds, or one column
     const int columns = n >= 1024 ? 1 : 1024 / n < 64 ? 1024 / n : 64;
     const unsigned groups = (unsigned)((t->table_width + columns - 1) / columns);
-    hipLaunchKernelGGL(pages_fork_kernel, dim3(groups + 1), dim3(256), (size_t)(2 + columns) * n * 4, (hipStream_t)stream, table_args(t), parents, children, n, columns);
+    int slots = 64;
+    while (2 * slots < 3 * n) slots *= 2;
+    const size_t words = (size_t)(1 + columns) * n + slots;      // (slots: n or more; 64 KB at the most)
+    hipLaunchKernelGGL(pages_fork_kernel, dim3(groups + 1), dim3(256), words * 4, (hipStream_t)stream, table_args(t), parents, children, n, columns, slots);
     return (int)hipGetLastError();
 }
 

@@ -201,6 +201,41 @@ def test_captured_steps_follow_counts_and_lengths():
         assert junk.isfinite()
 
 
+@pytest.mark.parametrize("n", [2731, 4096])
+def test_the_largest_forks(n):
+    """As many pairs as a call takes, to distinct children and to few of them, over and over."""
+    g = torch.Generator().manual_seed(n)
+    Z, width, page = 5000, 3, 16
+    start = make(g, 16000, Z, width, page, 3, SHAPES[1:2])
+    b = Books(*start, page)
+    refs, table, lens, pools = device(*start)
+    for children in (torch.randperm(Z, generator=g)[:n].tolist(), pick(g, 9, n), pick(g, Z, n)):
+        parents = pick(g, Z, n)
+        ifa.paged_fork(refs, table, lens, ints(parents), ints(children))
+        b.fork(parents, children)
+        b.check(refs, table, lens, pools)
+
+
+def test_the_largest_reservation_and_pool():
+    """8192 sequences, each group of eight on one last page, and a pool longer than a stretch of the books."""
+    Z, page, pages = 8192, 16, 40000
+    shared = list(range(pages - 1, pages - 1 - Z // 8, -1))
+    refs = [0] * pages
+    for i in shared:
+        refs[i] = 8
+    for i in range(0, 30000, 3):
+        refs[i] = 1
+    start = (refs, [[shared[z % (Z // 8)], -1] for z in range(Z)], [5 + z % 9 for z in range(Z)], [torch.arange(pages, dtype=torch.int32)[:, None].repeat(1, 4)])
+    b = Books(*start, page)
+    refs, table, lens, pools = device(*start)
+    fresh = [z % 3 for z in range(Z)]
+    granted = ifa.paged_reserve(pools, refs, table, lens, ints(fresh), page)
+    assert granted.tolist() == b.reserve(fresh)
+    b.check(refs, table, lens, pools)
+    assert ifa.paged_compact(pools, refs, table).tolist() == b.compact()
+    b.check(refs, table, lens, pools)
+
+
 def test_refusals():
     start = ([1, 0], [[0]], [4], [torch.zeros(2, 3)])
     refs, table, lens, pools = device(*start)
