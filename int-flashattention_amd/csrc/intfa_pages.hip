@@ -2,7 +2,7 @@
 //
 // Counts, table and lengths stay on the device.  What has an order (free pages are dealt by their index, sequences served by theirs) is done by one workgroup, which
 // walks the counts 16384 at a time; it leaves the pages to copy as a list, and a second launch copies them with the whole card.  Bound by latency: the walk
-// takes about 2 us per 16384 counts.  The copies move 16 bytes a lane, four at a time, past the caches.
+// takes about 2 us per 16384 counts.  The copies move 16 bytes a lane, four at a time.
 #include "intfa_paged_host.h"
 
 using namespace intfa;
@@ -10,15 +10,19 @@ using namespace intfa;
 namespace {
 
 constexpr int kPoolsEach = 96;                 // pools of a launch (the argument block holds them)
-constexpr int kChunk = 16384;                  // bytes of a page that a workgroup copies at a time
+// Bytes of a page that a workgroup copies at a time: at most so many, a page's chunks alike (4000 pages of 36864 + 512 bytes: 67 us with chunks of 16384 and what is left, 62 with
+// equal ones, 57 without the hint that passes the caches).  A pool's small page goes with the chunk ahead of it, up to four in a row (57 -> 52 us, 5.8 TB/s; a workgroup of its own for 512
+// bytes costs what one for 12288 does, and 48 of them in one workgroup would be 48 trips).
+constexpr int kChunk = 16384, kSmall = 1024, kFollowing = 4;
 constexpr int kWalk = 1024;                    // threads that keep the books
 constexpr int kLeastBlocks = 4 * kComputeUnits;
 
 struct PoolArgs {
     char* data[kPoolsEach];
     int64_t stride[kPoolsEach], bytes[kPoolsEach];
-    int32_t first[kPoolsEach + 1];             // chunk at which each pool begins within a page
+    int32_t first[kPoolsEach + 1];             // chunk at which each pool begins within a page (one that follows another's last chunk: where that ends)
     int32_t width[kPoolsEach];                 // bytes of a lane's access
+    int32_t chunk[kPoolsEach];                 // bytes of a chunk
     int32_t pools, num_pages;
     FastDiv d_chunks;
 };
@@ -38,10 +42,10 @@ template <typename W> __device__ __forceinline__ void copy_chunk(const char* src
         W w[MANY];
 #pragma unroll
         for (int k = 0; k < MANY; ++k)
-            if (i0 + 256 * k < n) w[k] = __builtin_nontemporal_load((const W*)src + i0 + 256 * k);
+            if (i0 + 256 * k < n) w[k] = ((const W*)src)[i0 + 256 * k];
 #pragma unroll
         for (int k = 0; k < MANY; ++k)
-            if (i0 + 256 * k < n) __builtin_nontemporal_store(w[k], (W*)dst + i0 + 256 * k);
+            if (i0 + 256 * k < n) ((W*)dst)[i0 + 256 * k] = w[k];
     }
 }
 
@@ -54,12 +58,17 @@ __global__ void __launch_bounds__(256) pages_move_kernel(const PoolArgs a, const
         if ((unsigned)src >= (unsigned)a.num_pages || (unsigned)dst >= (unsigned)a.num_pages || src == dst) continue;
         int p = 0;
         while (chunk >= a.first[p + 1]) ++p;
-        const int64_t at = (int64_t)(chunk - a.first[p]) * kChunk, left = a.bytes[p] - at, bytes = left < kChunk ? left : kChunk;
-        const char* const from = a.data[p] + src * a.stride[p] + at;
-        char* const to = a.data[p] + dst * a.stride[p] + at;
-        if (a.width[p] == 16) copy_chunk<v4i>(from, to, bytes);
-        else if (a.width[p] == 4) copy_chunk<int32_t>(from, to, bytes);
-        else copy_chunk<int8_t>(from, to, bytes);
+        int64_t at = (int64_t)(chunk - a.first[p]) * a.chunk[p];
+        do {
+            const int64_t left = a.bytes[p] - at, bytes = left < a.chunk[p] ? left : a.chunk[p];
+            const char* const from = a.data[p] + src * a.stride[p] + at;
+            char* const to = a.data[p] + dst * a.stride[p] + at;
+            if (a.width[p] == 16) copy_chunk<v4i>(from, to, bytes);
+            else if (a.width[p] == 4) copy_chunk<int32_t>(from, to, bytes);
+            else copy_chunk<int8_t>(from, to, bytes);
+            at = 0;
+            ++p;
+        } while (p < a.pools && chunk + 1 == a.first[p] && a.first[p] == a.first[p + 1]);      // (small pools behind this chunk)
     }
     if (m.table == nullptr) return;
     const int64_t entries = (int64_t)m.batch * m.table_width;
@@ -96,9 +105,9 @@ __device__ __forceinline__ int scan_all(int mine, int* lds, int& total) {
 }
 // The counts that a thread has of a stretch of the pool (behind the last page: 0 or 1 as `pad` says)
 constexpr int kEach = 16, kStretch = kEach * kWalk;
+typedef int32_t Four __attribute__((ext_vector_type(4), aligned(4)));
 struct Counts { int32_t r[kEach]; };
 __device__ __forceinline__ Counts load_counts(const int32_t* refs, int at, int pages, int pad) {
-    typedef int32_t Four __attribute__((ext_vector_type(4), aligned(4)));
     Counts c;
     if (at + kEach <= pages) {
 #pragma unroll
@@ -149,8 +158,19 @@ __global__ void __launch_bounds__(kWalk) pages_compact_kernel(const CompactArgs 
             if (at + k >= pages) break;
             const bool is_used = c.r[k] > 0;
             if (is_used && at + k >= used) a.src[f++] = at + k;
-            else a.new_index[at + k] = is_used ? at + k : -1;
             if (!is_used && at + k < used) a.dst[t++] = at + k;
+        }
+        // (those that move get theirs below)
+        if (at + kEach <= pages) {
+#pragma unroll
+            for (int k = 0; k < kEach; k += 4) {
+                Four index;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) index[i] = c.r[k + i] > 0 ? at + k + i : -1;
+                *(Four*)(a.new_index + at + k) = index;
+            }
+        } else {
+            for (int k = 0; k < kEach && at + k < pages; ++k) a.new_index[at + k] = a.refs[at + k] > 0 ? at + k : -1;
         }
         from += both & 0xffff;
         to += both >> 16;
@@ -424,13 +444,18 @@ int launch_moves(const intfa_page_pool* pools, int num_pools, int num_pages, Mov
         a.pools = num_pools - at < kPoolsEach ? num_pools - at : kPoolsEach;
         a.num_pages = num_pages;
         int64_t chunks = 0;
+        int following = 0;
         for (int i = 0; i < a.pools; ++i) {
             const intfa_page_pool& p = pools[at + i];
             a.data[i] = (char*)p.data; a.stride[i] = p.page_stride; a.bytes[i] = p.page_bytes;
             const uint64_t all = (uint64_t)reinterpret_cast<uintptr_t>(p.data) | (uint64_t)p.page_stride | (uint64_t)p.page_bytes;
             a.width[i] = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
             a.first[i] = (int32_t)chunks;
-            chunks += (p.page_bytes + kChunk - 1) / kChunk;
+            const int64_t parts = (p.page_bytes + kChunk - 1) / kChunk;
+            a.chunk[i] = (int32_t)(((p.page_bytes + parts - 1) / parts + 15) / 16 * 16);
+            const bool follows = p.page_bytes <= kSmall && i > 0 && following < kFollowing;
+            following = follows ? following + 1 : 0;
+            chunks += follows ? 0 : parts;
             if (chunks >= 1ll << 31) return INTFA_ERR_POOL;
         }
         a.first[a.pools] = (int32_t)chunks;
