@@ -38,125 +38,155 @@ __device__ __forceinline__ bool latent_place(const LatentAppendParams& p, int to
     return real && a.i < fresh && column < p.table_width && named;
 }
 
-template <int LANES> __device__ __forceinline__ float over_lanes_max(float v) {
-#pragma unroll
-    for (int w = 1; w < LANES; w <<= 1) v = fmaxf(v, __shfl_xor(v, w));
+// f over the 8 or 16 neighbouring lanes of a token, for all of them: by the rows' own permutations (neighbours, pairs, halves of eight, mirrored)
+template <int LANES, typename T, typename F> __device__ __forceinline__ T over_lanes(T v, F f) {
+    static_assert(LANES == 8 || LANES == 16, "");
+    auto moved = [&](auto ctrl) __attribute__((always_inline)) { return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    v = f(v, moved(std::integral_constant<int, 0xb1>()));
+    v = f(v, moved(std::integral_constant<int, 0x4e>()));
+    v = f(v, moved(std::integral_constant<int, 0x141>()));
+    if (LANES == 16) v = f(v, moved(std::integral_constant<int, 0x140>()));
     return v;
 }
-template <int LANES> __device__ __forceinline__ float over_lanes_sum(float v) {
+template <int LANES> __device__ __forceinline__ float over_lanes_max(float v) { return over_lanes<LANES>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int LANES> __device__ __forceinline__ float over_lanes_sum(float v) { return over_lanes<LANES>(v, [](float a, float b) { return a + b; }); }
+
+// N values of a token's lane, all N * LANES of them, to int8: the scale, and the bytes four a word
+template <int N, int LANES> __device__ __forceinline__ float to_bytes(const float (&x)[N], uint32_t (&q)[N / 4]) {
+    float top = 0.f;
 #pragma unroll
-    for (int w = 1; w < LANES; w <<= 1) v += __shfl_xor(v, w);
-    return v;
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = over_lanes_max<LANES>(top);
+    const bool infinite = top > 3.402823466e38f;             // (of the token's lanes alike)
+    if (__any(infinite)) {
+        float finite = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) finite = fmaxf(finite, finite_magnitude(x[i]));
+        top = over_lanes_max<LANES>(finite);
+    }
+    const float scale = fmaxf(top / 127.0f, kLeastScale), reciprocal = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) q[i] = quantise4(x + 4 * i, scale, reciprocal);
+    if (infinite) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) q[i] = quantise(x[4 * i], scale) | quantise(x[4 * i + 1], scale) << 8 | quantise(x[4 * i + 2], scale) << 16 | quantise(x[4 * i + 3], scale) << 24;
+    }
+    return scale;
 }
 
-// A wave takes T tokens, nothing of it waits for another wave: DC / 8 lanes a token for the latent part, eight elements each, and DR / 2 for the rotary one, a pair each, since
-// an angle costs as much as all of a lane's other work (eight angles a lane: four prompts of 4096 tokens 20 us of angles alone).
+// A wave takes 64 / L tokens, nothing of it waits for another wave: L lanes a token, with units of sixteen elements of the latent part and some pairs of the rotary one.  Bound by its
+// arithmetic: with more lanes a token (64, and 32 for the rotary part) what a token costs once - its place, the norm's root, the divisions, the sums over its lanes - was more than what
+// its elements cost (16384 tokens of 512 + 64 16.2 us).
 template <int DT, int DC, int DR> __global__ void __launch_bounds__(256) latent_append_kernel(const LatentAppendParams p) {
-    constexpr int LL = DC / 8, RL = DR / 2, LT = 64 / LL, RT = 64 / RL, T = LT > RT ? LT : RT, LP = T / LT, RP = T / RT;
-    const int lane = threadIdx.x & 63, first = ((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6)) * T;
+    constexpr int L = DC == 512 ? 16 : 8, T = 64 / L, E = DC / L, U = E / 16, P = DR / 2 / L;
+    const int lane = threadIdx.x & 63, l = lane % L, first = ((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6)) * T;
     if (first >= p.tokens) return;
     // everything is requested before the first is used
-    LatentPlace at[LP], rat[RP];
-    bool put[LP], rput[RP];
-    v4i raw[LP];
-    uint16_t pair[RP][2];
-    const int col = lane % LL * 8, j = lane % RL;
-    const bool turns = p.rope.freqs != nullptr && j < p.rope.pairs;
-    const int one = turns && !p.rope.interleaved ? j : 2 * j, two = turns && !p.rope.interleaved ? p.rope.pairs + j : 2 * j + 1;
+    LatentPlace at;
+    const bool put = latent_place(p, first + lane / L, at);
+    const char* const c = p.c + at.z * p.c_sb + at.i * p.c_sn;
+    const char* const k = p.k + at.z * p.k_sb + at.i * p.k_sn;
+    v4i raw[2 * U], raw_weight[2 * U];
 #pragma unroll
-    for (int k = 0; k < LP; ++k) {
-        put[k] = latent_place(p, first + k * LT + lane / LL, at[k]);
-        raw[k] = __builtin_nontemporal_load((const v4i*)(p.c + at[k].z * p.c_sb + at[k].i * p.c_sn + 2 * col));
+    for (int u = 0; u < 2 * U; ++u) raw[u] = *(const v4i*)(c + 2 * (16 * (l + L * (u / 2)) + 8 * (u & 1)));
+    uint16_t pair[P][2];
+    double freq[P];
+    int one[P], two[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int j = l + L * i;
+        const bool turns = p.rope.freqs != nullptr && j < p.rope.pairs;
+        one[i] = turns && !p.rope.interleaved ? j : 2 * j;
+        two[i] = turns && !p.rope.interleaved ? p.rope.pairs + j : 2 * j + 1;
+        pair[i][0] = *(const uint16_t*)(k + 2 * one[i]);
+        pair[i][1] = *(const uint16_t*)(k + 2 * two[i]);
+        freq[i] = turns ? p.rope.freqs[j] : 0.0;
     }
+    if (p.weight != nullptr) {
 #pragma unroll
-    for (int k = 0; k < RP; ++k) {
-        rput[k] = latent_place(p, first + k * RT + lane / RL, rat[k]);
-        const char* const src = p.k + rat[k].z * p.k_sb + rat[k].i * p.k_sn;
-        pair[k][0] = *(const uint16_t*)(src + 2 * one);
-        pair[k][1] = *(const uint16_t*)(src + 2 * two);
+        for (int u = 0; u < 2 * U; ++u) raw_weight[u] = *(const v4i*)(p.weight + 2 * (16 * (l + L * (u / 2)) + 8 * (u & 1)));
     }
-    const double freq = turns ? p.rope.freqs[j] : 0.0;
-    float weight[8];
-    if (p.weight != nullptr) unpack8<DT>(*(const v4i*)(p.weight + 2 * col), weight);
+    // ---- the rotary part
+    {
+        float y[2 * P < 4 ? 4 : 2 * P];
 #pragma unroll
-    for (int k = 0; k < LP; ++k) {
-        float x[8];
-        unpack8<DT>(raw[k], x);
-        if (p.weight != nullptr) {
-            // The squares are those of x / 2^e, 2^e the size of the row's largest element: they stay in range whatever the row's size.  (e from -40, under which
-            // eps is all there is; 126 for a row with an infinity, which thereby becomes one of zeros, as its formula has it)
-            uint32_t top = 0;
+        for (int i = 2 * P; i < 4; ++i) y[i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t a = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
-                top = top > a ? top : a;
+        for (int i = 0; i < P; ++i) {
+            auto wide = [](uint16_t w) __attribute__((always_inline)) {
+                return DT == 0 ? (float)__builtin_bit_cast(_Float16, w) : __builtin_bit_cast(float, (uint32_t)w << 16);
+            };
+            float a = wide(pair[i][0]), b = wide(pair[i][1]);
+            if (p.rope.freqs != nullptr) {
+                float cosine, sine;
+                rope_angle(freq[i], (double)at.position, p.rope.magnitude, cosine, sine);
+                float ta = a, tb = b;
+                rope_turn(ta, tb, cosine, sine);
+                const bool turns = l + L * i < p.rope.pairs;
+                a = turns ? ta : a;
+                b = turns ? tb : b;
             }
-#pragma unroll
-            for (int w = 1; w < LL; w <<= 1) {
-                const uint32_t a = (uint32_t)__shfl_xor((int)top, w);
-                top = top > a ? top : a;
-            }
-            int e = (int)(top >> 23) - 127;
-            e = e < -40 ? -40 : e > 126 ? 126 : e;
-            const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] *= down;
-                sum = fmaf(x[i], x[i], sum);
-            }
-            sum = over_lanes_sum<LL>(sum);
-            const float r = 1.0f / sqrtf(sum * (1.0f / DC) + p.eps * down * down);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * r * weight[i];
+            y[2 * i] = a;
+            y[2 * i + 1] = b;
         }
-        float top = 0.f;
+        uint32_t q[sizeof(y) / 16];
+        const float scale = to_bytes<sizeof(y) / 4, L>(y, q);
+        if (put) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-        top = over_lanes_max<LL>(top);
-        const bool infinite = top > 3.402823466e38f;         // (of the token's lanes alike)
-        if (__any(infinite)) {
-            float finite = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) finite = fmaxf(finite, finite_magnitude(x[i]));
-            finite = over_lanes_max<LL>(finite);
-            top = finite;
-        }
-        const float scale = fmaxf(top / 127.0f, kLeastScale), reciprocal = 1.0f / scale;
-        if (put[k]) {
-            uint32_t q[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float* const y = x + 4 * h;
-                q[h] = !infinite ? quantise4(y, scale, reciprocal)
-                                 : quantise(y[0], scale) | quantise(y[1], scale) << 8 | quantise(y[2], scale) << 16 | quantise(y[3], scale) << 24;
+            for (int i = 0; i < P; ++i) {
+                at.row[DC + one[i]] = (char)(q[i / 2] >> (16 * (i & 1)));
+                at.row[DC + two[i]] = (char)(q[i / 2] >> (16 * (i & 1) + 8));
             }
-            *(v2i*)(at[k].row + col) = (v2i){(int)q[0], (int)q[1]};
-            if (col == 0) at[k].scale[0] = scale;
+            if (l == 0) at.scale[1] = scale;
         }
     }
+    // ---- the latent part
+    float x[E];
 #pragma unroll
-    for (int k = 0; k < RP; ++k) {
-        auto wide = [](uint16_t w) __attribute__((always_inline)) {
-            return DT == 0 ? (float)__builtin_bit_cast(_Float16, w) : __builtin_bit_cast(float, (uint32_t)w << 16);
-        };
-        float a = wide(pair[k][0]), b = wide(pair[k][1]);
-        if (turns) {
-            float c, s;
-            rope_angle(freq, (double)rat[k].position, p.rope.magnitude, c, s);
-            rope_turn(a, b, c, s);
+    for (int u = 0; u < 2 * U; ++u) unpack8<DT>(raw[u], x + 8 * u);
+    if (p.weight != nullptr) {
+        // The squares are those of x / 2^e, 2^e the size of the row's largest element: they stay in range whatever the row's size.  (e from -40, under which
+        // eps is all there is; 126 for a row with an infinity, which thereby becomes one of zeros, as its formula has it)
+        typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+        v2us most = {0, 0};                    // (magnitudes of 16-bit numbers are ordered as their bits are)
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, raw[u][w] & 0x7fff7fff));
+        float two_tops[8];
+        unpack8<DT>((v4i){__builtin_bit_cast(int, most), 0, 0, 0}, two_tops);
+        uint32_t top = __builtin_bit_cast(uint32_t, two_tops[0]), other = __builtin_bit_cast(uint32_t, two_tops[1]);
+        top = over_lanes<L>(top > other ? top : other, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        int e = (int)(top >> 23) - 127;
+        e = e < -40 ? -40 : e > 126 ? 126 : e;
+        const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] *= down;
+            sum = fmaf(x[i], x[i], sum);
         }
-        const float top = over_lanes_max<RL>(fmaxf(finite_magnitude(a), finite_magnitude(b))), scale = fmaxf(top / 127.0f, kLeastScale);
-        if (rput[k]) {
-            rat[k].row[DC + one] = (char)quantise(a, scale);
-            rat[k].row[DC + two] = (char)quantise(b, scale);
-            if (j == 0) rat[k].scale[1] = scale;
+        sum = over_lanes_sum<L>(sum);
+        const float r = 1.0f / sqrtf(sum * (1.0f / DC) + p.eps * down * down);
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+            float weight[8];
+            unpack8<DT>(raw_weight[u], weight);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[8 * u + i] = x[8 * u + i] * r * weight[i];
         }
+    }
+    uint32_t q[E / 4];
+    const float scale = to_bytes<E, L>(x, q);
+    if (put) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) *(v4i*)(at.row + 16 * (l + L * u)) = (v4i){(int)q[4 * u], (int)q[4 * u + 1], (int)q[4 * u + 2], (int)q[4 * u + 3]};
+        if (l == 0) at.scale[0] = scale;
     }
 }
 
 template <int DT> void launch(const LatentAppendParams& p, int dc, int dr, hipStream_t stream) {
-    const int each = dc == 128 || dr == 32 ? 4 : 2;          // tokens of a wave (T above)
+    const int each = dc == 512 ? 4 : 8;        // tokens of a wave (T above)
     const dim3 grid((unsigned)((p.tokens + 4 * each - 1) / (4 * each)));
 #define INTFA_CALL(DC) do { \
         if (dr == 64) hipLaunchKernelGGL((latent_append_kernel<DT, DC, 64>), grid, dim3(256), 0, stream, p); \
