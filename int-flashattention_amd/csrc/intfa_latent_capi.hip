@@ -102,8 +102,10 @@ int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream) {
     if (p->seqlen > 1 << 30 || p->seqlen_k > 1 << 30) return INTFA_ERR_SHAPE;
     ExpandedParams ep{};
     ep.tiles = (p->seqlen + 127) / 128;
-    ep.pairs = (ep.tiles + 1) / 2;
-    const int64_t units = size_product(p->batch, p->heads), groups = size_product(units, ep.pairs);
+    const int64_t units = size_product(p->batch, p->heads);
+    ep.split = size_product(units, ep.tiles) <= kComputeUnits;
+    ep.pairs = ep.split ? ep.tiles : (ep.tiles + 1) / 2;
+    const int64_t groups = size_product(units, ep.pairs);
     if (groups * 512 >= 1ll << 32 || groups >= 1ll << 31) return INTFA_ERR_SHAPE;
     ep.qn = (const char*)p->q_nope; ep.qr = (const char*)p->q_rope; ep.kn = (const char*)p->k_nope; ep.kr = (const char*)p->k_rope; ep.v = (const char*)p->v;
     ep.out = (char*)p->out; ep.lse = p->lse; ep.seqlens_q = p->seqlens_q; ep.seqlens_k = p->seqlens_k;

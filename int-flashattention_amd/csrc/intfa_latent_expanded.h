@@ -3,6 +3,9 @@
 // A workgroup of eight waves takes two tiles of 128 query rows of a head, four waves each, 32 rows a wave; both walk the same blocks of 64 keys, which asynchronous copies bring into two
 // stages of LDS.  With a causal mask the tiles are the n-th from the end and the n-th from the start, so that all workgroups have the same work.
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 in the inputs' type, a row in one lane and its pair (l ^ 32), so that P goes from accumulator to operand in its lane.
+// Where the tiles are no more than the compute units, a workgroup has one, and each half of it half of each block's keys; the halves' rows are joined in the end (SPLIT: 10 heads of
+// 64 + 32, 3 x 777 rows over up to 1555 keys 32 -> 25 us, 16 heads of 128 + 64 over 2048 unmasked tokens 65 -> 47; with twice the tiles, 4096 causal tokens, it would be 106 for 97).
+// A third stage of LDS, requested two steps ahead, changed nothing (47 -> 48 us).
 // The blocks run as a software pipeline: each product of block n + 1's scores and of block n - 1's values is followed by its share of block n's softmax.
 #pragma once
 #include "intfa_latent_expanded_host.h"
@@ -34,11 +37,11 @@ template <int DN, int DR, int DV> struct ExpandedShape {
     static constexpr int KN = DN / 16, KS = (DN + DR) / 16, DT = DV / 32;
 };
 
-template <int DN, int DR, int DV, int DT_, bool CAUSAL>
+template <int DN, int DR, int DV, int DT_, bool CAUSAL, bool SPLIT>
 __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef ExpandedShape<DN, DR, DV> S;
-    constexpr int KEYS = S::KEYS, KN = S::KN, KS = S::KS, DT = S::DT, NST = 2;
+    constexpr int KEYS = S::KEYS, KN = S::KN, KS = S::KS, DT = S::DT, NST = SPLIT ? 1 : 2, OWN = 32 * NST, PER = 16 * NST;      // keys of a block that a half has, and a lane's of them
     // P = 2^(x - frame) times this: fp16 keeps its 11 bits down to 2^-21 of the frame's; bf16 has the range, and leaves room for sums of 2^12 of its largest values
     constexpr float kShift = DT_ == 0 ? 7.f : -20.f;
     __shared__ __align__(1024) char lds[S::LDS];
@@ -55,8 +58,10 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         pair = (int)blockIdx.x - unit * p.pairs;
     }
     const int z = fast_div(unit, p.d_heads), head = unit - z * p.heads;
-    const int tile = CAUSAL ? (half == 0 ? p.tiles - 1 - pair : pair) : 2 * pair + half;
-    const bool mine = CAUSAL ? half == 0 || pair != p.tiles - 1 - pair : tile < p.tiles;
+    // (split: the last tiles, which see the most keys, first)
+    const int tile = SPLIT ? p.tiles - 1 - pair : CAUSAL ? (half == 0 ? p.tiles - 1 - pair : pair) : 2 * pair + half;
+    const bool mine = SPLIT || (CAUSAL ? half == 0 || pair != p.tiles - 1 - pair : tile < p.tiles);
+    const int key0 = SPLIT ? 32 * half : 0;    // of the half's keys in a block
     auto length = [&](const int32_t* lens, int most) __attribute__((always_inline)) {
         if (lens == nullptr) return most;
         const int n = lens[z];
@@ -69,7 +74,8 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         return seen <= 0 ? 0 : ((seen < n_keys ? seen : n_keys) + KEYS - 1) / KEYS;
     };
     const int blocks = mine ? blocks_of(tile) : 0;
-    const int first = blocks_of(CAUSAL ? p.tiles - 1 - pair : 2 * pair), second = blocks_of(CAUSAL ? pair : 2 * pair + 1), all_blocks = first > second ? first : second;
+    const int first = blocks_of(SPLIT ? tile : CAUSAL ? p.tiles - 1 - pair : 2 * pair), second = blocks_of(SPLIT ? tile : CAUSAL ? pair : 2 * pair + 1);
+    const int all_blocks = first > second ? first : second;
     const int row = tile * S::ROWS + 32 * wave + lq, row_ld = row < p.seqlen ? row : p.seqlen - 1;
     // ---- copies: a wave's share of a block
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -112,8 +118,8 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     }
     const float scale = fmaxf(fabsf(p.qk_scale_log2), 0x1p-126f);      // (never zero: hidden keys are -infinity times it)
     // ---- a lane's places in the tiles
-    const uint32_t n_lane = S::OFF_N + S::N::at(lq) + 16 * lh, r_lane = S::OFF_R + S::R::at(lq) + 16 * lh;
-    const uint32_t v_lane = S::OFF_V + S::V::at(4 * lh + ((lane & 15) >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    const uint32_t n_lane = S::OFF_N + S::N::at(key0) + S::N::at(lq) + 16 * lh, r_lane = S::OFF_R + S::R::at(key0) + S::R::at(lq) + 16 * lh;
+    const uint32_t v_lane = S::OFF_V + S::V::at(key0) + S::V::at(4 * lh + ((lane & 15) >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     auto product = [&](v4i a, v4i b, v16f c) __attribute__((always_inline)) -> v16f {
         if (DT_ == 0) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         return (v4i){lo[0], lo[1], hi[0], hi[1]};
     };
     // ---- state, by the parity of the block
-    constexpr int NQ = NST * KS, NP = 4 * DT, AHEAD = 4;      // products of scores and of values in a block; operands are requested AHEAD products ahead
+    constexpr int NQ = NST * KS, NP = 2 * NST * DT, AHEAD = 4;      // products of scores and of values in a block; operands are requested AHEAD products ahead
     v16f s[2][NST], acc[DT];
     v4i pf[2][NST][2];
     float m = -INFINITY, l = 0.f, mx = -INFINITY;
@@ -144,21 +150,21 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         constexpr bool QK = decltype(qk_tag)::value, E = decltype(e_tag)::value, PV = decltype(pv_tag)::value;
         constexpr int NQS = QK ? NQ : 0, NM = NQS + (PV ? NP : 0);
         v4i fr[AHEAD];
-        float x[32], e[32], sum = 0.f;
+        float x[PER], e[PER], sum = 0.f;
         auto fetch = [&](int i) __attribute__((always_inline)) {
             if (i < NQS) fr[i % AHEAD] = key_fragment(i);
             else if (i < NM) fr[i % AHEAD] = value_fragment(i - NQS);
         };
         // element j of P: its argument two elements ahead, the exponential one ahead, then sum and conversion, so that none waits for the one before it
         auto argument = [&](int j) __attribute__((always_inline)) {
-            if (j < 32) {
+            if (j < PER) {
                 x[j] = fmaf(s[PAR][j / 16][j % 16], factor, -frame);
                 asm volatile("" : "+v"(x[j]));
             }
         };
         auto element = [&](int j) __attribute__((always_inline)) {
             argument(j + 2);
-            if (j + 1 < 32) {
+            if (j + 1 < PER) {
                 e[j + 1] = fast_exp2(x[j + 1]);
                 asm volatile("" : "+v"(e[j + 1]));
             }
@@ -196,23 +202,23 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
             fetch(i + AHEAD);
             if (E) {
 #pragma unroll
-                for (int j = i * 32 / (NM + !NM); j < (i + 1) * 32 / (NM + !NM); ++j) element(j);
+                for (int j = i * PER / (NM + !NM); j < (i + 1) * PER / (NM + !NM); ++j) element(j);
             }
             if (QK && PV && i >= C0) {
 #pragma unroll
-                for (int j = (i - C0) * 16 / (NM - C0); j < (i + 1 - C0) * 16 / (NM - C0); ++j) maximum(j);
+                for (int j = (i - C0) * (PER / 2) / (NM - C0); j < (i + 1 - C0) * (PER / 2) / (NM - C0); ++j) maximum(j);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if (E && NM == 0) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) element(j);
+            for (int j = 0; j < PER; ++j) element(j);
         }
         if (QK && !PV) {
 #pragma unroll
             for (int st = 0; st < NST; ++st) wait_for_product(s[PAR ^ 1][st]);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) maximum(j);
+            for (int j = 0; j < PER / 2; ++j) maximum(j);
         }
         return sum;
     };
@@ -221,11 +227,11 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     // Step n of the half's blocks.  The copies that it needs have been waited for; those of the next are requested.
     auto block = [&](auto par_tag, auto qk_tag, auto pv_tag, int n) __attribute__((always_inline)) {
         constexpr int PAR = decltype(par_tag)::value ? 1 : 0;
-        const int lim = lowest - n * KEYS;
-        const bool masked = lim < KEYS - 1 || (n + 1) * KEYS > n_keys;
+        const int at = n * KEYS + key0, lim = lowest - at;
+        const bool masked = lim < OWN - 1 || at + OWN > n_keys;
         if (masked) {
             int last = CAUSAL ? lim + lq : lim;
-            const int end = n_keys - 1 - n * KEYS;
+            const int end = n_keys - 1 - at;
             last = (last < end ? last : end) - 4 * lh;
             mx = -INFINITY;
 #pragma unroll
@@ -320,6 +326,35 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) wait_for_product(acc[dt]);
+    if (SPLIT) {                               // the second half's rows to the first
+        char* const acc_lds = lds + (wave * DT * 4 * 64 + lane) * 16;
+        v2f* const stats = (v2f*)(lds + 4 * DT * 4096) + wave * 64 + lane;
+        static_assert(4 * DT * 4096 + 2048 <= S::LDS, "");
+        if (half == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *(v4f*)(acc_lds + (dt * 4 + k) * 1024) = (v4f){acc[dt][4 * k], acc[dt][4 * k + 1], acc[dt][4 * k + 2], acc[dt][4 * k + 3]};
+            *stats = (v2f){m, l};
+        }
+        __syncthreads();
+        if (half == 0) {
+            const v2f other = *stats;
+            const float top = fmaxf(m, other[0]), base = top == -INFINITY ? 0.f : top, a = fast_exp2(m - base), b = fast_exp2(other[0] - base);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const v4f o = *(const v4f*)(acc_lds + (dt * 4 + k) * 1024);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[dt][4 * k + i] = acc[dt][4 * k + i] * a + o[i] * b;
+                }
+            l = l * a + other[1] * b;
+            m = top;
+        }
+        __syncthreads();
+        if (half == 1) return;
+    }
     if (!mine) return;
     const bool padding = row >= m_rows, empty = padding || m == -INFINITY;
     const float inv = empty ? 0.f : 1.f / l;
@@ -345,8 +380,11 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
 
 template <int DN, int DR, int DV, int DT_> int launch_expanded(const ExpandedParams& p, bool causal, hipStream_t stream) {
     const dim3 grid((unsigned)(p.batch * p.heads * p.pairs));
-    if (causal) hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, true>), grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, false>), grid, dim3(512), 0, stream, p);
+    if (p.split) {
+        if (causal) hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, true, true>), grid, dim3(512), 0, stream, p);
+        else hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, false, true>), grid, dim3(512), 0, stream, p);
+    } else if (causal) hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, true, false>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((latent_expanded_kernel<DN, DR, DV, DT_, false, false>), grid, dim3(512), 0, stream, p);
     return (int)hipGetLastError();
 }
 

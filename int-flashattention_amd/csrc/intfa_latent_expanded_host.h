@@ -9,7 +9,8 @@ struct ExpandedParams {
     const int32_t* seqlens_q; const int32_t* seqlens_k;
     int64_t qn_sb, qn_sh, qn_sn, qr_sb, qr_sh, qr_sn, kn_sb, kn_sh, kr_sb, v_sb, v_sh, o_sb, o_sh, o_sn;      // bytes
     uint32_t kn_sn, kr_sn, v_sn;                     // bytes
-    int32_t batch, heads, seqlen, seqlen_k, tiles, pairs, whole;      // tiles of a head, pairs of them; workgroups of the (sequence, head)s that are dealt whole to the XCDs
+    int32_t batch, heads, seqlen, seqlen_k, tiles, pairs, whole;      // tiles of a head, pairs of them (split: the tiles again); workgroups of the (sequence, head)s that are dealt whole to the XCDs
+    bool split;                                      // a workgroup has one tile, each half of it half of the keys
     float qk_scale_log2;
     FastDiv d_pairs, d_heads;
 };

@@ -25,15 +25,20 @@ def inputs(g, Z, H, N, Nk, dims, dtype, size=1.2):
     return r(Z, H, N, dn), r(Z, H, N, dr), r(Z, H, Nk, dn), r(Z, 1, Nk, dr), torch.randn((Z, H, Nk, dv), generator=g).to(dtype)
 
 
-def run(x, causal, sm, nq=None, nk=None):
+def run(x, causal, sm, nq=None, nk=None, copies=1):
+    """copies: of the heads, side by side; all give the same."""
     i32 = dict(dtype=torch.int32, device="cuda")
-    out, lse = ifa.attention_latent(*(t.cuda() for t in x), causal, sm, seqlens_q=None if nq is None else torch.tensor(nq, **i32),
+    heads = x[0].shape[1]
+    x = [t.cuda() if t.shape[1] == 1 and heads > 1 else t.cuda().repeat(1, copies, 1, 1) for t in x]
+    out, lse = ifa.attention_latent(*x, causal, sm, seqlens_q=None if nq is None else torch.tensor(nq, **i32),
                                     seqlens_k=None if nk is None else torch.tensor(nk, **i32), return_lse=True)
-    return out.cpu(), lse.cpu()
+    for i in range(heads, heads * copies, heads):
+        assert torch.equal(out[:, i:i + heads].nan_to_num(7.0), out[:, :heads].nan_to_num(7.0)) and torch.equal(lse[:, i:i + heads].nan_to_num(7.0), lse[:, :heads].nan_to_num(7.0))
+    return out[:, :heads].cpu(), lse[:, :heads].cpu()
 
 
-def check(x, causal, sm=0.07, nq=None, nk=None):
-    out, lse = run(x, causal, sm, nq, nk)
+def check(x, causal, sm=0.07, nq=None, nk=None, copies=1):
+    out, lse = run(x, causal, sm, nq, nk, copies)
     want, want_lse, mean_v, size = expanded(*x, causal, sm, nq, nk)
     assert out.dtype == x[4].dtype and out.shape == want.shape
     # (inputs past their type's range are infinities, and where the formula has no number the kernel has none)
@@ -56,6 +61,26 @@ def test_lengths(dtype, dims, causal, N, Nk):
     """One query and many, one tile and pairs of them, an odd number of tiles, fewer keys than queries (rows that see none)."""
     g = torch.Generator().manual_seed(N + Nk)
     check(inputs(g, 2, 3, N, Nk, dims, dtype), causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("N,Nk", [(1, 1), (5, 5), (64, 64), (65, 200), (128, 127), (200, 130), (257, 257), (300, 700), (1, 1000), (900, 40)])
+def test_lengths_of_many_heads(dtype, dims, causal, N, Nk):
+    """More tiles than compute units: a workgroup has pairs of them, each half one with all keys."""
+    g = torch.Generator().manual_seed(N + Nk + 1)
+    check(inputs(g, 2, 3, N, Nk, dims, dtype), causal, copies=43)
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths_that_differ_of_many_heads(dims, causal):
+    g = torch.Generator().manual_seed(4)
+    nq, nk = [300, 0, 1, 129, 7, -3, 999], [300, 300, 10, 64, 0, 50, 255]
+    check(inputs(g, 7, 2, 300, 310, dims, torch.bfloat16), causal, nq=nq, nk=nk, copies=13)
+    check(inputs(g, 7, 2, 300, 310, dims, torch.float16), causal, nk=nk, copies=13)
+    check(inputs(g, 7, 2, 300, 310, dims, torch.float16), causal, nq=nq, copies=13)
 
 
 @pytest.mark.parametrize("dims", DIMS)
@@ -104,14 +129,16 @@ def test_strides():
 
 @pytest.mark.parametrize("sm", [-0.07, 0.0, 3.0])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_scales_of_scores(sm, dtype):
+@pytest.mark.parametrize("copies", [1, 65])
+def test_scales_of_scores(sm, dtype, copies):
     g = torch.Generator().manual_seed(9)
-    check(inputs(g, 1, 2, 140, 200, DIMS[0], dtype, 1.2 if abs(sm) < 1 else 0.2), True, sm)
-    check(inputs(g, 1, 2, 140, 200, DIMS[1], dtype, 1.2 if abs(sm) < 1 else 0.2), False, sm)
+    check(inputs(g, 1, 2, 140, 200, DIMS[0], dtype, 1.2 if abs(sm) < 1 else 0.2), True, sm, copies=copies)
+    check(inputs(g, 1, 2, 140, 200, DIMS[1], dtype, 1.2 if abs(sm) < 1 else 0.2), False, sm, copies=copies)
 
 
 @pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 14])
-def test_large_scores(size):
+@pytest.mark.parametrize("copies", [1, 65])
+def test_large_scores(size, copies):
     """Scores far past what an exponent's rounding leaves: the largest key has the row, to the bit of a tie."""
     g = torch.Generator().manual_seed(11)
     for dtype in (torch.float16, torch.bfloat16):
@@ -120,25 +147,27 @@ def test_large_scores(size):
         qr, kr = (qr * 0).to(dtype), (kr * 0).to(dtype)
         qn[..., 0] = size
         kn[..., 0] = (size * (1 + torch.arange(200) % 7)).to(dtype)            # exact products: seven sizes of score, ties among them
-        check((qn, qr, kn, kr, v), False, 1.0)
-        check((qn, qr, kn, kr, v), True, 1.0)
+        check((qn, qr, kn, kr, v), False, 1.0, copies=copies)
+        check((qn, qr, kn, kr, v), True, 1.0, copies=copies)
 
 
 @pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 2.0 ** 120), (torch.float16, 3e4), (torch.bfloat16, 2.0 ** -100)])
-def test_values_of_any_size(dtype, size):
+@pytest.mark.parametrize("copies", [1, 65])
+def test_values_of_any_size(dtype, size, copies):
     g = torch.Generator().manual_seed(13)
     x = list(inputs(g, 1, 2, 200, 1500, DIMS[0], dtype))
     x[4] = (torch.rand(x[4].shape, generator=g) * size).to(dtype)
-    check(tuple(x), False)
+    check(tuple(x), False, copies=copies)
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_queries_that_hold_no_number(bad):
+@pytest.mark.parametrize("copies", [1, 65])
+def test_queries_that_hold_no_number(bad, copies):
     g = torch.Generator().manual_seed(15)
     x = inputs(g, 1, 2, 200, 200, DIMS[0], torch.float16)
-    want, want_lse = run(x, True, 0.07)
+    want, want_lse = run(x, True, 0.07, copies=copies)
     x[0][0, 1, 50, 3] = bad
-    out, lse = run(x, True, 0.07)
+    out, lse = run(x, True, 0.07, copies=copies)
     assert out[0, 1, 50].isnan().all() and lse[0, 1, 50].isnan()
     keep = torch.ones((1, 2, 200), dtype=torch.bool)
     keep[0, 1, 50] = False
