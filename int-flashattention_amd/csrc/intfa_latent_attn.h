@@ -800,14 +800,16 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
     constexpr int SLICES = ROWS / 32 * (DC / 32), MANY = 8, WAVES = 8;
     constexpr int SETS = (SLICES + WAVES - 1) / WAVES;         // of slices, an eight of waves each
     __shared__ __align__(16) float joined[WAVES - 1][64][18];
-    __shared__ int items[512 + 1], first[512 + 1], count;      // the open items; their first unit of work
+    __shared__ v4i items[kComputeUnits];       // the open items
+    __shared__ int first[kComputeUnits + 1], count;      // their first unit of work
     LatentArgs p = latent_args();
     const auto& d = p->deal;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (wave == 0) {
         int found = 0, units = 0;
         for (int i0 = 0; i0 < d.grid; i0 += 64) {
-            const int pieces = i0 + lane < d.grid ? p->open_items[i0 + lane][0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
+            const v4i item = p->open_items[i0 + lane < d.grid ? i0 + lane : 0];
+            const int pieces = i0 + lane < d.grid ? item[0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
             int upto = mine;
 #pragma unroll
             for (int w = 1; w < 64; w <<= 1) {
@@ -817,7 +819,7 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
             const uint64_t open = __ballot(pieces != 0);
             const int at = found + __popcll(open & ((1ull << lane) - 1));
             if (pieces != 0) {
-                items[at] = i0 + lane;
+                items[at] = item;
                 first[at] = units + upto - mine;
             }
             found += __popcll(open);
@@ -836,15 +838,15 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
             const int mid = (lo + hi) / 2;
             if (first[mid] <= unit) lo = mid; else hi = mid;
         }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        const v4i open = ((const __attribute__((address_space(4))) v4i*)p->open_items)[__builtin_amdgcn_readfirstlane(items[lo])];
-        const int pieces = open[0], z = open[1], part = unit - __builtin_amdgcn_readfirstlane(first[lo]);
+        const v4i item = items[lo];
+        const int pieces = __builtin_amdgcn_readfirstlane(item[0]), z = __builtin_amdgcn_readfirstlane(item[1]), tile = __builtin_amdgcn_readfirstlane(item[2]);
+        const int part = unit - __builtin_amdgcn_readfirstlane(first[lo]);
         const bool share = pieces > MANY;      // the waves share a slice's pieces
         const int slice = share ? part : part * WAVES + wave, g = slice / (DC / 32), ct = slice % (DC / 32);
-        const int r = 32 * g + (lane & 31), row = open[2] * ROWS + r;
+        const int r = 32 * g + (lane & 31), row = tile * ROWS + r;
         const bool valid = row < d.rows && slice < SLICES;
         const int token = paged_div(valid ? row : 0, d.d_group), head = (valid ? row : 0) - token * d.group;
-        const int64_t slot0 = open[3];
+        const int64_t slot0 = __builtin_amdgcn_readfirstlane(item[3]);
         float acc[16], top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = 0.f;
