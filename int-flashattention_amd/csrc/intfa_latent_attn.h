@@ -799,7 +799,8 @@ template <int DC, int DT, int ROWS>
 __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
     constexpr int SLICES = ROWS / 32 * (DC / 32), MANY = 8, WAVES = 8;
     constexpr int SETS = (SLICES + WAVES - 1) / WAVES;         // of slices, an eight of waves each
-    __shared__ __align__(16) float joined[WAVES - 1][64][18];
+    __shared__ v4f joined[WAVES][4][64];
+    __shared__ v2f joined_stats[WAVES][64];
     __shared__ v4i items[kComputeUnits];       // the open items
     __shared__ int first[kComputeUnits + 1], count;      // their first unit of work
     LatentArgs p = latent_args();
@@ -884,28 +885,38 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
                 }
             }
         if (share) {
-            if (wave > 0) {
-                float* const to = joined[wave - 1][lane];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) to[i] = acc[i];
-                to[16] = top;
-                to[17] = sum;
-            }
+            for (int k = 0; k < 4; ++k) joined[wave][k][lane] = (v4f){acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]};
+            joined_stats[wave][lane] = (v2f){top, sum};
             __syncthreads();
-            if (wave == 0) {
-#pragma unroll 1
-                for (int w = 0; w < WAVES - 1; ++w) {
-                    const float* const from = joined[w][lane];
-                    const float grown = fmaxf(top, from[16]), frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame), b = fast_exp2(from[16] - frame);
+            if (wave < 4) {                    // a wave has eight of the columns now: as if they were its first
+                v4f x[WAVES];
+                v2f st[WAVES];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[i] = fmaf(b, from[i], a * acc[i]);
-                    sum = fmaf(b, from[17], a * sum);
-                    top = grown;
+                for (int w = 0; w < WAVES; ++w) {
+                    x[w] = joined[w][wave][lane];
+                    st[w] = joined_stats[w][lane];
                 }
+                float grown = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) grown = fmaxf(grown, st[w][0]);
+                const float frame = grown == -INFINITY ? 0.f : grown;
+                v4f all = {0.f, 0.f, 0.f, 0.f};
+                sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float a = fast_exp2(st[w][0] - frame);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) all[i] = fmaf(a, x[w][i], all[i]);
+                    sum = fmaf(a, st[w][1], sum);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = all[i];
+                top = grown;
             }
             __syncthreads();
         }
-        if (valid && (!share || wave == 0)) {
+        if (valid && (!share || wave < 4)) {
             int m = d.seqlen;
             if (d.seqlens_q != nullptr) {
                 const int n = d.seqlens_q[z];
@@ -913,15 +924,15 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
             }
             const bool beyond = token >= m;
             const float weight = beyond || top == -INFINITY ? 0.f : kWeightUnit / sum;
-            char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * (32 * ct + 4 * (lane >> 5));
+            char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * (32 * ct + 4 * (lane >> 5) + (share ? 8 * wave : 0));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 v4f o = {acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]};
                 o *= weight;
                 if (beyond) o = (v4f){0.f, 0.f, 0.f, 0.f};
-                store_out4<DT>(dst + 16 * k, o);
+                if (k == 0 || !share) store_out4<DT>(dst + 16 * k, o);
             }
-            if (d.lse != nullptr && ct == 0 && lane < 32)
+            if (d.lse != nullptr && ct == 0 && lane < 32 && (!share || wave == 0))
                 d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = beyond ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
         }
     }
