@@ -472,7 +472,8 @@ int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream);
  * Sequence b has m = seqlens_q[b] queries (optional; clamped to [0, seqlen]; NULL: seqlen) and n = seqlens_k[b] keys (optional; clamped to [0, seqlen_k]; NULL: seqlen_k); with causal row i
  * sees keys 0 .. n - m + i.  Rows from m onward and rows that see no key are zeros with lse = -infinity; lse as in intfa_fwd_params.
  * Scores and sums are fp32, probabilities are rounded to the type of v; values that are not finite reach the rows that are computed together with those that see them (at
- * most 128 rows, and 64 keys behind a row's last).  Nothing behind a sequence's n keys is read. */
+ * most 128 rows, and 64 keys behind a row's last).  Nothing behind a sequence's n keys is read.  seqlen_k + 64 rows of k_nope, of k_rope and of v (one head's, by their stride) must span
+ * less than 2^31 elements. */
 typedef struct intfa_latent_expanded_params {
     const void* q_nope; const void* q_rope; const void* k_nope; const void* k_rope; const void* v; void* out;
     int64_t qn_stride_b, qn_stride_h, qn_stride_n;
@@ -496,14 +497,14 @@ int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream);
  * number of layers that share the table): what is copied of a page is page_bytes bytes of each. */
 typedef struct intfa_page_pool {
     void* data;
-    int64_t page_stride;               /* bytes from page to page */
+    int64_t page_stride;               /* bytes from page to page: pages must not overlap */
     int64_t page_bytes;
 } intfa_page_pool;
 #define INTFA_MAX_POOLS 4096
 
 typedef struct intfa_page_table {
     int32_t* refs;                     /* [num_pages] */
-    int32_t* block_table;              /* [batch, table_width], columns contiguous */
+    int32_t* block_table;              /* [batch, table_width], columns contiguous, rows that do not overlap */
     int64_t bt_stride_b;
     int32_t* seqlens_k;                /* [batch]; not used by intfa_pages_compact */
     int32_t num_pages, page_size, table_width, batch;      /* page_size: not used by intfa_pages_fork and intfa_pages_compact; positive */

@@ -417,18 +417,19 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
 }
 
 // ---- host
-int check_pools(const intfa_page_pool* pools, int32_t n) {
+int check_pools(const intfa_page_pool* pools, int32_t n, int32_t num_pages) {
     if (n < 0 || n > INTFA_MAX_POOLS || (n > 0 && pools == nullptr)) return INTFA_ERR_POOL;
     for (int i = 0; i < n; ++i) {
         if (pools[i].data == nullptr) return INTFA_ERR_NULL;
         if (pools[i].page_bytes <= 0 || pools[i].page_bytes > 1ll << 40) return INTFA_ERR_POOL;
+        if (num_pages > 1 && pools[i].page_stride < pools[i].page_bytes && -pools[i].page_stride < pools[i].page_bytes) return INTFA_ERR_POOL;      // (pages that overlap)
     }
     return INTFA_OK;
 }
 int check_table(const intfa_page_table* t, bool lens, bool page) {
     if (t == nullptr || t->refs == nullptr || t->block_table == nullptr || (lens && t->seqlens_k == nullptr)) return INTFA_ERR_NULL;
     if (t->num_pages <= 0 || t->num_pages >= 1 << 30 || t->table_width <= 0 || t->table_width >= 1 << 30) return INTFA_ERR_PAGE;
-    if (t->batch <= 0) return INTFA_ERR_SHAPE;
+    if (t->batch <= 0 || (t->batch > 1 && t->bt_stride_b < t->table_width && -t->bt_stride_b < t->table_width)) return INTFA_ERR_SHAPE;      // (rows that overlap)
     if (page && (t->page_size < 16 || t->page_size > 256 || (t->page_size & (t->page_size - 1)))) return INTFA_ERR_PAGE;
     if ((reinterpret_cast<uintptr_t>(t->refs) | reinterpret_cast<uintptr_t>(t->block_table) | reinterpret_cast<uintptr_t>(t->seqlens_k)) & 3u) return INTFA_ERR_ALIGN;
     return INTFA_OK;
@@ -482,7 +483,7 @@ extern "C" {
 
 int intfa_pages_copy(const intfa_page_pool* pools, int32_t num_pools, int32_t num_pages, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
     if (num_pools <= 0) return INTFA_ERR_POOL;
-    const int rc = check_pools(pools, num_pools);
+    const int rc = check_pools(pools, num_pools, num_pages);
     if (rc != INTFA_OK) return rc;
     if (src == nullptr || dst == nullptr) return INTFA_ERR_NULL;
     if (num_pages <= 0) return INTFA_ERR_PAGE;
@@ -529,7 +530,7 @@ int intfa_pages_reserve(const intfa_page_table* t, const intfa_page_pool* pools,
                         void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_table(t, true, true);
     if (rc != INTFA_OK) return rc;
-    rc = check_pools(pools, num_pools);
+    rc = check_pools(pools, num_pools, t->num_pages);
     if (rc != INTFA_OK) return rc;
     if (granted == nullptr) return INTFA_ERR_NULL;
     if (t->batch > 8192 || size_product(t->batch, t->table_width) >= 1ll << 31) return INTFA_ERR_SHAPE;
@@ -554,7 +555,7 @@ int intfa_pages_compact(const intfa_page_table* t, const intfa_page_pool* pools,
                         void* stream) {
     int rc = check_table(t, false, false);
     if (rc != INTFA_OK) return rc;
-    rc = check_pools(pools, num_pools);
+    rc = check_pools(pools, num_pools, t->num_pages);
     if (rc != INTFA_OK) return rc;
     if (new_index == nullptr) return INTFA_ERR_NULL;
     if (reinterpret_cast<uintptr_t>(new_index) & 3u) return INTFA_ERR_ALIGN;

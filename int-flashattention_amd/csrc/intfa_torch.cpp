@@ -811,7 +811,8 @@ std::vector<Tensor> pools_arg(PyObject* o, std::vector<intfa_page_pool>* pools) 
         if (!t.is_cuda()) fail(PyExc_RuntimeError, "int_flashattention_amd kernels run on the GPU only; got a CPU tensor");
         require_on(t, held[0], "every cache");
         if (t.size(0) != held[0].size(0)) fail(PyExc_ValueError, "caches must have one number of pages");
-        if (!t.select(0, 0).is_contiguous()) fail(PyExc_ValueError, "a page of a cache must be contiguous (pages may lie apart)");
+        if (!t.select(0, 0).is_contiguous() || (t.size(0) > 1 && t.stride(0) < t.numel() / t.size(0)))
+            fail(PyExc_ValueError, "a page of a cache must be contiguous, and pages must not overlap (they may lie apart)");
         pools->push_back({t.data_ptr(), t.stride(0) * (int64_t)t.element_size(), t.numel() / t.size(0) * (int64_t)t.element_size()});
     }
     return held;
@@ -828,6 +829,7 @@ intfa_page_table page_table_arg(const Tensor& refs, const Tensor& table, const T
     books_arg(table, 2, refs, "block_table");
     if (refs.size(0) == 0 || refs.size(0) >= 1 << 30) fail(PyExc_ValueError, "refs must hold a count for each page, at least one and fewer than 2^30");
     if (table.size(1) >= 1 << 30 || table.size(0) > INT_MAX) fail(PyExc_ValueError, "block_table has too many columns or rows");
+    if (table.size(0) > 1 && table.stride(0) < table.size(1)) fail(PyExc_ValueError, "rows of block_table must not overlap (it is changed in place)");
     intfa_page_table t{};
     if (lens.defined()) {
         books_arg(lens, 1, refs, "seqlens_k");
