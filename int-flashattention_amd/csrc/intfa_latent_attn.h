@@ -40,9 +40,11 @@ template <int DC, int DR, int ROWS> struct LatentShape {
     static constexpr int WHOLE = UNITS / 4, HALF = UNITS % 4 / 2;      // asynchronous copies of a wave and stage, of 64 and of 32 lanes: its 16 rows
     static constexpr int COPIES = WHOLE + HALF + 1;            // ... and their scales
     static_assert(UNITS % 4 == 0 || UNITS % 4 == 2, "");
-    // The first block comes into the first stage while the queries are in the last two and the angles in the second one (or behind them, where stages are small).
-    static constexpr int QUERY_AT = 2 * STAGE, QUERY_END = QUERY_AT + ROWS * 2 * ROW, ANGLES = ROWS * (DR / 2) * 8;
-    static constexpr bool ANGLES_IN = ANGLES <= STAGE;
+    // The first blocks come into the first stages while the queries' bytes are in the last one or two.  The angles are behind the tiles, or, of 64 wide rows, in the second stage.
+    static constexpr int QUERY_BYTES = ROWS * 2 * ROW, QUERY_AT = (STAGES - (QUERY_BYTES + STAGE - 1) / STAGE) * STAGE, QUERY_END = QUERY_AT + QUERY_BYTES, ANGLES = ROWS * (DR / 2) * 8;
+    static constexpr bool ANGLES_IN = ROWS == 64 && DC == 512;
+    static_assert(!ANGLES_IN || ANGLES <= STAGE, "");
+    static_assert(QUERY_AT >= (ROWS == 32 ? 3 : 2) * STAGE, "copies of the first steps would meet the queries");
     static constexpr int TILES_END = STAGES * STAGE > QUERY_END ? STAGES * STAGE : QUERY_END, ANGLES_AT = ANGLES_IN ? STAGE : TILES_END;
     static constexpr int P_AT = ANGLES_IN ? TILES_END : TILES_END + ANGLES, P_BYTES = ROWS * KEYS * 2;
     static constexpr int SCALES_AT = P_AT + P_BYTES, SCALE_STAGE = KEYS * 8;
@@ -326,12 +328,16 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         copy_rows(c.rows, copy_off, c.to);
         copy_rest(c);
     };
-    // ======== the queries, by all waves, while the first block comes
+    // ======== the queries, by all waves, while the first blocks come
+    const bool early = blocks > 1 && (!S::ANGLES_IN || deal->rope.freqs == nullptr);      // (nothing else is in the second stage)
     {
         Queries queries;
         if (blocks > 0) {
             queries.load(p, t, row0, tid);
-            if (!scoring) copy(0, look(0));
+            if (!scoring) {
+                copy(0, look(0));
+                if (early) copy(1, look(1));
+            }
             const int first_token = paged_div(row0, deal->d_group);
             if (deal->rope.freqs != nullptr) {     // the angles of the tile's tokens, each once
                 const int last_row = row0 + ROWS < deal->rows ? row0 + ROWS - 1 : deal->rows - 1, pairs = deal->rope.pairs;
@@ -346,7 +352,9 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             }
             queries.form(p, lds, (const v2f*)(lds + S::ANGLES_AT), first_token, alphas);
         }
-        if (!scoring) wait_copies<0>();
+        if (!scoring) {
+            if (early) wait_copies<S::COPIES>(); else wait_copies<0>();
+        }
         lds_barrier();                         // queries and first block are there
     }
     if (scoring) {
@@ -376,7 +384,6 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             m[q] = -INFINITY;
             l[q] = 0.f;
         }
-        if (SMALL) lds_barrier();              // (the queries have been read)
         if constexpr (!SMALL)
         {
             // A step forms the scores of block i + 1 while it takes the exponentials of block i: the first fragments' products run while the rows' maxima are settled, and with each of
@@ -618,7 +625,6 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         lds_barrier();
     } else {
         // ======== copies, and the values' product
-        const int id_second = look(1);
         int id_next = look(2);
         int value_at[2];
         {
@@ -635,8 +641,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[g][ct][r] = 0.f;
-        if (SMALL) lds_barrier();
-        if (blocks > 1) copy(1, id_second);
+        if (blocks > 1 && !early) copy(1, look(1));
         for (int i = 0; i <= blocks; ++i) {
             if (!SMALL) {
                 wait_copies<0>();
