@@ -70,34 +70,40 @@ __device__ __forceinline__ void lds_barrier() {
 }
 // A wave's copies of a stage: N times 64 x 16 bytes from base + each lane's offset to consecutive KB of LDS from `lds` on (the last one of 32 lanes, if HALF), without a register on the
 // way.  (As the copies of intfa_device.h: M0 is nobody else's.  One statement, which counts M0 on: with one each, the compiler keeps a scalar for every place of every stage, in lanes
-// of vector registers.)
-#define INTFA_COPY(o) "\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 " o ", %1"
-#define INTFA_FIRST "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1"
-template <int N> __device__ __forceinline__ void copy_rows(const char* base, const uint32_t (&o)[N], uint32_t lds) {
+// of vector registers.)  NT: past the caches, for rows that one workgroup alone reads (256 x 16 heads over 4096 tokens 117 -> 104 us, 5.9 TB/s; but 32 x 128 heads, whose two tiles of
+// rows share them, 66 -> 70).
+#define INTFA_COPY(o, nt) "\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 " o ", %1" nt
+#define INTFA_COPIES(nt) \
+    if constexpr (N == 2) asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]) : "memory", "scc"); \
+    else if constexpr (N == 3) asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]) : "memory", "scc"); \
+    else if constexpr (N == 4) \
+        asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) INTFA_COPY("%5", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]) : "memory", "scc"); \
+    else if constexpr (N == 5) \
+        asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) INTFA_COPY("%5", nt) INTFA_COPY("%6", nt) \
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]) : "memory", "scc"); \
+    else if constexpr (N == 8) \
+        asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) INTFA_COPY("%5", nt) INTFA_COPY("%6", nt) INTFA_COPY("%7", nt) INTFA_COPY("%8", nt) INTFA_COPY("%9", nt) \
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]) : "memory", "scc"); \
+    else \
+        asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) INTFA_COPY("%5", nt) INTFA_COPY("%6", nt) INTFA_COPY("%7", nt) INTFA_COPY("%8", nt) INTFA_COPY("%9", nt) INTFA_COPY("%10", nt) \
+                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]), "v"(o[8]) : "memory", "scc")
+#define INTFA_FIRST(nt) "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1" nt
+template <bool NT, int N> __device__ __forceinline__ void copy_rows(const char* base, const uint32_t (&o)[N], uint32_t lds) {
     static_assert(N == 2 || N == 3 || N == 4 || N == 5 || N == 8 || N == 9, "");
-    if constexpr (N == 2) asm volatile(INTFA_FIRST INTFA_COPY("%3") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]) : "memory", "scc");
-    else if constexpr (N == 3) asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]) : "memory", "scc");
-    else if constexpr (N == 4) asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]) : "memory", "scc");
-    else if constexpr (N == 5)
-        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6")
-                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]) : "memory", "scc");
-    else if constexpr (N == 8)
-        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6") INTFA_COPY("%7") INTFA_COPY("%8") INTFA_COPY("%9")
-                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]) : "memory", "scc");
-    else
-        asm volatile(INTFA_FIRST INTFA_COPY("%3") INTFA_COPY("%4") INTFA_COPY("%5") INTFA_COPY("%6") INTFA_COPY("%7") INTFA_COPY("%8") INTFA_COPY("%9") INTFA_COPY("%10")
-                     :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]), "v"(o[8]) : "memory", "scc");
+    if constexpr (NT) { INTFA_COPIES(" nt"); } else { INTFA_COPIES(""); }
 }
 #undef INTFA_COPY
 #undef INTFA_FIRST
+#undef INTFA_COPIES
 // 64 x 16 bytes and 64 x 4 alone
 __device__ __forceinline__ void copy_units(const char* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
-// 64 x 16 bytes to lds + at, if `wanted`.  (The branch is the statement's own: among the products, a branch of the compiler's costs it its schedule.)
-__device__ __forceinline__ void copy_units_if(int wanted, const char* base, uint32_t off, uint32_t lds, int at) {
-    asm volatile("s_cmp_eq_u32 %4, 0\n\ts_cbranch_scc1 .Lskip_copy%=\n\ts_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n.Lskip_copy%=:"
-                 :: "s"(lds), "v"(off), "s"(base), "i"(at), "s"(wanted) : "memory", "scc");
+// 64 x 16 bytes to lds + at.  how: 0 none, 1 so, 2 past the caches.  (The branches are the statement's own: among the products, a branch of the compiler's costs it its schedule.)
+__device__ __forceinline__ void copy_units_if(int how, const char* base, uint32_t off, uint32_t lds, int at) {
+    asm volatile("s_cmp_eq_u32 %4, 0\n\ts_cbranch_scc1 .Lskip_copy%=\n\ts_add_u32 m0, %0, %3\n\ts_cmp_eq_u32 %4, 1\n\ts_cbranch_scc1 .Lcached_copy%=\n\t"
+                 "global_load_lds_dwordx4 %1, %2 nt\n\ts_branch .Lskip_copy%=\n.Lcached_copy%=:\n\tglobal_load_lds_dwordx4 %1, %2\n.Lskip_copy%=:"
+                 :: "s"(lds), "v"(off), "s"(base), "i"(at), "s"(how) : "memory", "scc");
 }
 __device__ __forceinline__ void copy_words(const char* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
@@ -304,6 +310,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     int page_log2 = deal->page_log2, last_column = deal->table_width - 1, num_pages = deal->num_pages, ks_sh = (int)deal->ks_sh;
     asm volatile("" : "+s"(table), "+s"(all_rows), "+s"(all_scales), "+s"(k_sp), "+s"(ks_sp), "+s"(page_log2), "+s"(last_column), "+s"(num_pages), "+s"(ks_sh));
     const int page_mask = (1 << page_log2) - 1;
+    const bool streams = deal->tiles == 1;     // (nobody else reads these keys)
     auto look = [&](int block) __attribute__((always_inline)) {
         const int column = (key_first + KEYS * block + 16 * wave) >> page_log2;
         return table[column < last_column ? column : last_column];      // (behind the last key the table may hold anything)
@@ -325,7 +332,8 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     };
     auto copy = [&](int block, int id) __attribute__((always_inline)) {
         const BlockCopy c = block_copy(block, id);
-        copy_rows(c.rows, copy_off, c.to);
+        if (streams) copy_rows<true>(c.rows, copy_off, c.to);
+        else copy_rows<false>(c.rows, copy_off, c.to);
         copy_rest(c);
     };
     // ======== the queries, by all waves, while the first blocks come
@@ -658,7 +666,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             float alpha[RG];
             bool follow[RG];
             const bool more = !SMALL && i > 0 && i + 2 < blocks;
-            int wanted = __builtin_amdgcn_readfirstlane(more ? 1 : 0);
+            int wanted = __builtin_amdgcn_readfirstlane(!more ? 0 : streams ? 2 : 1);
             asm volatile("" : "+s"(wanted));
             BlockCopy next{};
             // (values two steps ahead of their products; a copy of block i + 2 behind each column tile's products)
