@@ -303,7 +303,7 @@ const char* intfa_error_string(int code) {
         case INTFA_ERR_SCRATCH: return "the split-KV partials of this call exceed INTFA_STATIC_SCRATCH_BYTES (or the device index exceeds 63)";
         case INTFA_ERR_PAGE: return "page_size must be 16, 32, 64, 128 or 256, with at least one page and one column in the block table";
         case INTFA_ERR_ROPE: return "rotated pairs must be a multiple of 8 and at most half of head_dim, the magnitude a positive number";
-        case INTFA_ERR_POOL: return "pools of pages must be given where pages are copied, at most INTFA_MAX_POOLS, with pages of positive size";
+        case INTFA_ERR_POOL: return "pools of pages must be given where pages are copied, at most INTFA_MAX_POOLS, with pages of positive size that do not overlap";
         default: return code > 0 ? "hip error" : "unknown error";
     }
 }

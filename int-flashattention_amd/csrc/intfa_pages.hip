@@ -303,15 +303,18 @@ __device__ __forceinline__ Span reserve_span(const ReserveArgs& a, int z) {
 
 // Every sequence needs so many pages: those that it lacks, and copies of those that others hold.  Its page of the first column, which holds its last tokens, is the one that
 // forked sequences share: of all that want a copy of it in this call, the last takes none if nobody else is left.  (A thread keeps what it knows of its first sequence; of
-// batches over 1024 it reads the others' again.)
+// batches over 1024 it reads the others' again.  Columns behind the first are its own work too while they are few, and a wave's where they are kLong or more: a trip to memory each, one
+// after the other, a prompt of 16384 tokens on pages of 16 would take 2 ms.)
+constexpr int kLong = 6;
 __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs a) {
     extern __shared__ __align__(16) int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
     int32_t* const plan_lds = head_lds + a.t.batch;      // [batch]: what becomes of its first column
     enum { kLacks, kKeep, kCopy, kLeft, kNone };      // (left: kept if all that share it and come earlier get their copies, else kNone)
     __shared__ int lds[kWalk / 64];
+    __shared__ int long_z[kWalk], long_count[kWalk], longs;      // sequences of many columns, and what is counted of them
     __shared__ int moves_lds;
-    const int pages = a.t.num_pages, Z = a.t.batch;
-    if (threadIdx.x == 0) moves_lds = 0;
+    const int pages = a.t.num_pages, Z = a.t.batch, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) moves_lds = longs = 0;
     const Counts stretch = load_counts(a.t.refs, kEach * (int)threadIdx.x, pages, 1);      // (asked for ahead of its use)
     Span own = {0, 0, 0, 0};
     int own_head = -1, own_holders = 0;
@@ -354,10 +357,34 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
                 plan_lds[z] = holders - before > 1 ? kCopy : before > 0 ? kLeft : kKeep;
             }
             needs = s.first < s.end && (plan_lds[z] == kLacks || plan_lds[z] == kCopy);
-            for (int c = s.first + 1; c < s.end; ++c) {
-                const int id = a.t.table[z * a.t.bt_sb + c];
-                needs += (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
+            if (s.end - s.first >= kLong) long_z[atomicAdd(&longs, 1)] = z;
+            else
+                for (int c = s.first + 1; c < s.end; ++c) {
+                    const int id = a.t.table[z * a.t.bt_sb + c];
+                    needs += (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
+                }
+        }
+        __syncthreads();
+        if (longs > 0) {
+            for (int i = wave; i < longs; i += kWalk / 64) {
+                const int zl = long_z[i];
+                const Span s = reserve_span(a, zl);
+                int count = 0;
+                for (int c0 = s.first + 1; c0 < s.end; c0 += 64) {
+                    bool takes = false;
+                    if (c0 + lane < s.end) {
+                        const int id = a.t.table[zl * a.t.bt_sb + c0 + lane];
+                        takes = (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
+                    }
+                    count += __popcll(__ballot(takes));
+                }
+                if (lane == 0) long_count[zl - z0] = count;
             }
+            __syncthreads();
+            const Span s = z >= Z ? Span{0, 0, 0, 0} : z < kWalk ? own : reserve_span(a, z);
+            if (s.end - s.first >= kLong) needs += long_count[threadIdx.x];
+            __syncthreads();
+            if (threadIdx.x == 0) longs = 0;
         }
         int total;
         const int ahead = scan_all(needs, lds, total);
@@ -384,32 +411,64 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
     found = found < dealt ? found : dealt;
     __threadfence_block();
     __syncthreads();
-    for (int z = threadIdx.x; z < Z; z += kWalk) {
-        const Span s = z < kWalk ? own : reserve_span(a, z);
-        int rank = a.granted[z], room = s.end, plan = plan_lds[z];       // columns before `room` can be written
-        if (plan == kLeft && rank > found) plan = kNone;
-        if (plan == kNone) room = s.first;
-        for (int c = s.first; c < room; ++c) {
-            int32_t* const at = a.t.table + z * a.t.bt_sb + c;
-            const int id = *at;
-            const bool named = (unsigned)id < (unsigned)pages;
-            const bool copy = named && (c == s.first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
-            if (named && !copy) continue;
-            if (rank >= found) {
-                room = c;
-                break;
-            }
-            const int page = a.free_list[rank++];
-            a.t.refs[page] = 1;
-            if (copy) {
-                const int m = atomicAdd(&moves_lds, 1);
-                a.src[m] = id;
-                a.dst[m] = page;
-            }
-            *at = page;
+    // (the table's entry at `column`, which names `id`, becomes `page`)
+    auto give = [&](int z, int column, int id, bool copy, int page) __attribute__((always_inline)) {
+        a.t.refs[page] = 1;
+        if (copy) {
+            const int m = atomicAdd(&moves_lds, 1);
+            a.src[m] = id;
+            a.dst[m] = page;
         }
+        a.t.table[z * a.t.bt_sb + column] = page;
+    };
+    auto grant = [&](int z, const Span& s, int room) __attribute__((always_inline)) {      // columns before `room` can be written
         const int64_t places = ((int64_t)room << a.t.page_log2) - s.held;
         a.granted[z] = places <= 0 ? 0 : places < s.fresh ? (int)places : s.fresh;
+    };
+    for (int z0 = 0; z0 < Z; z0 += kWalk) {
+        const int z = z0 + (int)threadIdx.x;
+        if (z < Z) {
+            const Span s = z < kWalk ? own : reserve_span(a, z);
+            int rank = a.granted[z], plan = plan_lds[z];
+            if (plan == kLeft && rank > found) plan = kNone;
+            const bool many = s.end - s.first >= kLong;
+            int room = plan == kNone ? s.first : many ? s.first + 1 : s.end;
+            for (int c = s.first; c < room; ++c) {
+                const int id = a.t.table[z * a.t.bt_sb + c];
+                const bool named = (unsigned)id < (unsigned)pages;
+                const bool copy = named && (c == s.first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
+                if (named && !copy) continue;
+                if (rank >= found) {
+                    room = c;
+                    break;
+                }
+                give(z, c, id, copy, a.free_list[rank++]);
+            }
+            if (many && room > s.first) {
+                long_z[atomicAdd(&longs, 1)] = z;
+                long_count[threadIdx.x] = rank;
+            } else grant(z, s, room);
+        }
+        __syncthreads();
+        for (int i = wave; i < longs; i += kWalk / 64) {
+            const int zl = long_z[i];
+            const Span s = reserve_span(a, zl);
+            int rank = long_count[zl - z0], room = s.end;
+            for (int c0 = s.first + 1; c0 < s.end && room == s.end; c0 += 64) {
+                const int c = c0 + lane, id = c < s.end ? a.t.table[zl * a.t.bt_sb + c] : -1;
+                const bool named = (unsigned)id < (unsigned)pages, copy = named && a.t.refs[id] > 1, takes = c < s.end && (!named || copy);
+                const uint64_t all = __ballot(takes);
+                const int mine = rank + __popcll(all & ((1ull << lane) - 1));
+                if (takes && mine < found) give(zl, c, id, copy, a.free_list[mine]);
+                const uint64_t out = __ballot(takes && mine >= found);
+                if (out != 0) room = c0 + __builtin_ctzll(out);
+                rank += __popcll(all);
+            }
+            if (lane == 0) grant(zl, s, room);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) longs = 0;
+        __syncthreads();
     }
     __threadfence_block();
     __syncthreads();
@@ -504,6 +563,7 @@ int intfa_pages_fork(const intfa_page_table* t, const int32_t* parents, const in
     // Columns of a workgroup: 1024 entries in four rounds, or one column
     const int columns = n >= 1024 ? 1 : 1024 / n < 64 ? 1024 / n : 64;
     const unsigned groups = (unsigned)((t->table_width + columns - 1) / columns);
+    if ((groups + 1ll) * 256 >= 1ll << 32) return INTFA_ERR_SHAPE;
     int slots = 64;
     while (2 * slots < 3 * n) slots *= 2;
     const size_t words = (size_t)(1 + columns) * n + slots;      // (slots: n or more; 64 KB at the most)

@@ -201,6 +201,35 @@ def test_captured_steps_follow_counts_and_lengths():
         assert junk.isfinite()
 
 
+@pytest.mark.parametrize("pages", [3000, 700])
+def test_prompts_of_many_columns(pages):
+    """Reservations of hundreds of columns beside short ones, over entries that are named already, shared ones among them; where the pages run out, in the middle of such a span."""
+    g = torch.Generator().manual_seed(pages)
+    Z, width, page = 40, 170, 16
+    refs, table, lens = [0] * pages, [[-1] * width for _ in range(Z)], []
+    order = torch.randperm(pages, generator=g).tolist()
+    for z in range(Z):
+        lens.append(pick(g, 60, 1)[0] if z % 3 else 0)
+        for c in range(lens[z] // page + 1):
+            table[z][c] = order.pop()
+        if z % 5 == 1:                         # entries ahead of the tokens, one's own and shared ones
+            for c in (7, 8, 70, 130):
+                table[z][c] = order[c % 3] if c % 2 == 0 else order.pop()
+    for row in table:
+        for i in row:
+            if i >= 0:
+                refs[i] += 1
+    start = (refs, table, lens, [torch.arange(pages, dtype=torch.int32)[:, None].repeat(1, 5)])
+    b = Books(*start, page)
+    refs, table, lens, pools = device(*start)
+    fresh = [(2600, 3, 1500, 0, 90, 1040, 200)[z % 7] for z in range(Z)]
+    granted = ifa.paged_reserve(pools, refs, table, lens, ints(fresh), page)
+    want = b.reserve(fresh)
+    assert granted.tolist() == want
+    assert (sum(want) < sum(fresh)) == (pages == 700) or max(fresh) > width * page - 60
+    b.check(refs, table, lens, pools)
+
+
 @pytest.mark.parametrize("n", [2731, 4096])
 def test_the_largest_forks(n):
     """As many pairs as a call takes, to distinct children and to few of them, over and over."""
