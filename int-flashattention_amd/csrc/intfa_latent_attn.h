@@ -512,18 +512,17 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             const int key0 = key_first + KEYS * block, tile = (block % STAGES) * S::STAGE;
             const float* const scales = (const float*)(lds + S::SCALES_AT + (block % STAGES) * S::SCALE_STAGE);
             // ---- scores, as t = score + log2 of the value's scale
-            constexpr int PER = SMALL ? 4 : 16;    // a lane's keys
-            typedef typename std::conditional<SMALL, v4i, v16i>::type Sums;
+            constexpr int PER = 4;             // a lane's keys
             float s[QT][PER];
             // (lane i of a row of sixteen has the scales of the row's i-th key, from where all of the row take them)
-            const int tile_key = SMALL ? 16 * wave : 32 * kg, lane_key = tile_key + (SMALL ? 4 * c16 + (x16 & 3) : (int)scale_lane_key(lane));
+            const int tile_key = 16 * wave, lane_key = tile_key + 4 * c16 + (x16 & 3);
             const v2f two = *(const v2f*)(scales + 2 * lane_key);
             // the rotary part first, then the latent one, two fragments ahead of the products
             auto fragment = [&](int i) __attribute__((always_inline)) {
                 const int k = i < KS - KC ? KC + i : i - (KS - KC);
                 return *(const v4i*)(lds + tile + fragment_at(key_at, k));
             };
-            Sums hi[QT], lo[QT];
+            v4i hi[QT], lo[QT];
             auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int q = 0; q < QT; ++q)
@@ -548,13 +547,8 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 }
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
-                    if constexpr (SMALL) {
-                        hi[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_hi[q][k], hi[q], 0, 0, 0);
-                        lo[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_lo[q][k], lo[q], 0, 0, 0);
-                    } else {
-                        hi[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query_hi[q][k], hi[q], 0, 0, 0);
-                        lo[q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[i % 4], query_lo[q][k], lo[q], 0, 0, 0);
-                    }
+                    hi[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_hi[q][k], hi[q], 0, 0, 0);
+                    lo[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[i % 4], query_lo[q][k], lo[q], 0, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -567,7 +561,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 if (key0 + KEYS > least) {
 #pragma unroll
                     for (int i = 0; i < PER; ++i) {
-                        const int key = key0 + tile_key + (SMALL ? 4 * c16 + i : 8 * (i / 4) + 4 * lh + i % 4);
+                        const int key = key0 + tile_key + 4 * c16 + i;
                         s[q][i] = key < seen[q] ? s[q][i] : -INFINITY;
                     }
                 }
@@ -575,27 +569,26 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 top[q] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) top[q] = fmaxf(top[q], s[q][i]);
-                if constexpr (SMALL) top[q] = reduce_row_lanes(top[q], [](float a, float b) { return fmaxf(a, b); });
-                else top[q] = half_pair_max(top[q]);
-                if (SMALL ? c16 == 0 : lh == 0) tops[kg * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)] = top[q];
+                top[q] = reduce_row_lanes(top[q], [](float a, float b) { return fmaxf(a, b); });
+                if (c16 == 0) tops[kg * ROWS + 16 * q + x16] = top[q];
             }
             lds_barrier();                     // A: the maxima are there, and P of the block before has been read
             bool grows[QT], any = false;
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
 #pragma unroll
-                for (int k = 0; k < KG; ++k) top[q] = fmaxf(top[q], tops[k * ROWS + (SMALL ? 16 * q + x16 : 32 * rg + lq)]);
+                for (int k = 0; k < KG; ++k) top[q] = fmaxf(top[q], tops[k * ROWS + 16 * q + x16]);
                 grows[q] = top[q] - m[q] > kLatentSlack;
                 any = any || grows[q];
             }
-            const bool follow = __any(any);    // (of a row group's waves alike; rows that do not need it stay: what a row gets does not depend on the others)
+            const bool follow = __any(any);    // (of all waves alike; rows that do not need it stay: what a row gets does not depend on the others)
             if (follow) {
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
                     const float alpha = grows[q] ? fast_exp2(m[q] - top[q]) : 1.f;
                     m[q] = grows[q] ? top[q] : m[q];
                     l[q] *= alpha;
-                    if (kg == 0 && (SMALL ? c16 == 0 : lh == 0)) alphas[SMALL ? 16 * q + x16 : 32 * rg + lq] = alpha;
+                    if (kg == 0 && c16 == 0) alphas[16 * q + x16] = alpha;
                 }
             }
             if (kg == 0 && lane == 0) flags[rg] = follow;
@@ -611,13 +604,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 uint32_t w[PER / 2];
 #pragma unroll
                 for (int h = 0; h < PER / 2; ++h) w[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){s[q][2 * h], s[q][2 * h + 1]}, v2h));
-                if constexpr (SMALL) {
-                    *(v2i*)(lds + S::P_AT + (64 * wave + 16 * q + x16 + 32 * (c16 & 1)) * 16 + 8 * (c16 >> 1)) = (v2i){(int)w[0], (int)w[1]};
-                } else {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        *(v4i*)(lds + S::P_AT + ((rg * 4 + 2 * kg + half) * 64 + lane) * 16) = (v4i){(int)w[4 * half], (int)w[4 * half + 1], (int)w[4 * half + 2], (int)w[4 * half + 3]};
-                }
+                *(v2i*)(lds + S::P_AT + (64 * wave + 16 * q + x16 + 32 * (c16 & 1)) * 16 + 8 * (c16 >> 1)) = (v2i){(int)w[0], (int)w[1]};
             }
             lds_barrier();                     // B: P is there, and so is the next block
         }
