@@ -125,6 +125,38 @@ def scan_lanes(asm: str) -> List[str]:
     return findings
 
 
+_TRANS = re.compile(r"^v_(exp|log|rcp|rsq|sqrt|sin|cos)_(f16|f32|legacy_f32|iflag_f32)")
+
+
+def scan_trans(asm: str) -> List[str]:
+    """Returns one line per vector instruction that reads the result of an exponential, logarithm, root, reciprocal, sine or cosine right behind it (another such instruction may): it needs one
+    wait state, which the compiler leaves ahead of its own instructions only.  A hand-written sum of weights right behind their exponentials read the registers' old contents in some lanes."""
+    findings: List[str] = []
+    for kernel, blocks in spill_check.kernels(asm):
+        code = [[(n, *m.groups()) for n, t in b["lines"] for m in [_INSTRUCTION.match(t)] if m] for b in blocks]
+        ways = spill_check.successors(blocks)
+        for k, lines in enumerate(code):
+            for i, (n, op, operands) in enumerate(lines):
+                if not _TRANS.match(op):
+                    continue
+                following, seen = lines[i + 1:i + 2], set()
+                if not following:              # the next instruction of every way on, past empty blocks
+                    work = list(ways[k])
+                    while work:
+                        j = work.pop()
+                        if j not in seen:
+                            seen.add(j)
+                            following += code[j][:1]
+                            work += [] if code[j] else ways[j]
+                result = set(_registers(re.split(r",\s*(?![^\[]*\])", operands.strip())[0]))
+                for at, reader, read in following:
+                    args = re.split(r",\s*(?![^\[]*\])", read.strip())
+                    sources = args if reader.startswith(("v_fmac", "v_mac", "v_dot", "v_writelane")) else args[1:]
+                    if reader.startswith("v_") and not _TRANS.match(reader) and result & set(_registers(", ".join(sources))):
+                        findings.append(f"{kernel}: line {at}: `{reader} {read.strip()}` comes 1 wait state too early for the result of line {n}")
+    return findings
+
+
 _LOAD_WAIT = re.compile(r"^\s+s_waitcnt\b.*\bvmcnt\(")
 
 
