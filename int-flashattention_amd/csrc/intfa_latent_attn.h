@@ -813,9 +813,13 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (wave == 0) {
         int found = 0, units = 0;
-        for (int i0 = 0; i0 < d.grid; i0 += 64) {
-            const v4i item = p->open_items[i0 + lane < d.grid ? i0 + lane : 0];
-            const int pieces = i0 + lane < d.grid ? item[0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
+        v4i all[kComputeUnits / 64];           // (one trip for all of them)
+#pragma unroll
+        for (int i = 0; i < kComputeUnits / 64; ++i) all[i] = p->open_items[64 * i + lane < d.grid ? 64 * i + lane : 0];
+#pragma unroll
+        for (int i = 0; i < kComputeUnits / 64; ++i) {
+            const v4i item = all[i];
+            const int pieces = 64 * i + lane < d.grid ? item[0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
             int upto = mine;
 #pragma unroll
             for (int w = 1; w < 64; w <<= 1) {
