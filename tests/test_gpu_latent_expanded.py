@@ -29,7 +29,7 @@ def run(x, causal, sm, nq=None, nk=None, copies=1):
     """copies: of the heads, side by side; all give the same."""
     i32 = dict(dtype=torch.int32, device="cuda")
     heads = x[0].shape[1]
-    x = [t.cuda() if t.shape[1] == 1 and heads > 1 else t.cuda().repeat(1, copies, 1, 1) for t in x]
+    x = [t.cuda() if i == 3 else t.cuda().repeat(1, copies, 1, 1) for i, t in enumerate(x)]      # (the rotary keys are all heads')
     out, lse = ifa.attention_latent(*x, causal, sm, seqlens_q=None if nq is None else torch.tensor(nq, **i32),
                                     seqlens_k=None if nk is None else torch.tensor(nk, **i32), return_lse=True)
     for i in range(heads, heads * copies, heads):
