@@ -11,7 +11,7 @@
 // scales' sizes, P is within fp16 and the accumulators are plain sums of int8 numbers times P; the output is their quotient.
 // Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 106 us with the merge, 5.75 TB/s (memory; the same pages over and over would be 99);
 // 128 heads of 32 requests 55 us and 11 of merging, 650 TFLOP/s without it (4560 clocks a block of 64 rows, where products take 2176 and vector instructions 1840: two waves a SIMD, in order, hide little of either
-// under the other).  32 rows where a tile of 64 would be half empty: 16 of its rows cost what 32 do in the values' product, which is not what bounds few rows.
+// under the other).  Tiles of 32 rows are for few rows, and where there is little work (make_plan): 16 of their rows cost what 32 do in the values' product, which is not what bounds few rows.
 #pragma once
 #include "intfa_latent_host.h"
 #include "intfa_paged_device.h"

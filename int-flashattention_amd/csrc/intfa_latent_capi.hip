@@ -28,11 +28,15 @@ struct Plan { int rows, tiles, unit_log2, lead, grid; size_t stats_at, items_at,
 Plan make_plan(const intfa_latent_attn_params* p) {
     Plan a{};
     const int rows = p->heads * p->seqlen;
-    a.rows = rows <= 32 ? 32 : 64;
+    const int64_t keys = (int64_t)p->cache.table_width * p->cache.page_size;
+    // Tiles of 64 rows take a block of keys in 1.6 times the time of 32 rows, and twice as long until their first and from their last one: with few blocks a compute unit tiles of 32 are
+    // faster (128 heads of one request over 8192 tokens 35 -> 27 us, 64 heads of 16 over 2048 34 -> 28; 128 heads of 32 over 2048, eight blocks a unit, 48 both; over 4096 65 -> 75).
+    // (The keys that the table has room for; the lengths are on the device.)
+    a.rows = rows <= 32 || size_product((int64_t)p->batch * ((rows + 63) / 64), (keys + 63) / 64) <= 8 * kComputeUnits ? 32 : 64;
     a.tiles = (rows + a.rows - 1) / a.rows;
     a.lead = 2;
     a.unit_log2 = 6;
-    const int64_t items = (int64_t)p->batch * a.tiles, keys = (int64_t)p->cache.table_width * p->cache.page_size;
+    const int64_t items = (int64_t)p->batch * a.tiles;
     auto units = [&] { return items * (a.lead + ((keys + (1ll << a.unit_log2) - 1) >> a.unit_log2)); };
     a.grid = (int)(units() < kComputeUnits ? units() : kComputeUnits);
     while (units() * a.grid >= 1ll << 32 && a.unit_log2 < 30) ++a.unit_log2;      // (units are numbered in 32 bits, times the workgroups)

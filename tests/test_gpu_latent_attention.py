@@ -27,7 +27,25 @@ def queries(g, Z, H, N, dc, dr, dtype, size=1.5):
     return (torch.randn((Z, H, N, dc), generator=g) * size * (64.0 / dc) ** 0.5).to(dtype), (torch.randn((Z, H, N, dr), generator=g) * size).to(dtype)
 
 
+WIDE = {"on": False}
+
+
+@pytest.fixture(autouse=True, params=[False, True], ids=["", "wide"])
+def wide(request, monkeypatch):
+    """Tables with room for few keys and for many, behind the same lengths: calls of more than 32 rows take tiles of 32 rows with the one and of 64 with the other."""
+    monkeypatch.setitem(WIDE, "on", request.param)
+
+
+def widened(table, q, page, lens):
+    if not WIDE["on"] or max(lens) > table.shape[1] * page:      # (a length behind the table's end stays there)
+        return table
+    Z, H, N = q.shape[:3]
+    more = 2100 * 64 // (Z * -(-H * N // 64) * page) + 1
+    return torch.cat([table, torch.full((table.shape[0], more), -1, dtype=torch.int32)], 1)
+
+
 def run(q, pool, table, lens, causal, sm=0.1, fresh=None, rope=None, **kw):
+    table = widened(table, q[0], pool[0].shape[1], lens)
     i32 = dict(dtype=torch.int32, device="cuda")
     rope_kw = {} if rope is None else dict(freqs=rope["freqs"].cuda(), magnitude=rope.get("magnitude", 1.0), interleaved=rope.get("interleaved", False))
     return ifa.attention_paged_latent_int8(q[0].cuda(), q[1].cuda(), pool[0].cuda(), pool[1].cuda(), table.cuda(), torch.tensor(lens, **i32), causal, sm,
@@ -202,6 +220,7 @@ def test_strides():
     want = run(tuple(x.contiguous() for x in q), pool, table, lens, True)
     rows = torch.zeros((20, 2, 16, 608), dtype=torch.int8)
     rows[:, 1, :, 16:592] = pool[0]
+    table = widened(table, q[0], 16, lens)
     scales = torch.zeros((20, 16, 4))
     scales[..., 2:] = pool[1]
     i32 = dict(dtype=torch.int32, device="cuda")
@@ -228,5 +247,6 @@ def test_cache_behind_4_gib():
     i32 = dict(dtype=torch.int32, device="cuda")
     for H in (16, 64):
         q = [x.cuda() for x in queries(g, 1, H, 1, 512, 64, torch.float16)]
+        table = widened(table, q[0], 64, [300])
         outs = [ifa.attention_paged_latent_int8(*q, cache, scale, (table + off).cuda(), torch.tensor([300], **i32), False, 0.1) for off in (0, pages - 8)]
         assert torch.equal(*outs) and outs[0].abs().max() > 0

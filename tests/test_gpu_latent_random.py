@@ -4,6 +4,7 @@ import random
 import pytest
 import torch
 
+import test_gpu_latent_attention as A
 import test_gpu_latent_expanded as E
 from latent_reference import make_pool
 from paged_reference import make_table
@@ -13,7 +14,8 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("seed", range(120))
-def test_absorbed(seed):
+def test_absorbed(seed, monkeypatch):
+    monkeypatch.setitem(A.WIDE, "on", seed % 2 == 1)
     r, g = random.Random(seed), torch.Generator().manual_seed(seed)
     dc, dr, page = r.choice((128, 256, 512)), r.choice((32, 64)), r.choice((16, 32, 64, 128, 256))
     Z, N = r.choice((1, 2, 3, 7)), r.choice((1, 1, 1, 2, 3, 8, 17))

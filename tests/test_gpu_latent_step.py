@@ -139,10 +139,10 @@ def _captured(f):
     return graph
 
 
-@pytest.mark.parametrize("H", [4, 40])
-def test_a_captured_step_replays_like_eager_ones(H):
+@pytest.mark.parametrize("H,width", [(4, 6), (40, 6), (40, 800)])
+def test_a_captured_step_replays_like_eager_ones(H, width):
     """Reservation, appends, lengths and attention captured once, replayed over new tokens with forks, frees and eager work in between; eager steps on a second server give the same bits."""
-    a, b = Server(6, 80, 6), Server(6, 80, 6)
+    a, b = Server(6, 80, width), Server(6, 80, width)
     start = [t.clone() for t in a.books()]
     q = [torch.zeros((6, H, 1, d), dtype=torch.bfloat16, device=DEV) for d in (DC, DR)]
     new, fresh = [tuple(torch.zeros_like(t) for t in pair) for pair in a.new(3)], ints(*[0] * 6)
@@ -224,8 +224,9 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, y) for x, y in zip(servers[i].books(), servers[2 + i].books()))
 
 
-def test_calls_repeat_to_the_bit():
-    s = Server(5, 200, 40, layers=1)
+@pytest.mark.parametrize("width", [40, 1000])
+def test_calls_repeat_to_the_bit(width):
+    s = Server(5, 200, width, layers=1)
     s.step(s.new(1200), ints(1200, 700, 3, 64, 999))
     for H, N in ((16, 1), (30, 1), (128, 1), (10, 6)):
         q = [t.to(DEV) for t in queries(s.g, 5, H, N, DC, DR, torch.bfloat16)]
