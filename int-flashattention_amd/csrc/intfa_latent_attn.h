@@ -10,7 +10,7 @@
 // A token's value scale s goes into the exponent: rows follow the maximum of t = score + log2 s, P = 2^(t - frame), and the sum of weights is that of P / s.  Whatever the
 // scales' sizes, P is within fp16 and the accumulators are plain sums of int8 numbers times P; the output is their quotient.
 // Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 106 us with the merge, 5.75 TB/s (memory; the same pages over and over would be 99);
-// 128 heads of 32 requests 55 us and 11 of merging, 650 TFLOP/s without it (4560 clocks a block of 64 rows, where products take 2176 and vector instructions 1840: two waves a SIMD, in order, hide little of either
+// 128 heads of 32 requests 54 us and 10 of merging, 670 TFLOP/s without it (4560 clocks a block of 64 rows, where products take 2176 and vector instructions 1840: two waves a SIMD, in order, hide little of either
 // under the other).  Tiles of 32 rows are for few rows, and where there is little work (make_plan): 16 of their rows cost what 32 do in the values' product, which is not what bounds few rows.
 #pragma once
 #include "intfa_latent_host.h"
@@ -796,15 +796,51 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     if (threadIdx.x == 0) latent_args()->open_items[blockIdx.x] = open;
 }
 
-// The items that lie in several pieces, a launch later.  A slice is 32 rows by 32 columns; a wave takes one, or, of an item of many pieces, an eighth of the pieces of one, and the
-// eight join theirs.  The workgroups deal the open items' slices among themselves (a grid over all items would be mostly workgroups without work, and of
-// 65536 tokens of one request, 256 pieces, sixteen workgroups read all: 49 us with the attention, 33 so).  Bound by a chain of four trips to memory, about 4 us, and by what the parts are: 128 heads of 32
-// requests 33 MB in 11 us.
+// Pieces first, first + step .. of an item: a lane's Q groups of four columns (1024 bytes apart) of the weighted sums, the row's maximum and sum of weights.  PER: pieces under way at a time.
+template <int Q, int PER> __device__ __forceinline__ void latent_gather(const float* parts, const float* stats, int64_t slot0, int64_t slot_bytes, int rows, int pieces, int first, int step,
+                                                                        v4f (&acc)[Q], float& top, float& sum) {
+    for (int j0 = first; j0 < pieces; j0 += PER * step) {
+        v4f x[PER][Q];
+        v2f st[PER];
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int j = j0 + u * step;
+            st[u] = (v2f){-INFINITY, 0.f};
+            if (j >= pieces) continue;
+            // the pieces: the first in its workgroup's own slot, the others first items of theirs
+            const int64_t slot = j == 0 ? slot0 : 2 * ((slot0 >> 1) + j);
+            st[u] = *(const v2f*)(stats + slot * rows * 2);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) x[u][k] = *(const v4f*)((const char*)parts + slot * slot_bytes + 1024 * k);
+        }
+        float grown = top;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) grown = fmaxf(grown, st[u][0]);
+        const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
+#pragma unroll
+        for (int k = 0; k < Q; ++k) acc[k] *= a;
+        sum *= a;
+        top = grown;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            if (j0 + u * step >= pieces) continue;
+            const float w = fast_exp2(st[u][0] - frame);
+#pragma unroll
+            for (int k = 0; k < Q; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[k][i] = fmaf(w, x[u][k][i], acc[k][i]);
+            sum = fmaf(w, st[u][1], sum);
+        }
+    }
+}
+// The items that lie in several pieces, a launch later.  A slice is 32 rows by 32 columns; a wave takes one, or, of an item of many pieces, eight waves share a quarter of one, an eighth of
+// the pieces each, and the first joins theirs.  The workgroups deal the open items' slices among themselves (a grid over all items would be mostly workgroups without work).  Bound by a
+// chain of four trips to memory, about 4 us, and by what the parts are: 128 heads of 32 requests 33 MB in 9.6 us; one request of 256 pieces, 8 MB, 8.5 (in whole slices 14.5).
 template <int DC, int DT, int ROWS>
 __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
     constexpr int SLICES = ROWS / 32 * (DC / 32), MANY = 8, WAVES = 8;
     constexpr int SETS = (SLICES + WAVES - 1) / WAVES;         // of slices, an eight of waves each
-    __shared__ v4f joined[WAVES][4][64];
+    __shared__ v4f joined[WAVES][64];
     __shared__ v2f joined_stats[WAVES][64];
     __shared__ v4i items[kComputeUnits];       // the open items
     __shared__ int first[kComputeUnits + 1], count;      // their first unit of work
@@ -819,7 +855,7 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
 #pragma unroll
         for (int i = 0; i < kComputeUnits / 64; ++i) {
             const v4i item = all[i];
-            const int pieces = 64 * i + lane < d.grid ? item[0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? SLICES : SETS;
+            const int pieces = 64 * i + lane < d.grid ? item[0] : 0, mine = pieces == 0 ? 0 : pieces > MANY ? 4 * SLICES : SETS;
             int upto = mine;
 #pragma unroll
             for (int w = 1; w < 64; w <<= 1) {
@@ -851,81 +887,47 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
         const v4i item = items[lo];
         const int pieces = __builtin_amdgcn_readfirstlane(item[0]), z = __builtin_amdgcn_readfirstlane(item[1]), tile = __builtin_amdgcn_readfirstlane(item[2]);
         const int part = unit - __builtin_amdgcn_readfirstlane(first[lo]);
-        const bool share = pieces > MANY;      // the waves share a slice's pieces
-        const int slice = share ? part : part * WAVES + wave, g = slice / (DC / 32), ct = slice % (DC / 32);
+        const bool share = pieces > MANY;      // the waves share a quarter of a slice
+        const int slice = share ? part / 4 : part * WAVES + wave, quarter = share ? part % 4 : 0, g = slice / (DC / 32), ct = slice % (DC / 32);
         const int r = 32 * g + (lane & 31), row = tile * ROWS + r;
         const bool valid = row < d.rows && slice < SLICES;
         const int token = paged_div(valid ? row : 0, d.d_group), head = (valid ? row : 0) - token * d.group;
         const int64_t slot0 = __builtin_amdgcn_readfirstlane(item[3]);
-        float acc[16], top = -INFINITY, sum = 0.f;
+        const float* const parts = d.parts + ((slice * 4 + quarter) * 64 + lane) * 4;
+        const float* const stats = d.part_stats + r * 2;
+        v4f acc[4];
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-        const int step = share ? WAVES : 1;
-        if (valid)
-            for (int j0 = share ? wave : 0; j0 < pieces; j0 += MANY / 2 * step) {
-                v4f x[MANY / 2][4];
-                v2f st[MANY / 2];
-#pragma unroll
-                for (int u = 0; u < MANY / 2; ++u) {
-                    const int j = j0 + u * step;
-                    st[u] = (v2f){-INFINITY, 0.f};
-                    if (j >= pieces) continue;
-                    // the pieces: the first in its workgroup's own slot, the others first items of theirs
-                    const int64_t slot = j == 0 ? slot0 : 2 * ((slot0 >> 1) + j);
-                    st[u] = *(const v2f*)(d.part_stats + (slot * ROWS + r) * 2);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) x[u][k] = *(const v4f*)(d.parts + slot * ROWS * DC + ((slice * 4 + k) * 64 + lane) * 4);
-                }
-                float grown = top;
-#pragma unroll
-                for (int u = 0; u < MANY / 2; ++u) grown = fmaxf(grown, st[u][0]);
-                const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] *= a;
-                sum *= a;
-                top = grown;
-#pragma unroll
-                for (int u = 0; u < MANY / 2; ++u) {
-                    if (j0 + u * step >= pieces) continue;
-                    const float w = fast_exp2(st[u][0] - frame);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[i] = fmaf(w, x[u][i / 4][i % 4], acc[i]);
-                    sum = fmaf(w, st[u][1], sum);
-                }
-            }
+        for (int k = 0; k < 4; ++k) acc[k] = (v4f){0.f, 0.f, 0.f, 0.f};
         if (share) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) joined[wave][k][lane] = (v4f){acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]};
+            v4f one[1] = {acc[0]};
+            if (valid) latent_gather<1, MANY>(parts, stats, slot0, (int64_t)ROWS * DC * 4, ROWS, pieces, wave, WAVES, one, top, sum);
+            joined[wave][lane] = one[0];
             joined_stats[wave][lane] = (v2f){top, sum};
             __syncthreads();
-            if (wave < 4) {                    // a wave has eight of the columns now: as if they were its first
-                v4f x[WAVES];
+            if (wave == 0) {
                 v2f st[WAVES];
-#pragma unroll
-                for (int w = 0; w < WAVES; ++w) {
-                    x[w] = joined[w][wave][lane];
-                    st[w] = joined_stats[w][lane];
-                }
                 float grown = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) grown = fmaxf(grown, st[w][0]);
+                for (int w = 0; w < WAVES; ++w) {
+                    st[w] = joined_stats[w][lane];
+                    grown = fmaxf(grown, st[w][0]);
+                }
                 const float frame = grown == -INFINITY ? 0.f : grown;
-                v4f all = {0.f, 0.f, 0.f, 0.f};
                 sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
                     const float a = fast_exp2(st[w][0] - frame);
+                    const v4f x = joined[w][lane];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) all[i] = fmaf(a, x[w][i], all[i]);
+                    for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(a, x[i], acc[0][i]);
                     sum = fmaf(a, st[w][1], sum);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = all[i];
                 top = grown;
             }
             __syncthreads();
-        }
-        if (valid && (!share || wave < 4)) {
+        } else if (valid) latent_gather<4, MANY / 2>(parts, stats, slot0, (int64_t)ROWS * DC * 4, ROWS, pieces, 0, 1, acc, top, sum);
+        if (valid && (!share || wave == 0)) {
             int m = d.seqlen;
             if (d.seqlens_q != nullptr) {
                 const int n = d.seqlens_q[z];
@@ -933,15 +935,14 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
             }
             const bool beyond = token >= m;
             const float weight = beyond || top == -INFINITY ? 0.f : kWeightUnit / sum;
-            char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * (32 * ct + 4 * (lane >> 5) + (share ? 8 * wave : 0));
+            char* const dst = d.out + z * d.o_sb + head * d.o_sh + token * d.o_sn + 2 * (32 * ct + 4 * (lane >> 5) + 8 * quarter);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v4f o = {acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]};
-                o *= weight;
+                v4f o = acc[k] * weight;
                 if (beyond) o = (v4f){0.f, 0.f, 0.f, 0.f};
                 if (k == 0 || !share) store_out4<DT>(dst + 16 * k, o);
             }
-            if (d.lse != nullptr && ct == 0 && lane < 32 && (!share || wave == 0))
+            if (d.lse != nullptr && ct == 0 && quarter == 0 && lane < 32)
                 d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = beyond ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
         }
     }
@@ -951,9 +952,9 @@ template <int DC, int DR, int DT, int ROWS, int QT> int launch_latent_rows(const
     hipLaunchKernelGGL((latent_attn_kernel<DC, DR, DT, ROWS, QT>), dim3((unsigned)p.deal.grid), dim3(512), 0, stream, p);
     const int rc = (int)hipGetLastError();
     if (rc != 0) return rc;
-    // (an item of few pieces is SLICES / 8 units of work, one of nine or more SLICES)
+    // (an item of few pieces is SLICES / 8 units of work, one of nine or more 4 SLICES)
     constexpr int SLICES = ROWS / 32 * (DC / 32);
-    const int units = p.deal.grid * SLICES / 8 + SLICES;
+    const int units = p.deal.grid * SLICES / 8 + 4 * SLICES;
     hipLaunchKernelGGL((latent_merge_kernel<DC, DT, ROWS>), dim3((unsigned)(units < 2 * kComputeUnits ? units : 2 * kComputeUnits)), dim3(512), 0, stream, p);
     return (int)hipGetLastError();
 }
