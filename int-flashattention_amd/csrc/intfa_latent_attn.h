@@ -9,7 +9,7 @@
 //                  the columns for all rows, so that no byte is converted twice.  P goes through LDS in the operand's own layout.
 // A token's value scale s goes into the exponent: rows follow the maximum of t = score + log2 s, P = 2^(t - frame), and the sum of weights is that of P / s.  Whatever the
 // scales' sizes, P is within fp16 and the accumulators are plain sums of int8 numbers times P; the output is their quotient.
-// Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 106 us with the merge, 5.75 TB/s (memory; the same pages over and over would be 99);
+// Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 100 us with the merge, 6.1 TB/s (memory; the same pages over and over would be 86);
 // 128 heads of 32 requests 54 us and 10 of merging, 670 TFLOP/s without it (4560 clocks a block of 64 rows, where products take 2176 and vector instructions 1840: two waves a SIMD, in order, hide little of either
 // under the other).  Tiles of 32 rows are for few rows, and where there is little work (make_plan): 16 of their rows cost what 32 do in the values' product, which is not what bounds few rows.
 #pragma once
@@ -77,7 +77,8 @@ __device__ __forceinline__ void lds_barrier() {
 // rows share them, 66 -> 70).
 #define INTFA_COPY(o, nt) "\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 " o ", %1" nt
 #define INTFA_COPIES(nt) \
-    if constexpr (N == 2) asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]) : "memory", "scc"); \
+    if constexpr (N == 1) asm volatile(INTFA_FIRST(nt) :: "s"(lds), "s"(base), "v"(o[0]) : "memory"); \
+    else if constexpr (N == 2) asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]) : "memory", "scc"); \
     else if constexpr (N == 3) asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]) : "memory", "scc"); \
     else if constexpr (N == 4) \
         asm volatile(INTFA_FIRST(nt) INTFA_COPY("%3", nt) INTFA_COPY("%4", nt) INTFA_COPY("%5", nt) :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]) : "memory", "scc"); \
@@ -92,7 +93,7 @@ __device__ __forceinline__ void lds_barrier() {
                      :: "s"(lds), "s"(base), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "v"(o[4]), "v"(o[5]), "v"(o[6]), "v"(o[7]), "v"(o[8]) : "memory", "scc")
 #define INTFA_FIRST(nt) "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1" nt
 template <bool NT, int N> __device__ __forceinline__ void copy_rows(const char* base, const uint32_t (&o)[N], uint32_t lds) {
-    static_assert(N == 2 || N == 3 || N == 4 || N == 5 || N == 8 || N == 9, "");
+    static_assert((N >= 1 && N <= 5) || N == 8 || N == 9, "");
     if constexpr (NT) { INTFA_COPIES(" nt"); } else { INTFA_COPIES(""); }
 }
 #undef INTFA_COPY
@@ -256,6 +257,9 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
     constexpr bool SMALL = ROWS == 32;         // scores in tiles of 16 keys by 16 rows: a wave has 16 keys of a block; else of 32 by 32
     constexpr int STEP = SMALL ? 64 : 32;
     static_assert(SMALL || (QT == 1 && RG == 2), "");
+    // The copies are the scoring waves' with few rows, which would wait for half of their time else (256 x 16 heads over 4096 tokens 106 us with the others' copies, 100 so), and
+    // the others' with 64, among their products.
+    constexpr bool SCORES_COPY = SMALL;
     constexpr int KC = DC / STEP, KR = (DR + STEP - 1) / STEP, KS = KC + KR;      // steps of the score's products: latent part, rotary part
     typedef LatentQueries<DC, DR, DT, ROWS> Queries;
     __shared__ __align__(16) char lds[S::LDS];
@@ -295,7 +299,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         const int bit = DR == 32 && S::LATENT_UNITS >= 16 ? UPF * k >> 3 & 1 : 0;
         return w.at[bit] + 16 * (UPF * k - 8 * bit);
     };
-    // ======== copies: wave w of the second half copies rows 16 w .. 16 w + 15 of every block
+    // ======== copies: wave w of a half copies rows 16 w .. 16 w + 15 of every block
     const int k_sn = deal->k_sn;
     auto offset_of = [&](int i) __attribute__((always_inline)) {
         const int unit = 64 * i + lane, r = unit / S::UNITS < 16 ? unit / S::UNITS : 15, u = unit % S::UNITS;
@@ -333,6 +337,15 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         if (S::HALF && lane < 32) copy_units(c.rows, copy_half, c.to + 1024u * S::WHOLE);
         if (lane < 32) copy_words(c.scales, c.named ? scale_off : (uint32_t)lane * 4, c.scales_to);
     };
+    constexpr int FIRST = (S::WHOLE + 1) / 2;
+    auto copy_some = [&](const BlockCopy& c, auto second) __attribute__((always_inline)) {      // half of the whole ones
+        constexpr int AT = decltype(second)::value ? FIRST : 0, N = decltype(second)::value ? S::WHOLE - FIRST : FIRST;
+        uint32_t off[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) off[i] = copy_off[AT + i];
+        if (streams) copy_rows<true>(c.rows, off, c.to + 1024u * AT);
+        else copy_rows<false>(c.rows, off, c.to + 1024u * AT);
+    };
     auto copy = [&](int block, int id) __attribute__((always_inline)) {
         const BlockCopy c = block_copy(block, id);
         if (streams) copy_rows<true>(c.rows, copy_off, c.to);
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         Queries queries;
         if (blocks > 0) {
             queries.load(p, t, row0, tid);
-            if (!scoring) {
+            if (SCORES_COPY ? scoring : !scoring) {
                 copy(0, look(0));
                 if (early) copy(1, look(1));
             }
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             }
             queries.form(p, lds, (const v2f*)(lds + S::ANGLES_AT), first_token, alphas);
         }
-        if (!scoring) {
+        if (SCORES_COPY ? scoring : !scoring) {
             if (early) wait_copies<S::COPIES>(); else wait_copies<0>();
         }
         lds_barrier();                         // queries and first block are there
@@ -507,8 +520,12 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 step(F, T, blocks, (blocks - 1) & 1);
             }
         }
-        else
+        else {
+        int id_next = look(2);
         for (int block = 0; block < blocks; ++block) {
+            const bool more = block + 2 < blocks;
+            const BlockCopy next = block_copy(block + 2, id_next);
+            if (more) id_next = look(block + 3);
             const int key0 = key_first + KEYS * block, tile = (block % STAGES) * S::STAGE;
             const float* const scales = (const float*)(lds + S::SCALES_AT + (block % STAGES) * S::SCALE_STAGE);
             // ---- scores, as t = score + log2 of the value's scale
@@ -572,6 +589,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 top[q] = reduce_row_lanes(top[q], [](float a, float b) { return fmaxf(a, b); });
                 if (c16 == 0) tops[kg * ROWS + 16 * q + x16] = top[q];
             }
+            if (more) copy_some(next, BoolTag<false>{});
             lds_barrier();                     // A: the maxima are there, and P of the block before has been read
             bool grows[QT], any = false;
 #pragma unroll
@@ -606,7 +624,13 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 for (int h = 0; h < PER / 2; ++h) w[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){s[q][2 * h], s[q][2 * h + 1]}, v2h));
                 *(v2i*)(lds + S::P_AT + (64 * wave + 16 * q + x16 + 32 * (c16 & 1)) * 16 + 8 * (c16 >> 1)) = (v2i){(int)w[0], (int)w[1]};
             }
+            if (more) {
+                copy_some(next, BoolTag<true>{});
+                copy_rest(next);
+                wait_copies<S::COPIES>();
+            } else wait_copies<0>();
             lds_barrier();                     // B: P is there, and so is the next block
+        }
         }
         lds_barrier();                         // (the other half's last block)
         lds_barrier();
@@ -639,7 +663,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[g][ct][r] = 0.f;
-        if (blocks > 1 && !early) copy(1, look(1));
+        if (!SMALL && blocks > 1 && !early) copy(1, look(1));
         for (int i = 0; i <= blocks; ++i) {
             if (!SMALL) {
                 wait_copies<0>();
@@ -704,8 +728,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 fetch(1);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (SMALL) copy_next();
-            else {
+            if (!SMALL) {
                 if (more) {
                     next = block_copy(i + 2, id_next);
                     id_next = look(i + 3);
@@ -737,10 +760,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 product(2);
                 product(3);
             }
-            if (SMALL) {
-                if (i + 2 < blocks) wait_copies<S::COPIES>(); else wait_copies<0>();
-                lds_barrier();                 // B
-            }
+            if (SMALL) lds_barrier();          // B
         }
         lds_barrier();                         // (the rows' sums are there)
         p = latent_args();
