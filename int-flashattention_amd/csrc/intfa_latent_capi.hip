@@ -101,7 +101,7 @@ int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream) {
         !rows16(p->v, p->v_stride_b, p->v_stride_h, p->v_stride_n) || !rows16(p->out, p->o_stride_b, p->o_stride_h, p->o_stride_n) || !aligned_to(p->lse, 4) ||
         !aligned_to(p->seqlens_q, 4) || !aligned_to(p->seqlens_k, 4)) return INTFA_ERR_ALIGN;
     // the keys of a (sequence, head) are addressed with 32 bits, those of a block behind the last one among them
-    auto fits = [&](int64_t row, int64_t dim) { return row >= dim && size_product((int64_t)p->seqlen_k + 64, row) < 1ll << 31; };
+    auto fits = [&](int64_t row, int64_t dim) { return row >= dim && size_product((int64_t)p->seqlen_k + 128, row) < 1ll << 31; };
     if (!fits(p->kn_stride_n, p->nope_dim) || !fits(p->kr_stride_n, p->rope_dim) || !fits(p->v_stride_n, p->v_dim)) return INTFA_ERR_SHAPE;
     if (p->seqlen > 1 << 30 || p->seqlen_k > 1 << 30) return INTFA_ERR_SHAPE;
     ExpandedParams ep{};

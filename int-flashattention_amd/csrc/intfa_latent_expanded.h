@@ -3,8 +3,8 @@
 // A workgroup of eight waves takes two tiles of 128 query rows of a head, four waves each, 32 rows a wave; both walk the same blocks of 64 keys, which asynchronous copies bring into two
 // stages of LDS.  With a causal mask the tiles are the n-th from the end and the n-th from the start, so that all workgroups have the same work.
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 in the inputs' type, a row in one lane and its pair (l ^ 32), so that P goes from accumulator to operand in its lane.
-// Where the tiles are no more than the compute units, a workgroup has one, and each half of it half of each block's keys; the halves' rows are joined in the end (SPLIT: 10 heads of
-// 64 + 32, 3 x 777 rows over up to 1555 keys 32 -> 25 us, 16 heads of 128 + 64 over 2048 unmasked tokens 65 -> 47; with twice the tiles, 4096 causal tokens, it would be 106 for 97).
+// Where the tiles are no more than the compute units, a workgroup has one, and each half of it half of the keys - of every block, or (small heads) every second block; the halves' rows are joined in the end
+// (SPLIT: 10 heads of 64 + 32, 3 x 777 rows over up to 1555 keys 32 -> 24 us, 16 heads of 128 + 64 over 2048 unmasked tokens 65 -> 47; with twice the tiles, 4096 causal tokens, it would be 106 for 97).
 // A third stage of LDS, requested two steps ahead, changed nothing (47 -> 48 us).
 // The blocks run as a software pipeline: each product of block n + 1's scores and of block n - 1's values is followed by its share of block n's softmax.
 #pragma once
@@ -26,13 +26,14 @@ template <int ROW, int PAD> struct PaddedTile {
     static __device__ __forceinline__ uint32_t source(int inst, int lane, uint32_t stride) { return (uint32_t)(inst + lane / (ROW / 16) * NI) * stride + 16u * (uint32_t)(lane % (ROW / 16)); }
 };
 
-template <int DN, int DR, int DV> struct ExpandedShape {
-    static constexpr int KEYS = 64, ROWS = 128;      // of a half of the workgroup
+template <int DN, int DR, int DV, bool SPLIT> struct ExpandedShape {
+    // split: of the small heads a step takes two tiles of keys, one for each half; of the large ones half of a tile for each (two of them twice over have no room)
+    static constexpr int PER_STEP = SPLIT && DN == 64 ? 2 : 1, KEYS = 64 * PER_STEP, ROWS = 128;      // of a half of the workgroup
     static constexpr int NROW = 2 * DN, RROW = 2 * DR, VROW = 2 * DV;
     typedef PaddedTile<NROW, 16> N;
     typedef PaddedTile<RROW, 16> R;
     typedef PaddedTile<VROW, 64> V;
-    static constexpr int OFF_N = 0, OFF_R = 2 * N::BYTES, OFF_V = OFF_R + 2 * R::BYTES, TILES = OFF_V + 2 * V::BYTES;
+    static constexpr int OFF_N = 0, OFF_R = 2 * PER_STEP * N::BYTES, OFF_V = OFF_R + 2 * PER_STEP * R::BYTES, TILES = OFF_V + 2 * PER_STEP * V::BYTES;
     static constexpr int LDS = TILES > 8 * OutStage<DV>::BYTES ? TILES : 8 * OutStage<DV>::BYTES;
     static constexpr int KN = DN / 16, KS = (DN + DR) / 16, DT = DV / 32;
 };
@@ -40,8 +41,8 @@ template <int DN, int DR, int DV> struct ExpandedShape {
 template <int DN, int DR, int DV, int DT_, bool CAUSAL, bool SPLIT>
 __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    typedef ExpandedShape<DN, DR, DV> S;
-    constexpr int KEYS = S::KEYS, KN = S::KN, KS = S::KS, DT = S::DT, NST = SPLIT ? 1 : 2, OWN = 32 * NST, PER = 16 * NST;      // keys of a block that a half has, and a lane's of them
+    typedef ExpandedShape<DN, DR, DV, SPLIT> S;
+    constexpr int KEYS = S::KEYS, KN = S::KN, KS = S::KS, DT = S::DT, TILES = S::PER_STEP, NST = SPLIT && TILES == 1 ? 1 : 2, OWN = 32 * NST, PER = 16 * NST;      // keys of a block that a half has, and a lane's of them
     // P = 2^(x - frame) times this: fp16 keeps its 11 bits down to 2^-21 of the frame's; bf16 has the range, and leaves room for sums of 2^12 of its largest values
     constexpr float kShift = DT_ == 0 ? 7.f : -20.f;
     __shared__ __align__(1024) char lds[S::LDS];
@@ -61,7 +62,8 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     // (split: the last tiles, which see the most keys, first)
     const int tile = SPLIT ? p.tiles - 1 - pair : CAUSAL ? (half == 0 ? p.tiles - 1 - pair : pair) : 2 * pair + half;
     const bool mine = SPLIT || (CAUSAL ? half == 0 || pair != p.tiles - 1 - pair : tile < p.tiles);
-    const int key0 = SPLIT ? 32 * half : 0;    // of the half's keys in a block
+    const int key0 = SPLIT ? OWN * half : 0;   // of the half's keys in a block
+    const int own_tile = TILES == 2 ? half : 0, own_row = TILES == 2 ? 0 : key0;
     auto length = [&](const int32_t* lens, int most) __attribute__((always_inline)) {
         if (lens == nullptr) return most;
         const int n = lens[z];
@@ -92,15 +94,21 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     const uint32_t r_off = S::R::source(all_wave % S::R::NI, lane, p.kr_sn);
     static_assert(S::N::NI % 8 == 0 && S::V::NI % 8 == 0 && S::R::NI <= 8, "");
     auto copy_k = [&](int block, int buf) __attribute__((always_inline)) {
-        const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS);
 #pragma unroll
-        for (int i = 0; i < NE; ++i) issue_copy_1k<false>(n_rsrc, n_off[i], at * p.kn_sn, lds0 + S::OFF_N + buf * S::N::BYTES + S::N::INST * (all_wave + 8 * i));
-        if (all_wave < S::R::NI) issue_copy_1k<false>(r_rsrc, r_off, at * p.kr_sn, lds0 + S::OFF_R + buf * S::R::BYTES + S::R::INST * all_wave);
+        for (int t = 0; t < TILES; ++t) {
+            const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS + 64 * t);
+#pragma unroll
+            for (int i = 0; i < NE; ++i) issue_copy_1k<false>(n_rsrc, n_off[i], at * p.kn_sn, lds0 + S::OFF_N + (buf * TILES + t) * S::N::BYTES + S::N::INST * (all_wave + 8 * i));
+            if (all_wave < S::R::NI) issue_copy_1k<false>(r_rsrc, r_off, at * p.kr_sn, lds0 + S::OFF_R + (buf * TILES + t) * S::R::BYTES + S::R::INST * all_wave);
+        }
     };
     auto copy_v = [&](int block, int buf) __attribute__((always_inline)) {
-        const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) issue_copy_1k<false>(v_rsrc, v_off[i], at * p.v_sn, lds0 + S::OFF_V + buf * S::V::BYTES + S::V::INST * (all_wave + 8 * i));
+        for (int t = 0; t < TILES; ++t) {
+            const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS + 64 * t);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) issue_copy_1k<false>(v_rsrc, v_off[i], at * p.v_sn, lds0 + S::OFF_V + (buf * TILES + t) * S::V::BYTES + S::V::INST * (all_wave + 8 * i));
+        }
     };
     if (all_blocks > 0) copy_k(0, 0);
     // ---- queries (B operand of S^T): sixteen bytes a step; a negative scale of scores turns them
@@ -118,8 +126,9 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     }
     const float scale = fmaxf(fabsf(p.qk_scale_log2), 0x1p-126f);      // (never zero: hidden keys are -infinity times it)
     // ---- a lane's places in the tiles
-    const uint32_t n_lane = S::OFF_N + S::N::at(key0) + S::N::at(lq) + 16 * lh, r_lane = S::OFF_R + S::R::at(key0) + S::R::at(lq) + 16 * lh;
-    const uint32_t v_lane = S::OFF_V + S::V::at(key0) + S::V::at(4 * lh + ((lane & 15) >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    const uint32_t n_lane = S::OFF_N + own_tile * S::N::BYTES + S::N::at(own_row) + S::N::at(lq) + 16 * lh;
+    const uint32_t r_lane = S::OFF_R + own_tile * S::R::BYTES + S::R::at(own_row) + S::R::at(lq) + 16 * lh;
+    const uint32_t v_lane = S::OFF_V + own_tile * S::V::BYTES + S::V::at(own_row) + S::V::at(4 * lh + ((lane & 15) >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     auto product = [&](v4i a, v4i b, v16f c) __attribute__((always_inline)) -> v16f {
         if (DT_ == 0) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -284,9 +293,9 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         const int buf = n & 1;
         if (n + 2 < all_blocks) copy_k(n + 2, buf);
         if (n >= 0 && n < all_blocks) copy_v(n, buf);
-        n_now = n_lane + (uint32_t)((buf ^ 1) * S::N::BYTES);
-        r_now = r_lane + (uint32_t)((buf ^ 1) * S::R::BYTES);
-        v_now = v_lane + (uint32_t)((buf ^ 1) * S::V::BYTES);
+        n_now = n_lane + (uint32_t)((buf ^ 1) * TILES * S::N::BYTES);
+        r_now = r_lane + (uint32_t)((buf ^ 1) * TILES * S::R::BYTES);
+        v_now = v_lane + (uint32_t)((buf ^ 1) * TILES * S::V::BYTES);
     };
     auto next = [&](auto par_tag, auto qk_tag, auto pv_tag) __attribute__((always_inline)) {
         sync();
