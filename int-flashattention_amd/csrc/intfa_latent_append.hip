@@ -76,7 +76,7 @@ template <int N, int LANES> __device__ __forceinline__ float to_bytes(const floa
 
 // A wave takes 64 / L tokens, nothing of it waits for another wave: L lanes a token, with units of sixteen elements of the latent part and some pairs of the rotary one.  Bound by its
 // arithmetic: with more lanes a token (64, and 32 for the rotary part) what a token costs once - its place, the norm's root, the divisions, the sums over its lanes - was more than what
-// its elements cost (16384 tokens of 512 + 64 16.2 us, and 11.9 so; 28.6 MB, 2.4 TB/s; one token 3.4 us).
+// its elements cost (16384 tokens of 512 + 64 16.2 us, and 11.9 so, 28.6 MB; 65536 tokens 24.5, 4.7 TB/s; one token 3.4).
 template <int DT, int DC, int DR> __global__ void __launch_bounds__(256) latent_append_kernel(const LatentAppendParams p) {
     constexpr int L = DC == 512 ? 16 : 8, T = 64 / L, E = DC / L, U = E / 16, P = DR / 2 / L;
     const int lane = threadIdx.x & 63, l = lane % L, first = ((int)blockIdx.x * 4 + ((int)threadIdx.x >> 6)) * T;
