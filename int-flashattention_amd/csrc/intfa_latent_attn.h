@@ -29,12 +29,31 @@ __device__ __forceinline__ LatentArgs latent_args() {
 constexpr float kLatentShift = 11.f, kLatentSlack = 4.f;
 // Scales enter scores as 2^-20 of themselves and the query's step as 2^20 of itself: products of up to 2^31 with scales of up to 2^117 fit.
 constexpr float kScoreUnit = 0x1p-20f;
-// Weights are summed as 2^-5 of themselves: 1 / s of scales of 2^121 is a normal number then, and sums of 2^21 of 2^-100 fit.
-constexpr float kWeightUnit = 0x1p-5f;
+// Weights are summed as 2^-18 of themselves: a term P / s is at most 2^97 (of s = 2^-100), and 2^30 keys fit; a row's largest is at least 2^-124 (its frame goes by another key, of s = 2^117),
+// where fp32 still has steps of 2^-25 of it.
+constexpr float kWeightLog = 18.f, kWeightUnit = 0x1p-18f;
+// P / s is P times a key's 1 / s, short of keys that lie so far under the row's frame, for their scale alone, that P leaves fp32 and P / s does not.  Where no scale that an item
+// has met is over this, those have weights of less than 2^-33 of the row's largest; from the first larger one on (latent vectors of 2000 and more) a second exponential, of the
+// score alone, takes the place of the product.
+constexpr float kLargeScale = 16.f;
 constexpr float kQuerySteps = 32512.f;         // 127 * 256: the high byte of a step count rounds to at most 127
 
 // What the scale of a token on a page that the table does not name is read from
 static __device__ const float kHiddenScale[32] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+
+// Sums of weights follow their row's frame, which the scales alone may move by 2^217.  A factor 2^d of one exponential ends at 2^-126: where it goes further than kOneFactor, it
+// is taken in two.  (Seldom: what checks for it does so for a wave, and for several factors at a time.)
+constexpr float kOneFactor = -125.f;
+__device__ __forceinline__ float add_moved(float sum, float a, float d) {
+    const bool far = d < kOneFactor;
+    return fmaf(fast_exp2(far ? kOneFactor : d), a * fast_exp2(far ? d - kOneFactor : 0.f), sum);
+}
+// sum + 2^x, down to fp32's last place (the exponential itself ends at 2^-126)
+__device__ __forceinline__ float add_exp2(float sum, float x) {
+    const float e = fast_exp2(0.5f * x);
+    return fmaf(e, e, sum);
+}
+__device__ __forceinline__ float log2_of_weights(float sum) { return sum < 0x1p100f ? __builtin_log2f(sum * (1.f / kWeightUnit)) : __builtin_log2f(sum) + kWeightLog; }
 
 template <int DC, int DR, int ROWS> struct LatentShape {
     static constexpr int ROW = DC + DR, UNITS = ROW / 16, LATENT_UNITS = DC / 16, KEYS = 64, THREADS = 512;
@@ -229,6 +248,9 @@ __device__ __forceinline__ LatentScale latent_scale(float c, float r, bool beyon
     return s;
 }
 
+// What takes log2 of the value's scale out of an exponent again, and the weights' unit in (0 for a hidden key: its exponent is -infinity)
+__device__ __forceinline__ float less_log(float c, bool beyond) { return beyond || c < 0.f ? 0.f : -__builtin_amdgcn_logf(fmaxf(c, 0x1p-100f)) - kWeightLog; }
+
 // Scales that come as lanes of a register (scale_lane_key), in the instruction that uses them: c = f * scale, c += scale of the lane's i-th key.  (Hand-written as fmac_lane_scale:
 // the compiler takes sixteen copies of the register first, which have no room here.)
 __device__ __forceinline__ float mul_lane_scale(float f, float scales, int i) {
@@ -415,6 +437,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             constexpr int AHEAD = 3, EARLY = KC / 8 > 1 ? KC / 8 : 1;      // fragments ahead of the products; of the latent part ahead of the weights
             static_assert(KC >= 4, "");
             float s[16], inv = 0.f, e_last = 0.f;
+            bool large = false;                // (of all waves alike)
             uint32_t w[4];
             auto element = [&](int j, float frame, int ln) __attribute__((always_inline)) {
                 const float e = fast_exp2(s[j] - frame);
@@ -460,12 +483,21 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                     const bool grows = top - m[0] > kLatentSlack, follow = __any(grows);      // (rows that do not need it stay: what a row gets does not depend on the others)
                     if (follow) {
                         const float alpha = grows ? fast_exp2(m[0] - top) : 1.f;
+                        const float d = grows && l[0] != 0.f ? m[0] - top : 0.f, was = l[0];
                         m[0] = grows ? top : m[0];
                         l[0] *= alpha;
+                        if (__builtin_expect(__any(d < kOneFactor), 0)) l[0] = add_moved(0.f, was, d);
                         if (kg == 0 && lh == 0) alphas[parity * ROWS + 32 * rg + lq] = alpha;
                     }
                     if (kg == 0 && ln == 0) flags[2 * parity + rg] = follow;
                     frame = (m[0] == -INFINITY ? 0.f : m[0]) - kLatentShift;
+                    if (__builtin_expect(large, 0)) {      // (the scales of the block: its stage is written two blocks later)
+                        const int key = 32 * kg + (int)scale_lane_key(ln);
+                        float take = less_log(*(const float*)(lds + S::SCALES_AT + ((next + STAGES - 1) % STAGES) * S::SCALE_STAGE + 8 * key), key0 - KEYS + key >= most);
+                        asm volatile("s_nop 1" : "+v"(take));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) l[0] = add_exp2(l[0], add_lane_scale(s[i] - frame, take, i));
+                    }
                     lds_barrier();             // A: P of the block before has been read
                 }
 #pragma unroll
@@ -480,7 +512,8 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                 if (QK) {
                     const v2f two = *(const v2f*)(lds + S::SCALES_AT + (next % STAGES) * S::SCALE_STAGE + 8 * (32 * kg + (int)scale_lane_key(ln)));
                     LatentScale sc = latent_scale(two[0], two[1], key0 + 32 * kg + (int)scale_lane_key(ln) >= most);
-                    inv = sc.inv;
+                    large = large || __any(*(const float*)(lds + S::SCALES_AT + (next % STAGES) * S::SCALE_STAGE + 8 * ln) > kLargeScale && key0 + ln < most);
+                    inv = large ? 0.f : sc.inv;
                     asm volatile("s_nop 1" : "+v"(sc.c), "+v"(sc.r), "+v"(sc.log), "+v"(inv));      // (two wait states to other lanes' reads)
                     wait_for_product(hi);
                     wait_for_product(lo);
@@ -522,6 +555,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
         }
         else {
         int id_next = look(2);
+        bool large = false;                    // (of all waves alike)
         for (int block = 0; block < blocks; ++block) {
             const bool more = block + 2 < blocks;
             const BlockCopy next = block_copy(block + 2, id_next);
@@ -549,7 +583,9 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
             v4i f[4];
             f[0] = fragment(0);
             f[1] = fragment(1);
-            const LatentScale sc = latent_scale(two[0], two[1], key0 + lane_key >= most);
+            LatentScale sc = latent_scale(two[0], two[1], key0 + lane_key >= most);
+            large = large || __any(scales[2 * lane] > kLargeScale && key0 + lane < most);
+            sc.inv = large ? 0.f : sc.inv;
             clear();
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
@@ -604,8 +640,10 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
 #pragma unroll
                 for (int q = 0; q < QT; ++q) {
                     const float alpha = grows[q] ? fast_exp2(m[q] - top[q]) : 1.f;
+                    const float d = grows[q] && l[q] != 0.f ? m[q] - top[q] : 0.f, was = l[q];
                     m[q] = grows[q] ? top[q] : m[q];
                     l[q] *= alpha;
+                    if (__builtin_expect(__any(d < kOneFactor), 0)) l[q] = add_moved(0.f, was, d);
                     if (kg == 0 && c16 == 0) alphas[16 * q + x16] = alpha;
                 }
             }
@@ -614,6 +652,11 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
 #pragma unroll
             for (int q = 0; q < QT; ++q) {
                 const float frame = (m[q] == -INFINITY ? 0.f : m[q]) - kLatentShift;
+                if (__builtin_expect(large, 0)) {
+                    const float take = less_log(two[0], key0 + lane_key >= most);
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) l[q] = add_exp2(l[q], s[q][i] - frame + lane_scale(take, i));
+                }
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     s[q][i] = fast_exp2(s[q][i] - frame);
@@ -788,7 +831,7 @@ __global__ void __launch_bounds__(512, 2) latent_attn_kernel(const LatentParams)
                     }
                 if (p->deal.lse != nullptr && wave == 0 && lh == 0)
                     p->deal.lse[((int64_t)t.z * p->deal.heads + head) * p->deal.seqlen + token] =
-                        token >= t.m ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+                        token >= t.m ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + log2_of_weights(sum);
             } else {
                 float* const slot = p->deal.parts + (int64_t)part.slot * ROWS * DC;
 #pragma unroll
@@ -836,7 +879,8 @@ template <int Q, int PER> __device__ __forceinline__ void latent_gather(const fl
         float grown = top;
 #pragma unroll
         for (int u = 0; u < PER; ++u) grown = fmaxf(grown, st[u][0]);
-        const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame);
+        const float frame = grown == -INFINITY ? 0.f : grown, a = fast_exp2(top - frame), was = sum, moved = sum != 0.f ? top - frame : 0.f;
+        float furthest = moved;
 #pragma unroll
         for (int k = 0; k < Q; ++k) acc[k] *= a;
         sum *= a;
@@ -845,11 +889,17 @@ template <int Q, int PER> __device__ __forceinline__ void latent_gather(const fl
         for (int u = 0; u < PER; ++u) {
             if (j0 + u * step >= pieces) continue;
             const float w = fast_exp2(st[u][0] - frame);
+            furthest = fminf(furthest, st[u][0] - frame);
 #pragma unroll
             for (int k = 0; k < Q; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[k][i] = fmaf(w, x[u][k][i], acc[k][i]);
             sum = fmaf(w, st[u][1], sum);
+        }
+        if (__builtin_expect(__any(furthest < kOneFactor), 0)) {
+            sum = add_moved(0.f, was, moved);
+#pragma unroll
+            for (int u = 0; u < PER; ++u) sum = add_moved(sum, st[u][1], st[u][0] - frame);
         }
     }
 }
@@ -934,6 +984,7 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
                     grown = fmaxf(grown, st[w][0]);
                 }
                 const float frame = grown == -INFINITY ? 0.f : grown;
+                float furthest = 0.f;
                 sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) {
@@ -942,6 +993,12 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[0][i] = fmaf(a, x[i], acc[0][i]);
                     sum = fmaf(a, st[w][1], sum);
+                    furthest = fminf(furthest, st[w][0] - frame);
+                }
+                if (__builtin_expect(__any(furthest < kOneFactor), 0)) {
+                    sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) sum = add_moved(sum, st[w][1], st[w][0] - frame);
                 }
                 top = grown;
             }
@@ -963,7 +1020,7 @@ __global__ void __launch_bounds__(512) latent_merge_kernel(const LatentParams) {
                 if (k == 0 || !share) store_out4<DT>(dst + 16 * k, o);
             }
             if (d.lse != nullptr && ct == 0 && quarter == 0 && lane < 32)
-                d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = beyond ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + __builtin_log2f(sum * (1.f / kWeightUnit));
+                d.lse[((int64_t)z * d.heads + head) * d.seqlen + token] = beyond ? -INFINITY : (top == -INFINITY ? 0.f : top) - kLatentShift + log2_of_weights(sum);
         }
     }
 }
