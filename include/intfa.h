@@ -525,8 +525,8 @@ int intfa_pages_fork(const intfa_page_table* t, const int32_t* parents, const in
 int intfa_pages_free(const intfa_page_table* t, const int32_t* sequences, const int32_t* keep, int32_t n, void* stream);
 
 /* Room for fresh[b] tokens (or fresh_all, where fresh is NULL) behind the seqlens_k[b] of each sequence.  Columns that these tokens reach and that name no page
- * get a free one; a page among them that others hold too is replaced by a copy (in every pool) of the sequence's own, unless all others that hold it in the same column get
- * copies in this call: the last one keeps it.  Free pages are dealt in their order, to sequence 0 first.  granted[b]: tokens that there is room for now, fewer
+ * get a free one; a page among them that others hold too is replaced by a copy (in every pool) of the sequence's own, unless all others that hold it get copies in this
+ * call: the last one keeps it.  (Tokens or not: pages reserved ahead of a fork are copied like those behind them.)  Free pages are dealt in their order, to sequence 0 first.  granted[b]: tokens that there is room for now, fewer
  * than asked where the pages ran out or the table ends; pass it to the append as seqlens_new.  (Once the pages have run out, sequences behind are granted
  * nothing in a page that had to be shared out.)  Lengths are not changed.  batch is at most 8192.
  * workspace: intfa_pages_reserve_workspace_bytes(t), 16-byte aligned, nothing to clear. */

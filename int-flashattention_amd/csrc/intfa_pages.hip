@@ -295,6 +295,7 @@ struct ReserveArgs {
     const int32_t* fresh; int32_t fresh_all;
     int32_t* granted;
     int32_t* free_list; int32_t* src; int32_t* dst; int32_t* count;      // src, dst: as long as the free list
+    int32_t* reached; int32_t* last;           // [pages]: of a page that is held more than once, the entries that a call reaches, and the last of them
 };
 
 // The columns that a sequence's fresh tokens reach: [first, end), end at most the table's width.
@@ -312,10 +313,11 @@ __device__ __forceinline__ Span reserve_span(const ReserveArgs& a, int z) {
     return s;
 }
 
-// Every sequence needs so many pages: those that it lacks, and copies of those that others hold.  Its page of the first column, which holds its last tokens, is the one that
-// forked sequences share: of all that want a copy of it in this call, the last takes none if nobody else is left.  (A thread keeps what it knows of its first sequence; of
-// batches over 1024 it reads the others' again.  Columns behind the first are its own work too while they are few, and a wave's where they are kLong or more: a trip to memory each, one
-// after the other, a prompt of 16384 tokens on pages of 16 took 400 us, and 17 so.)
+// Every sequence needs so many pages: those that it lacks, and copies of those that others hold; of all that want a copy of a page in this call, the last takes none if nobody else is
+// left.  The page that forked sequences share is that of their first column, which holds their last tokens: who is the last there is found among the first columns, in LDS.  Where
+// a later column is shared too (sequences forked after a reservation ahead), the entries that the call reaches are counted page by page in memory, and what the sequences need is
+// counted again (256 sequences of 4, three columns ahead: 31 us).  (A thread keeps what it knows of its first sequence; of batches over 1024 it reads the others' again.  Columns behind the first are its own work too while they
+// are few, and a wave's where they are kLong or more: a trip to memory each, one after the other, a prompt of 16384 tokens on pages of 16 took 400 us, and 17 so.)
 constexpr int kLong = 6;
 __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs a) {
     extern __shared__ __align__(16) int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
@@ -323,9 +325,9 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
     enum { kLacks, kKeep, kCopy, kLeft, kNone };      // (left: kept if all that share it and come earlier get their copies, else kNone)
     __shared__ int lds[kWalk / 64];
     __shared__ int long_z[kWalk], long_count[kWalk], longs;      // sequences of many columns, and what is counted of them
-    __shared__ int moves_lds;
+    __shared__ int moves_lds, deep_lds;
     const int pages = a.t.num_pages, Z = a.t.batch, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) moves_lds = longs = 0;
+    if (threadIdx.x == 0) moves_lds = longs = deep_lds = 0;
     const Counts stretch = load_counts(a.t.refs, kEach * (int)threadIdx.x, pages, 1);      // (asked for ahead of their use)
     Span own = {0, 0, 0, 0};
     int own_head = -1, own_holders = 0;
@@ -349,59 +351,116 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
         }
     }
     __syncthreads();
-    // needs, in the order of the sequences: granted[z] holds the pages that were dealt before it until its own are
-    int dealt = 0;
-    for (int z0 = 0; z0 < Z; z0 += kWalk) {
-        const int z = z0 + (int)threadIdx.x;
-        int needs = 0;
-        if (z < Z) {
-            const Span s = z < kWalk ? own : reserve_span(a, z);
-            const int head = z < kWalk ? own_head : head_lds[z];
-            if (head >= 0) {
-                const int holders = z < kWalk ? own_holders : a.t.refs[head];
-                int before = 0, o = 0;
-#pragma unroll 8
-                for (; o + 4 <= z; o += 4) {
-                    const v4i h = *(const v4i*)(head_lds + o);
-                    before += (h[0] == head) + (h[1] == head) + (h[2] == head) + (h[3] == head);
-                }
-                for (; o < z; ++o) before += head_lds[o] == head;
-                plan_lds[z] = holders - before > 1 ? kCopy : before > 0 ? kLeft : kKeep;
+    auto cell = [&](int z, int c) __attribute__((always_inline)) { return z * a.t.table_width + c; };      // (below 2^31)
+    // f(z, c, id) for the entries that are reached and name pages which others hold too
+    auto each_shared = [&](auto f) __attribute__((always_inline)) {
+        for (int z0 = 0; z0 < Z; z0 += kWalk) {
+            const int z = z0 + (int)threadIdx.x;
+            if (z < Z) {
+                const Span s = z < kWalk ? own : reserve_span(a, z);
+                if (s.end - s.first >= kLong) long_z[atomicAdd(&longs, 1)] = z;
+                else
+                    for (int c = s.first; c < s.end; ++c) {
+                        const int id = a.t.table[z * a.t.bt_sb + c];
+                        if ((unsigned)id < (unsigned)pages && a.t.refs[id] > 1) f(z, c, id);
+                    }
             }
-            needs = s.first < s.end && (plan_lds[z] == kLacks || plan_lds[z] == kCopy);
-            if (s.end - s.first >= kLong) long_z[atomicAdd(&longs, 1)] = z;
-            else
-                for (int c = s.first + 1; c < s.end; ++c) {
-                    const int id = a.t.table[z * a.t.bt_sb + c];
-                    needs += (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
-                }
-        }
-        __syncthreads();
-        if (longs > 0) {
+            __syncthreads();
             for (int i = wave; i < longs; i += kWalk / 64) {
                 const int zl = long_z[i];
                 const Span s = reserve_span(a, zl);
-                int count = 0;
-                for (int c0 = s.first + 1; c0 < s.end; c0 += 64) {
-                    bool takes = false;
-                    if (c0 + lane < s.end) {
-                        const int id = a.t.table[zl * a.t.bt_sb + c0 + lane];
-                        takes = (unsigned)id >= (unsigned)pages || a.t.refs[id] > 1;
-                    }
-                    count += __popcll(__ballot(takes));
+                for (int c = s.first + lane; c < s.end; c += 64) {
+                    const int id = a.t.table[zl * a.t.bt_sb + c];
+                    if ((unsigned)id < (unsigned)pages && a.t.refs[id] > 1) f(zl, c, id);
                 }
-                if (lane == 0) long_count[zl - z0] = count;
             }
-            __syncthreads();
-            const Span s = z >= Z ? Span{0, 0, 0, 0} : z < kWalk ? own : reserve_span(a, z);
-            if (s.end - s.first >= kLong) needs += long_count[threadIdx.x];
+            __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) longs = 0;
+            __syncthreads();
         }
-        int total;
-        const int ahead = scan_all(needs, lds, total);
-        if (z < Z) a.granted[z] = dealt + ahead;
-        dealt += total;
+    };
+    // An entry that names a page which others hold too: by it alone in the end?  (Known where the entries have been counted; both ways of the code below are of their own, for
+    // the sake of the usual one, which has no such entries behind the first columns: 2048 sequences 55 us, and 60 with the question in it.)
+    auto kept = [&](auto counted, int z, int c, int id) __attribute__((always_inline)) {
+        return decltype(counted)::value && __hip_atomic_load(a.last + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == cell(z, c) &&
+               __hip_atomic_load(a.reached + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.t.refs[id];
+    };
+    // needs, in the order of the sequences: granted[z] holds the pages that were dealt before it until its own are
+    int dealt = 0;
+    auto count_needs = [&](auto counted) __attribute__((always_inline)) {
+        for (int z0 = 0; z0 < Z; z0 += kWalk) {
+            const int z = z0 + (int)threadIdx.x;
+            int needs = 0;
+            if (z < Z) {
+                const Span s = z < kWalk ? own : reserve_span(a, z);
+                const int head = z < kWalk ? own_head : head_lds[z];
+                if (decltype(counted)::value && head >= 0) plan_lds[z] = kept(counted, z, s.first, head) ? kLeft : kCopy;
+                else if (head >= 0) {
+                    const int holders = z < kWalk ? own_holders : a.t.refs[head];
+                    int before = 0, o = 0;
+#pragma unroll 8
+                    for (; o + 4 <= z; o += 4) {
+                        const v4i h = *(const v4i*)(head_lds + o);
+                        before += (h[0] == head) + (h[1] == head) + (h[2] == head) + (h[3] == head);
+                    }
+                    for (; o < z; ++o) before += head_lds[o] == head;
+                    plan_lds[z] = holders - before > 1 ? kCopy : before > 0 ? kLeft : kKeep;
+                }
+                needs = s.first < s.end && (plan_lds[z] == kLacks || plan_lds[z] == kCopy);
+                if (s.end - s.first >= kLong) long_z[atomicAdd(&longs, 1)] = z;
+                else
+                    for (int c = s.first + 1; c < s.end; ++c) {
+                        const int id = a.t.table[z * a.t.bt_sb + c];
+                        const bool named = (unsigned)id < (unsigned)pages, shared = named && a.t.refs[id] > 1;
+                        if (shared) deep_lds = 1;
+                        needs += !named || (shared && !kept(counted, z, c, id));
+                    }
+            }
+            __syncthreads();
+            if (longs > 0) {
+                for (int i = wave; i < longs; i += kWalk / 64) {
+                    const int zl = long_z[i];
+                    const Span s = reserve_span(a, zl);
+                    int count = 0;
+                    for (int c0 = s.first + 1; c0 < s.end; c0 += 64) {
+                        bool takes = false;
+                        if (c0 + lane < s.end) {
+                            const int id = a.t.table[zl * a.t.bt_sb + c0 + lane];
+                            const bool named = (unsigned)id < (unsigned)pages, shared = named && a.t.refs[id] > 1;
+                            if (shared) deep_lds = 1;
+                            takes = !named || (shared && !kept(counted, zl, c0 + lane, id));
+                        }
+                        count += __popcll(__ballot(takes));
+                    }
+                    if (lane == 0) long_count[zl - z0] = count;
+                }
+                __syncthreads();
+                const Span s = z >= Z ? Span{0, 0, 0, 0} : z < kWalk ? own : reserve_span(a, z);
+                if (s.end - s.first >= kLong) needs += long_count[threadIdx.x];
+                __syncthreads();
+                if (threadIdx.x == 0) longs = 0;
+            }
+            int total;
+            const int ahead = scan_all(needs, lds, total);
+            if (z < Z) a.granted[z] = dealt + ahead;
+            dealt += total;
+        }
+    };
+    count_needs(std::false_type());
+    __syncthreads();
+    const bool deep = deep_lds != 0;
+    if (__builtin_expect(deep, 0)) {
+        each_shared([&](int, int, int id) __attribute__((always_inline)) {
+            __hip_atomic_store(a.reached + id, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(a.last + id, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
+        each_shared([&](int z, int c, int id) __attribute__((always_inline)) {
+            atomicAdd(a.reached + id, 1);
+            atomicMax(a.last + id, cell(z, c));
+        });
+        dealt = 0;
+        count_needs(std::true_type());
     }
     // as many free pages, in their order
     int found = 0;
@@ -429,51 +488,63 @@ __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs 
         const int64_t places = ((int64_t)room << a.t.page_log2) - s.held;
         a.granted[z] = places <= 0 ? 0 : places < s.fresh ? (int)places : s.fresh;
     };
-    for (int z0 = 0; z0 < Z; z0 += kWalk) {
-        const int z = z0 + (int)threadIdx.x;
-        if (z < Z) {
-            const Span s = z < kWalk ? own : reserve_span(a, z);
-            int rank = a.granted[z], plan = plan_lds[z];
-            if (plan == kLeft && rank > found) plan = kNone;
-            const bool many = s.end - s.first >= kLong;
-            int room = plan == kNone ? s.first : many ? s.first + 1 : s.end;
-            for (int c = s.first; c < room; ++c) {
-                const int id = a.t.table[z * a.t.bt_sb + c];
-                const bool named = (unsigned)id < (unsigned)pages;
-                const bool copy = named && (c == s.first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
-                if (named && !copy) continue;
-                if (rank >= found) {
-                    room = c;
-                    break;
+    auto deal = [&](auto counted) __attribute__((always_inline)) {
+        for (int z0 = 0; z0 < Z; z0 += kWalk) {
+            const int z = z0 + (int)threadIdx.x;
+            if (z < Z) {
+                const Span s = z < kWalk ? own : reserve_span(a, z);
+                int rank = a.granted[z], plan = plan_lds[z];
+                if (plan == kLeft && rank > found) plan = kNone;
+                const bool many = s.end - s.first >= kLong;
+                int room = plan == kNone ? s.first : many ? s.first + 1 : s.end;
+                for (int c = s.first; c < room; ++c) {
+                    const int id = a.t.table[z * a.t.bt_sb + c];
+                    const bool named = (unsigned)id < (unsigned)pages;
+                    bool copy = named && (c == s.first ? plan == kCopy : a.t.refs[id] > 1);      // (counts that are over 0 change behind the barrier below)
+                    if (copy && c != s.first && kept(counted, z, c, id)) {
+                        copy = false;
+                        if (rank > found) {        // (another could not leave)
+                            room = c;
+                            break;
+                        }
+                    }
+                    if (named && !copy) continue;
+                    if (rank >= found) {
+                        room = c;
+                        break;
+                    }
+                    give(z, c, id, copy, a.free_list[rank++]);
                 }
-                give(z, c, id, copy, a.free_list[rank++]);
+                if (many && room > s.first) {
+                    long_z[atomicAdd(&longs, 1)] = z;
+                    long_count[threadIdx.x] = rank;
+                } else grant(z, s, room);
             }
-            if (many && room > s.first) {
-                long_z[atomicAdd(&longs, 1)] = z;
-                long_count[threadIdx.x] = rank;
-            } else grant(z, s, room);
-        }
-        __syncthreads();
-        for (int i = wave; i < longs; i += kWalk / 64) {
-            const int zl = long_z[i];
-            const Span s = reserve_span(a, zl);
-            int rank = long_count[zl - z0], room = s.end;
-            for (int c0 = s.first + 1; c0 < s.end && room == s.end; c0 += 64) {
-                const int c = c0 + lane, id = c < s.end ? a.t.table[zl * a.t.bt_sb + c] : -1;
-                const bool named = (unsigned)id < (unsigned)pages, copy = named && a.t.refs[id] > 1, takes = c < s.end && (!named || copy);
-                const uint64_t all = __ballot(takes);
-                const int mine = rank + __popcll(all & ((1ull << lane) - 1));
-                if (takes && mine < found) give(zl, c, id, copy, a.free_list[mine]);
-                const uint64_t out = __ballot(takes && mine >= found);
-                if (out != 0) room = c0 + __builtin_ctzll(out);
-                rank += __popcll(all);
+            __syncthreads();
+            for (int i = wave; i < longs; i += kWalk / 64) {
+                const int zl = long_z[i];
+                const Span s = reserve_span(a, zl);
+                int rank = long_count[zl - z0], room = s.end;
+                for (int c0 = s.first + 1; c0 < s.end && room == s.end; c0 += 64) {
+                    const int c = c0 + lane, id = c < s.end ? a.t.table[zl * a.t.bt_sb + c] : -1;
+                    const bool named = (unsigned)id < (unsigned)pages, shared = named && a.t.refs[id] > 1, left = shared && kept(counted, zl, c, id), copy = shared && !left;
+                    const bool takes = c < s.end && (!named || copy);
+                    const uint64_t all = __ballot(takes);
+                    const int mine = rank + __popcll(all & ((1ull << lane) - 1));
+                    if (takes && mine < found) give(zl, c, id, copy, a.free_list[mine]);
+                    const uint64_t out = __ballot((takes && mine >= found) || (left && mine > found));
+                    if (out != 0) room = c0 + __builtin_ctzll(out);
+                    rank += __popcll(all);
+                }
+                if (lane == 0) grant(zl, s, room);
             }
-            if (lane == 0) grant(zl, s, room);
+            __syncthreads();
+            if (threadIdx.x == 0) longs = 0;
+            __syncthreads();
         }
-        __syncthreads();
-        if (threadIdx.x == 0) longs = 0;
-        __syncthreads();
-    }
+    };
+    if (__builtin_expect(deep, 0)) deal(std::true_type());
+    else deal(std::false_type());
     __threadfence_block();
     __syncthreads();
     for (int m = threadIdx.x; m < moves_lds; m += kWalk) atomicSub(a.t.refs + a.src[m], 1);
@@ -540,6 +611,7 @@ int64_t reserve_most(const intfa_page_table* t) {       // pages that a call can
     const int64_t entries = size_product(t->batch, t->table_width);
     return entries < t->num_pages ? entries : t->num_pages;
 }
+size_t reserve_bytes(const intfa_page_table* t) { return 16 + 12 * (size_t)reserve_most(t) + 8 * (size_t)t->num_pages; }
 
 }  // namespace
 
@@ -588,7 +660,7 @@ int intfa_pages_free(const intfa_page_table* t, const int32_t* sequences, const 
 }
 
 size_t intfa_pages_reserve_workspace_bytes(const intfa_page_table* t) {
-    return check_table(t, true, true) == INTFA_OK ? (size_t)(16 + 12 * reserve_most(t)) : 0;
+    return check_table(t, true, true) == INTFA_OK ? reserve_bytes(t) : 0;
 }
 
 int intfa_pages_reserve(const intfa_page_table* t, const intfa_page_pool* pools, int32_t num_pools, const int32_t* fresh, int32_t fresh_all, int32_t* granted,
@@ -601,9 +673,9 @@ int intfa_pages_reserve(const intfa_page_table* t, const intfa_page_pool* pools,
     if (t->batch > 8192 || size_product(t->batch, t->table_width) >= 1ll << 31) return INTFA_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(fresh) | reinterpret_cast<uintptr_t>(granted)) & 3u) return INTFA_ERR_ALIGN;
     const int64_t most = reserve_most(t);
-    if (workspace == nullptr || workspace_bytes < (size_t)(16 + 12 * most) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return INTFA_ERR_WORKSPACE;
+    if (workspace == nullptr || workspace_bytes < reserve_bytes(t) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return INTFA_ERR_WORKSPACE;
     int32_t* const words = (int32_t*)workspace;
-    ReserveArgs a{table_args(t), fresh, fresh_all, granted, words + 4, words + 4 + most, words + 4 + 2 * most, words};
+    ReserveArgs a{table_args(t), fresh, fresh_all, granted, words + 4, words + 4 + most, words + 4 + 2 * most, words, words + 4 + 3 * most, words + 4 + 3 * most + t->num_pages};
     hipLaunchKernelGGL(pages_reserve_kernel, dim3(1), dim3(kWalk), (size_t)t->batch * 8, (hipStream_t)stream, a);
     rc = (int)hipGetLastError();
     if (rc != 0 || num_pools == 0) return rc;

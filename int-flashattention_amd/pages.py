@@ -34,7 +34,7 @@ def paged_reserve(caches, refs, block_table, seqlens_k, seqlens_new, page_size):
     room for, int32 [Z]: fewer where the pages ran out or the table ends.  Pass that on as ``seqlens_new`` of the append.  Lengths are not changed.
 
     Columns that the tokens reach and that name no page get a free one: free pages are dealt in their order, to sequence 0 first.  A page among them that other sequences hold too is
-    replaced by a copy in every cache; of sequences that all want a copy of their last page in one call, the last keeps the page itself if nobody else holds it.
+    replaced by a copy in every cache; of sequences that all want a copy of a page in one call, the last keeps the page itself if nobody else holds it.
     (Once the pages have run out, sequences behind that are granted nothing in a page that others were to leave.)"""
     return (_host._native or _host.native()).paged_reserve(caches, refs, block_table, seqlens_k, seqlens_new, page_size)
 
