@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         const int n = lens[z];
         return n < 0 ? 0 : n < most ? n : most;
     };
-    const int m_rows = length(p.seqlens_q, p.seqlen), n_keys = length(p.seqlens_k, p.seqlen_k), off = n_keys - m_rows;
+    const int m_rows = length(p.seqlens_q, p.seqlen), n_keys = __builtin_amdgcn_readfirstlane(length(p.seqlens_k, p.seqlen_k)), off = n_keys - m_rows;
     auto blocks_of = [&](int t) __attribute__((always_inline)) {
         if (t >= p.tiles || t * S::ROWS >= m_rows) return 0;
         const int last = t * S::ROWS + S::ROWS < m_rows ? t * S::ROWS + S::ROWS : m_rows, seen = CAUSAL ? last + off : n_keys;
@@ -81,10 +81,24 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     const int row = tile * S::ROWS + 32 * wave + lq, row_ld = row < p.seqlen ? row : p.seqlen - 1;
     // ---- copies: a wave's share of a block
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    const uint32_t keys_1 = (uint32_t)(n_keys > 0 ? n_keys - 1 : 0);
-    const v4i n_rsrc = make_rsrc(p.kn + z * p.kn_sb + head * p.kn_sh, n_keys > 0 ? keys_1 * p.kn_sn + S::NROW : 0);
-    const v4i r_rsrc = make_rsrc(p.kr + z * p.kr_sb, n_keys > 0 ? keys_1 * p.kr_sn + S::RROW : 0);
-    const v4i v_rsrc = make_rsrc(p.v + z * p.v_sb + head * p.v_sh, n_keys > 0 ? keys_1 * p.v_sn + S::VROW : 0);
+    // A resource for each tile, which ends with its keys: rows behind the last one come as zeros.  (One for the whole, from which a tile is an offset in a scalar register, would not
+    // do: the hardware takes that from the resource's size ahead of its check, and of a tile that begins behind the last key nothing is left to check against.)  The addresses
+    // go on by a block's rows.
+    struct Rows { uint64_t at; uint32_t stride; };
+    auto rows_at = [](const char* at, uint32_t stride) __attribute__((always_inline)) {
+        const uint64_t a = (uint64_t)at;
+        return Rows{(uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), stride};
+    };
+    Rows n_rows = rows_at(p.kn + z * p.kn_sb + head * p.kn_sh, p.kn_sn), r_rows = rows_at(p.kr + z * p.kr_sb, p.kr_sn), v_rows = rows_at(p.v + z * p.v_sb + head * p.v_sh, p.v_sn);
+    auto tile_of = [&](const Rows& t, int i, int block) __attribute__((always_inline)) {
+        int keys = n_keys - block * KEYS - 64 * i;
+        keys = keys < 64 ? keys : 64;
+        asm("" : "+s"(keys));                  // (both bounds at once would be a vector instruction's)
+        keys = keys > 0 ? keys : 0;
+        const uint64_t at = t.at + (uint64_t)((uint32_t)i * 64 * t.stride);
+        return (v4i){(int)(uint32_t)at, (int)(uint32_t)(at >> 32), (int)((uint32_t)keys * t.stride), 0x00020000};      // (addresses end below 2^48: stride 0)
+    };
+    auto go_on = [&](Rows& t) __attribute__((always_inline)) { t.at += KEYS * t.stride; };      // (a block's rows span less than 2^32 bytes)
     constexpr int NE = (S::N::NI + 7) / 8, VE = (S::V::NI + 7) / 8;      // instructions of a wave (all eight have as many; those of the rotary part: one of some waves)
     uint32_t n_off[NE], v_off[VE];
 #pragma unroll
@@ -96,19 +110,22 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
     auto copy_k = [&](int block, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS + 64 * t);
+            const v4i n_rsrc = tile_of(n_rows, t, block);
 #pragma unroll
-            for (int i = 0; i < NE; ++i) issue_copy_1k<false>(n_rsrc, n_off[i], at * p.kn_sn, lds0 + S::OFF_N + (buf * TILES + t) * S::N::BYTES + S::N::INST * (all_wave + 8 * i));
-            if (all_wave < S::R::NI) issue_copy_1k<false>(r_rsrc, r_off, at * p.kr_sn, lds0 + S::OFF_R + (buf * TILES + t) * S::R::BYTES + S::R::INST * all_wave);
+            for (int i = 0; i < NE; ++i) issue_copy_1k<false>(n_rsrc, n_off[i], 0u, lds0 + S::OFF_N + (buf * TILES + t) * S::N::BYTES + S::N::INST * (all_wave + 8 * i));
+            if (all_wave < S::R::NI) issue_copy_1k<false>(tile_of(r_rows, t, block), r_off, 0u, lds0 + S::OFF_R + (buf * TILES + t) * S::R::BYTES + S::R::INST * all_wave);
         }
+        go_on(n_rows);
+        go_on(r_rows);
     };
     auto copy_v = [&](int block, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const uint32_t at = __builtin_amdgcn_readfirstlane(block * KEYS + 64 * t);
+            const v4i v_rsrc = tile_of(v_rows, t, block);
 #pragma unroll
-            for (int i = 0; i < VE; ++i) issue_copy_1k<false>(v_rsrc, v_off[i], at * p.v_sn, lds0 + S::OFF_V + (buf * TILES + t) * S::V::BYTES + S::V::INST * (all_wave + 8 * i));
+            for (int i = 0; i < VE; ++i) issue_copy_1k<false>(v_rsrc, v_off[i], 0u, lds0 + S::OFF_V + (buf * TILES + t) * S::V::BYTES + S::V::INST * (all_wave + 8 * i));
         }
+        go_on(v_rows);
     };
     if (all_blocks > 0) copy_k(0, 0);
     // ---- queries (B operand of S^T): sixteen bytes a step; a negative scale of scores turns them
