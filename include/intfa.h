@@ -473,8 +473,8 @@ int intfa_latent_attn_int8(const intfa_latent_attn_params* p, void* stream);
  * Sequence b has m = seqlens_q[b] queries (optional; clamped to [0, seqlen]; NULL: seqlen) and n = seqlens_k[b] keys (optional; clamped to [0, seqlen_k]; NULL: seqlen_k); with causal row i
  * sees keys 0 .. n - m + i.  Rows from m onward and rows that see no key are zeros with lse = -infinity; lse as in intfa_fwd_params.
  * Scores and sums are fp32, probabilities are rounded to the type of v; values that are not finite reach the rows that are computed together with those that see them (at
- * most 128 rows, and 128 keys behind a row's last).  Nothing behind a sequence's n keys is read.  seqlen_k + 128 rows of k_nope, of k_rope and of v (one head's, by their stride) must span
- * less than 2^31 elements. */
+ * most 128 rows, and 128 keys behind a row's last).  Nothing behind a sequence's n keys is read.  seqlen_k is less than 2^25, and rows of k_nope, of k_rope and of v are at least as far apart
+ * as they are long and less than 2^24 elements. */
 typedef struct intfa_latent_expanded_params {
     const void* q_nope; const void* q_rope; const void* k_nope; const void* k_rope; const void* v; void* out;
     int64_t qn_stride_b, qn_stride_h, qn_stride_n;

@@ -100,11 +100,14 @@ int intfa_latent_expanded(const intfa_latent_expanded_params* p, void* stream) {
         !rows16(p->k_nope, p->kn_stride_b, p->kn_stride_h, p->kn_stride_n) || !rows16(p->k_rope, p->kr_stride_b, 0, p->kr_stride_n) ||
         !rows16(p->v, p->v_stride_b, p->v_stride_h, p->v_stride_n) || !rows16(p->out, p->o_stride_b, p->o_stride_h, p->o_stride_n) || !aligned_to(p->lse, 4) ||
         !aligned_to(p->seqlens_q, 4) || !aligned_to(p->seqlens_k, 4)) return INTFA_ERR_ALIGN;
-    // the keys of a (sequence, head) are addressed with 32 bits, those of a block behind the last one among them
-    auto fits = [&](int64_t row, int64_t dim) { return row >= dim && size_product((int64_t)p->seqlen_k + 128, row) < 1ll << 31; };
+    // a block of 128 keys spans less than 2^32 bytes
+    auto fits = [&](int64_t row, int64_t dim) { return row >= dim && row < 1 << 24; };
     if (!fits(p->kn_stride_n, p->nope_dim) || !fits(p->kr_stride_n, p->rope_dim) || !fits(p->v_stride_n, p->v_dim)) return INTFA_ERR_SHAPE;
-    if (p->seqlen > 1 << 30 || p->seqlen_k > 1 << 30) return INTFA_ERR_SHAPE;
+    if (p->seqlen > 1 << 30 || p->seqlen_k >= 1 << 25) return INTFA_ERR_SHAPE;
     ExpandedParams ep{};
+    // those of a (sequence, head) together, and of the block behind the last one, may span more
+    auto far = [&](int64_t row) { return size_product((int64_t)p->seqlen_k + 128, row) >= 1ll << 31; };
+    ep.far = far(p->kn_stride_n) || far(p->kr_stride_n) || far(p->v_stride_n);
     ep.tiles = (p->seqlen + 127) / 128;
     const int64_t units = size_product(p->batch, p->heads);
     ep.split = size_product(units, ep.tiles) <= kComputeUnits;

@@ -11,6 +11,7 @@ struct ExpandedParams {
     uint32_t kn_sn, kr_sn, v_sn;                     // bytes
     int32_t batch, heads, seqlen, seqlen_k, tiles, pairs, whole;      // tiles of a head, pairs of them (split: the tiles again); workgroups of the (sequence, head)s that are dealt whole to the XCDs
     bool split;                                      // a workgroup has one tile, each half of it half of the keys
+    bool far;                                        // keys or values of a head span more than 32 bits
     float qk_scale_log2;
     FastDiv d_pairs, d_heads;
 };
