@@ -421,7 +421,8 @@ typedef struct intfa_latent_cache {
  * normalised first: c * w / sqrt(mean(c^2) + norm_eps).  All of it in fp32 and without a rounding in between; then for either part x
  *     scale = max(A / 127, 2^-100), A the part's largest magnitude;   q = rint(x / scale) within +-127.
  * A NaN becomes 0 and an infinity +-127, and neither counts for A.  Rows past the table's last column, of a page that it does not name, or from
- * seqlens_new[b] onward (optional; clamped to [0, seqlen_new]) are dropped.  The lengths are the caller's to advance.  No other token of a page is touched. */
+ * seqlens_new[b] onward (optional; clamped to [0, seqlen_new]) are dropped.  The lengths are the caller's to advance.  No other token of a page is touched.
+ * batch * seqlen_new is less than 2^28 - 15 where latent_dim is 512, else less than 2^29 - 31. */
 typedef struct intfa_latent_append_params {
     intfa_latent_cache cache;
     const void* c_new;                 /* fp16 or bf16 [batch, seqlen_new, latent_dim] and [batch, seqlen_new, rope_dim], rows contiguous, 16-byte aligned */

@@ -185,12 +185,16 @@ template <int DT, int DC, int DR> __global__ void __launch_bounds__(256) latent_
     }
 }
 
+constexpr int kAppendThreads = 256;
+int64_t append_groups(int64_t tokens, int dc) {
+    const int each = 4 * (dc == 512 ? 4 : 8);  // tokens of a workgroup: of its waves, T each
+    return tokens / each + (tokens % each != 0);
+}
 template <int DT> void launch(const LatentAppendParams& p, int dc, int dr, hipStream_t stream) {
-    const int each = dc == 512 ? 4 : 8;        // tokens of a wave (T above)
-    const dim3 grid((unsigned)((p.tokens + 4 * each - 1) / (4 * each)));
+    const dim3 grid((unsigned)append_groups(p.tokens, dc));
 #define INTFA_CALL(DC) do { \
-        if (dr == 64) hipLaunchKernelGGL((latent_append_kernel<DT, DC, 64>), grid, dim3(256), 0, stream, p); \
-        else hipLaunchKernelGGL((latent_append_kernel<DT, DC, 32>), grid, dim3(256), 0, stream, p); } while (0)
+        if (dr == 64) hipLaunchKernelGGL((latent_append_kernel<DT, DC, 64>), grid, dim3(kAppendThreads), 0, stream, p); \
+        else hipLaunchKernelGGL((latent_append_kernel<DT, DC, 32>), grid, dim3(kAppendThreads), 0, stream, p); } while (0)
     if (dc == 512) INTFA_CALL(512); else if (dc == 256) INTFA_CALL(256); else INTFA_CALL(128);
 #undef INTFA_CALL
 }
@@ -212,9 +216,9 @@ int intfa_latent_append_int8(const intfa_latent_append_params* p, void* stream) 
         !aligned_to(p->norm_weight, 16) || !aligned_to(p->seqlens_k, 4) || !aligned_to(p->seqlens_new, 4) || !aligned_to(p->rope.freqs, 8)) return INTFA_ERR_ALIGN;
     if (p->norm_weight != nullptr && (!(p->norm_eps > 0.f) || p->norm_eps > 3.402823466e38f)) return INTFA_ERR_SHAPE;
     const int64_t tokens = size_product(p->batch, p->seqlen_new);
-    if (tokens > 1ll << 30) return INTFA_ERR_SHAPE;          // (tokens are 32-bit numbers, and so are the threads of a launch)
+    // (tokens are 32-bit numbers, and so are the threads of a launch)
+    if (tokens > 1ll << 30 || append_groups(tokens, c.latent_dim) * kAppendThreads >= 1ll << 32) return INTFA_ERR_SHAPE;
     LatentAppendParams ap{};
-    if (size_product(tokens, 64) >= 1ll << 32) return INTFA_ERR_SHAPE;
     ap.c = (const char*)p->c_new; ap.k = (const char*)p->k_new; ap.weight = (const char*)p->norm_weight;
     ap.c_sb = p->cn_stride_b * 2; ap.c_sn = p->cn_stride_n * 2; ap.k_sb = p->kn_stride_b * 2; ap.k_sn = p->kn_stride_n * 2;
     ap.rows = (char*)c.rows; ap.scale = c.scale; ap.r_sp = c.r_stride_p; ap.s_sp = c.s_stride_p; ap.r_sn = (int32_t)c.r_stride_n; ap.s_sn = (int32_t)c.s_stride_n;
