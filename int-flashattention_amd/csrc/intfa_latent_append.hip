@@ -16,6 +16,7 @@ struct LatentAppendParams {
     const int32_t* seqlens_k; const int32_t* seqlens_new;
     RopeArgs rope;
     float eps;
+    int32_t least_e;                                 // the least power of two that a row counts as for its norm
     int32_t tokens, seqlen_new, page_log2, num_pages, table_width;
     FastDiv d_seqlen;
 };
@@ -145,8 +146,8 @@ template <int DT, int DC, int DR> __global__ void __launch_bounds__(256) latent_
 #pragma unroll
     for (int u = 0; u < 2 * U; ++u) unpack8<DT>(raw[u], x + 8 * u);
     if (p.weight != nullptr) {
-        // The squares are those of x / 2^e, 2^e the size of the row's largest element: they stay in range whatever the row's size.  (e from -40, under which
-        // eps is all there is; 126 for a row with an infinity, which thereby becomes one of zeros, as its formula has it)
+        // The squares are those of x / 2^e, 2^e the size of the row's largest element: they stay in range whatever the row's size.  (e from -40, or from 2^-50 of eps' root, under which
+        // eps is all there is and eps / 4^e would leave fp32; 126 for a row with an infinity, which thereby becomes one of zeros, as its formula has it)
         typedef unsigned short v2us __attribute__((ext_vector_type(2)));
         v2us most = {0, 0};                    // (magnitudes of 16-bit numbers are ordered as their bits are)
 #pragma unroll
@@ -158,7 +159,7 @@ template <int DT, int DC, int DR> __global__ void __launch_bounds__(256) latent_
         uint32_t top = __builtin_bit_cast(uint32_t, two_tops[0]), other = __builtin_bit_cast(uint32_t, two_tops[1]);
         top = over_lanes<L>(top > other ? top : other, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
         int e = (int)(top >> 23) - 127;
-        e = e < -40 ? -40 : e > 126 ? 126 : e;
+        e = e < p.least_e ? p.least_e : e > 126 ? 126 : e;
         const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
         float sum = 0.f;
 #pragma unroll
@@ -225,6 +226,8 @@ int intfa_latent_append_int8(const intfa_latent_append_params* p, void* stream) 
     ap.table = c.block_table; ap.bt_sb = c.bt_stride_b; ap.seqlens_k = p->seqlens_k; ap.seqlens_new = p->seqlens_new;
     ap.rope = {p->rope.freqs, p->rope.freqs != nullptr ? p->rope.pairs : 0, p->rope.interleaved, p->rope.magnitude};
     ap.eps = p->norm_eps;
+    const int root = p->norm_weight != nullptr ? ((int)(__builtin_bit_cast(uint32_t, p->norm_eps) >> 23) - 127) / 2 : 0;
+    ap.least_e = root - 50 > -40 ? root - 50 : -40;
     ap.tokens = (int32_t)tokens; ap.seqlen_new = p->seqlen_new;
     ap.page_log2 = __builtin_ctz((unsigned)c.page_size); ap.num_pages = c.num_pages; ap.table_width = c.table_width;
     ap.d_seqlen = make_fast_div(p->seqlen_new);
