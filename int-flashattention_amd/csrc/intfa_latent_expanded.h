@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         if (half == 1) return;
     }
     if (!mine) return;
-    const bool padding = row >= m_rows, empty = padding || m == -INFINITY;
+    const bool padding = row >= m_rows, empty = padding || m == -INFINITY, zeros = padding || l == 0.f;      // (a row without a key: its products may hold 0 times an infinite value)
     const float inv = empty ? 0.f : 1.f / l;
     if (p.lse != nullptr && lh == 0 && row < p.seqlen)
         p.lse[((int64_t)z * p.heads + head) * p.seqlen + row] = padding ? -INFINITY : (m == -INFINITY ? 0.f : m) - kShift + __builtin_log2f(l);
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(512, 2) latent_expanded_kernel(const ExpandedP
         for (int k = 0; k < 4; ++k) {
             v4f o = {acc[dt][4 * k], acc[dt][4 * k + 1], acc[dt][4 * k + 2], acc[dt][4 * k + 3]};
             o *= inv;
-            if (padding) o = (v4f){0.f, 0.f, 0.f, 0.f};
+            if (zeros) o = (v4f){0.f, 0.f, 0.f, 0.f};
             v2i bits;
             store_out4<DT_>((char*)&bits, o);
             out_stage_put<DV>(stage, lq, 32 * dt + 8 * k + 4 * lh, bits);
