@@ -297,7 +297,7 @@ const char* intfa_error_string(int code) {
         case INTFA_ERR_ALIGN: return "pointers and row/head/batch strides must be 16-byte aligned";
         case INTFA_ERR_DTYPE: return "unknown dtype enum";
         case INTFA_ERR_WORKSPACE: return "workspace missing, misaligned or too small for num_splits";
-        case INTFA_ERR_SHAPE: return "batch and heads must be positive and the grid must fit 31 bits";
+        case INTFA_ERR_SHAPE: return "batch and heads must be positive, sizes and strides within what the entry point's declaration allows, the eps of a norm a positive number, and the grid must fit 31 bits";
         case INTFA_ERR_SPLITS: return "num_splits must be at most 64";
         case INTFA_ERR_VSCALE: return "v_scale_block must be a multiple of the key-block length (or 64 at head_dim 128) and vs_stride_blk at least head_dim";
         case INTFA_ERR_SCRATCH: return "the split-KV partials of this call exceed INTFA_STATIC_SCRATCH_BYTES (or the device index exceeds 63)";

@@ -1,6 +1,9 @@
 """Sizes and strides that are past what the latent cache's entry points take, refused ahead of any GPU call (the largest that they do take are run in the GPU tests)."""
+import math
+
 import pytest
 
+from int_flashattention_amd import _capi
 from test_latent_host import _append, _attn_bytes, _expanded
 
 
@@ -24,3 +27,8 @@ def test_appends_of_too_many_tokens(kw):
 def test_workspace_where_the_workgroups_become_fewer(kw, rows, workgroups):
     """Two slots of fp32 rows for each, their maxima and sums, and an open item: units are numbered in 32 bits, times the workgroups."""
     assert _attn_bytes(**kw) == workgroups * (2 * rows * (512 * 4 + 8) + 16)
+
+
+def test_what_a_refusal_says():
+    text = _capi.load().intfa_error_string(_append(norm_eps=math.nan)).decode()
+    assert _append(norm_eps=math.nan) == _expanded(kn_stride_n=1 << 24) == -7 and "eps" in text and "strides" in text and "sizes" in text
