@@ -757,9 +757,14 @@ PyObject* attention_latent(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto is = [&](int i, int64_t h, int64_t rows, int64_t d) { return in[i]->size(0) == Z && in[i]->size(1) == h && in[i]->size(2) == rows && in[i]->size(3) == d; };
     if (!is(1, H, N, dr) || !is(2, H, Nk, dn) || !is(3, 1, Nk, dr) || !is(4, H, Nk, dv))
         fail(PyExc_ValueError, "q_nope and q_rope must be [Z, H, N, d], k_nope and v [Z, H, N_k, d], k_rope [Z, 1, N_k, d]");
+    if (Nk >= 1 << 25) fail(PyExc_ValueError, "there must be fewer than 2^25 keys, got " + std::to_string(Nk));
     const CallDevice dev(*in[0]);
     Tensor x[5];
-    for (int i = 0; i < 5; ++i) x[i] = row_major(*in[i], in[i]->size(3), 2);
+    for (int i = 0; i < 5; ++i) {
+        x[i] = row_major(*in[i], in[i]->size(3), 2);
+        // (rows of keys that lie over each other, broadcast ones among them, or further apart than the kernel's addresses go)
+        if (i >= 2 && Nk > 1 && (x[i].stride(2) < x[i].size(3) || x[i].stride(2) >= 1 << 24)) x[i] = x[i].contiguous();
+    }
     const Tensor &lens_q = optional_tensor_arg(a[7], "seqlens_q"), &lens_k = optional_tensor_arg(a[8], "seqlens_k");
     Tensor lens_q_, lens_k_, lse, out = dev.empty({Z, H, N, dv}, x[0].scalar_type());
     const bool return_lse = bool_arg(a[9]);
@@ -777,6 +782,7 @@ PyObject* attention_latent(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
         set_strides(&p.qn_stride_b, x[0]); set_strides(&p.qr_stride_b, x[1]); set_strides(&p.kn_stride_b, x[2]); set_strides(&p.v_stride_b, x[4]); set_strides(&p.o_stride_b, out);
         p.kr_stride_b = x[3].stride(0); p.kr_stride_n = x[3].stride(2);
+        if (Nk == 1) { p.kn_stride_n = dn; p.kr_stride_n = dr; p.v_stride_n = dv; }      // (a single row's stride may be anything)
         p.seqlens_q = lens_q_.defined() ? lens_q_.data_ptr<int32_t>() : nullptr;
         p.seqlens_k = lens_k_.defined() ? lens_k_.data_ptr<int32_t>() : nullptr;
         p.batch = (int)Z; p.heads = (int)H; p.seqlen = (int)N; p.seqlen_k = (int)Nk; p.nope_dim = (int)dn; p.rope_dim = (int)dr; p.v_dim = (int)dv; p.dtype = quant_dtype(x[0]);

@@ -38,7 +38,7 @@ def attention_paged_latent_int8(q_latent, q_rope, cache, scale, block_table, seq
 def attention_latent(q_nope, q_rope, k_nope, k_rope, v, causal, sm_scale, *, seqlens_q=None, seqlens_k=None, return_lse=False):
     """The same attention with keys and values expanded for every head, which prompts are cheaper with: ``q_nope`` [Z, H, N, dn], ``q_rope`` [Z, H, N, dr], ``k_nope`` [Z, H, N_k, dn],
     ``k_rope`` [Z, 1, N_k, dr] (shared by the heads), ``v`` [Z, H, N_k, dv], all fp16 or all bf16; (dn, dr, dv) is (128, 64, 128) or (64, 32, 64).  Slices of projections will do:
-    only the last dimension has to be contiguous (N_k is less than 2^25, and keys of a head are less than 2^24 elements apart).  Rotary parts come rotated (``rotary``).  Returns a new contiguous [Z, H, N, dv] tensor, and with ``return_lse`` also
+    only the last dimension has to be contiguous (rows of keys that overlap or are 2^24 elements and more apart are copied first).  N_k is less than 2^25.  Rotary parts come rotated (``rotary``).  Returns a new contiguous [Z, H, N, dv] tensor, and with ``return_lse`` also
     m + log2(l) of each row, fp32 [Z, H, N].
 
     ``seqlens_q`` and ``seqlens_k`` (int32 [Z] on the device): queries and keys of each sequence where they are fewer; nothing behind a sequence's keys is read.  With ``causal`` row i
