@@ -121,7 +121,8 @@ Tensor row_major(const Tensor& t, int64_t d_to, int elem_bytes) {
     const Tensor x = t.size(-1) == d_to ? t : at::constant_pad_nd(t, {0, d_to - t.size(-1)});
     bool ok = x.stride(-1) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) ok = ok && (x.stride(i) * elem_bytes) % 16 == 0;
-    return ok ? x : x.contiguous();
+    // (one that is contiguous as it is, off its 16 bytes or with a stride of a single entry that is, stays itself in contiguous())
+    return ok ? x : x.is_contiguous() ? x.clone(at::MemoryFormat::Contiguous) : x.contiguous();
 }
 // True if the rows of consecutive heads of t ([Z, H, N, ...]) lie at one constant stride.
 bool can_fold(const Tensor& t, int64_t n) { return n == 1 || t.stride(1) == n * t.stride(2); }
