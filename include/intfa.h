@@ -448,6 +448,7 @@ int intfa_latent_append_int8(const intfa_latent_append_params* p, void* stream);
  * magnitudes times sm_scale; a row that holds no number gives none.  Products are exact in integers, scores and sums fp32 (a score past 2^128 is no number; so are scores of keys past
  * 2^124 or queries past 2^120).  Probabilities times their token's scale are rounded to 11 bits, those under 2^-25 of the row's largest to steps of 2^-35 of it.
  * What a token weighs does not go by its scale: the sum of a row's weights, and lse, have those down to 2^-25 of its largest, whatever scales (to 2^117) lie beside each other.
+ * The work is dealt by table_width, batch, heads and seqlen: with another width the same call may differ in its last bits (calls of one shape repeat to the bit).
  * workspace: at least intfa_latent_attn_workspace_bytes(p) bytes of device memory, 16-byte aligned, nothing to clear; two launches that may run at the same
  * time must not share it. */
 typedef struct intfa_latent_attn_params {

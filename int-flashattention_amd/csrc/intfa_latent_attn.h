@@ -9,7 +9,7 @@
 //                  the columns for all rows, so that no byte is converted twice.  P goes through LDS in the operand's own layout.
 // A token's value scale s goes into the exponent: rows follow the maximum of t = score + log2 s, P = 2^(t - frame), and the sum of weights is that of P / s.  Whatever the
 // scales' sizes, P is within fp16 and the accumulators are plain sums of int8 numbers times P; the output is their quotient.
-// Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 100 us with the merge, 6.1 TB/s (memory; the same pages over and over would be 86);
+// Measured, latent part 512 and rotary part 64: 16 heads of 256 requests over 4096 tokens 101 us with the merge, 6.1 TB/s (memory; the same pages over and over would be 86);
 // 128 heads of 32 requests 54 us and 10 of merging, 670 TFLOP/s without it (4560 clocks a block of 64 rows, where products take 2176 and vector instructions 1840: two waves a SIMD, in order, hide little of either
 // under the other).  Tiles of 32 rows are for few rows, and where there is little work (make_plan): 16 of their rows cost what 32 do in the values' product, which is not what bounds few rows.
 #pragma once

@@ -316,8 +316,9 @@ __device__ __forceinline__ Span reserve_span(const ReserveArgs& a, int z) {
 // Every sequence needs so many pages: those that it lacks, and copies of those that others hold; of all that want a copy of a page in this call, the last takes none if nobody else is
 // left.  The page that forked sequences share is that of their first column, which holds their last tokens: who is the last there is found among the first columns, in LDS.  Where
 // a later column is shared too (sequences forked after a reservation ahead), the entries that the call reaches are counted page by page in memory, and what the sequences need is
-// counted again (256 sequences of 4, three columns ahead: 31 us).  (A thread keeps what it knows of its first sequence; of batches over 1024 it reads the others' again.  Columns behind the first are its own work too while they
-// are few, and a wave's where they are kLong or more: a trip to memory each, one after the other, a prompt of 16384 tokens on pages of 16 took 400 us, and 17 so.)
+// counted again (256 sequences in groups of four, three columns ahead: 31 us).  (A thread keeps what it knows of its first sequence; of batches over 1024 it reads the others' again.
+// Columns behind the first are its own work too while they are few, and a wave's where they are kLong or more: a trip to memory each, one after the other, a prompt of 16384 tokens
+// on pages of 16 took 400 us, and 17 so.)
 constexpr int kLong = 6;
 __global__ void __launch_bounds__(kWalk) pages_reserve_kernel(const ReserveArgs a) {
     extern __shared__ __align__(16) int32_t head_lds[];      // [batch]: the shared page of a sequence's first column, or -1
